@@ -42,7 +42,8 @@ typedef enum {
   IPUC_ERR_ALIGNMENT = 3,        /* pointer or leading-dimension alignment */
   IPUC_ERR_CUDA = 4,             /* a CUDA runtime/driver call failed */
   IPUC_ERR_NCCL = 5,             /* a collective failed */
-  IPUC_ERR_DEVICE_TIMEOUT = 6    /* a bounded device wait gave up (error word set) */
+  IPUC_ERR_DEVICE_TIMEOUT = 6,   /* a bounded device wait gave up (error word set) */
+  IPUC_ERR_DEVICE_INDEX = 7      /* an index in device memory was out of range (error word set) */
 } ipuc_status;
 
 /* Precision (operator.rs Precision, F16/F32 only). */
@@ -66,7 +67,9 @@ const char *ipuc_status_string(ipuc_status status);
 /* Thread-local description of the last error returned on this thread. */
 const char *ipuc_last_error_string(void);
 /* Reads and clears the device error word set by bounded waits inside kernels
- * on the current device (synchronises `stream`).  Reference: the device
+ * (IPUC_ERR_DEVICE_TIMEOUT) and by their range checks of indices in device
+ * memory (IPUC_ERR_DEVICE_INDEX) on the current device (synchronises `stream`;
+ * the word keeps the first error).  Reference: the device
  * "fails" only by host-side timeout (device/static_runtime.S:487-488). */
 ipuc_status ipuc_device_status(ipuc_stream stream);
 
@@ -441,6 +444,136 @@ ipuc_status ipuc_ipc_close(void *device_ptr);
  * IPUC_ERR_DEVICE_TIMEOUT) and returns. */
 ipuc_status ipuc_peer_all_reduce_f16(void *const *inputs, void *const *outputs, void *const *signals, int32_t rank,
                                      int32_t world, uint64_t element_count, ipuc_stream stream);
+
+/* ---- Serving with positions and a paged key/value cache -------------------
+ * No counterpart in the reference, whose graphs have no positions and no
+ * cache: what a transformer block needs next to ipuc_gemm_f16 and
+ * ipuc_flash_attention_f16 when it generates tokens.  Values are f16, all
+ * arithmetic is f32 with one rounding at the store (the products inside
+ * attention take f16 operands, as ipuc_flash_attention_f16).  Forward only.
+ *
+ * Indices in device memory (positions, lengths, row offsets, page ids) are
+ * checked by the kernels: one out of range leaves its access out and makes
+ * the next ipuc_device_status() return IPUC_ERR_DEVICE_INDEX; what else the
+ * call writes for that sequence is then unspecified. */
+
+/* Angles theta(p, i) = p * f_i of pair i at position p, from f_i = base^(-2i/R)
+ * with R = rotary_dim, scaled for contexts longer than the model's own:
+ *   NONE    f_i
+ *   LINEAR  f_i / factor
+ *   BASE    base * factor^(R / (R - 2)) in place of base
+ *   BANDS   w_i f_i + (1 - w_i) f_i / factor, where w_i goes from 0 to 1 as
+ *           the turns that pair i makes over `original` positions,
+ *           original * f_i / 2pi, go from `low` to `high`
+ * Cosines and sines are multiplied by `magnitude` (1 where unused). */
+typedef enum {
+  IPUC_ROTARY_SCALE_NONE = 0,
+  IPUC_ROTARY_SCALE_LINEAR = 1,
+  IPUC_ROTARY_SCALE_BASE = 2,
+  IPUC_ROTARY_SCALE_BANDS = 3
+} ipuc_rotary_scale;
+typedef struct {
+  int32_t kind;          /* ipuc_rotary_scale */
+  double base;           /* > 1 */
+  double factor;         /* >= 1 (LINEAR, BASE, BANDS) */
+  double low, high;      /* BANDS: low < high */
+  double original;       /* BANDS: > 0 */
+  double magnitude;      /* > 0 */
+} ipuc_rotary_scaling;
+/* table f32 [positions][rotary_dim]: the cosines of a position's rotary_dim / 2
+ * pairs, then their sines.  Angles are reduced in 64 bits, so far positions
+ * keep f32 accuracy.  rotary_dim even, at most 256.  Built once per model. */
+ipuc_status ipuc_rotary_table(float *table, int64_t positions, int64_t rotary_dim,
+                              const ipuc_rotary_scaling *scaling, ipuc_stream stream);
+
+/* Which elements of a head form pair i of the first rotary_dim: (x_i,
+ * x_{i + rotary_dim/2}) or (x_2i, x_{2i+1}).  Elements from rotary_dim on pass. */
+typedef enum { IPUC_ROTARY_HALF = 0, IPUC_ROTARY_INTERLEAVED = 1 } ipuc_rotary_layout;
+typedef struct {
+  const float *table;    /* ipuc_rotary_table's */
+  int64_t positions;     /* its rows */
+  int32_t rotary_dim;    /* its columns; even, <= head_dim; 0: no rotation */
+  int32_t layout;        /* ipuc_rotary_layout */
+} ipuc_rotary;
+
+/* Rotates the heads of [tokens][heads][head_dim] rows: token t lies at t *
+ * stride elements (a slice of a projection; stride >= heads * head_dim), in
+ * f16 or f32 (a projection written with IPUC_GEMM_OUT_F32); out f16.
+ * positions: device int32 [tokens], NULL for 0, 1, ...; a token with a
+ * negative position is padding and its output is left as it is.  In place
+ * (out == in, f16, equal strides) or apart; head_dim even, at most 256; any
+ * alignment of f16 elements (16 bytes are fastest). */
+ipuc_status ipuc_rotary_f16(void *out, int64_t out_stride, const void *in, int64_t in_stride,
+                            ipuc_precision in_precision, int64_t tokens, int64_t heads, int64_t head_dim,
+                            const ipuc_rotary *rotary, const int32_t *positions, ipuc_stream stream);
+
+/* Norm of queries and keys over each head, y = x / sqrt(mean(x^2) + eps) *
+ * weight (f16 [head_dim], NULL for ones), and their rotation (NULL: none) in
+ * one pass.  Rows, precisions, positions and in-place use as ipuc_rotary_f16;
+ * q_heads or k_heads may be 0 (that tensor's pointers are then not read). */
+ipuc_status ipuc_qk_norm_rotary_f16(void *q_out, int64_t q_out_stride, void *k_out, int64_t k_out_stride,
+                                    const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                                    ipuc_precision in_precision, const void *q_weight, const void *k_weight,
+                                    float eps, int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t head_dim,
+                                    const ipuc_rotary *rotary, const int32_t *positions, ipuc_stream stream);
+
+/* A paged cache: slot s of page p of head h holds head_dim f16 at p *
+ * page_stride + h * head_stride + s * row_stride elements of keys and of
+ * values ([pages][heads][page_size][head_dim] and [pages][page_size][heads]
+ * [head_dim] are both such).  The caller owns the memory and hands out pages. */
+typedef struct {
+  void *keys, *values;
+  int64_t pages;
+  int32_t page_size, heads, head_dim;
+  int64_t page_stride, head_stride, row_stride;
+} ipuc_paged_cache;
+
+/* The sequences of a call.  Position p of sequence b is slot p % page_size of
+ * page page_table[b * table_stride + p / page_size].  lengths[b] counts the
+ * positions of sequence b with this call's rows; its rows are its newest
+ * positions.  row_offsets [sequences + 1] (non-decreasing): sequence b has rows
+ * [row_offsets[b], row_offsets[b + 1]); rows from row_offsets[sequences] on
+ * are padding and are left as they are.  NULL: one row per sequence (rows ==
+ * sequences).  Rows at negative positions (length 0: an idle slot) append
+ * nothing and attend to nothing.  All arrays are int32 in device memory. */
+typedef struct {
+  const int32_t *page_table, *lengths, *row_offsets;
+  int64_t table_stride;  /* >= max_pages */
+  int64_t rows;
+  int32_t sequences;
+  int32_t max_pages;     /* entries of a table row; max_pages * page_size < 2^31 */
+} ipuc_paged_batch;
+
+/* Writes the new rows' keys (rotated by their positions unless rotary is
+ * NULL) and values into the cache: k, v [rows][heads][head_dim] at strides
+ * k_stride, v_stride, f16 or f32.  A slot that two rows of the call share
+ * (one page in two places of the table) holds either's elements. */
+ipuc_status ipuc_paged_append_f16(const ipuc_paged_cache *cache, const ipuc_paged_batch *batch, const void *k,
+                                  int64_t k_stride, const void *v, int64_t v_stride, ipuc_precision in_precision,
+                                  const ipuc_rotary *rotary, ipuc_stream stream);
+
+/* Attention of the batch's rows over the cache: the row of sequence b at
+ * position p attends to positions 0..p of its sequence, softmax(q k^T * scale)
+ * v per head; query head h reads key head h / (q_heads / heads).  q [rows]
+ * [q_heads][head_dim] f16 at stride q_stride, out [rows][q_heads][head_dim]
+ * f16, dense.  scale <= 0 selects 1/sqrt(head_dim).  A row that attends to
+ * nothing gives 0.
+ * prefix_rows: positions below it are the same for all sequences and are read
+ * through prefix_pages (device int32, ceil(prefix_rows / page_size) entries)
+ * once for all rows, not through the table, whose entries for them are not
+ * read.  Slots behind a sequence's length may hold anything, NaN included.
+ * A non-finite value at a position that a sequence's later rows attend to may
+ * turn the call's earlier rows of that sequence NaN too (0 * inf).
+ * head_dim a multiple of 8, at most 128; q_heads / heads at most 128; 16-byte
+ * aligned pointers, strides multiples of 8 elements.
+ * workspace: ipuc_paged_attention_workspace_bytes() bytes, 256-byte aligned,
+ * contents need no clearing; two calls that may overlap need one each. */
+uint64_t ipuc_paged_attention_workspace_bytes(int64_t rows, int64_t sequences, int64_t q_heads, int64_t heads,
+                                              int64_t head_dim, int64_t prefix_rows, int32_t ragged);
+ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_t q_stride, int64_t q_heads,
+                                     const ipuc_paged_cache *cache, const ipuc_paged_batch *batch,
+                                     int64_t prefix_rows, const int32_t *prefix_pages, float scale, void *workspace,
+                                     uint64_t workspace_bytes, ipuc_stream stream);
 
 #ifdef __cplusplus
 }

@@ -40,11 +40,19 @@ enum : uint32_t {
   ERR_SITE_PRODUCER = 1,
   ERR_SITE_MMA = 2,
   ERR_SITE_EPILOGUE = 3,
+  // Sites from ERR_SITE_INDEX on are range checks (IPUC_ERR_DEVICE_INDEX).
+  ERR_SITE_INDEX = 16,
+  ERR_SITE_POSITION = 16,
+  ERR_SITE_LENGTH = 17,
+  ERR_SITE_PAGE = 18,
+  ERR_SITE_OFFSET = 19,
   ERR_KERNEL_GEMM_F16 = 1u << 16,
   ERR_KERNEL_GEMM_F32 = 2u << 16,
   ERR_KERNEL_ATTENTION = 3u << 16,
   ERR_KERNEL_SELFTEST = 4u << 16,
   ERR_KERNEL_LAYOUT = 5u << 16,
+  ERR_KERNEL_HEADS = 7u << 16,
+  ERR_KERNEL_PAGED_ATTENTION = 8u << 16,
 };
 
 __device__ __forceinline__ void record_device_error(uint32_t *word, uint32_t code) {

@@ -1,0 +1,452 @@
+// Rotary positions and what is fused with them: the table of cosines and
+// sines, the rotation of a projection's heads, the per-head norm of queries
+// and keys with the rotation in the same pass, and the append of keys and
+// values to a paged cache with the rotation applied on the way.
+//
+// Pair i of a head's first `rotary_dim` elements turns by the angle
+// theta(p, i) = p * f_i at position p: (a, b) -> (a c - b s, b c + a s).  The
+// pairs are (x_i, x_{i+R/2}) (half) or (x_2i, x_2i+1) (interleaved); elements
+// from rotary_dim on pass unturned.  All arithmetic is f32 with one rounding
+// to f16 at the store.
+#include <math.h>
+
+#include "common.cuh"
+#include "paged.cuh"
+
+namespace ipuc {
+namespace {
+
+// ---- the table ----------------------------------------------------------------
+
+constexpr int kMaxPairs = 128;
+
+struct TableParams {
+  float *table;
+  int64_t positions;
+  int32_t pairs;
+  float magnitude;
+  double quarter_turns[kMaxPairs];  // f_i * 2 / pi: quarter turns per position
+};
+
+// Angles of far positions need more than 32 bits (131072 * f leaves 7 bits of
+// a fraction in f32), so position times frequency is formed in f64 in units of
+// a quarter turn; what is left after the nearest whole quarter is at most half
+// a quarter, which f32 holds to 2^-26 of a turn, and the whole quarters swap
+// and negate the f32 sine and cosine.
+__global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant__ TableParams p) {
+  const int64_t n = p.positions * p.pairs;
+  const int64_t stride = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += stride) {
+    const int64_t pos = e / p.pairs;
+    const int i = (int)(e - pos * p.pairs);
+    const double t = (double)pos * p.quarter_turns[i];
+    const double whole = rint(t);
+    float s, c;
+    sincospif(0.5f * (float)(t - whole), &s, &c);
+    const int q = (int)((long long)whole & 3);
+    const float cs = q == 0 ? c : q == 1 ? -s : q == 2 ? -c : s;
+    const float sn = q == 0 ? s : q == 1 ? c : q == 2 ? -s : -c;
+    p.table[pos * 2 * p.pairs + i] = cs * p.magnitude;
+    p.table[pos * 2 * p.pairs + p.pairs + i] = sn * p.magnitude;
+  }
+}
+
+// ---- heads: rotate, norm, append -------------------------------------------------
+
+// One of the (at most two) tensors of a call: [tokens][heads][head_dim].
+struct Segment {
+  const void *in;
+  uint16_t *out;          // dense output, or a paged cache's base
+  const uint16_t *weight; // norm: [head_dim] or null (ones)
+  int64_t in_stride, out_stride;  // elements from token to token (paged: unused)
+  int32_t heads;
+  int32_t rotate;
+};
+
+struct HeadsParams {
+  Segment seg[2];
+  const float *table;       // [table_rows][rotary_dim]: cosines, then sines; null: no rotation
+  const int32_t *positions; // null: the token's index (paged: its position in the cache)
+  PagedView paged;
+  int64_t table_rows;
+  int64_t tokens;
+  int32_t head_dim, rotary_dim;
+  int32_t interleaved;
+  int32_t lane_shift;  // log2 of the lanes that share a head
+  int32_t slots;       // head slots per token: a thread takes heads slot, slot + slots, ...
+  float eps;
+  uint32_t *err;
+};
+
+template <typename T, int V>
+struct alignas(V * sizeof(T) < 16 ? V * sizeof(T) : 16) Vec {
+  T v[V];
+};
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(uint16_t x) { return h2f(x); }
+
+// An item is two vectors of V elements that one lane holds: the two sides of V
+// pairs, or 2V neighbouring elements.  A head's head_dim / 2V items are spread
+// over 2^lane_shift neighbouring lanes, so the norm's sum is a shuffle tree.
+template <int V, typename TIN, bool kNorm, bool kPaged>
+__global__ void __launch_bounds__(256) heads_kernel(const __grid_constant__ HeadsParams p) {
+  constexpr int IPL = V >= 4 ? 1 : V == 2 ? 2 : 4;  // items per lane (head_dim <= 256)
+  constexpr int U = IPL > 1 ? 1 : sizeof(TIN) == 2 ? 4 : 2;  // heads per thread
+  const uint32_t lanes = 1u << p.lane_shift;
+  const uint32_t lane = threadIdx.x & (lanes - 1);
+  const uint32_t group = (blockIdx.x * (256u >> p.lane_shift)) + (threadIdx.x >> p.lane_shift);
+  const uint32_t token = group / (uint32_t)p.slots;
+  const int slot = (int)(group - token * (uint32_t)p.slots);
+  bool live = token < p.tokens;
+  int64_t pos = 0;
+  int64_t page_at = 0;
+  if (live) {
+    if constexpr (kPaged) {
+      PagedRow r;
+      live = paged_row(p.paged, token, r);
+      if (live) {
+        pos = r.position;
+        const int64_t cap = (int64_t)p.paged.max_pages * p.paged.page_size;
+        if (pos < 0) {
+          live = false;
+        } else if (pos >= cap) {
+          live = false;
+          record_device_error(p.err, ERR_KERNEL_HEADS | ERR_SITE_LENGTH);
+        } else {
+          const int32_t page = (int32_t)pos / p.paged.page_size;
+          const int32_t id = p.paged.page_table[r.sequence * p.paged.table_stride + page];
+          if (id < 0 || id >= p.paged.pages) {
+            live = false;
+            record_device_error(p.err, ERR_KERNEL_HEADS | ERR_SITE_PAGE);
+          }
+          page_at = id * p.paged.page_stride + (pos - (int64_t)page * p.paged.page_size) * p.paged.row_stride;
+        }
+      }
+    } else if (p.table) {
+      pos = p.positions ? p.positions[token] : (int64_t)token;
+      if (pos < 0) live = false;
+    }
+    if (live && p.table && pos >= p.table_rows) {
+      live = false;
+      record_device_error(p.err, ERR_KERNEL_HEADS | ERR_SITE_POSITION);
+    }
+  }
+  const int items = p.head_dim / (2 * V), turned = p.rotary_dim / (2 * V);
+  const int total = p.seg[0].heads + p.seg[1].heads;
+  // Every load of the thread is issued before the first is used.
+  Vec<TIN, V> x[U][IPL][2];
+  Vec<float, V> cs[IPL], sn[IPL];
+  int e0[IPL], e1[IPL];
+#pragma unroll
+  for (int k = 0; k < IPL; ++k) {
+    const int item = (int)(lane + k * lanes);
+    const bool turn = p.table && item < turned;
+    const bool split = turn && !p.interleaved;
+    e0[k] = split ? item * V : 2 * V * item;
+    e1[k] = split ? p.rotary_dim / 2 + item * V : e0[k] + V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      cs[k].v[j] = 1.0f;
+      sn[k].v[j] = 0.0f;
+    }
+    if (live && turn) {
+      const float *row = p.table + pos * p.rotary_dim + item * V;
+      cs[k] = *reinterpret_cast<const Vec<float, V> *>(row);
+      sn[k] = *reinterpret_cast<const Vec<float, V> *>(row + p.rotary_dim / 2);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = slot + u * p.slots;
+      if (live && item < items && h < total) {
+        const Segment &g = p.seg[h < p.seg[0].heads ? 0 : 1];
+        const int hh = h < p.seg[0].heads ? h : h - p.seg[0].heads;
+        const TIN *in = static_cast<const TIN *>(g.in) + token * g.in_stride + hh * p.head_dim;
+        x[u][k][0] = *reinterpret_cast<const Vec<TIN, V> *>(in + e0[k]);
+        x[u][k][1] = *reinterpret_cast<const Vec<TIN, V> *>(in + e1[k]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[u][k][0].v[j] = x[u][k][1].v[j] = TIN(0);
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int h = slot + u * p.slots;
+    const Segment &g = p.seg[h < p.seg[0].heads ? 0 : 1];
+    const int hh = h < p.seg[0].heads ? h : h - p.seg[0].heads;
+    float rstd = 1.0f;
+    if constexpr (kNorm) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int k = 0; k < IPL; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float a = to_f32(x[u][k][0].v[j]), b = to_f32(x[u][k][1].v[j]);
+          sum = fmaf(a, a, fmaf(b, b, sum));
+        }
+      for (uint32_t m = lanes >> 1; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+      rstd = rsqrtf(sum / (float)p.head_dim + p.eps);
+    }
+    if (!live || h >= total) continue;
+#pragma unroll
+    for (int k = 0; k < IPL; ++k) {
+      if ((int)(lane + k * lanes) >= items) continue;
+      float y[2 * V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        y[j] = to_f32(x[u][k][0].v[j]);
+        y[V + j] = to_f32(x[u][k][1].v[j]);
+      }
+      if constexpr (kNorm) {
+        if (g.weight) {
+          const Vec<uint16_t, V> w0 = *reinterpret_cast<const Vec<uint16_t, V> *>(g.weight + e0[k]);
+          const Vec<uint16_t, V> w1 = *reinterpret_cast<const Vec<uint16_t, V> *>(g.weight + e1[k]);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            y[j] *= rstd * h2f(w0.v[j]);
+            y[V + j] *= rstd * h2f(w1.v[j]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 2 * V; ++j) y[j] *= rstd;
+        }
+      }
+      if (p.table && g.rotate && (int)(lane + k * lanes) < turned) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const int ia = p.interleaved ? 2 * j : j, ib = p.interleaved ? 2 * j + 1 : V + j;
+          const float a = y[ia], b = y[ib];
+          y[ia] = a * cs[k].v[j] - b * sn[k].v[j];
+          y[ib] = b * cs[k].v[j] + a * sn[k].v[j];
+        }
+      }
+      uint16_t *out = g.out + (kPaged ? page_at + hh * p.paged.head_stride : token * g.out_stride + hh * p.head_dim);
+      Vec<uint16_t, V> o0, o1;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        o0.v[j] = f2h(y[j]);
+        o1.v[j] = f2h(y[V + j]);
+      }
+      *reinterpret_cast<Vec<uint16_t, V> *>(out + e0[k]) = o0;
+      *reinterpret_cast<Vec<uint16_t, V> *>(out + e1[k]) = o1;
+    }
+  }
+}
+
+// Largest vector width that every address of the call allows: 2V divides the
+// turned part and the head, and pointers and strides are multiples of V.
+int vector_width(const HeadsParams &p, size_t in_bytes, bool paged) {
+  for (int v = 8; v > 1; v /= 2) {
+    bool ok = p.head_dim % (2 * v) == 0 && p.rotary_dim % (2 * v) == 0;
+    for (const Segment &g : p.seg) {
+      if (!g.heads) continue;
+      const uintptr_t in_align = v * in_bytes < 16 ? v * in_bytes : 16;
+      ok = ok && aligned(g.in, in_align) && aligned(g.out, v * 2) && g.in_stride % v == 0;
+      if (g.weight) ok = ok && aligned(g.weight, v * 2);
+      if (!paged) ok = ok && g.out_stride % v == 0;
+    }
+    if (paged)
+      ok = ok && p.paged.page_stride % v == 0 && p.paged.head_stride % v == 0 && p.paged.row_stride % v == 0;
+    if (p.table) ok = ok && aligned(p.table, 16);
+    if (ok) return v;
+  }
+  return 1;
+}
+
+template <typename TIN, bool kNorm, bool kPaged>
+ipuc_status launch_heads(HeadsParams &p, cudaStream_t stream) {
+  const int v = vector_width(p, sizeof(TIN), kPaged);
+  const int items = p.head_dim / (2 * v);
+  p.lane_shift = 0;
+  while ((1 << p.lane_shift) < items && p.lane_shift < 5) ++p.lane_shift;
+  const int per_thread = v < 4 ? 1 : sizeof(TIN) == 2 ? 4 : 2;
+  const int total = p.seg[0].heads + p.seg[1].heads;
+  p.slots = (total + per_thread - 1) / per_thread;
+  const int64_t groups = p.tokens * p.slots, per_block = 256 >> p.lane_shift;
+  IPUC_CHECK_ARG(groups < (1ll << 31), "heads: extent too large");
+  const unsigned grid = (unsigned)((groups + per_block - 1) / per_block);
+  switch (v) {
+    case 8: heads_kernel<8, TIN, kNorm, kPaged><<<grid, 256, 0, stream>>>(p); break;
+    case 4: heads_kernel<4, TIN, kNorm, kPaged><<<grid, 256, 0, stream>>>(p); break;
+    case 2: heads_kernel<2, TIN, kNorm, kPaged><<<grid, 256, 0, stream>>>(p); break;
+    default: heads_kernel<1, TIN, kNorm, kPaged><<<grid, 256, 0, stream>>>(p); break;
+  }
+  return check_launch("heads_kernel");
+}
+
+ipuc_status check_rotary(const char *who, const ipuc_rotary *r, int64_t head_dim, HeadsParams &p) {
+  p.table = nullptr;
+  p.table_rows = 0;
+  p.rotary_dim = 0;
+  p.interleaved = 0;
+  if (!r || r->rotary_dim == 0) return IPUC_OK;
+  const std::string w = who;
+  IPUC_CHECK_ARG(r->rotary_dim > 0 && r->rotary_dim % 2 == 0 && r->rotary_dim <= head_dim,
+                 w + ": rotary_dim must be even and within the head");
+  IPUC_CHECK_ARG(r->layout == IPUC_ROTARY_HALF || r->layout == IPUC_ROTARY_INTERLEAVED, w + ": bad rotary layout");
+  IPUC_CHECK_ARG(r->table != nullptr && r->positions > 0, w + ": rotary table missing");
+  IPUC_CHECK_ALIGN(aligned(r->table, 4), w + ": rotary table must be 4-byte aligned");
+  p.table = r->table;
+  p.table_rows = r->positions;
+  p.rotary_dim = r->rotary_dim;
+  p.interleaved = r->layout == IPUC_ROTARY_INTERLEAVED;
+  return IPUC_OK;
+}
+
+// One dense tensor [tokens][heads][head_dim] of a call; rows may lie further
+// apart than heads * head_dim (a projection's slice).
+ipuc_status check_segment(const char *who, Segment &g, void *out, int64_t out_stride, const void *in,
+                          int64_t in_stride, ipuc_precision precision, int64_t heads, int64_t head_dim, bool dense) {
+  const std::string w = who;
+  IPUC_CHECK_ARG(out && in, w + ": null pointer");
+  IPUC_CHECK_ALIGN(aligned(in, precision == IPUC_F32 ? 4 : 2) && aligned(out, 2),
+                   w + ": pointers must be element-aligned");
+  IPUC_CHECK_ARG(in_stride >= heads * head_dim && (!dense || out_stride >= heads * head_dim),
+                 w + ": token stride shorter than heads * head_dim");
+  IPUC_CHECK_ARG(in != out || (precision == IPUC_F16 && in_stride == out_stride),
+                 w + ": in place needs f16 input and equal strides");
+  g.in = in;
+  g.out = static_cast<uint16_t *>(out);
+  g.in_stride = in_stride;
+  g.out_stride = out_stride;
+  g.heads = (int32_t)heads;
+  g.rotate = 1;
+  g.weight = nullptr;
+  return IPUC_OK;
+}
+
+ipuc_status check_heads(const char *who, int64_t tokens, int64_t heads, int64_t head_dim, ipuc_precision precision) {
+  const std::string w = who;
+  IPUC_CHECK_ARG(precision == IPUC_F16 || precision == IPUC_F32, w + ": bad input precision");
+  IPUC_CHECK_ARG(tokens >= 0 && heads >= 0 && tokens < (1ll << 31) && heads < (1ll << 16),
+                 w + ": extent out of range");
+  IPUC_CHECK_ARG(head_dim > 0 && head_dim % 2 == 0, w + ": head_dim must be even and positive");
+  if (head_dim > 256) return fail(IPUC_ERR_UNSUPPORTED, w + ": head_dim above 256 is not supported");
+  return IPUC_OK;
+}
+
+}  // namespace
+}  // namespace ipuc
+
+using namespace ipuc;
+
+extern "C" ipuc_status ipuc_rotary_table(float *table, int64_t positions, int64_t rotary_dim,
+                                         const ipuc_rotary_scaling *scaling, ipuc_stream stream) {
+  IPUC_CHECK_ARG(scaling != nullptr, "rotary_table: null scaling");
+  IPUC_CHECK_ARG(positions >= 0 && positions < (1ll << 31), "rotary_table: positions out of range");
+  IPUC_CHECK_ARG(rotary_dim > 0 && rotary_dim % 2 == 0, "rotary_table: rotary_dim must be even and positive");
+  if (rotary_dim > 2 * kMaxPairs) return fail(IPUC_ERR_UNSUPPORTED, "rotary_table: rotary_dim above 256 is not supported");
+  const ipuc_rotary_scaling &c = *scaling;
+  IPUC_CHECK_ARG(c.kind >= IPUC_ROTARY_SCALE_NONE && c.kind <= IPUC_ROTARY_SCALE_BANDS, "rotary_table: bad scaling kind");
+  IPUC_CHECK_ARG(isfinite(c.base) && c.base > 1.0, "rotary_table: base must be above 1");
+  IPUC_CHECK_ARG(isfinite(c.magnitude) && c.magnitude > 0.0, "rotary_table: magnitude must be positive");
+  if (c.kind != IPUC_ROTARY_SCALE_NONE)
+    IPUC_CHECK_ARG(isfinite(c.factor) && c.factor >= 1.0, "rotary_table: factor must be at least 1");
+  if (c.kind == IPUC_ROTARY_SCALE_BASE)
+    IPUC_CHECK_ARG(rotary_dim > 2, "rotary_table: base scaling needs rotary_dim above 2");
+  if (c.kind == IPUC_ROTARY_SCALE_BANDS)
+    IPUC_CHECK_ARG(isfinite(c.low) && isfinite(c.high) && c.low < c.high && isfinite(c.original) && c.original > 0.0,
+                   "rotary_table: bands need low < high and a positive original length");
+  if (positions == 0) return IPUC_OK;
+  IPUC_CHECK_ARG(table != nullptr, "rotary_table: null pointer");
+  IPUC_CHECK_ALIGN(aligned(table, 4), "rotary_table: table must be 4-byte aligned");
+  TableParams p;
+  p.table = table;
+  p.positions = positions;
+  p.pairs = (int32_t)(rotary_dim / 2);
+  p.magnitude = (float)c.magnitude;
+  const double pi = 3.14159265358979323846, r = (double)rotary_dim;
+  const double base = c.kind == IPUC_ROTARY_SCALE_BASE ? c.base * pow(c.factor, r / (r - 2.0)) : c.base;
+  for (int i = 0; i < p.pairs; ++i) {
+    double f = pow(base, -2.0 * i / r);
+    if (c.kind == IPUC_ROTARY_SCALE_LINEAR) f /= c.factor;
+    if (c.kind == IPUC_ROTARY_SCALE_BANDS) {
+      const double turns = c.original * f / (2.0 * pi);
+      const double keep = fmin(1.0, fmax(0.0, (turns - c.low) / (c.high - c.low)));
+      f *= keep + (1.0 - keep) / c.factor;
+    }
+    p.quarter_turns[i] = f * (2.0 / pi);
+  }
+  const int64_t want = (positions * p.pairs + 255) / 256, cap = (int64_t)sm_count() * 8;
+  rotary_table_kernel<<<(unsigned)(want < cap ? want : cap), 256, 0, stream>>>(p);
+  return check_launch("rotary_table_kernel");
+}
+
+extern "C" ipuc_status ipuc_rotary_f16(void *out, int64_t out_stride, const void *in, int64_t in_stride,
+                                       ipuc_precision in_precision, int64_t tokens, int64_t heads, int64_t head_dim,
+                                       const ipuc_rotary *rotary, const int32_t *positions, ipuc_stream stream) {
+  ipuc_status st = check_heads("rotary", tokens, heads, head_dim, in_precision);
+  if (st != IPUC_OK) return st;
+  HeadsParams p = {};
+  if ((st = check_rotary("rotary", rotary, head_dim, p)) != IPUC_OK) return st;
+  IPUC_CHECK_ARG(p.table != nullptr, "rotary: rotary table missing");
+  if (tokens == 0 || heads == 0) return IPUC_OK;
+  st = check_segment("rotary", p.seg[0], out, out_stride, in, in_stride, in_precision, heads, head_dim, true);
+  if (st != IPUC_OK) return st;
+  p.positions = positions;
+  p.tokens = tokens;
+  p.head_dim = (int32_t)head_dim;
+  p.err = device_error_word();
+  return in_precision == IPUC_F16 ? launch_heads<uint16_t, false, false>(p, stream)
+                                  : launch_heads<float, false, false>(p, stream);
+}
+
+extern "C" ipuc_status ipuc_qk_norm_rotary_f16(void *q_out, int64_t q_out_stride, void *k_out, int64_t k_out_stride,
+                                               const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                                               ipuc_precision in_precision, const void *q_weight,
+                                               const void *k_weight, float eps, int64_t tokens, int64_t q_heads,
+                                               int64_t k_heads, int64_t head_dim, const ipuc_rotary *rotary,
+                                               const int32_t *positions, ipuc_stream stream) {
+  ipuc_status st = check_heads("qk_norm_rotary", tokens, q_heads, head_dim, in_precision);
+  if (st == IPUC_OK) st = check_heads("qk_norm_rotary", tokens, k_heads, head_dim, in_precision);
+  if (st != IPUC_OK) return st;
+  IPUC_CHECK_ARG(isfinite(eps) && eps >= 0.0f, "qk_norm_rotary: eps must be finite and not negative");
+  HeadsParams p = {};
+  if ((st = check_rotary("qk_norm_rotary", rotary, head_dim, p)) != IPUC_OK) return st;
+  if (tokens == 0 || q_heads + k_heads == 0) return IPUC_OK;
+  if (q_heads) {
+    st = check_segment("qk_norm_rotary", p.seg[0], q_out, q_out_stride, q, q_stride, in_precision, q_heads, head_dim, true);
+    if (st != IPUC_OK) return st;
+  }
+  if (k_heads) {
+    st = check_segment("qk_norm_rotary", p.seg[1], k_out, k_out_stride, k, k_stride, in_precision, k_heads, head_dim, true);
+    if (st != IPUC_OK) return st;
+  }
+  IPUC_CHECK_ALIGN(aligned(q_weight, 2) && aligned(k_weight, 2), "qk_norm_rotary: pointers must be element-aligned");
+  p.seg[0].weight = static_cast<const uint16_t *>(q_weight);
+  p.seg[1].weight = static_cast<const uint16_t *>(k_weight);
+  p.positions = positions;
+  p.tokens = tokens;
+  p.head_dim = (int32_t)head_dim;
+  p.eps = eps;
+  p.err = device_error_word();
+  return in_precision == IPUC_F16 ? launch_heads<uint16_t, true, false>(p, stream)
+                                  : launch_heads<float, true, false>(p, stream);
+}
+
+extern "C" ipuc_status ipuc_paged_append_f16(const ipuc_paged_cache *cache, const ipuc_paged_batch *batch,
+                                             const void *k, int64_t k_stride, const void *v, int64_t v_stride,
+                                             ipuc_precision in_precision, const ipuc_rotary *rotary,
+                                             ipuc_stream stream) {
+  ipuc_status st = check_paged("paged_append", cache, batch);
+  if (st != IPUC_OK) return st;
+  st = check_heads("paged_append", batch->rows, cache->heads, cache->head_dim, in_precision);
+  if (st != IPUC_OK) return st;
+  HeadsParams p = {};
+  if ((st = check_rotary("paged_append", rotary, cache->head_dim, p)) != IPUC_OK) return st;
+  if (batch->rows == 0 || batch->sequences == 0) return IPUC_OK;
+  st = check_segment("paged_append", p.seg[0], cache->keys, 0, k, k_stride, in_precision, cache->heads,
+                     cache->head_dim, false);
+  if (st == IPUC_OK)
+    st = check_segment("paged_append", p.seg[1], cache->values, 0, v, v_stride, in_precision, cache->heads,
+                       cache->head_dim, false);
+  if (st != IPUC_OK) return st;
+  p.seg[1].rotate = 0;
+  p.paged = paged_view(cache, batch);
+  p.tokens = batch->rows;
+  p.head_dim = cache->head_dim;
+  p.err = device_error_word();
+  return in_precision == IPUC_F16 ? launch_heads<uint16_t, false, true>(p, stream)
+                                  : launch_heads<float, false, true>(p, stream);
+}

@@ -67,6 +67,7 @@ extern "C" const char *ipuc_status_string(ipuc_status status) {
     case IPUC_ERR_CUDA: return "IPUC_ERR_CUDA";
     case IPUC_ERR_NCCL: return "IPUC_ERR_NCCL";
     case IPUC_ERR_DEVICE_TIMEOUT: return "IPUC_ERR_DEVICE_TIMEOUT";
+    case IPUC_ERR_DEVICE_INDEX: return "IPUC_ERR_DEVICE_INDEX";
   }
   return "IPUC_ERR_UNKNOWN";
 }
@@ -83,6 +84,13 @@ extern "C" ipuc_status ipuc_device_status(ipuc_stream stream) {
     const uint32_t zero = 0;
     IPUC_CUDA(cudaMemcpy(word, &zero, sizeof(zero), cudaMemcpyHostToDevice));
     char buf[128];
+    const uint32_t site = value & 0xffffu;
+    if (site >= ERR_SITE_INDEX) {
+      static const char *const what[] = {"position", "length", "page id", "row offset"};
+      snprintf(buf, sizeof(buf), "index in device memory out of range: kernel %u, %s", value >> 16,
+               site - ERR_SITE_INDEX < 4 ? what[site - ERR_SITE_INDEX] : "index");
+      return fail(IPUC_ERR_DEVICE_INDEX, buf);
+    }
     snprintf(buf, sizeof(buf), "device wait timed out: kernel %u site %u", value >> 16, value & 0xffffu);
     return fail(IPUC_ERR_DEVICE_TIMEOUT, buf);
   }

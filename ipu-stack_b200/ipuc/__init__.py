@@ -19,7 +19,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libipuc.so")
 
 # ipuc_status
-OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_ALIGNMENT, ERR_CUDA, ERR_NCCL, ERR_DEVICE_TIMEOUT = range(7)
+(OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_ALIGNMENT, ERR_CUDA, ERR_NCCL, ERR_DEVICE_TIMEOUT,
+ ERR_DEVICE_INDEX) = range(8)
 # ipuc_precision
 F16, F32 = 0, 1
 # ipuc_order
@@ -68,6 +69,13 @@ SIGNATURES = {
     "ipuc_ipc_open": (_i32, [_vp, _u64, ctypes.POINTER(_vp)]),
     "ipuc_ipc_close": (_i32, [_vp]),
     "ipuc_peer_all_reduce_f16": (_i32, [_vp, _vp, _vp, _i32, _i32, _u64, _vp]),
+    "ipuc_rotary_table": (_i32, [_vp, _i64, _i64, _vp, _vp]),
+    "ipuc_rotary_f16": (_i32, [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "ipuc_qk_norm_rotary_f16": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _vp, _f32, _i64, _i64,
+                                       _i64, _i64, _vp, _vp, _vp]),
+    "ipuc_paged_append_f16": (_i32, [_vp, _vp, _vp, _i64, _vp, _i64, _i32, _vp, _vp]),
+    "ipuc_paged_attention_workspace_bytes": (_u64, [_i64, _i64, _i64, _i64, _i64, _i64, _i32]),
+    "ipuc_paged_attention_f16": (_i32, [_vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp, _f32, _vp, _u64, _vp]),
 }
 
 
@@ -80,7 +88,7 @@ class IpucError(RuntimeError):
 
 STATUS_NAMES = {OK: "IPUC_OK", ERR_INVALID_ARGUMENT: "IPUC_ERR_INVALID_ARGUMENT", ERR_UNSUPPORTED: "IPUC_ERR_UNSUPPORTED",
                 ERR_ALIGNMENT: "IPUC_ERR_ALIGNMENT", ERR_CUDA: "IPUC_ERR_CUDA", ERR_NCCL: "IPUC_ERR_NCCL",
-                ERR_DEVICE_TIMEOUT: "IPUC_ERR_DEVICE_TIMEOUT"}
+                ERR_DEVICE_TIMEOUT: "IPUC_ERR_DEVICE_TIMEOUT", ERR_DEVICE_INDEX: "IPUC_ERR_DEVICE_INDEX"}
 
 _lib = None
 
@@ -431,6 +439,219 @@ def launch(spec, out, inputs=(), scalars=(), workspace=None, stream=None):
     ws = workspace.numel() * workspace.element_size() if workspace is not None else 0
     call("ipuc_launch", ctypes.byref(spec), ctypes.byref(o), arr, len(ins), sc, len(scalars), _ptr(workspace), ws,
          _stream(stream))
+
+
+# ---- serving with positions and a paged key/value cache --------------------
+# These wrappers take torch tensors, read sizes and strides from them and
+# refuse tensors that the kernels could not address (other types, shapes or
+# devices) with the library's own status codes.
+
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1
+ROTARY_SCALE_NONE, ROTARY_SCALE_LINEAR, ROTARY_SCALE_BASE, ROTARY_SCALE_BANDS = range(4)
+
+
+class _RotaryScaling(ctypes.Structure):
+    _fields_ = [("kind", _i32), ("base", ctypes.c_double), ("factor", ctypes.c_double), ("low", ctypes.c_double),
+                ("high", ctypes.c_double), ("original", ctypes.c_double), ("magnitude", ctypes.c_double)]
+
+
+class _Rotary(ctypes.Structure):
+    _fields_ = [("table", _vp), ("positions", _i64), ("rotary_dim", _i32), ("layout", _i32)]
+
+
+class _PagedCache(ctypes.Structure):
+    _fields_ = [("keys", _vp), ("values", _vp), ("pages", _i64), ("page_size", _i32), ("heads", _i32),
+                ("head_dim", _i32), ("page_stride", _i64), ("head_stride", _i64), ("row_stride", _i64)]
+
+
+class _PagedBatch(ctypes.Structure):
+    _fields_ = [("page_table", _vp), ("lengths", _vp), ("row_offsets", _vp), ("table_stride", _i64), ("rows", _i64),
+                ("sequences", _i32), ("max_pages", _i32)]
+
+
+def _refuse(fn, text):
+    raise IpucError(fn, ERR_INVALID_ARGUMENT, f"{fn[5:]}: {text}")
+
+
+def _want(fn, name, t, dtype, ndim, dense=None):
+    """`t` is a CUDA tensor of the current device with this type and rank, its last `dense` dimensions dense."""
+    import torch
+    if not isinstance(t, torch.Tensor) or t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
+        _refuse(fn, f"{name} has the wrong type")
+    if t.dim() != ndim:
+        _refuse(fn, f"{name} must have {ndim} dimensions")
+    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+        _refuse(fn, f"{name} is not on the current device")
+    expect = 1
+    for i in range(1, (ndim if dense is None else dense) + 1):
+        if t.size(-i) != 1 and t.stride(-i) != expect:
+            _refuse(fn, f"{name} must be dense in its last {ndim if dense is None else dense} dimensions")
+        expect *= t.size(-i)
+
+
+def _token_rows(fn, name, t, dtype):
+    """[tokens, heads, head_dim] with dense heads: (token stride, precision)."""
+    import torch
+    _want(fn, name, t, dtype, 3, 2)
+    return t.stride(0) if t.size(0) > 1 else t.size(1) * t.size(2), F16 if t.dtype == torch.float16 else F32
+
+
+def rotary_table(out, base=10000.0, scaling=ROTARY_SCALE_NONE, factor=1.0, low=1.0, high=32.0, original=1.0,
+                 magnitude=1.0, stream=None):
+    """Fills out (f32 [positions, rotary_dim]) with the cosines and sines of every position; see ipuc_rotary_scaling."""
+    import torch
+    _want("ipuc_rotary_table", "table", out, torch.float32, 2)
+    s = _RotaryScaling(scaling, base, factor, low, high, original, magnitude)
+    call("ipuc_rotary_table", out.data_ptr(), out.size(0), out.size(1), ctypes.byref(s), _stream(stream))
+
+
+class Rotary:
+    """A rotary table (rotary_table's output) with the layout of the pairs; keeps the table alive."""
+
+    def __init__(self, table, layout=ROTARY_HALF):
+        import torch
+        _want("ipuc_rotary_f16", "table", table, torch.float32, 2)
+        self.table = table
+        self.spec = _Rotary(table.data_ptr(), table.size(0), table.size(1), layout)
+
+
+def _rotary_spec(rotary):
+    return None if rotary is None else ctypes.byref(rotary.spec)
+
+
+def _positions(fn, positions, tokens):
+    import torch
+    if positions is None:
+        return None
+    _want(fn, "positions", positions, torch.int32, 1)
+    if positions.size(0) != tokens:
+        _refuse(fn, "positions must have one entry per token")
+    return positions.data_ptr()
+
+
+def rotary_f16(out, x, rotary, positions=None, stream=None):
+    """out = x with the heads rotated: x [tokens, heads, head_dim] f16 or f32, out f16 of that shape."""
+    import torch
+    fn = "ipuc_rotary_f16"
+    xs, precision = _token_rows(fn, "x", x, (torch.float16, torch.float32))
+    os_, _ = _token_rows(fn, "out", out, torch.float16)
+    if out.shape != x.shape:
+        _refuse(fn, "out and x must have the same shape")
+    call(fn, out.data_ptr(), os_, x.data_ptr(), xs, precision, x.size(0), x.size(1), x.size(2), _rotary_spec(rotary),
+         _positions(fn, positions, x.size(0)), _stream(stream))
+
+
+def qk_norm_rotary_f16(q_out, k_out, q, k, q_weight=None, k_weight=None, eps=1e-6, rotary=None, positions=None,
+                       stream=None):
+    """Per-head norm of q and k, then their rotation: q [tokens, q_heads, head_dim], k [tokens, k_heads, head_dim]."""
+    import torch
+    fn = "ipuc_qk_norm_rotary_f16"
+    qs, precision = _token_rows(fn, "q", q, (torch.float16, torch.float32))
+    ks, k_precision = _token_rows(fn, "k", k, (torch.float16, torch.float32))
+    qos, _ = _token_rows(fn, "q_out", q_out, torch.float16)
+    kos, _ = _token_rows(fn, "k_out", k_out, torch.float16)
+    if precision != k_precision or q.size(0) != k.size(0) or q.size(2) != k.size(2):
+        _refuse(fn, "q and k must have the same type, tokens and head_dim")
+    if q_out.shape != q.shape or k_out.shape != k.shape:
+        _refuse(fn, "outputs must have their inputs' shapes")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None:
+            _want(fn, name, w, torch.float16, 1)
+            if w.size(0) != q.size(2):
+                _refuse(fn, f"{name} must have head_dim entries")
+    call(fn, q_out.data_ptr(), qos, k_out.data_ptr(), kos, q.data_ptr(), qs, k.data_ptr(), ks, precision,
+         _ptr(q_weight), _ptr(k_weight), eps, q.size(0), q.size(1), k.size(1), q.size(2), _rotary_spec(rotary),
+         _positions(fn, positions, q.size(0)), _stream(stream))
+
+
+class PagedCache:
+    """Keys and values [pages, heads, page_size, head_dim] f16 of equal strides (any order of the first three
+    dimensions in memory: pass a transposed view of [pages, page_size, heads, head_dim]); keeps them alive."""
+
+    def __init__(self, keys, values):
+        import torch
+        fn = "ipuc_paged_cache"
+        _want(fn, "keys", keys, torch.float16, 4, 1)
+        _want(fn, "values", values, torch.float16, 4, 1)
+        if keys.shape != values.shape or keys.stride() != values.stride():
+            _refuse(fn, "keys and values must have the same shape and strides")
+        self.keys, self.values = keys, values
+        pages, heads, page_size, d = keys.shape
+        # a dimension of one element has no meaningful stride
+        strides = [keys.stride(i) if keys.size(i) > 1 else max(keys.stride(i), d) for i in range(3)]
+        self.spec = _PagedCache(keys.data_ptr(), values.data_ptr(), pages, page_size, heads, d, *strides)
+
+
+class PagedBatch:
+    """The sequences of a call: page_table [sequences, max_pages], lengths [sequences] and, unless every sequence
+    has one row, row_offsets [sequences + 1], int32.  rows: the rows of the tensors that go with row_offsets (its
+    last entry, or more: the rest is padding); read from the tensors of each call where it is not given."""
+
+    def __init__(self, page_table, lengths, row_offsets=None, rows=None):
+        import torch
+        fn = "ipuc_paged_batch"
+        _want(fn, "page_table", page_table, torch.int32, 2, 1)
+        _want(fn, "lengths", lengths, torch.int32, 1)
+        n = lengths.size(0)
+        if page_table.size(0) != n:
+            _refuse(fn, "page_table must have one row per sequence")
+        if row_offsets is not None:
+            _want(fn, "row_offsets", row_offsets, torch.int32, 1)
+            if row_offsets.size(0) != n + 1:
+                _refuse(fn, "row_offsets must have one entry more than sequences")
+        self._keep = (page_table, lengths, row_offsets)
+        width = page_table.size(1)
+        self._rows = rows
+        self.spec = _PagedBatch(page_table.data_ptr(), lengths.data_ptr(), _ptr(row_offsets),
+                                page_table.stride(0) if n > 1 else width, 0 if rows is None else rows, n, width)
+
+    def _with_rows(self, fn, rows):
+        if self._rows is not None and self._rows != rows:
+            _refuse(fn, "tensors must have the batch's rows")
+        self.spec.rows = rows
+        return ctypes.byref(self.spec)
+
+
+def paged_append_f16(cache, batch, k, v, rotary=None, stream=None):
+    """Writes the new rows k, v [rows, heads, head_dim] (f16 or f32) into the cache, keys rotated by their positions."""
+    import torch
+    fn = "ipuc_paged_append_f16"
+    ks, precision = _token_rows(fn, "k", k, (torch.float16, torch.float32))
+    vs, v_precision = _token_rows(fn, "v", v, (torch.float16, torch.float32))
+    if precision != v_precision or k.shape != v.shape:
+        _refuse(fn, "k and v must have the same type and shape")
+    if k.size(1) != cache.spec.heads or k.size(2) != cache.spec.head_dim:
+        _refuse(fn, "rows must have the cache's heads and head_dim")
+    call(fn, ctypes.byref(cache.spec), batch._with_rows(fn, k.size(0)), k.data_ptr(), ks, v.data_ptr(), vs, precision,
+         _rotary_spec(rotary), _stream(stream))
+
+
+def paged_attention_workspace_bytes(rows, sequences, q_heads, heads, head_dim, prefix_rows=0, ragged=False) -> int:
+    """Bytes for paged_attention_f16; ragged: the batch has row_offsets."""
+    return int(lib().ipuc_paged_attention_workspace_bytes(rows, sequences, q_heads, heads, head_dim, prefix_rows,
+                                                          int(ragged)))
+
+
+def paged_attention_f16(out, q, cache, batch, workspace, prefix_rows=0, prefix_pages=None, scale=0.0, stream=None):
+    """Attention of q [rows, q_heads, head_dim] over the cache into out (dense); positions below prefix_rows are read
+    once for all rows through prefix_pages."""
+    import torch
+    fn = "ipuc_paged_attention_f16"
+    qs, _ = _token_rows(fn, "q", q, torch.float16)
+    _want(fn, "out", out, torch.float16, 3)
+    if out.shape != q.shape:
+        _refuse(fn, "out and q must have the same shape")
+    if q.size(2) != cache.spec.head_dim:
+        _refuse(fn, "rows must have the cache's head_dim")
+    if prefix_rows:
+        if prefix_pages is None:
+            _refuse(fn, "prefix_rows without prefix_pages")
+        _want(fn, "prefix_pages", prefix_pages, torch.int32, 1)
+        if prefix_pages.size(0) * cache.spec.page_size < prefix_rows:
+            _refuse(fn, "prefix_pages do not hold prefix_rows")
+    call(fn, out.data_ptr(), q.data_ptr(), qs, q.size(1), ctypes.byref(cache.spec), batch._with_rows(fn, q.size(0)),
+         prefix_rows, _ptr(prefix_pages), scale, _ptr(workspace),
+         workspace.numel() * workspace.element_size() if workspace is not None else 0, _stream(stream))
 
 
 # ---- peer-memory all-reduce over NVLink (one process per GPU) -------------
