@@ -34,12 +34,13 @@ struct TableParams {
 // a quarter, which f32 holds to 2^-26 of a turn, and the whole quarters swap
 // and negate the f32 sine and cosine.
 __global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant__ TableParams p) {
-  const int64_t n = p.positions * p.pairs;
-  const int64_t stride = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += stride) {
-    const int64_t pos = e / p.pairs;
-    const int i = (int)(e - pos * p.pairs);
-    const double t = (double)pos * p.quarter_turns[i];
+  const int rows = 256 / p.pairs;  // positions per block and step
+  const int i = threadIdx.x % p.pairs;
+  if ((int)threadIdx.x >= rows * p.pairs) return;
+  const double f = p.quarter_turns[i];
+  for (int64_t pos = (int64_t)blockIdx.x * rows + threadIdx.x / p.pairs; pos < p.positions;
+       pos += (int64_t)gridDim.x * rows) {
+    const double t = (double)pos * f;
     const double whole = rint(t);
     float s, c;
     sincospif(0.5f * (float)(t - whole), &s, &c);
@@ -73,7 +74,8 @@ struct HeadsParams {
   int32_t head_dim, rotary_dim;
   int32_t interleaved;
   int32_t lane_shift;  // log2 of the lanes that share a head
-  int32_t slots;       // head slots per token: a thread takes heads slot, slot + slots, ...
+  int32_t heads;       // of both tensors
+  float inv_dim;       // 1 / head_dim
   float eps;
   uint32_t *err;
 };
@@ -86,151 +88,183 @@ struct alignas(V * sizeof(T) < 16 ? V * sizeof(T) : 16) Vec {
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(uint16_t x) { return h2f(x); }
 
-// An item is two vectors of V elements that one lane holds: the two sides of V
-// pairs, or 2V neighbouring elements.  A head's head_dim / 2V items are spread
-// over 2^lane_shift neighbouring lanes, so the norm's sum is a shuffle tree.
-template <int V, typename TIN, bool kNorm, bool kPaged>
-__global__ void __launch_bounds__(256) heads_kernel(const __grid_constant__ HeadsParams p) {
-  constexpr int IPL = V >= 4 ? 1 : V == 2 ? 2 : 4;  // items per lane (head_dim <= 256)
-  constexpr int U = IPL > 1 ? 1 : sizeof(TIN) == 2 ? 4 : 2;  // heads per thread
-  const uint32_t lanes = 1u << p.lane_shift;
-  const uint32_t lane = threadIdx.x & (lanes - 1);
-  const uint32_t group = (blockIdx.x * (256u >> p.lane_shift)) + (threadIdx.x >> p.lane_shift);
-  const uint32_t token = group / (uint32_t)p.slots;
-  const int slot = (int)(group - token * (uint32_t)p.slots);
-  bool live = token < p.tokens;
-  int64_t pos = 0;
-  int64_t page_at = 0;
-  if (live) {
-    if constexpr (kPaged) {
-      PagedRow r;
-      live = paged_row(p.paged, token, r);
-      if (live) {
-        pos = r.position;
-        const int64_t cap = (int64_t)p.paged.max_pages * p.paged.page_size;
-        if (pos < 0) {
-          live = false;
-        } else if (pos >= cap) {
-          live = false;
-          record_device_error(p.err, ERR_KERNEL_HEADS | ERR_SITE_LENGTH);
-        } else {
-          const int32_t page = (int32_t)pos / p.paged.page_size;
-          const int32_t id = p.paged.page_table[r.sequence * p.paged.table_stride + page];
-          if (id < 0 || id >= p.paged.pages) {
-            live = false;
-            record_device_error(p.err, ERR_KERNEL_HEADS | ERR_SITE_PAGE);
-          }
-          page_at = id * p.paged.page_stride + (pos - (int64_t)page * p.paged.page_size) * p.paged.row_stride;
-        }
-      }
-    } else if (p.table) {
-      pos = p.positions ? p.positions[token] : (int64_t)token;
-      if (pos < 0) live = false;
-    }
-    if (live && p.table && pos >= p.table_rows) {
-      live = false;
-      record_device_error(p.err, ERR_KERNEL_HEADS | ERR_SITE_POSITION);
+template <int V>
+__device__ __forceinline__ Vec<uint16_t, V> to_f16(const float *y) {
+  Vec<uint16_t, V> o;
+  if constexpr (V == 1) {
+    o.v[0] = f2h(y[0]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      const __half2 h = __floats2half2_rn(y[j], y[j + 1]);
+      o.v[j] = __half_as_ushort(__low2half(h));
+      o.v[j + 1] = __half_as_ushort(__high2half(h));
     }
   }
+  return o;
+}
+
+// Rows are read and written once: streaming hints on both sides keep them from
+// pushing the table out of L2 (8192 x 32 x 128: 31.8 -> 27.5 us).
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> load(const T *p) {
+  if constexpr (sizeof(T) * V % 16 == 0) {
+    Vec<T, V> o;
+    uint4 *q = reinterpret_cast<uint4 *>(&o);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(T) * V / 16); ++i) q[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+    return o;
+  } else {
+    return *reinterpret_cast<const Vec<T, V> *>(p);
+  }
+}
+template <int V>
+__device__ __forceinline__ void store(uint16_t *p, const Vec<uint16_t, V> &v) {
+  if constexpr (V == 8) __stcs(reinterpret_cast<uint4 *>(p), *reinterpret_cast<const uint4 *>(&v));
+  else *reinterpret_cast<Vec<uint16_t, V> *>(p) = v;
+}
+
+// An item is two vectors of V elements that one lane holds: the two sides of V
+// pairs, or 2V neighbouring elements.  A head's head_dim / 2V items are spread
+// over 2^lane_shift neighbouring lanes (a group), IPL to a lane, so the norm's
+// sum is a shuffle tree.
+//
+// HBM-bound: x is read and written once, and the rows' loads are issued before
+// the chain position -> table row, which they do not depend on.  One head per
+// group: two or four heads that share the lookups and the table row measured
+// the same on 8192 x 32 x 128 (27.8 us, torch's copy of the same bytes 22.4) and
+// slower on 32 tokens (2.6 and 3.4 against 2.2 us), and so did resident blocks
+// that loop with the next group's loads in flight (35.8 us).
+template <int V, typename TIN, bool kNorm, bool kPaged>
+__global__ void __launch_bounds__(256) heads_kernel(const __grid_constant__ HeadsParams p) {
+  constexpr int IPL = V >= 4 ? 1 : V == 2 ? 2 : 4;  // head_dim <= 256
+  const uint32_t lanes = 1u << p.lane_shift;
+  const uint32_t lane = threadIdx.x & (lanes - 1);
+  const uint32_t group = blockIdx.x * (256u >> p.lane_shift) + (threadIdx.x >> p.lane_shift);
+  const uint32_t token = group / (uint32_t)p.heads, head = group - token * (uint32_t)p.heads;
+  const bool inside = token < p.tokens;
   const int items = p.head_dim / (2 * V), turned = p.rotary_dim / (2 * V);
-  const int total = p.seg[0].heads + p.seg[1].heads;
-  // Every load of the thread is issued before the first is used.
-  Vec<TIN, V> x[U][IPL][2];
-  Vec<float, V> cs[IPL], sn[IPL];
+  const bool second = head >= (uint32_t)p.seg[0].heads;
+  const Segment &g = p.seg[second ? 1 : 0];
+  const int at = second ? (int)head - p.seg[0].heads : (int)head;
   int e0[IPL], e1[IPL];
 #pragma unroll
   for (int k = 0; k < IPL; ++k) {
     const int item = (int)(lane + k * lanes);
-    const bool turn = p.table && item < turned;
-    const bool split = turn && !p.interleaved;
+    const bool split = item < turned && !p.interleaved;
     e0[k] = split ? item * V : 2 * V * item;
     e1[k] = split ? p.rotary_dim / 2 + item * V : e0[k] + V;
+  }
+  Vec<TIN, V> x[IPL][2];
+  const TIN *in = static_cast<const TIN *>(g.in) + token * g.in_stride + at * p.head_dim;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      cs[k].v[j] = 1.0f;
-      sn[k].v[j] = 0.0f;
+  for (int k = 0; k < IPL; ++k) {
+    if (inside && (int)(lane + k * lanes) < items) {
+      x[k][0] = load<TIN, V>(in + e0[k]);
+      x[k][1] = load<TIN, V>(in + e1[k]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[k][0].v[j] = x[k][1].v[j] = TIN(0);
     }
-    if (live && turn) {
-      const float *row = p.table + pos * p.rotary_dim + item * V;
+  }
+  // The token's position (-1: nothing is written) and, in a cache, its slot.
+  int32_t position = 0;
+  int64_t page_at = 0;
+  if (!inside) {
+    position = -1;
+  } else if constexpr (kPaged) {
+    PagedRow r;
+    if (!paged_row(p.paged, token, r) || r.position < 0) {
+      position = -1;
+    } else if (r.position >= (int64_t)p.paged.max_pages * p.paged.page_size) {
+      position = -1;
+      record_device_error(p.err, ERR_KERNEL_HEADS | ERR_SITE_LENGTH);
+    } else {
+      position = (int32_t)r.position;
+      const int32_t page = position / p.paged.page_size;
+      const int32_t id = p.paged.page_table[r.sequence * p.paged.table_stride + page];
+      page_at = id * p.paged.page_stride + (int64_t)(position - page * p.paged.page_size) * p.paged.row_stride;
+      if (id < 0 || id >= p.paged.pages) {
+        position = -1;
+        record_device_error(p.err, ERR_KERNEL_HEADS | ERR_SITE_PAGE);
+      }
+    }
+  } else if (p.table) {
+    position = p.positions ? p.positions[token] : (int32_t)token;
+  }
+  if (p.table && position >= p.table_rows) {
+    position = -1;
+    record_device_error(p.err, ERR_KERNEL_HEADS | ERR_SITE_POSITION);
+  }
+  Vec<float, V> cs[IPL], sn[IPL];
+#pragma unroll
+  for (int k = 0; k < IPL; ++k) {
+    const int item = (int)(lane + k * lanes);
+    if (p.table && item < turned && position >= 0) {
+      const float *row = p.table + (int64_t)position * p.rotary_dim + item * V;
       cs[k] = *reinterpret_cast<const Vec<float, V> *>(row);
       sn[k] = *reinterpret_cast<const Vec<float, V> *>(row + p.rotary_dim / 2);
     }
+  }
+  float rstd = 1.0f;
+  if constexpr (kNorm) {
+    float sum = 0.0f;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = slot + u * p.slots;
-      if (live && item < items && h < total) {
-        const Segment &g = p.seg[h < p.seg[0].heads ? 0 : 1];
-        const int hh = h < p.seg[0].heads ? h : h - p.seg[0].heads;
-        const TIN *in = static_cast<const TIN *>(g.in) + token * g.in_stride + hh * p.head_dim;
-        x[u][k][0] = *reinterpret_cast<const Vec<TIN, V> *>(in + e0[k]);
-        x[u][k][1] = *reinterpret_cast<const Vec<TIN, V> *>(in + e1[k]);
+    for (int k = 0; k < IPL; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float a = to_f32(x[k][0].v[j]), b = to_f32(x[k][1].v[j]);
+        sum = fmaf(a, a, fmaf(b, b, sum));
+      }
+    for (uint32_t m = lanes >> 1; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+    rstd = rsqrtf(sum * p.inv_dim + p.eps);
+  }
+  if (position < 0) return;
+  uint16_t *out = g.out + (kPaged ? page_at + at * p.paged.head_stride : token * g.out_stride + at * p.head_dim);
+#pragma unroll
+  for (int k = 0; k < IPL; ++k) {
+    const int item = (int)(lane + k * lanes);
+    if (item >= items) continue;
+    float y[2 * V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      y[j] = to_f32(x[k][0].v[j]);
+      y[V + j] = to_f32(x[k][1].v[j]);
+    }
+    if constexpr (kNorm) {
+      if (g.weight) {
+        const Vec<uint16_t, V> w0 = *reinterpret_cast<const Vec<uint16_t, V> *>(g.weight + e0[k]);
+        const Vec<uint16_t, V> w1 = *reinterpret_cast<const Vec<uint16_t, V> *>(g.weight + e1[k]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          y[j] *= rstd * h2f(w0.v[j]);
+          y[V + j] *= rstd * h2f(w1.v[j]);
+        }
       } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[u][k][0].v[j] = x[u][k][1].v[j] = TIN(0);
+        for (int j = 0; j < 2 * V; ++j) y[j] *= rstd;
       }
     }
-  }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int h = slot + u * p.slots;
-    const Segment &g = p.seg[h < p.seg[0].heads ? 0 : 1];
-    const int hh = h < p.seg[0].heads ? h : h - p.seg[0].heads;
-    float rstd = 1.0f;
-    if constexpr (kNorm) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int k = 0; k < IPL; ++k)
+    if (p.table && g.rotate && item < turned) {
+      // (two loops: indices known at compile time keep y in registers)
+      if (p.interleaved) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float a = to_f32(x[u][k][0].v[j]), b = to_f32(x[u][k][1].v[j]);
-          sum = fmaf(a, a, fmaf(b, b, sum));
+          const float a = y[2 * j], b = y[2 * j + 1];
+          y[2 * j] = a * cs[k].v[j] - b * sn[k].v[j];
+          y[2 * j + 1] = b * cs[k].v[j] + a * sn[k].v[j];
         }
-      for (uint32_t m = lanes >> 1; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-      rstd = rsqrtf(sum / (float)p.head_dim + p.eps);
-    }
-    if (!live || h >= total) continue;
-#pragma unroll
-    for (int k = 0; k < IPL; ++k) {
-      if ((int)(lane + k * lanes) >= items) continue;
-      float y[2 * V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        y[j] = to_f32(x[u][k][0].v[j]);
-        y[V + j] = to_f32(x[u][k][1].v[j]);
-      }
-      if constexpr (kNorm) {
-        if (g.weight) {
-          const Vec<uint16_t, V> w0 = *reinterpret_cast<const Vec<uint16_t, V> *>(g.weight + e0[k]);
-          const Vec<uint16_t, V> w1 = *reinterpret_cast<const Vec<uint16_t, V> *>(g.weight + e1[k]);
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            y[j] *= rstd * h2f(w0.v[j]);
-            y[V + j] *= rstd * h2f(w1.v[j]);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 2 * V; ++j) y[j] *= rstd;
-        }
-      }
-      if (p.table && g.rotate && (int)(lane + k * lanes) < turned) {
+      } else {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const int ia = p.interleaved ? 2 * j : j, ib = p.interleaved ? 2 * j + 1 : V + j;
-          const float a = y[ia], b = y[ib];
-          y[ia] = a * cs[k].v[j] - b * sn[k].v[j];
-          y[ib] = b * cs[k].v[j] + a * sn[k].v[j];
+          const float a = y[j], b = y[V + j];
+          y[j] = a * cs[k].v[j] - b * sn[k].v[j];
+          y[V + j] = b * cs[k].v[j] + a * sn[k].v[j];
         }
       }
-      uint16_t *out = g.out + (kPaged ? page_at + hh * p.paged.head_stride : token * g.out_stride + hh * p.head_dim);
-      Vec<uint16_t, V> o0, o1;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        o0.v[j] = f2h(y[j]);
-        o1.v[j] = f2h(y[V + j]);
-      }
-      *reinterpret_cast<Vec<uint16_t, V> *>(out + e0[k]) = o0;
-      *reinterpret_cast<Vec<uint16_t, V> *>(out + e1[k]) = o1;
     }
+    store(out + e0[k], to_f16<V>(y));
+    store(out + e1[k], to_f16<V>(y + V));
   }
 }
 
@@ -260,10 +294,9 @@ ipuc_status launch_heads(HeadsParams &p, cudaStream_t stream) {
   const int items = p.head_dim / (2 * v);
   p.lane_shift = 0;
   while ((1 << p.lane_shift) < items && p.lane_shift < 5) ++p.lane_shift;
-  const int per_thread = v < 4 ? 1 : sizeof(TIN) == 2 ? 4 : 2;
-  const int total = p.seg[0].heads + p.seg[1].heads;
-  p.slots = (total + per_thread - 1) / per_thread;
-  const int64_t groups = p.tokens * p.slots, per_block = 256 >> p.lane_shift;
+  p.heads = p.seg[0].heads + p.seg[1].heads;
+  p.inv_dim = 1.0f / (float)p.head_dim;
+  const int64_t groups = p.tokens * p.heads, per_block = 256 >> p.lane_shift;
   IPUC_CHECK_ARG(groups < (1ll << 31), "heads: extent too large");
   const unsigned grid = (unsigned)((groups + per_block - 1) / per_block);
   switch (v) {
@@ -368,7 +401,7 @@ extern "C" ipuc_status ipuc_rotary_table(float *table, int64_t positions, int64_
     }
     p.quarter_turns[i] = f * (2.0 / pi);
   }
-  const int64_t want = (positions * p.pairs + 255) / 256, cap = (int64_t)sm_count() * 8;
+  const int64_t rows = 256 / p.pairs, want = (positions + rows - 1) / rows, cap = (int64_t)sm_count() * 8;
   rotary_table_kernel<<<(unsigned)(want < cap ? want : cap), 256, 0, stream>>>(p);
   return check_launch("rotary_table_kernel");
 }

@@ -108,11 +108,16 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_cuda_found = False  # torch.cuda.is_available() asks the driver each time; it does not change once true
+
+
 def _stream(stream) -> int | None:
+    global _cuda_found
     if stream is None:
         try:
             import torch
-            if torch.cuda.is_available():
+            if _cuda_found or torch.cuda.is_available():
+                _cuda_found = True
                 return torch.cuda.current_stream().cuda_stream
         except Exception:  # pragma: no cover
             pass
@@ -473,95 +478,123 @@ def _refuse(fn, text):
     raise IpucError(fn, ERR_INVALID_ARGUMENT, f"{fn[5:]}: {text}")
 
 
-def _want(fn, name, t, dtype, ndim, dense=None):
-    """`t` is a CUDA tensor of the current device with this type and rank, its last `dense` dimensions dense."""
+_torch = _get_device = _raw_stream = None
+
+
+def _load_torch():
+    """torch and its two per-call queries, looked up once: a decode step makes these calls for every layer, and
+    torch.cuda.current_stream() alone costs as much host time as a launch."""
+    global _torch, _get_device, _raw_stream
     import torch
-    if not isinstance(t, torch.Tensor) or t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
+    _get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    _torch = torch
+    return torch
+
+
+def _device():
+    """(torch, index of the current device; -2, which no tensor has, before CUDA is initialised)."""
+    torch = _torch or _load_torch()
+    return torch, _get_device() if torch.cuda.is_initialized() else -2
+
+
+def _stream_on(device, stream):
+    if stream is None and _raw_stream is not None:
+        return _raw_stream(device)
+    return _stream(stream)
+
+
+def _want(fn, name, t, device, dtype, ndim):
+    """Shape and strides of `t`, a CUDA tensor of the current device with this type and rank."""
+    if not isinstance(t, _torch.Tensor) or t.dtype is not dtype:
         _refuse(fn, f"{name} has the wrong type")
-    if t.dim() != ndim:
+    shape = t.shape
+    if len(shape) != ndim:
         _refuse(fn, f"{name} must have {ndim} dimensions")
-    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+    if t.get_device() != device:
         _refuse(fn, f"{name} is not on the current device")
-    expect = 1
-    for i in range(1, (ndim if dense is None else dense) + 1):
-        if t.size(-i) != 1 and t.stride(-i) != expect:
-            _refuse(fn, f"{name} must be dense in its last {ndim if dense is None else dense} dimensions")
-        expect *= t.size(-i)
+    return shape, t.stride()
 
 
-def _token_rows(fn, name, t, dtype):
-    """[tokens, heads, head_dim] with dense heads: (token stride, precision)."""
-    import torch
-    _want(fn, name, t, dtype, 3, 2)
-    return t.stride(0) if t.size(0) > 1 else t.size(1) * t.size(2), F16 if t.dtype == torch.float16 else F32
+def _vector(fn, name, t, device, dtype, size):
+    """Address of a dense vector."""
+    shape, stride = _want(fn, name, t, device, dtype, 1)
+    if shape[0] != size or (size > 1 and stride[0] != 1):
+        _refuse(fn, f"{name} must be a dense vector of {size} entries")
+    return t.data_ptr()
+
+
+def _token_rows(fn, name, t, device, dtype, shape=None):
+    """[tokens, heads, head_dim] with dense heads: (shape, token stride)."""
+    size, stride = _want(fn, name, t, device, dtype, 3)
+    tokens, heads, d = size
+    if shape is not None and (tokens, heads, d) != tuple(shape):
+        _refuse(fn, f"{name} has the wrong shape")
+    if (d > 1 and stride[2] != 1) or (heads > 1 and stride[1] != d):
+        _refuse(fn, f"{name} must be dense in its last 2 dimensions")
+    return size, stride[0] if tokens > 1 else heads * d
+
+
+def _precision(fn, name, t):
+    """(dtype, ipuc_precision) of an f16 or f32 input."""
+    dtype = getattr(t, "dtype", None)
+    if dtype is _torch.float16:
+        return dtype, F16
+    if dtype is _torch.float32:
+        return dtype, F32
+    return _refuse(fn, f"{name} has the wrong type")
 
 
 def rotary_table(out, base=10000.0, scaling=ROTARY_SCALE_NONE, factor=1.0, low=1.0, high=32.0, original=1.0,
                  magnitude=1.0, stream=None):
     """Fills out (f32 [positions, rotary_dim]) with the cosines and sines of every position; see ipuc_rotary_scaling."""
-    import torch
-    _want("ipuc_rotary_table", "table", out, torch.float32, 2)
+    fn, (_, device) = "ipuc_rotary_table", _device()
+    spec = Rotary(out).spec
     s = _RotaryScaling(scaling, base, factor, low, high, original, magnitude)
-    call("ipuc_rotary_table", out.data_ptr(), out.size(0), out.size(1), ctypes.byref(s), _stream(stream))
+    call(fn, spec.table, spec.positions, spec.rotary_dim, ctypes.byref(s), _stream_on(device, stream))
 
 
 class Rotary:
     """A rotary table (rotary_table's output) with the layout of the pairs; keeps the table alive."""
 
     def __init__(self, table, layout=ROTARY_HALF):
-        import torch
-        _want("ipuc_rotary_f16", "table", table, torch.float32, 2)
+        fn, (torch, device) = "ipuc_rotary_table", _device()
+        (positions, columns), stride = _want(fn, "table", table, device, torch.float32, 2)
+        if stride[1] != 1 or (positions > 1 and stride[0] != columns):
+            _refuse(fn, "table must be dense")
         self.table = table
-        self.spec = _Rotary(table.data_ptr(), table.size(0), table.size(1), layout)
-
-
-def _rotary_spec(rotary):
-    return None if rotary is None else ctypes.byref(rotary.spec)
-
-
-def _positions(fn, positions, tokens):
-    import torch
-    if positions is None:
-        return None
-    _want(fn, "positions", positions, torch.int32, 1)
-    if positions.size(0) != tokens:
-        _refuse(fn, "positions must have one entry per token")
-    return positions.data_ptr()
+        self.spec = _Rotary(table.data_ptr(), positions, columns, layout)
+        self._ref = ctypes.byref(self.spec)
 
 
 def rotary_f16(out, x, rotary, positions=None, stream=None):
     """out = x with the heads rotated: x [tokens, heads, head_dim] f16 or f32, out f16 of that shape."""
-    import torch
-    fn = "ipuc_rotary_f16"
-    xs, precision = _token_rows(fn, "x", x, (torch.float16, torch.float32))
-    os_, _ = _token_rows(fn, "out", out, torch.float16)
-    if out.shape != x.shape:
-        _refuse(fn, "out and x must have the same shape")
-    call(fn, out.data_ptr(), os_, x.data_ptr(), xs, precision, x.size(0), x.size(1), x.size(2), _rotary_spec(rotary),
-         _positions(fn, positions, x.size(0)), _stream(stream))
+    fn, (torch, device) = "ipuc_rotary_f16", _device()
+    dtype, precision = _precision(fn, "x", x)
+    shape, xs = _token_rows(fn, "x", x, device, dtype)
+    _, os_ = _token_rows(fn, "out", out, device, torch.float16, shape)
+    at = None if positions is None else _vector(fn, "positions", positions, device, torch.int32, shape[0])
+    call(fn, out.data_ptr(), os_, x.data_ptr(), xs, precision, *shape, None if rotary is None else rotary._ref, at,
+         _stream_on(device, stream))
 
 
 def qk_norm_rotary_f16(q_out, k_out, q, k, q_weight=None, k_weight=None, eps=1e-6, rotary=None, positions=None,
                        stream=None):
-    """Per-head norm of q and k, then their rotation: q [tokens, q_heads, head_dim], k [tokens, k_heads, head_dim]."""
-    import torch
-    fn = "ipuc_qk_norm_rotary_f16"
-    qs, precision = _token_rows(fn, "q", q, (torch.float16, torch.float32))
-    ks, k_precision = _token_rows(fn, "k", k, (torch.float16, torch.float32))
-    qos, _ = _token_rows(fn, "q_out", q_out, torch.float16)
-    kos, _ = _token_rows(fn, "k_out", k_out, torch.float16)
-    if precision != k_precision or q.size(0) != k.size(0) or q.size(2) != k.size(2):
-        _refuse(fn, "q and k must have the same type, tokens and head_dim")
-    if q_out.shape != q.shape or k_out.shape != k.shape:
-        _refuse(fn, "outputs must have their inputs' shapes")
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None:
-            _want(fn, name, w, torch.float16, 1)
-            if w.size(0) != q.size(2):
-                _refuse(fn, f"{name} must have head_dim entries")
-    call(fn, q_out.data_ptr(), qos, k_out.data_ptr(), kos, q.data_ptr(), qs, k.data_ptr(), ks, precision,
-         _ptr(q_weight), _ptr(k_weight), eps, q.size(0), q.size(1), k.size(1), q.size(2), _rotary_spec(rotary),
-         _positions(fn, positions, q.size(0)), _stream(stream))
+    """Per-head norm of q and k, then their rotation: q [tokens, q_heads, head_dim], k [tokens, k_heads, head_dim]
+    of one type, weights f16 [head_dim] (None: ones)."""
+    fn, (torch, device) = "ipuc_qk_norm_rotary_f16", _device()
+    dtype, precision = _precision(fn, "q", q)
+    q_shape, qs = _token_rows(fn, "q", q, device, dtype)
+    tokens, q_heads, d = q_shape
+    k_heads = k.shape[1] if k.dim() == 3 else 0
+    k_shape, ks = _token_rows(fn, "k", k, device, dtype, (tokens, k_heads, d))
+    _, qos = _token_rows(fn, "q_out", q_out, device, torch.float16, q_shape)
+    _, kos = _token_rows(fn, "k_out", k_out, device, torch.float16, k_shape)
+    wq = None if q_weight is None else _vector(fn, "q_weight", q_weight, device, torch.float16, d)
+    wk = None if k_weight is None else _vector(fn, "k_weight", k_weight, device, torch.float16, d)
+    at = None if positions is None else _vector(fn, "positions", positions, device, torch.int32, tokens)
+    call(fn, q_out.data_ptr(), qos, k_out.data_ptr(), kos, q.data_ptr(), qs, k.data_ptr(), ks, precision, wq, wk, eps,
+         tokens, q_heads, k_heads, d, None if rotary is None else rotary._ref, at, _stream_on(device, stream))
 
 
 class PagedCache:
@@ -569,61 +602,53 @@ class PagedCache:
     dimensions in memory: pass a transposed view of [pages, page_size, heads, head_dim]); keeps them alive."""
 
     def __init__(self, keys, values):
-        import torch
-        fn = "ipuc_paged_cache"
-        _want(fn, "keys", keys, torch.float16, 4, 1)
-        _want(fn, "values", values, torch.float16, 4, 1)
-        if keys.shape != values.shape or keys.stride() != values.stride():
+        fn, (torch, device) = "ipuc_paged_cache", _device()
+        shape, stride = _want(fn, "keys", keys, device, torch.float16, 4)
+        if _want(fn, "values", values, device, torch.float16, 4) != (shape, stride):
             _refuse(fn, "keys and values must have the same shape and strides")
-        self.keys, self.values = keys, values
-        pages, heads, page_size, d = keys.shape
+        pages, heads, page_size, d = shape
+        if d > 1 and stride[3] != 1:
+            _refuse(fn, "head_dim must be dense")
         # a dimension of one element has no meaningful stride
-        strides = [keys.stride(i) if keys.size(i) > 1 else max(keys.stride(i), d) for i in range(3)]
-        self.spec = _PagedCache(keys.data_ptr(), values.data_ptr(), pages, page_size, heads, d, *strides)
+        page_stride, head_stride, row_stride = [s if n > 1 else max(s, d) for s, n in zip(stride, shape[:3])]
+        self.keys, self.values = keys, values
+        self.spec = _PagedCache(keys.data_ptr(), values.data_ptr(), pages, page_size, heads, d, page_stride,
+                                head_stride, row_stride)
+        self._ref = ctypes.byref(self.spec)
 
 
 class PagedBatch:
     """The sequences of a call: page_table [sequences, max_pages], lengths [sequences] and, unless every sequence
-    has one row, row_offsets [sequences + 1], int32.  rows: the rows of the tensors that go with row_offsets (its
-    last entry, or more: the rest is padding); read from the tensors of each call where it is not given."""
+    has one row, row_offsets [sequences + 1], int32.  The number of rows is that of the tensors of each call (with
+    row_offsets: its last entry, or more; the rest is padding)."""
 
-    def __init__(self, page_table, lengths, row_offsets=None, rows=None):
-        import torch
-        fn = "ipuc_paged_batch"
-        _want(fn, "page_table", page_table, torch.int32, 2, 1)
-        _want(fn, "lengths", lengths, torch.int32, 1)
-        n = lengths.size(0)
-        if page_table.size(0) != n:
-            _refuse(fn, "page_table must have one row per sequence")
-        if row_offsets is not None:
-            _want(fn, "row_offsets", row_offsets, torch.int32, 1)
-            if row_offsets.size(0) != n + 1:
-                _refuse(fn, "row_offsets must have one entry more than sequences")
+    def __init__(self, page_table, lengths, row_offsets=None):
+        fn, (torch, device) = "ipuc_paged_batch", _device()
+        (n, width), stride = _want(fn, "page_table", page_table, device, torch.int32, 2)
+        if width > 1 and stride[1] != 1:
+            _refuse(fn, "page_table must be dense in its last dimension")
+        at = _vector(fn, "lengths", lengths, device, torch.int32, n)
+        offsets = None if row_offsets is None else _vector(fn, "row_offsets", row_offsets, device, torch.int32, n + 1)
         self._keep = (page_table, lengths, row_offsets)
-        width = page_table.size(1)
-        self._rows = rows
-        self.spec = _PagedBatch(page_table.data_ptr(), lengths.data_ptr(), _ptr(row_offsets),
-                                page_table.stride(0) if n > 1 else width, 0 if rows is None else rows, n, width)
+        self.spec = _PagedBatch(page_table.data_ptr(), at, offsets, stride[0] if n > 1 else width, 0, n, width)
 
-    def _with_rows(self, fn, rows):
-        if self._rows is not None and self._rows != rows:
-            _refuse(fn, "tensors must have the batch's rows")
-        self.spec.rows = rows
-        return ctypes.byref(self.spec)
+    def _with_rows(self, rows):
+        # a struct of its own for each call: two threads may use one batch
+        s = self.spec
+        return ctypes.byref(_PagedBatch(s.page_table, s.lengths, s.row_offsets, s.table_stride, rows, s.sequences,
+                                        s.max_pages))
 
 
 def paged_append_f16(cache, batch, k, v, rotary=None, stream=None):
     """Writes the new rows k, v [rows, heads, head_dim] (f16 or f32) into the cache, keys rotated by their positions."""
-    import torch
-    fn = "ipuc_paged_append_f16"
-    ks, precision = _token_rows(fn, "k", k, (torch.float16, torch.float32))
-    vs, v_precision = _token_rows(fn, "v", v, (torch.float16, torch.float32))
-    if precision != v_precision or k.shape != v.shape:
-        _refuse(fn, "k and v must have the same type and shape")
-    if k.size(1) != cache.spec.heads or k.size(2) != cache.spec.head_dim:
-        _refuse(fn, "rows must have the cache's heads and head_dim")
-    call(fn, ctypes.byref(cache.spec), batch._with_rows(fn, k.size(0)), k.data_ptr(), ks, v.data_ptr(), vs, precision,
-         _rotary_spec(rotary), _stream(stream))
+    fn, (_, device) = "ipuc_paged_append_f16", _device()
+    dtype, precision = _precision(fn, "k", k)
+    rows = k.shape[0] if k.dim() else 0
+    shape = (rows, cache.spec.heads, cache.spec.head_dim)
+    _, ks = _token_rows(fn, "k", k, device, dtype, shape)
+    _, vs = _token_rows(fn, "v", v, device, dtype, shape)
+    call(fn, cache._ref, batch._with_rows(rows), k.data_ptr(), ks, v.data_ptr(), vs, precision,
+         None if rotary is None else rotary._ref, _stream_on(device, stream))
 
 
 def paged_attention_workspace_bytes(rows, sequences, q_heads, heads, head_dim, prefix_rows=0, ragged=False) -> int:
@@ -635,23 +660,27 @@ def paged_attention_workspace_bytes(rows, sequences, q_heads, heads, head_dim, p
 def paged_attention_f16(out, q, cache, batch, workspace, prefix_rows=0, prefix_pages=None, scale=0.0, stream=None):
     """Attention of q [rows, q_heads, head_dim] over the cache into out (dense); positions below prefix_rows are read
     once for all rows through prefix_pages."""
-    import torch
-    fn = "ipuc_paged_attention_f16"
-    qs, _ = _token_rows(fn, "q", q, torch.float16)
-    _want(fn, "out", out, torch.float16, 3)
-    if out.shape != q.shape:
-        _refuse(fn, "out and q must have the same shape")
-    if q.size(2) != cache.spec.head_dim:
+    fn, (torch, device) = "ipuc_paged_attention_f16", _device()
+    shape, qs = _token_rows(fn, "q", q, device, torch.float16)
+    rows, heads, d = shape
+    _, os_ = _token_rows(fn, "out", out, device, torch.float16, shape)
+    if os_ != heads * d:
+        _refuse(fn, "out must be dense")
+    if d != cache.spec.head_dim:
         _refuse(fn, "rows must have the cache's head_dim")
+    at = None
     if prefix_rows:
         if prefix_pages is None:
             _refuse(fn, "prefix_rows without prefix_pages")
-        _want(fn, "prefix_pages", prefix_pages, torch.int32, 1)
-        if prefix_pages.size(0) * cache.spec.page_size < prefix_rows:
-            _refuse(fn, "prefix_pages do not hold prefix_rows")
-    call(fn, out.data_ptr(), q.data_ptr(), qs, q.size(1), ctypes.byref(cache.spec), batch._with_rows(fn, q.size(0)),
-         prefix_rows, _ptr(prefix_pages), scale, _ptr(workspace),
-         workspace.numel() * workspace.element_size() if workspace is not None else 0, _stream(stream))
+        (n,), stride = _want(fn, "prefix_pages", prefix_pages, device, torch.int32, 1)
+        if n * cache.spec.page_size < prefix_rows or (n > 1 and stride[0] != 1):
+            _refuse(fn, "prefix_pages must be dense and hold prefix_rows")
+        at = prefix_pages.data_ptr()
+    if workspace is not None and workspace.get_device() != device:
+        _refuse(fn, "workspace is not on the current device")
+    call(fn, out.data_ptr(), q.data_ptr(), qs, heads, cache._ref, batch._with_rows(rows), prefix_rows, at, scale,
+         _ptr(workspace), workspace.numel() * workspace.element_size() if workspace is not None else 0,
+         _stream_on(device, stream))
 
 
 # ---- peer-memory all-reduce over NVLink (one process per GPU) -------------

@@ -126,7 +126,7 @@ def test_wrappers_refuse_host_tensors_and_wrong_shapes():
     x = torch.zeros((4, 2, 64), dtype=torch.float16)
     with pytest.raises(ipuc.IpucError, match="type"):
         ipuc.rotary_f16(x, x.double(), None)
-    with pytest.raises(ipuc.IpucError, match="3 dimensions"):
+    with pytest.raises(ipuc.IpucError, match="dimensions"):
         ipuc.rotary_f16(x, x[0], None)
     if torch.cuda.is_available():
         with pytest.raises(ipuc.IpucError, match="current device"):
