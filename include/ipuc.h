@@ -541,7 +541,7 @@ typedef struct {
   int64_t table_stride;  /* >= max_pages */
   int64_t rows;
   int32_t sequences;
-  int32_t max_pages;     /* entries of a table row; max_pages * page_size < 2^31 */
+  int32_t max_pages;     /* entries of a table row; max_pages * page_size < 2^31 - 256 */
 } ipuc_paged_batch;
 
 /* Writes the new rows' keys (rotated by their positions unless rotary is
