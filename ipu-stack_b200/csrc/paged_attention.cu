@@ -68,18 +68,44 @@ struct PagedAttnParams {
   int32_t q_heads, heads, group, head_dim, prefix;
   int32_t chunk;          // keys per TMA box: gcd(page_size, 64)
   float scale_log2;       // softmax scale * log2(e)
-  // Partial results: unnormalised O (f32, head_dim wide) and (running maximum
-  // in log2 units, sum of weights) per row and query head.
-  float *own_o, *prefix_o;
-  float2 *own_ml, *prefix_ml;
-  int64_t *tile_sums;     // single rows: own key tiles of the sequences before b, [sequences + 1]
-  int32_t stream_ctas;    // single rows: CTAs of the own-part kernel; 0: the tile kernel took it
-  int32_t own_splits, prefix_splits;
-  int32_t row_units;      // tile kernel: units of 2 * tile_rows rows per head
+  // Each kernel cuts a line of key tiles into equal pieces, one per CTA.  A
+  // unit (rows that read the same keys of one head) that a piece ends in has
+  // several partial results: unnormalised O (f32, head_dim wide) and (running
+  // maximum in log2 units, sum of weights) per row, in slot (unit + CTA).
+  float *stream_o, *tile_o;
+  float2 *stream_ml, *tile_ml;
+  int32_t stream_rows, tile_slot_rows;  // rows of a slot
+  // Written by CTA 0 of either kernel for the join: key tiles before sequence
+  // b (stream) or row unit u (tile), then (tile) the whole line's, then the
+  // number of pieces; and row units before sequence b.
+  int64_t *stream_sums, *unit_sums;
+  int32_t *unit_base;
+  int32_t sms;                     // CTAs of each kernel
+  int32_t stream, tile;            // which of the two run
+  int32_t stream_prefix;  // the stream kernel takes the prefix too
+  int32_t tile_own;       // the tile kernel takes the own parts, in at most max_units row units
+  int32_t max_units;
+  int32_t prefix_units;   // tile kernel: row units of the prefix
   int32_t tile_rows;      // tile kernel: batch rows per 128-row MMA tile, 128 / group
-  int32_t direct;         // the tile kernel's result is final
   uint32_t *err;
 };
+
+// Two f32 to packed f16 in one conversion.
+__device__ __forceinline__ uint32_t to_h2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Named barrier over `count` threads that says whether `pred` holds for any of them.
+__device__ __forceinline__ bool barrier_any(uint32_t id, uint32_t count, bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %3, 0;\n bar.red.or.pred q, %1, %2, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"(id), "r"(count), "r"((uint32_t)pred)
+      : "memory");
+  return r != 0;
+}
 
 // Length of sequence b as far as its table row can hold it.
 __device__ __forceinline__ int32_t checked_length(const PagedAttnParams &p, int32_t b, bool report) {
@@ -138,14 +164,17 @@ __device__ __forceinline__ int32_t page_of(const PagedAttnParams &p, const int32
 // and K and V are streamed once: HBM-bound.  The key tiles (64 keys, at
 // absolute multiples of 64) of all (sequence, head) units form one line that
 // is cut into equal pieces, one per CTA, so ragged lengths leave no CTA idle.
-// A producer warp fills a ring of tiles by TMA, box by box of gcd(page_size,
-// 64) keys; four warps take 16 keys of every tile each, with a running
-// maximum, sum and O of their own, and meet once per unit.
-constexpr int kStreamKeys = 64, kStreamStages = 3, kStreamThreads = 160, kMergeLd = 36;
+// When all rows of the call fit one m16 tile, the shared prefix is on the line
+// too, as a first unit per head.
+// A CTA is two workers with a piece each: a producer warp fills a ring of
+// tiles by TMA, box by box of gcd(page_size, 64) keys; four warps take 16 keys
+// of every tile each, with a running maximum, sum and O of their own, and meet
+// once per unit.
+constexpr int kStreamKeys = 64, kStreamStages = 3, kStreamWorkers = 2, kStreamThreads = kStreamWorkers * 160, kMergeLd = 36;
 
 template <int DP>
 constexpr int stream_smem_bytes() {
-  return kStreamStages * 2 * kStreamKeys * DP * 2 + 4 * 16 * kMergeLd * 4 + 1024;
+  return kStreamWorkers * (kStreamStages * 2 * kStreamKeys * DP * 2 + 4 * 16 * kMergeLd * 4) + 1024;
 }
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
@@ -167,13 +196,26 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A CTA's place on the line of key tiles: unit (b, h), tile i of its n.
+// A CTA's place on the line of key tiles: tile i of the n of unit (b, h), keys
+// [lo, hi); b = -1: the prefix.
 struct StreamWalk {
-  int32_t b, h, i, n, len;
+  int32_t b, h, i, n, lo, hi;
   int64_t left;
 
   __device__ __forceinline__ static int32_t tiles(const PagedAttnParams &p, int32_t len) {
     return len > p.prefix ? (len + kStreamKeys - 1) / kStreamKeys - p.prefix / kStreamKeys : 0;
+  }
+  __device__ __forceinline__ void enter(const PagedAttnParams &p, int32_t sequence) {
+    b = sequence;
+    if (b < 0) {
+      lo = 0;
+      hi = p.prefix;
+      n = (hi + kStreamKeys - 1) / kStreamKeys;
+    } else {
+      lo = p.prefix;
+      hi = checked_length(p, b, false);
+      n = tiles(p, hi);
+    }
   }
   __device__ __forceinline__ void step(const PagedAttnParams &p, int32_t count) {
     left -= count;
@@ -183,77 +225,106 @@ struct StreamWalk {
     if (++h < p.heads) return;
     h = 0;
     do {
-      if (++b >= p.paged.sequences) {
+      if (b + 1 >= p.paged.sequences) {
         left = 0;
         return;
       }
-      len = checked_length(p, b, false);
-      n = tiles(p, len);
+      enter(p, b + 1);
     } while (n == 0);
   }
 };
 
+// SMs that stream own parts while the others work on the prefix: so many that
+// both take the same time, at 55 GB/s an SM streaming (up to what saturates
+// HBM) and 2.5 us a key tile of two row tiles.  Every CTA of both kernels comes
+// to the same number.
+constexpr float kStreamBytesPerUs = 55e3f, kTileUs = 2.5f;
+constexpr int kStreamSaturated = 112;
+__device__ __forceinline__ int32_t stream_sms(const PagedAttnParams &p, int64_t own_tiles) {
+  if (own_tiles == 0) return 0;
+  if (p.prefix_units == 0) return p.sms;
+  const float stream = (float)own_tiles * p.heads * (2.0f * 64 * 2 * p.head_dim) / kStreamBytesPerUs;
+  const float tile = (float)p.prefix_units * p.heads * ((p.prefix + 127) / 128) * kTileUs;
+  const int32_t x = (int32_t)(p.sms * (stream / (stream + tile)) + 0.5f);
+  return max(1, min(min(x, kStreamSaturated), p.sms - 1));
+}
+
 template <int DP>
-__global__ void __launch_bounds__(kStreamThreads, 2)
+__global__ void __launch_bounds__(kStreamThreads, 1)
     paged_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const __grid_constant__ PagedAttnParams p) {
   constexpr int HALVES = DP / 64, KS = DP / 16, NT = DP / 8;
   constexpr int HALF_BYTES = kStreamKeys * 128, TILE_BYTES = HALVES * HALF_BYTES;  // K or V of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float *merge = reinterpret_cast<float *>(smem + kStreamStages * 2 * TILE_BYTES);  // [4][16][kMergeLd]
-  __shared__ uint64_t full[kStreamStages], empty[kStreamStages];
-  __shared__ int64_t scratch[kStreamThreads / 32], first_left[2];
-  __shared__ int32_t first_unit[4];
-  __shared__ float warp_m[4][16], warp_l[4][16];
+  constexpr int RING_BYTES = kStreamStages * 2 * TILE_BYTES;
+  __shared__ uint64_t all_full[kStreamWorkers][kStreamStages], all_empty[kStreamWorkers][kStreamStages];
+  __shared__ int64_t scratch[kStreamThreads / 32];
+  __shared__ int32_t first_unit[kStreamWorkers][3];
+  __shared__ float all_m[kStreamWorkers][4][16], all_l[kStreamWorkers][4][16];
   __shared__ int aborted;
   volatile int *abort_flag = &aborted;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int worker = threadIdx.x / 160, warp = (threadIdx.x >> 5) % 5, lane = threadIdx.x & 31;
+  uint64_t *full = all_full[worker], *empty = all_empty[worker];
+  float(&warp_m)[4][16] = all_m[worker], (&warp_l)[4][16] = all_l[worker];
+  float *merge = reinterpret_cast<float *>(smem + kStreamWorkers * RING_BYTES) + worker * 4 * 16 * kMergeLd;
+  smem += worker * RING_BYTES;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStreamStages; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 4);
-    }
+    for (int w = 0; w < kStreamWorkers; ++w)
+      for (int i = 0; i < kStreamStages; ++i) {
+        mbar_init(&all_full[w][i], 1);
+        mbar_init(&all_empty[w][i], 4);
+      }
     aborted = 0;
-    first_left[1] = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  const int64_t cta = blockIdx.x;
-  auto count = [&](int32_t b) { return StreamWalk::tiles(p, checked_length(p, b, cta == 0)); };
-  // Sums first, then this CTA's piece [W c / C, W (c + 1) / C) of the line of W tiles.
-  int64_t starts[2] = {0, 0};
-  const int64_t total = block_sums<kStreamThreads>(p.paged.sequences, scratch, count, [&](int32_t b, int64_t sum) {
-    if (cta == 0) p.tile_sums[b] = sum;
-  });
-  if (cta == 0 && threadIdx.x == 0) p.tile_sums[p.paged.sequences] = total;
   griddep_launch_dependents();
-  const int64_t line = total * p.heads, ctas = min((int64_t)gridDim.x, line);  // no piece is empty
-  if (cta >= ctas) return;
-  starts[0] = line * cta / ctas;
-  starts[1] = line * (cta + 1) / ctas;
+  auto count = [&](int32_t b) { return StreamWalk::tiles(p, checked_length(p, b, blockIdx.x == 0)); };
+  // Sums first, then this worker's piece [W c / C, W (c + 1) / C) of the line of W tiles.
+  const int64_t total = block_sums<kStreamThreads>(p.paged.sequences, scratch, count, [&](int32_t b, int64_t sum) {
+    if (blockIdx.x == 0) p.stream_sums[b] = sum;
+  });
+  const int64_t ahead = p.stream_prefix ? (int64_t)((p.prefix + kStreamKeys - 1) / kStreamKeys) * p.heads : 0;
+  const int64_t line = ahead + total * p.heads;
+  const int64_t share = p.stream_prefix ? p.sms : stream_sms(p, total);
+  const int64_t pieces = min(kStreamWorkers * share, line);  // no piece is empty
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    p.stream_sums[p.paged.sequences] = total;
+    p.stream_sums[p.paged.sequences + 1] = pieces;
+  }
+  if ((int64_t)blockIdx.x >= share || blockIdx.x >= pieces) return;
+  // Worker w of CTA c has piece w * share + c: few pieces spread over many SMs.
+  auto piece_of = [&](int w) { return w * share + (int64_t)blockIdx.x; };
+  auto start_of = [&](int w) { return line * piece_of(w) / pieces; };
   __syncthreads();  // scratch is read before it is written again
   block_sums<kStreamThreads>(p.paged.sequences, scratch, count, [&](int32_t b, int64_t sum) {
     const int32_t n = count(b);
-    const int64_t at = starts[0] - sum * p.heads;
-    if (at >= 0 && at < (int64_t)n * p.heads) {
-      first_unit[0] = b;
-      first_unit[1] = (int32_t)(at / n);
-      first_unit[2] = (int32_t)(at % n);
-      first_unit[3] = n;
+    for (int w = 0; w < kStreamWorkers; ++w) {
+      const int64_t at = start_of(w) - ahead - sum * p.heads;
+      if (at >= 0 && at < (int64_t)n * p.heads) {
+        first_unit[w][0] = b;
+        first_unit[w][1] = (int32_t)(at / n);
+        first_unit[w][2] = (int32_t)(at % n);
+      }
     }
   });
-  __syncthreads();
+  __syncthreads();  // (the barriers' initialisation too)
+  const int64_t cta = piece_of(worker), start = start_of(worker);
+  if (cta >= pieces) return;
   StreamWalk w;
-  w.b = first_unit[0];
-  w.h = first_unit[1];
-  w.i = first_unit[2];
-  w.n = first_unit[3];
-  w.len = checked_length(p, w.b, false);
-  w.left = starts[1] - starts[0];
-  const int32_t tile0 = p.prefix / kStreamKeys;  // first key tile of every unit
+  w.left = line * (cta + 1) / pieces - start;
+  if (start < ahead) {
+    w.enter(p, -1);
+    w.h = (int32_t)(start / w.n);
+    w.i = (int32_t)(start % w.n);
+  } else {
+    w.enter(p, first_unit[worker][0]);
+    w.h = first_unit[worker][1];
+    w.i = first_unit[worker][2];
+  }
 
   if (warp == 4) {
     // Producer: lane l issues boxes l, l + 32, ... of a tile: (K or V, half, chunk).
@@ -262,10 +333,10 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     uint32_t t = 0;
     for (; w.left > 0 && ok; ++t, w.step(p, 1)) {
       const int st = t % kStreamStages;
-      const int32_t key0 = (tile0 + w.i) * kStreamKeys;
-      const int32_t *ids = p.paged.page_table + w.b * p.paged.table_stride;
+      const int32_t key0 = (w.lo / kStreamKeys + w.i) * kStreamKeys;
+      const int32_t *ids = w.b < 0 ? p.prefix_pages : p.paged.page_table + w.b * p.paged.table_stride;
       // this lane's first box's page is looked up before the stage is free
-      int32_t page = lane < boxes ? page_of(p, ids, key0 + (lane % chunks) * p.chunk, p.prefix, w.len) : 0;
+      int32_t page = lane < boxes ? page_of(p, ids, key0 + (lane % chunks) * p.chunk, w.lo, w.hi) : 0;
       if (!mbar_wait_bounded(&empty[st], ((t / kStreamStages) & 1) ^ 1, abort_flag)) {
         ok = false;
         break;
@@ -276,7 +347,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
       for (int x = lane; x < boxes; x += 32) {
         const int chunk = x % chunks, half = (x / chunks) % HALVES, v = x / (chunks * HALVES);
         const int32_t pos = key0 + chunk * p.chunk;
-        if (x >= 32) page = page_of(p, ids, pos, p.prefix, w.len);
+        if (x >= 32) page = page_of(p, ids, pos, w.lo, w.hi);
         tma_load_4d(base + v * TILE_BYTES + half * HALF_BYTES + chunk * p.chunk * 128, v ? &tm_v : &tm_k, &full[st],
                     half * 64, pos % p.paged.page_size, w.h, page);
       }
@@ -291,18 +362,24 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     return;
   }
 
-  // Consumers.  A fragments: rows lane / 4 and lane / 4 + 8 of the group.
+  // Consumers.  A fragments: rows lane / 4 and lane / 4 + 8 of the unit: the
+  // group's heads, or (prefix) those of all rows of the call.
   const int r0 = lane >> 2, r1 = r0 + 8, cq = (lane & 3) * 2;
+  auto unit_rows = [&](const StreamWalk &u) { return u.b < 0 ? (int)p.rows * p.group : p.group; };
   auto load_q = [&](const StreamWalk &u, uint32_t (&a)[KS][4]) {
-    const uint16_t *base = p.q + u.b * p.q_stride + (int64_t)u.h * p.group * p.head_dim;
+    const int n = unit_rows(u);
+    const uint16_t *base[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int row = x ? r1 : r0, token = row / p.group;
+      base[x] = p.q + (u.b < 0 ? token : u.b) * p.q_stride + (u.h * p.group + row - token * p.group) * p.head_dim;
+    }
 #pragma unroll
     for (int k = 0; k < KS; ++k)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int row = j & 1 ? r1 : r0, col = k * 16 + cq + (j & 2 ? 8 : 0);
-        a[k][j] = row < p.group && col < p.head_dim
-                      ? *reinterpret_cast<const uint32_t *>(base + row * p.head_dim + col)
-                      : 0u;
+        a[k][j] = row < n && col < p.head_dim ? *reinterpret_cast<const uint32_t *>(base[j & 1] + col) : 0u;
       }
   };
   uint32_t q[KS][4];
@@ -317,6 +394,13 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
   uint32_t t = 0;
   while (w.left > 0) {
     const int32_t count_here = (int32_t)min((int64_t)(w.n - w.i), w.left);
+    // Keys a row attends to end at the unit's end, in the prefix perhaps before it.
+    int32_t end0 = w.hi, end1 = w.hi, end = w.hi;
+    if (w.b < 0) {
+      if (r0 < (int)p.rows * p.group) end0 = min(w.hi, max(0, p.paged.lengths[r0 / p.group]));
+      if (r1 < (int)p.rows * p.group) end1 = min(w.hi, max(0, p.paged.lengths[r1 / p.group]));
+      end = __reduce_min_sync(0xffffffffu, min(end0, end1));
+    }
     float o[NT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
@@ -325,7 +409,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
       // (a wait that ran out is not left early: the barriers below need every warp)
       if (ok && !mbar_wait_bounded(&full[st], (t / kStreamStages) & 1, abort_flag)) ok = false;
       const uint32_t ks = sbase + st * 2 * TILE_BYTES, vs = ks + TILE_BYTES;
-      const int32_t key0 = (tile0 + w.i + k) * kStreamKeys + warp * 16;
+      const int32_t key0 = (w.lo / kStreamKeys + w.i + k) * kStreamKeys + warp * 16;
       float s[2][4] = {}, s2[2][4] = {};  // even and odd steps: two chains
 #pragma unroll
       for (int d = 0; d < KS; ++d) {
@@ -340,7 +424,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         s[0][j] += s2[0][j];
         s[1][j] += s2[1][j];
       }
-      if (key0 < p.prefix || key0 + 16 > w.len) {
+      if (key0 < w.lo || key0 + 16 > end) {
         // The unit's first or last tile: scores of keys that are not its own
         // are dropped, and the warp's V rows of such keys, which may hold
         // anything, are zeroed (0 * NaN is NaN).
@@ -349,11 +433,11 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int32_t key = key0 + x * 8 + cq + (j & 1);
-            if (key < p.prefix || key >= w.len) s[x][j] = -INFINITY;
+            if (key < w.lo || key >= (j & 2 ? end1 : end0)) s[x][j] = -INFINITY;
           }
         for (int x = lane; x < 16 * HALVES * 8; x += 32) {
           const int row = x / (HALVES * 8), half = (x >> 3) % HALVES;
-          if (key0 + row < p.prefix || key0 + row >= w.len) {
+          if (key0 + row < w.lo || key0 + row >= w.hi) {
             const uint32_t at = vs + half * HALF_BYTES + (warp * 16 + row) * 128 + (x & 7) * 16;
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
           }
@@ -392,8 +476,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         const float p2 = ex2_approx(fmaf(s[x][2], c, n1)), p3 = ex2_approx(fmaf(s[x][3], c, n1));
         l0 += p0 + p1;
         l1 += p2 + p3;
-        a[2 * x] = pack_h2(p0, p1);
-        a[2 * x + 1] = pack_h2(p2, p3);
+        a[2 * x] = to_h2(p0, p1);
+        a[2 * x + 1] = to_h2(p2, p3);
       }
 #pragma unroll
       for (int d = 0; d < NT; d += 2) {
@@ -421,12 +505,12 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
       warp_l[warp][r0] = l0;
       warp_l[warp][r1] = l1;
     }
-    named_barrier_sync(1, 128);
+    named_barrier_sync(1 + worker, 128);
     const float t0 = fmaxf(fmaxf(warp_m[0][r0], warp_m[1][r0]), fmaxf(warp_m[2][r0], warp_m[3][r0]));
     const float t1 = fmaxf(fmaxf(warp_m[0][r1], warp_m[1][r1]), fmaxf(warp_m[2][r1], warp_m[3][r1]));
     const float a0 = m0 == -INFINITY ? 0.0f : ex2_approx((m0 - t0) * c);
     const float a1 = m1 == -INFINITY ? 0.0f : ex2_approx((m1 - t1) * c);
-    const int orow = threadIdx.x >> 3, ocol = (threadIdx.x & 7) * 4;  // this thread's share of the sums
+    const int orow = warp * 4 + (lane >> 3), ocol = (lane & 7) * 4;  // this thread's share of the sums
     float top = -INFINITY, sum = 0.0f;
 #pragma unroll
     for (int x = 0; x < 4; ++x) top = fmaxf(top, warp_m[x][orow]);
@@ -434,9 +518,11 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     for (int x = 0; x < 4; ++x)
       if (warp_m[x][orow] != -INFINITY) sum += warp_l[x][orow] * ex2_approx((warp_m[x][orow] - top) * c);
     const bool whole = p.prefix == 0 && count_here == w.n;
-    const int64_t slot = ((int64_t)w.b * p.heads + w.h + cta) * p.group + orow;
+    const int64_t unit = (int64_t)(w.b + p.stream_prefix) * p.heads + w.h;
+    const int64_t slot = (unit + cta) * p.stream_rows + orow;
+    const int rows_here = unit_rows(w);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (!whole && orow < p.group && ocol == 0) p.own_ml[slot] = make_float2(top == -INFINITY ? top : top * c, sum);
+    if (!whole && orow < rows_here && ocol == 0) p.stream_ml[slot] = make_float2(top == -INFINITY ? top : top * c, sum);
 #pragma unroll
     for (int round = 0; round < DP / 32; ++round) {
       float *mine = merge + warp * 16 * kMergeLd;
@@ -446,9 +532,9 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         *reinterpret_cast<float2 *>(mine + r0 * kMergeLd + i * 8 + cq) = make_float2(v[0] * a0, v[1] * a0);
         *reinterpret_cast<float2 *>(mine + r1 * kMergeLd + i * 8 + cq) = make_float2(v[2] * a1, v[3] * a1);
       }
-      named_barrier_sync(1, 128);
+      named_barrier_sync(1 + worker, 128);
       const int col = round * 32 + ocol;
-      if (orow < p.group && col < p.head_dim) {
+      if (orow < rows_here && col < p.head_dim) {
         float4 r = *reinterpret_cast<const float4 *>(merge + orow * kMergeLd + ocol);
 #pragma unroll
         for (int x = 1; x < 4; ++x) {
@@ -460,15 +546,15 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         }
         if (whole) {
           uint2 h;
-          h.x = pack_h2(r.x * inv, r.y * inv);
-          h.y = pack_h2(r.z * inv, r.w * inv);
+          h.x = to_h2(r.x * inv, r.y * inv);
+          h.y = to_h2(r.z * inv, r.w * inv);
           const int64_t head = (int64_t)w.b * p.q_heads + w.h * p.group + orow;
           *reinterpret_cast<uint2 *>(p.out + head * p.head_dim + col) = h;
         } else {
-          *reinterpret_cast<float4 *>(p.own_o + slot * p.head_dim + col) = r;
+          *reinterpret_cast<float4 *>(p.stream_o + slot * p.head_dim + col) = r;
         }
       }
-      named_barrier_sync(1, 128);
+      named_barrier_sync(1 + worker, 128);
     }
     w = next;
 #pragma unroll
@@ -486,104 +572,153 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
 
 // Rows that read the same keys (all rows of the call for the shared prefix;
 // one sequence's rows for its own part) are packed group by group into
-// 128-row MMA tiles, tile_rows = 128 / group batch rows to a tile.  One CTA
-// owns two tiles of one key head and a range of 128-key tiles:
-//   warp 0      loads: Q once, then K and V tiles through two-stage rings, box
+// 128-row MMA tiles, tile_rows = 128 / group batch rows to a tile, two tiles
+// to a unit.  As above, the 128-key tiles of all (row unit, head) units form a
+// line, the prefix's first, and each of the CTAs, one per SM, has an equal
+// piece of it:
+//   warp 0      loads: Q of a unit, K and V tiles through two-stage rings, box
 //               by box of gcd(page_size, 64) keys
 //   warp 1      S_t = Q_t K^T into TMEM, O_t += P_t V with P_t read from TMEM
 //               (it overwrites S_t as packed f16)
 //   warps 2-17  softmax: two warps per lane quarter of a tile, 64 keys each
-// so the tensor core works on one tile while the other's softmax runs.
+// so the tensor core works on one tile while the other's softmax runs, and a
+// unit's Q and first K tile load while the last unit's results are stored.
 constexpr int kTileRows = 128, kTileKeys = 128;
 constexpr int kTileBytes = 128 * 128 * 2, kTileHalf = kTileBytes / 2;
 constexpr int kTileThreads = 576, kTileSmem = 6 * kTileBytes + 1024;
 
-template <bool kPrefix>
+__device__ __forceinline__ int32_t first_row(const PagedAttnParams &p, int32_t b) {
+  return p.paged.row_offsets ? max(0, min(p.paged.row_offsets[b], (int32_t)p.rows)) : b;
+}
+
+// A CTA's place on the tile kernel's line: key tile i of the n of unit (row
+// unit, head h); `seq` < 0: the prefix, whose row units cover all rows.
+struct TileWalk {
+  int32_t seq, j, h, i, n;   // row unit j of its sequence (or of the prefix)
+  int32_t unit;              // own part: row units before it
+  int32_t rows, lo, hi;      // batch rows; keys [lo, hi)
+  int64_t row0, pos0;        // first batch row and (own part) its position
+  int64_t left;
+
+  __device__ __forceinline__ void own(const PagedAttnParams &p, int32_t b, int32_t row_unit) {
+    const int32_t begin = first_row(p, b), end = first_row(p, b + 1), per_unit = 2 * p.tile_rows;
+    seq = b;
+    j = row_unit;
+    row0 = begin + (int64_t)j * per_unit;
+    rows = (int32_t)max((int64_t)0, min((int64_t)per_unit, end - row0));
+    pos0 = (int64_t)p.paged.lengths[b] - (end - begin) + (row0 - begin);
+    lo = p.prefix;
+    hi = (int32_t)max((int64_t)0, min((int64_t)checked_length(p, b, false), pos0 + rows));
+    n = rows > 0 && hi > lo ? (hi + kTileKeys - 1) / kTileKeys - lo / kTileKeys : 0;
+  }
+  __device__ __forceinline__ void prefix(const PagedAttnParams &p, int32_t row_unit) {
+    const int32_t per_unit = 2 * p.tile_rows;
+    seq = -1;
+    j = row_unit;
+    row0 = (int64_t)j * per_unit;
+    rows = (int32_t)min((int64_t)per_unit, p.rows - row0);
+    pos0 = 0;
+    lo = 0;
+    hi = p.prefix;
+    n = (hi + kTileKeys - 1) / kTileKeys;
+  }
+  __device__ __forceinline__ static int32_t units(const PagedAttnParams &p, int32_t b) {
+    const int32_t per_unit = 2 * p.tile_rows;
+    return max(0, (first_row(p, b + 1) - first_row(p, b) + per_unit - 1) / per_unit);
+  }
+  // Key tiles of this unit that are this CTA's.
+  __device__ __forceinline__ int32_t here() const { return (int32_t)min((int64_t)(n - i), left); }
+  __device__ __forceinline__ int64_t slot_unit(const PagedAttnParams &p) const {
+    return seq < 0 ? (int64_t)h * p.prefix_units + j : (int64_t)(p.prefix_units + unit) * p.heads + h;
+  }
+  __device__ __forceinline__ void next(const PagedAttnParams &p) {
+    const int32_t count = here();
+    left -= count;
+    i += count;
+    if (i < n || left <= 0) return;
+    i = 0;
+    if (seq < 0) {  // units are in the order (head, row unit)
+      if (++j < p.prefix_units) {
+        prefix(p, j);
+        return;
+      }
+      if (++h < p.heads) {
+        prefix(p, 0);
+        return;
+      }
+      unit = -1;
+      j = 0;
+      h = 0;
+    } else if (++h < p.heads) {
+      return;
+    } else {
+      h = 0;
+      ++j;
+    }
+    // the next row unit with keys
+    ++unit;
+    if (seq < 0) seq = 0;
+    for (;; ++unit) {
+      while (j >= units(p, seq)) {
+        if (++seq >= p.paged.sequences) {
+          left = 0;
+          return;
+        }
+        j = 0;
+      }
+      own(p, seq, j);
+      if (n > 0) return;
+      ++j;
+    }
+  }
+};
+
+// One unit's share of a CTA's piece, as the load warp hands it to the others:
+// only that warp walks the line, which costs the softmax warps no registers.
+struct TileTask {
+  int64_t row0, pos0, slot;
+  int32_t rows, lo, hi, h, first, n;  // key tiles [first, first + n); n = 0: the piece is done
+  int32_t tiles;                      // row tiles in use
+  int32_t prefix, direct, store;
+  // V rows outside [lo, hi) of a chunk that has both kinds may hold anything
+  // and are zeroed in shared memory (0 * NaN is NaN); whole chunks outside are
+  // zero-filled by the TMA.
+  int32_t fix_first, fix_last;
+};
+
 __global__ void __launch_bounds__(kTileThreads, 1)
     paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedAttnParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *s_q = smem, *s_k = smem + 2 * kTileBytes, *s_v = smem + 4 * kTileBytes;
-  __shared__ uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_ready[2], v_fixed[2], o_final;
+  __shared__ uint64_t q_full, q_empty, k_full[2], v_full[2], k_empty[2], v_empty[2], v_fixed[2];  // per ring stage
+  __shared__ uint64_t s_full[2], p_ready[2], o_final[2], o_empty[2];                             // per row tile
   __shared__ uint32_t tmem_slot;
   __shared__ int aborted;
   __shared__ float x_max[2][2][kTileRows], x_sum[2][2][kTileRows];
   __shared__ int64_t scratch[kTileThreads / 32];
-  __shared__ int32_t found[2];
+  __shared__ int32_t found[5];
+  __shared__ uint64_t task_full[2], task_empty[2];
+  __shared__ TileTask tasks[2];
   volatile int *abort_flag = &aborted;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  // The unit: `rows` batch rows from row0 on (of sequence `seq` at position
-  // pos0, or of all sequences), key head h, share `split` of the key tiles of
-  // positions [lo, hi).
-  int32_t x = blockIdx.x;
-  const int32_t unit = x % p.row_units;
-  x /= p.row_units;
-  const int32_t h = x % p.heads, split = x / p.heads, splits = kPrefix ? p.prefix_splits : p.own_splits;
-  const int32_t per_unit = 2 * p.tile_rows;
-  int64_t row0 = (int64_t)unit * per_unit, pos0 = 0;
-  int32_t rows = 0, lo = 0, hi = 0, seq = 0;
-  if (kPrefix) {
-    rows = (int32_t)min((int64_t)per_unit, p.rows - row0);
-    hi = p.prefix;
-  } else {
-    // Sequence b has ceil(rows / per_unit) units.
-    auto first_row = [&](int32_t b) {
-      return p.paged.row_offsets ? max(0, min(p.paged.row_offsets[b], (int32_t)p.rows)) : b;
-    };
-    auto count = [&](int32_t b) { return max(0, (first_row(b + 1) - first_row(b) + per_unit - 1) / per_unit); };
-    if (threadIdx.x == 0) found[0] = -1;
-    __syncthreads();
-    block_sums<kTileThreads>(p.paged.sequences, scratch, count, [&](int32_t b, int64_t sum) {
-      if (unit >= sum && unit < sum + count(b)) {
-        found[0] = b;
-        found[1] = (int32_t)(unit - sum);
-      }
-    });
-    __syncthreads();
-    seq = found[0];
-    if (seq < 0) return;  // the grid is an upper bound
-    const int32_t begin = first_row(seq), end = first_row(seq + 1);
-    row0 = begin + (int64_t)found[1] * per_unit;
-    rows = (int32_t)min((int64_t)per_unit, end - row0);
-    const int32_t len = checked_length(p, seq, true);
-    pos0 = (int64_t)p.paged.lengths[seq] - (end - begin) + (row0 - begin);
-    lo = p.prefix;
-    hi = (int32_t)max((int64_t)0, min((int64_t)len, pos0 + rows));
-  }
-  const int32_t first = lo / kTileKeys, count = hi > lo ? (hi + kTileKeys - 1) / kTileKeys - first : 0;
-  const int32_t j_begin = first + (int32_t)((int64_t)count * split / splits);
-  const int32_t n_tiles = first + (int32_t)((int64_t)count * (split + 1) / splits) - j_begin;
-  float *part_o = kPrefix ? p.prefix_o : p.own_o;
-  float2 *part_ml = kPrefix ? p.prefix_ml : p.own_ml;
-  if (n_tiles == 0) {
-    // No keys: empty partials (O is not read where the maximum is -inf), or zero rows.
-    for (int32_t i = threadIdx.x; i < rows * p.group; i += kTileThreads) {
-      const int64_t head = (row0 + i / p.group) * p.q_heads + h * p.group + i % p.group;
-      if (!p.direct) {
-        part_ml[split * p.rows * p.q_heads + head] = make_float2(-INFINITY, 0.0f);
-      } else {
-        for (int d = 0; d < p.head_dim; d += 8)
-          *reinterpret_cast<uint4 *>(p.out + head * p.head_dim + d) = make_uint4(0u, 0u, 0u, 0u);
-      }
-    }
-    return;
-  }
-  const int tiles = rows > p.tile_rows ? 2 : 1;  // row tiles in use
-  const int halves = p.head_dim > 64 ? 2 : 1, k_steps = (p.head_dim + 15) / 16;
-
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1);
-    mbar_init(&o_final, 1);
+    mbar_init(&q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&v_full[i], 1);
       mbar_init(&k_empty[i], 1);
       mbar_init(&v_empty[i], 1);
+      mbar_init(&v_fixed[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_ready[i], 8);
-      mbar_init(&v_fixed[i], 1);
+      mbar_init(&o_final[i], 1);
+      mbar_init(&o_empty[i], 8);
+      mbar_init(&task_full[i], 1);
+      mbar_init(&task_empty[i], 17);  // the MMA thread and 16 softmax warps
     }
     aborted = 0;
     fence_barrier_init();
@@ -591,6 +726,91 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
+  // This CTA's piece of the line of W tiles, [W c / C, W (c + 1) / C).
+  const int64_t cta = blockIdx.x;
+  const int64_t ahead = (int64_t)p.prefix_units * p.heads * ((p.prefix + kTileKeys - 1) / kTileKeys);
+  // Row units (above 2^40) and key tiles of sequence b's own part, in one sum.
+  auto count = [&](int32_t b) {
+    const int32_t u = TileWalk::units(p, b);
+    int64_t sum = (int64_t)u << 40;
+    TileWalk w;
+    for (int32_t j = 0; j < u; ++j) {
+      w.own(p, b, j);
+      sum += w.n;
+    }
+    return sum;
+  };
+  int64_t total = 0;
+  int32_t share = p.sms;
+  if (p.stream) {
+    const int64_t own_tiles = block_sums<kTileThreads>(
+        p.paged.sequences, scratch, [&](int32_t b) { return StreamWalk::tiles(p, checked_length(p, b, false)); },
+        [](int32_t, int64_t) {});
+    share -= stream_sms(p, own_tiles);
+  }
+  if (p.tile_own) {
+    if (cta == 0)
+      for (int32_t b = threadIdx.x; b < p.paged.sequences; b += kTileThreads) checked_length(p, b, true);
+    total = block_sums<kTileThreads>(p.paged.sequences, scratch, count, [&](int32_t b, int64_t sum) {
+      if (cta != 0) return;
+      const int32_t base = (int32_t)(sum >> 40), u = TileWalk::units(p, b);
+      int64_t tiles = sum & ((1ll << 40) - 1);
+      p.unit_base[b] = base;
+      TileWalk w;
+      for (int32_t j = 0; j < u && base + j < p.max_units; ++j) {
+        p.unit_sums[base + j] = tiles;
+        w.own(p, b, j);
+        tiles += w.n;
+        p.unit_sums[base + j + 1] = tiles;
+      }
+    });
+  }
+  const int64_t line = ahead + (total & ((1ll << 40) - 1)) * p.heads, ctas = min((int64_t)share, line);
+  if (cta == 0 && threadIdx.x == 0) {
+    p.unit_sums[p.max_units + 1] = line;
+    p.unit_sums[p.max_units + 2] = ctas;
+  }
+  griddep_launch_dependents();
+  if (cta >= ctas) {  // no piece is empty
+    if (cta == 0) griddep_wait();
+    return;
+  }
+  const int64_t start = line * cta / ctas;
+  TileWalk walk;
+  walk.unit = -1;
+  if (start < ahead) {
+    walk.prefix(p, 0);
+    const int64_t u = start / walk.n;
+    walk.h = (int32_t)(u / p.prefix_units);
+    walk.prefix(p, (int32_t)(u % p.prefix_units));
+    walk.i = (int32_t)(start % walk.n);
+  } else {
+    __syncthreads();  // scratch is read before it is written again
+    block_sums<kTileThreads>(p.paged.sequences, scratch, count, [&](int32_t b, int64_t sum) {
+      int64_t at = start - ahead - (sum & ((1ll << 40) - 1)) * p.heads;
+      if (at < 0 || at >= (count(b) & ((1ll << 40) - 1)) * p.heads) return;
+      TileWalk w;
+      int32_t j = 0;
+      for (;; ++j) {
+        w.own(p, b, j);
+        if (at < (int64_t)w.n * p.heads) break;
+        at -= (int64_t)w.n * p.heads;
+      }
+      found[0] = b;
+      found[1] = j;
+      found[2] = (int32_t)(at / w.n);
+      found[3] = (int32_t)(at % w.n);
+      found[4] = (int32_t)(sum >> 40) + j;
+    });
+    __syncthreads();
+    walk.own(p, found[0], found[1]);
+    walk.h = found[2];
+    walk.i = found[3];
+    walk.unit = found[4];
+  }
+  walk.left = line * (cta + 1) / ctas - start;
+  const int halves = p.head_dim > 64 ? 2 : 1, k_steps = (p.head_dim + 15) / 16;
+
   if (warp == 1) {
     tmem_alloc(&tmem_slot, 512);
     tmem_relinquish();
@@ -599,77 +819,113 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;  // S_t at column t * 128, O_t at 256 + t * 128
-  // V rows outside [lo, hi) of a chunk that has both kinds may hold anything and
-  // are zeroed in shared memory (0 * NaN is NaN): in the first tile (0) and in
-  // the last one (1).  Whole chunks outside are zero-filled by the TMA.
-  const bool fix_first = j_begin * kTileKeys < lo && lo % p.chunk != 0;
-  const bool fix_last = (j_begin + n_tiles) * kTileKeys > hi && hi % p.chunk != 0;
-
   if (warp == 0) {
     const int chunks = kTileKeys / p.chunk, boxes = halves * chunks;
-    const int32_t *ids = kPrefix ? p.prefix_pages : p.paged.page_table + seq * p.paged.table_stride;
     bool ok = true;
-    int k_issued = 0, v_issued = 0;
-    if (lane == 0) {
-      mbar_arrive_expect_tx(&q_full, tiles * halves * p.tile_rows * p.group * 128);
-      for (int t = 0; t < tiles; ++t)
-        for (int half = 0; half < halves; ++half)
-          tma_load_4d(s_q + t * kTileBytes + half * kTileHalf, &tm_q, &q_full, half * 64, 0, h,
-                      (int32_t)row0 + t * p.tile_rows);
-    }
-    auto load = [&](uint8_t *base, const CUtensorMap *map, uint64_t *bar, int32_t key0) {
-      if (lane == 0) mbar_arrive_expect_tx(bar, halves * kTileHalf);
-      __syncwarp();
-      for (int i = lane; i < boxes; i += 32) {
-        const int chunk = i % chunks, half = i / chunks;
-        const int32_t pos = key0 + chunk * p.chunk;
-        tma_load_4d(base + half * kTileHalf + chunk * p.chunk * 128, map, bar, half * 64, pos % p.paged.page_size, h,
-                    page_of(p, ids, pos, lo, hi));
+    uint32_t unit = 0, k_issued = 0, v_issued = 0, q_issued = 0;
+    // Tasks are written two ahead of the last reader at most; after the last comes one with n = 0.
+    auto publish = [&](const TileTask &task, uint32_t index) {
+      const bool free = mbar_wait_bounded(&task_empty[index & 1], ((index >> 1) & 1) ^ 1, abort_flag);
+      if (free && lane == 0) {
+        tasks[index & 1] = task;
+        mbar_arrive(&task_full[index & 1]);
       }
+      return free;
     };
-    for (int j = 0; j < n_tiles && ok; ++j) {
-      const int st = j & 1;
-      const int32_t key0 = (j_begin + j) * kTileKeys;
-      if (!mbar_wait_bounded(&k_empty[st], ((j >> 1) & 1) ^ 1, abort_flag)) {
+    for (; walk.left > 0 && ok; walk.next(p), ++unit) {
+      TileTask task;
+      task.row0 = walk.row0;
+      task.pos0 = walk.pos0;
+      task.slot = walk.slot_unit(p) + cta;
+      task.rows = walk.rows;
+      task.lo = walk.lo;
+      task.hi = walk.hi;
+      task.h = walk.h;
+      task.n = walk.here();
+      task.first = walk.lo / kTileKeys + walk.i;
+      task.tiles = walk.rows > p.tile_rows ? 2 : 1;
+      task.prefix = walk.seq < 0;
+      task.direct = p.prefix == 0 && task.n == walk.n;
+      // (max_units holds for sorted row offsets; others write no partials past it)
+      task.store = walk.unit < p.max_units;
+      task.fix_first = task.first * kTileKeys < walk.lo && walk.lo % p.chunk != 0;
+      task.fix_last = (task.first + task.n) * kTileKeys > walk.hi && walk.hi % p.chunk != 0;
+      if (!publish(task, unit)) {
         ok = false;
         break;
       }
-      load(s_k + st * kTileBytes, &tm_k, &k_full[st], key0);
-      ++k_issued;
-      if (!mbar_wait_bounded(&v_empty[st], ((j >> 1) & 1) ^ 1, abort_flag)) {
-        ok = false;
-        break;
-      }
-      load(s_v + st * kTileBytes, &tm_v, &v_full[st], key0);
-      ++v_issued;
-      const bool is_last = j == n_tiles - 1;
-      if ((fix_first && j == 0) || (fix_last && is_last)) {
-        if (!mbar_wait_bounded(&v_full[st], (j >> 1) & 1, abort_flag)) {
+      const int32_t *ids = walk.seq < 0 ? p.prefix_pages : p.paged.page_table + walk.seq * p.paged.table_stride;
+      auto load = [&](uint8_t *base, const CUtensorMap *map, uint64_t *bar, int32_t key0) {
+        if (lane == 0) mbar_arrive_expect_tx(bar, halves * kTileHalf);
+        __syncwarp();
+        for (int i = lane; i < boxes; i += 32) {
+          const int chunk = i % chunks, half = i / chunks;
+          const int32_t pos = key0 + chunk * p.chunk;
+          tma_load_4d(base + half * kTileHalf + chunk * p.chunk * 128, map, bar, half * 64, pos % p.paged.page_size,
+                      walk.h, page_of(p, ids, pos, walk.lo, walk.hi));
+        }
+      };
+      for (int32_t j = 0; j < task.n; ++j) {
+        const int st = k_issued & 1;
+        const int32_t key0 = (task.first + j) * kTileKeys;
+        if (!mbar_wait_bounded(&k_empty[st], ((k_issued >> 1) & 1) ^ 1, abort_flag)) {
           ok = false;
           break;
         }
-        for (int i = lane; i < kTileKeys * halves * 8; i += 32) {
-          const int row = i / (halves * 8), half = (i >> 3) % halves;
-          if (key0 + row < lo || key0 + row >= hi)
-            *reinterpret_cast<uint4 *>(s_v + st * kTileBytes + half * kTileHalf + row * 128 + (i & 7) * 16) =
-                make_uint4(0u, 0u, 0u, 0u);
+        load(s_k + st * kTileBytes, &tm_k, &k_full[st], key0);
+        ++k_issued;
+        if (j == 0) {
+          // Q's buffer: the previous unit's S products are done
+          if (!mbar_wait_bounded(&q_empty, (unit & 1) ^ 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&q_full, task.tiles * halves * p.tile_rows * p.group * 128);
+            for (int t = 0; t < task.tiles; ++t)
+              for (int half = 0; half < halves; ++half)
+                tma_load_4d(s_q + t * kTileBytes + half * kTileHalf, &tm_q, &q_full, half * 64, 0, walk.h,
+                            (int32_t)walk.row0 + t * p.tile_rows);
+          }
+          ++q_issued;
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_fixed[fix_first && j == 0 ? 0 : 1]);
+        if (!mbar_wait_bounded(&v_empty[st], ((v_issued >> 1) & 1) ^ 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        load(s_v + st * kTileBytes, &tm_v, &v_full[st], key0);
+        ++v_issued;
+        if ((task.fix_first && j == 0) || (task.fix_last && j == task.n - 1)) {
+          if (!mbar_wait_bounded(&v_full[st], ((v_issued - 1) >> 1) & 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          for (int i = lane; i < kTileKeys * halves * 8; i += 32) {
+            const int row = i / (halves * 8), half = (i >> 3) % halves;
+            if (key0 + row < walk.lo || key0 + row >= walk.hi)
+              *reinterpret_cast<uint4 *>(s_v + st * kTileBytes + half * kTileHalf + row * 128 + (i & 7) * 16) =
+                  make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_fixed[st]);
+        }
       }
+    }
+    if (ok) {
+      TileTask done = {};
+      ok = publish(done, unit);
     }
     if (!ok) {
       if (lane == 0) record_device_error(p.err, ERR_KERNEL_PAGED_ATTENTION | ERR_SITE_PRODUCER);
       *abort_flag = 1;
+      // nothing leaves while copies into its shared memory are in flight
+      if (q_issued) mbar_wait_bounded(&q_full, (q_issued - 1) & 1, nullptr, 1000000000ull);
+      for (uint32_t i = k_issued > 2 ? k_issued - 2 : 0; i < k_issued; ++i)
+        mbar_wait_bounded(&k_full[i & 1], (i >> 1) & 1, nullptr, 1000000000ull);
+      for (uint32_t i = v_issued > 2 ? v_issued - 2 : 0; i < v_issued; ++i)
+        mbar_wait_bounded(&v_full[i & 1], (i >> 1) & 1, nullptr, 1000000000ull);
     }
-    // Nothing leaves while copies into its shared memory are in flight (at once
-    // unless a wait ran out above: the MMA warp has waited for all of them).
-    mbar_wait_bounded(&q_full, 0, nullptr, 1000000000ull);
-    for (int i = max(0, k_issued - 2); i < k_issued; ++i)
-      mbar_wait_bounded(&k_full[i & 1], (i >> 1) & 1, nullptr, 1000000000ull);
-    for (int i = max(0, v_issued - 2); i < v_issued; ++i)
-      mbar_wait_bounded(&v_full[i & 1], (i >> 1) & 1, nullptr, 1000000000ull);
   } else if (warp == 1) {
     if (lane == 0) {
       const uint32_t idesc_s = make_idesc(128, kTileKeys, 0, false, false);
@@ -688,40 +944,61 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         mma_commit(&s_full[t]);
       };
-      // Per key tile j: PV_t(j) as soon as P_t(j) is there, then S_t(j + 1) behind it.
-      bool ok = mbar_wait_bounded(&q_full, 0, abort_flag) && mbar_wait_bounded(&k_full[0], 0, abort_flag);
-      for (int t = 0; t < tiles && ok; ++t) issue_s(t, 0);
-      for (int j = 0; j < n_tiles && ok; ++j) {
-        const int st = j & 1;
-        const bool more = j + 1 < n_tiles, fix = (fix_first && j == 0) || (fix_last && !more);
-        const uint64_t vd = v_desc + (uint64_t)(st * (kTileBytes >> 4));
-        ok = fix ? mbar_wait_bounded(&v_fixed[fix_first && j == 0 ? 0 : 1], 0, abort_flag)
-                 : mbar_wait_bounded(&v_full[st], (j >> 1) & 1, abort_flag);
-        for (int t = 0; t < tiles && ok; ++t) {
-          if (!mbar_wait_bounded(&p_ready[t], j & 1, abort_flag)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
+      // Per key tile j: PV_t(j) as soon as P_t(j) is there, then S_t(j + 1)
+      // behind it.  A unit's first S products queue behind the last unit's last
+      // PV products, so its S tiles (which held the last P) are free by then.
+      bool ok = true;
+      uint32_t unit = 0, g = 0;          // units begun, key tiles done
+      uint32_t p_count[2] = {0, 0}, o_count[2] = {0, 0}, fixes[2] = {0, 0};
+      for (;; ++unit) {
+        ok = mbar_wait_bounded(&task_full[unit & 1], (unit >> 1) & 1, abort_flag);
+        if (!ok) break;
+        const TileTask &task = tasks[unit & 1];
+        const int tiles = task.tiles;
+        const int32_t n = task.n;
+        const bool fix_first = task.fix_first, fix_last = task.fix_last;
+        mbar_arrive(&task_empty[unit & 1]);
+        if (n == 0) break;
+        ok = mbar_wait_bounded(&k_full[g & 1], (g >> 1) & 1, abort_flag) && mbar_wait_bounded(&q_full, unit & 1, abort_flag);
+        if (!ok) break;
+        for (int t = 0; t < tiles; ++t) issue_s(t, g & 1);
+        if (n == 1) mma_commit(&q_empty);
+        for (int32_t j = 0; j < n && ok; ++j, ++g) {
+          const int st = g & 1;
+          const bool more = j + 1 < n;
+          const uint64_t vd = v_desc + (uint64_t)(st * (kTileBytes >> 4));
+          if ((fix_first && j == 0) || (fix_last && !more))
+            ok = mbar_wait_bounded(&v_fixed[st], fixes[st]++ & 1, abort_flag);
+          else
+            ok = mbar_wait_bounded(&v_full[st], (g >> 1) & 1, abort_flag);
+          for (int t = 0; t < tiles && ok; ++t) {
+            ok = mbar_wait_bounded(&p_ready[t], p_count[t]++ & 1, abort_flag);
+            // the last unit's O_t has been read out before this one's first PV_t
+            if (ok && j == 0 && o_count[t]) ok = mbar_wait_bounded(&o_empty[t], (o_count[t] - 1) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll
-          for (int k = 0; k < kTileKeys / 16; ++k)
-            mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, vd + (uint64_t)((k * 2048) >> 4), idesc_o,
-                       j > 0 || k > 0 ? 1u : 0u);
-          if (t == 0) {
-            // K's stage was last read by the S products that P_t(j) came from
-            mma_commit(&k_empty[st]);
-            if (more && !mbar_wait_bounded(&k_full[st ^ 1], ((j + 1) >> 1) & 1, abort_flag)) {
-              ok = false;
-              break;
+            for (int k = 0; k < kTileKeys / 16; ++k)
+              mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, vd + (uint64_t)((k * 2048) >> 4), idesc_o,
+                         j > 0 || k > 0 ? 1u : 0u);
+            if (t == 0) {
+              // K's stage was last read by the S products that P_t(j) came from
+              mma_commit(&k_empty[st]);
+              if (more && !mbar_wait_bounded(&k_full[st ^ 1], ((g + 1) >> 1) & 1, abort_flag)) {
+                ok = false;
+                break;
+              }
             }
+            if (t == tiles - 1) mma_commit(&v_empty[st]);
+            if (more) issue_s(t, st ^ 1);
+            else mma_commit(&o_final[t]);
           }
-          if (t == tiles - 1) mma_commit(&v_empty[st]);
-          if (more) issue_s(t, st ^ 1);
+          if (ok && j + 2 == n) mma_commit(&q_empty);
         }
+        if (!ok) break;
+        for (int t = 0; t < tiles; ++t) ++o_count[t];
       }
-      if (ok) {
-        mma_commit(&o_final);
-      } else {
+      if (!ok) {
         record_device_error(p.err, ERR_KERNEL_PAGED_ATTENTION | ERR_SITE_MMA);
         *abort_flag = 1;
       }
@@ -733,33 +1010,54 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_col = tmem + lane_off + t * 128, o_col = tmem + lane_off + 256 + t * 128 + half * 64;
     const float c = p.scale_log2;
-    if (t < tiles) {
-      // This row's keys: [lo, limit).
-      const int32_t local = t * p.tile_rows + row / p.group;  // batch row within the unit
-      const bool row_ok = row < p.tile_rows * p.group && local < rows;
-      const int64_t token = row0 + local;
-      int64_t limit = 0;
-      if (row_ok) {
-        if (kPrefix) {
-          PagedRow r;
-          limit = paged_row(p.paged, token, r) ? min((int64_t)hi, r.position + 1) : 0;
-        } else {
-          limit = min((int64_t)hi, pos0 + local + 1);
-        }
+    const int32_t local = t * p.tile_rows + row / p.group;  // batch row within a unit
+    const bool in_tile = row < p.tile_rows * p.group;
+    bool ok = true;
+    uint32_t g = 0, unit = 0;  // key tiles and units of this row tile so far
+    for (uint32_t index = 0;; ++index) {
+      // (the two warps of a lane quarter go on or stop together: they meet at barriers below)
+      const bool late = ok && !mbar_wait_bounded(&task_full[index & 1], (index >> 1) & 1, abort_flag);
+      if (barrier_any(bar_id, 64, late || !ok)) {
+        ok = false;
+        break;
       }
-      bool ok = true;
+      const TileTask &task = tasks[index & 1];
+      const int32_t n = task.n;
+      if (n == 0) break;
+      if (t >= task.tiles) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&task_empty[index & 1]);
+        continue;
+      }
+      // This row's keys: [lo, limit).
+      const bool row_ok = in_tile && local < task.rows && task.store;
+      const int64_t token = task.row0 + local;
+      const int32_t lo = task.lo, first = task.first;
+      const bool direct = task.direct;
+      const int64_t head = token * p.q_heads + task.h * p.group + row % p.group;
+      const int32_t slot_row = t * p.tile_rows * p.group + row;
+      const int64_t slot = task.slot;
+      int32_t limit = 0;
+      if (row_ok) {
+        PagedRow r;
+        int64_t position = task.pos0 + local;
+        if (task.prefix) position = paged_row(p.paged, token, r) ? r.position : -1;
+        limit = (int32_t)max((int64_t)0, min((int64_t)task.hi, position + 1));
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&task_empty[index & 1]);
       float m = -INFINITY, l = 0.0f;
-      for (int j = 0; j < n_tiles; ++j) {
+      for (int32_t j = 0; j < n; ++j, ++g) {
         // (a wait that ran out is not left early: the barriers below need every warp)
-        if (ok && !mbar_wait_bounded(&s_full[t], j & 1, abort_flag)) ok = false;
+        if (ok && !mbar_wait_bounded(&s_full[t], g & 1, abort_flag)) ok = false;
         tc_fence_after();
-        const int32_t key0 = (j_begin + j) * kTileKeys + half * 64;
+        const int32_t key0 = (first + j) * kTileKeys + half * 64;
         uint32_t a[32], b[32];
         tmem_ld_32x32b_x32(s_col + half * 64, a);
         tmem_ld_32x32b_x32(s_col + half * 64 + 32, b);
         tmem_wait_ld(a);
         tmem_regs_fence(b);
-        const int from = max(0, lo - key0), to = (int)max((int64_t)0, min((int64_t)64, limit - key0));
+        const int from = lo - key0, to = limit - key0;
         if (__any_sync(0xffffffffu, from > 0 || to < 64)) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
@@ -799,11 +1097,21 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           const float x0 = __uint_as_float(i < 16 ? a[2 * i] : b[2 * i - 32]);
           const float x1 = __uint_as_float(i < 16 ? a[2 * i + 1] : b[2 * i - 31]);
           const uint64_t tt = f2_fma(f2_pack(x0, x1), c2, nmc2);
-          float t0, t1;
-          f2_unpack(tt, t0, t1);
-          const float p0 = ex2_approx(t0), p1 = ex2_approx(t1);
-          sum2 = f2_add(sum2, f2_pack(p0, p1));
-          packed[i] = pack_h2(p0, p1);
+          // (one pair in three on the FMA pipe: the exponential unit alone would bound the kernel)
+          uint64_t pp;
+          float p0, p1;
+          if (i % 3 == 2) {
+            pp = exp2_poly2(tt);
+            f2_unpack(pp, p0, p1);
+          } else {
+            float t0, t1;
+            f2_unpack(tt, t0, t1);
+            p0 = ex2_approx(t0);
+            p1 = ex2_approx(t1);
+            pp = f2_pack(p0, p1);
+          }
+          sum2 = f2_add(sum2, pp);
+          packed[i] = to_h2(p0, p1);
         }
         tmem_st_32x32b_x32(s_col + half * 32, packed);
         float s0, s1;
@@ -829,46 +1137,53 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       x_sum[t][half][row] = l;
       named_barrier_sync(bar_id, 64);
       l += x_sum[t][half ^ 1][row];
-      if (ok && !mbar_wait_bounded(&o_final, 0, abort_flag)) ok = false;
+      if (ok && !mbar_wait_bounded(&o_final[t], unit & 1, abort_flag)) ok = false;
+      ++unit;
       tc_fence_after();
-      const int64_t head = token * p.q_heads + h * p.group + row % p.group;
-      const int64_t slot = split * p.rows * p.q_heads + head;
-      if (row_ok && !p.direct && half == 0) part_ml[slot] = make_float2(m == -INFINITY ? m : m * c, l);
+      if (row_ok && !direct && half == 0) p.tile_ml[slot * p.tile_slot_rows + slot_row] = make_float2(m == -INFINITY ? m : m * c, l);
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
       for (int ch = 0; ch < 2; ++ch) {
         uint32_t r[32];
         tmem_ld_32x32b_x32(o_col + ch * 32, r);
         tmem_wait_ld(r);
+        if (ch == 1) {
+          // O_t is read out: the next unit's first PV may overwrite it
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&o_empty[t]);
+        }
         const int col0 = half * 64 + ch * 32;
         if (!row_ok) continue;
-        if (p.direct) {
+        if (direct) {
           // (a row without keys: O is 0 * V, which a non-finite V of another row's keys makes NaN)
           uint16_t *o = p.out + head * p.head_dim + col0;
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             if (col0 + i >= p.head_dim) break;
             uint4 v;
-            v.x = pack_h2(__uint_as_float(r[i]) * inv, __uint_as_float(r[i + 1]) * inv);
-            v.y = pack_h2(__uint_as_float(r[i + 2]) * inv, __uint_as_float(r[i + 3]) * inv);
-            v.z = pack_h2(__uint_as_float(r[i + 4]) * inv, __uint_as_float(r[i + 5]) * inv);
-            v.w = pack_h2(__uint_as_float(r[i + 6]) * inv, __uint_as_float(r[i + 7]) * inv);
+            v.x = to_h2(__uint_as_float(r[i]) * inv, __uint_as_float(r[i + 1]) * inv);
+            v.y = to_h2(__uint_as_float(r[i + 2]) * inv, __uint_as_float(r[i + 3]) * inv);
+            v.z = to_h2(__uint_as_float(r[i + 4]) * inv, __uint_as_float(r[i + 5]) * inv);
+            v.w = to_h2(__uint_as_float(r[i + 6]) * inv, __uint_as_float(r[i + 7]) * inv);
             *reinterpret_cast<uint4 *>(o + i) = l == 0.0f ? make_uint4(0u, 0u, 0u, 0u) : v;
           }
         } else {
-          float *o = part_o + slot * p.head_dim + col0;
+          // [slot][dim / 4][row][4]: a lane holds a row, so a warp's 16-byte stores are
+          // neighbours (row by row they cost 15 us a unit on all SMs, half-filled sectors)
+          float *o = p.tile_o + ((slot * (p.head_dim >> 2) + (col0 >> 2)) * p.tile_slot_rows + slot_row) * 4;
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
             if (col0 + i >= p.head_dim) break;
-            *reinterpret_cast<float4 *>(o + i) = make_float4(__uint_as_float(r[i]), __uint_as_float(r[i + 1]),
+            *reinterpret_cast<float4 *>(o + (int64_t)i * p.tile_slot_rows) = make_float4(__uint_as_float(r[i]), __uint_as_float(r[i + 1]),
                                                              __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
           }
         }
       }
-      if (!ok) {
-        if (lane == 0) record_device_error(p.err, ERR_KERNEL_PAGED_ATTENTION | ERR_SITE_EPILOGUE);
-        *abort_flag = 1;
-      }
+    }
+    if (!ok) {
+      if (lane == 0) record_device_error(p.err, ERR_KERNEL_PAGED_ATTENTION | ERR_SITE_EPILOGUE);
+      *abort_flag = 1;
     }
   }
   tc_fence_before();
@@ -877,106 +1192,170 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  // The join waits for this grid alone: it ends after the stream kernel's, with which it runs.
+  if (cta == 0) griddep_wait();
 }
 
 // ---- the partial results' sum -----------------------------------------------------
 
-// One warp per row and query head, four dims per lane: the partials' weights
-// 2^(m - max m), then the weighted sum of their O over the weighted sum of l.
-__global__ void __launch_bounds__(256) paged_combine_kernel(const __grid_constant__ PagedAttnParams p) {
-  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const int64_t row = unit / p.q_heads;
-  const int32_t head = (int32_t)(unit - row * p.q_heads);
-  if (row >= p.rows) return;
-  if (p.paged.row_offsets && row >= p.paged.row_offsets[p.paged.sequences]) return;  // padding
-  if (p.paged.row_offsets && row < p.paged.row_offsets[0]) return;
-  // Own partials: slots own0 + i * own_step.
-  int64_t own0 = row * p.q_heads + head, own_step = p.rows * p.q_heads;
-  int32_t own_n = p.own_splits;
-  if (p.stream_ctas) {
-    const int64_t before = p.tile_sums[row], n = p.tile_sums[row + 1] - before;
-    const int64_t line = p.tile_sums[p.paged.sequences] * p.heads, ctas = min((int64_t)p.stream_ctas, line);
-    const int32_t kv = head / p.group;
-    own_n = 0;
-    if (n > 0) {
-      // CTA c has tiles [line c / C, line (c + 1) / C): tile t is c = ((t + 1) C - 1) / line's
-      const int64_t t0 = before * p.heads + kv * n;
-      const int64_t c0 = ((t0 + 1) * ctas - 1) / line, c1 = ((t0 + n) * ctas - 1) / line;
-      if (c0 == c1 && p.prefix == 0) return;  // written by that CTA
-      own_n = (int32_t)(c1 - c0 + 1);
-      own0 = (row * p.heads + kv + c0) * p.group + head % p.group;
-      own_step = p.group;
-    }
+// A block joins 8 neighbouring rows of one key head (batch row, head of the
+// group), a thread four dims of one of them: so 16-byte reads are neighbours
+// row by row (tile slots) or dim by dim (stream slots).  A row's partials are
+// the pieces of its prefix unit and those of its own unit, both runs of slots.
+template <int32_t N>
+struct Number {
+  static constexpr int32_t value = N;
+};
+
+struct Pieces {
+  int64_t slot;    // of the first
+  int32_t count, row;
+};
+// Pieces of unit `unit`, tiles [first, first + n) of a line of `line` tiles:
+// CTA c has [line c / C, line (c + 1) / C), so tile t is c = ((t + 1) C - 1) / line's.
+__device__ __forceinline__ Pieces pieces_of(int64_t line, int64_t c, int64_t first, int64_t n, int64_t unit,
+                                            int32_t row) {
+  Pieces r = {0, 0, row};
+  if (n <= 0) return r;
+  int32_t c0, c1;
+  if (line * c < (1ll << 31)) {  // (32-bit divisions: a quarter of the time)
+    c0 = (int32_t)(((uint32_t)(first + 1) * (uint32_t)c - 1) / (uint32_t)line);
+    c1 = (int32_t)(((uint32_t)(first + n) * (uint32_t)c - 1) / (uint32_t)line);
+  } else {
+    c0 = (int32_t)(((first + 1) * c - 1) / line);
+    c1 = (int32_t)(((first + n) * c - 1) / line);
   }
-  const int64_t pre0 = row * p.q_heads + head, pre_step = p.rows * p.q_heads;
-  float top = -INFINITY;
-  for (int32_t i = lane; i < p.prefix_splits; i += 32) top = fmaxf(top, p.prefix_ml[pre0 + i * pre_step].x);
-  for (int32_t i = lane; i < own_n; i += 32) top = fmaxf(top, p.own_ml[own0 + i * own_step].x);
-#pragma unroll
-  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  // (in bounds whatever the sums of unsorted row offsets are)
+  c0 = max(0, min(c0, (int32_t)c - 1));
+  c1 = max(c0, min(c1, (int32_t)c - 1));
+  r.slot = unit + c0;
+  r.count = c1 - c0 + 1;
+  return r;
+}
+
+__global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_constant__ PagedAttnParams p) {
+  const int32_t dim = (threadIdx.x >> 3) * 4;
+  const uint32_t index = blockIdx.x * 8 + (threadIdx.x & 7), row = index / (uint32_t)p.group;
+  const int32_t kv = blockIdx.y, in_group = (int32_t)(index - row * (uint32_t)p.group);
+  const int32_t stream_keys = p.stream_prefix ? (p.prefix + kStreamKeys - 1) / kStreamKeys : 0;
+  __shared__ Pieces shared_pieces[2][8];  // own, prefix
+  griddep_wait();
+  // One thread per row and kind finds the pieces.
+  if ((threadIdx.x & 31) < 8 && threadIdx.x < 64) {
+    const bool prefix = threadIdx.x >= 32;
+    Pieces r = {0, -1, 0};
+    PagedRow where;
+    if (row < p.rows && paged_row(p.paged, row, where)) {
+      r.count = 0;
+      const int32_t tile_keys = (p.prefix + kTileKeys - 1) / kTileKeys, per_unit = 2 * p.tile_rows;
+      if (prefix && stream_keys) {
+        const int64_t line = (int64_t)stream_keys * p.heads + p.stream_sums[p.paged.sequences] * p.heads;
+        r = pieces_of(line, p.stream_sums[p.paged.sequences + 1], (int64_t)kv * stream_keys, stream_keys, kv, (int32_t)index);
+      } else if (prefix && p.prefix_units) {
+        const int32_t unit = kv * p.prefix_units + (int32_t)row / per_unit;
+        r = pieces_of(p.unit_sums[p.max_units + 1], p.unit_sums[p.max_units + 2], (int64_t)unit * tile_keys, tile_keys, unit,
+                      (int32_t)row % per_unit * p.group + in_group);
+      } else if (!prefix && p.stream) {
+        const int64_t before = p.stream_sums[row], n = p.stream_sums[row + 1] - before;
+        const int64_t ahead = (int64_t)stream_keys * p.heads, line = ahead + p.stream_sums[p.paged.sequences] * p.heads;
+        r = pieces_of(line, p.stream_sums[p.paged.sequences + 1], ahead + before * p.heads + kv * n, n,
+                      (int64_t)((int32_t)row + p.stream_prefix) * p.heads + kv, in_group);
+      } else if (!prefix && p.tile_own) {
+        const int32_t place = (int32_t)row - first_row(p, where.sequence);
+        const int32_t unit = p.unit_base[where.sequence] + place / per_unit;
+        if (unit < p.max_units) {
+          const int64_t before = p.unit_sums[unit], n = p.unit_sums[unit + 1] - before;
+          r = pieces_of(p.unit_sums[p.max_units + 1], p.unit_sums[p.max_units + 2],
+                        ((int64_t)p.prefix_units * tile_keys + before) * p.heads + kv * n, n,
+                        (int64_t)(p.prefix_units + unit) * p.heads + kv, place % per_unit * p.group + in_group);
+        }
+      }
+    }
+    shared_pieces[prefix][threadIdx.x & 7] = r;
+  }
+  __syncthreads();
+  const Pieces own = shared_pieces[0][threadIdx.x & 7], pre = shared_pieces[1][threadIdx.x & 7];
+  if (own.count < 0 || dim >= p.head_dim) return;  // padding
+  if (p.prefix == 0 && own.count == 1) return;  // the whole unit was one CTA's, which wrote the result
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float l = 0.0f;
-  const bool mine = lane * 4 < p.head_dim;
-  auto add = [&](const float *part, const float2 *ml, int64_t slot) {
-    const float2 s = ml[slot];
-    if (s.x == -INFINITY) return;
-    const float w = ex2_approx(s.x - top);
-    l += w * s.y;
-    if (mine) {
-      const float4 x = *reinterpret_cast<const float4 *>(part + slot * p.head_dim + lane * 4);
-      o.x += w * x.x;
-      o.y += w * x.y;
-      o.z += w * x.z;
-      o.w += w * x.w;
+  float l = 0.0f, top = -INFINITY;
+  // `n` partials' loads are issued before the first is used, with no branch between them.
+  auto join = [&](const Pieces &r, bool stream, auto n) {
+    constexpr int32_t N = decltype(n)::value;
+    const int32_t rows = stream ? p.stream_rows : p.tile_slot_rows;
+    const float2 *ml = (stream ? p.stream_ml : p.tile_ml) + r.slot * rows + r.row;
+    const float *part = stream ? p.stream_o + (r.slot * rows + r.row) * p.head_dim + dim
+                               : p.tile_o + ((r.slot * (p.head_dim >> 2) + (dim >> 2)) * rows + r.row) * 4;
+    const int64_t step = (int64_t)rows * p.head_dim;
+    for (int32_t i = 0; i < r.count; i += N) {
+      float2 s[N];
+      float4 v[N];
+      float t = top;
+#pragma unroll
+      for (int32_t x = 0; x < N; ++x) {
+        s[x] = make_float2(-INFINITY, 0.0f);
+        v[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (i + x < r.count) {
+          s[x] = ml[(int64_t)(i + x) * rows];
+          v[x] = *reinterpret_cast<const float4 *>(part + (i + x) * step);
+        }
+      }
+#pragma unroll
+      for (int32_t x = 0; x < N; ++x) t = fmaxf(t, s[x].x);
+      if (t == -INFINITY) continue;  // no keys
+      const float a = ex2_approx(top - t);
+      top = t;
+      l *= a;
+      o.x *= a;
+      o.y *= a;
+      o.z *= a;
+      o.w *= a;
+#pragma unroll
+      for (int32_t x = 0; x < N; ++x) {
+        if (s[x].x == -INFINITY) continue;  // (its O was not written)
+        const float w = ex2_approx(s[x].x - t);
+        l = fmaf(s[x].y, w, l);
+        o.x = fmaf(v[x].x, w, o.x);
+        o.y = fmaf(v[x].y, w, o.y);
+        o.z = fmaf(v[x].z, w, o.z);
+        o.w = fmaf(v[x].w, w, o.w);
+      }
     }
   };
-#pragma unroll 4
-  for (int32_t i = 0; i < p.prefix_splits; ++i) add(p.prefix_o, p.prefix_ml, pre0 + i * pre_step);
-#pragma unroll 2
-  for (int32_t i = 0; i < own_n; ++i) add(p.own_o, p.own_ml, own0 + i * own_step);
-  if (!mine) return;
+  if (pre.count > 2) join(pre, stream_keys != 0, Number<4>());
+  else join(pre, stream_keys != 0, Number<2>());
+  join(own, p.stream != 0, Number<2>());
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint2 v;
-  v.x = pack_h2(o.x * inv, o.y * inv);
-  v.y = pack_h2(o.z * inv, o.w * inv);
-  *reinterpret_cast<uint2 *>(p.out + (row * p.q_heads + head) * p.head_dim + lane * 4) = v;
+  v.x = to_h2(o.x * inv, o.y * inv);
+  v.y = to_h2(o.z * inv, o.w * inv);
+  *reinterpret_cast<uint2 *>(p.out + ((int64_t)row * p.q_heads + kv * p.group + in_group) * p.head_dim + dim) = v;
 }
 
 // ---- host ---------------------------------------------------------------------------
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Key tiles split over `splits` CTAs per unit: the smallest time of whole waves,
-// counting a CTA's start and result as two tiles.
-int32_t splits_for(int64_t units, int64_t key_tiles) {
-  const int64_t sms = sm_count();
-  int64_t best = 1, cost = -1;
-  for (int64_t s = 1; s <= key_tiles && s <= 64 && (s == 1 || units * s <= 4 * sms); ++s) {
-    const int64_t c = ceil_div(units * s, sms) * (ceil_div(key_tiles, s) + 2);
-    if (cost < 0 || c < cost) {
-      best = s;
-      cost = c;
-    }
-  }
-  return (int32_t)best;
-}
-
 // How a call is cut up, from sizes the host knows, and its workspace.
 struct PagedPlan {
-  bool stream;             // single rows, group <= 16: paged_stream_kernel
-  bool own_direct;         // one partial per row: the tile kernel writes the result
-  int32_t stream_ctas, own_splits, prefix_splits, tile_rows;
-  int64_t own_units, prefix_units;
-  uint64_t own_o, own_ml, prefix_o, prefix_ml, tile_sums, bytes;
+  bool stream, stream_prefix;  // the stream kernel takes single rows, and their prefix if all fit one m16 tile
+  bool tile, tile_own;         // the tile kernel runs; takes the own parts
+  int32_t sms, stream_rows, tile_rows, tile_slot_rows;
+  int64_t prefix_units, max_units;
+  uint64_t stream_o, stream_ml, stream_sums, tile_o, tile_ml, unit_sums, unit_base, bytes;
 };
 
 PagedPlan paged_plan(int64_t rows, int64_t sequences, int64_t q_heads, int64_t heads, int64_t head_dim,
                      int64_t prefix_rows, bool ragged) {
   PagedPlan plan = {};
   const int64_t group = q_heads / heads;
+  plan.sms = sm_count();
   plan.stream = !ragged && group <= 16;
+  plan.tile_own = !plan.stream;
+  plan.stream_prefix = plan.stream && prefix_rows > 0 && rows * group <= 16;
   plan.tile_rows = (int32_t)(kTileRows / group);
+  plan.tile_slot_rows = (int32_t)(2 * plan.tile_rows * group);
+  plan.stream_rows = (int32_t)(plan.stream_prefix ? rows * group : group);
   const int64_t per_unit = 2 * plan.tile_rows;
   uint64_t at = 0;
   auto take = [&](uint64_t bytes) {
@@ -984,29 +1363,25 @@ PagedPlan paged_plan(int64_t rows, int64_t sequences, int64_t q_heads, int64_t h
     at += (bytes + 255) & ~uint64_t(255);
     return here;
   };
-  int64_t own_slots;
   if (plan.stream) {
-    plan.stream_ctas = 2 * sm_count();
-    plan.own_splits = 0;
-    own_slots = (sequences * heads + plan.stream_ctas) * group;
-    plan.tile_sums = take((sequences + 1) * 8);
-  } else {
-    plan.own_units = ragged ? rows / per_unit + sequences : sequences;
-    if (plan.own_units > rows) plan.own_units = rows;
-    // how many keys there are is not known here: as many CTAs as there are SMs
-    const int64_t want = sm_count() / (plan.own_units * heads > 0 ? plan.own_units * heads : 1);
-    plan.own_splits = (int32_t)(want < 1 ? 1 : want > 32 ? 32 : want);
-    plan.own_direct = plan.own_splits == 1 && prefix_rows == 0;
-    own_slots = plan.own_direct ? 0 : plan.own_splits * rows * q_heads;
+    const int64_t slots =
+        ((sequences + (plan.stream_prefix ? 1 : 0)) * heads + kStreamWorkers * plan.sms) * plan.stream_rows;
+    plan.stream_o = take(slots * head_dim * 4);
+    plan.stream_ml = take(slots * 8);
+    plan.stream_sums = take((sequences + 2) * 8);
   }
-  plan.own_o = take(own_slots * head_dim * 4);
-  plan.own_ml = take(own_slots * 8);
-  if (prefix_rows > 0) {
-    plan.prefix_units = ceil_div(rows, per_unit);
-    plan.prefix_splits = splits_for(plan.prefix_units * heads, ceil_div(prefix_rows, kTileKeys));
-    const int64_t slots = plan.prefix_splits * rows * q_heads;
-    plan.prefix_o = take(slots * head_dim * 4);
-    plan.prefix_ml = take(slots * 8);
+  if (prefix_rows > 0 && !plan.stream_prefix) plan.prefix_units = ceil_div(rows, per_unit);
+  if (plan.tile_own) {
+    plan.max_units = rows / per_unit + sequences;
+    if (plan.max_units > rows) plan.max_units = rows;
+  }
+  if (plan.prefix_units || plan.tile_own) {
+    plan.tile = true;
+    const int64_t slots = ((plan.prefix_units + plan.max_units) * heads + plan.sms) * plan.tile_slot_rows;
+    plan.tile_o = take(slots * head_dim * 4);
+    plan.tile_ml = take(slots * 8);
+    plan.unit_sums = take((plan.max_units + 3) * 8);
+    plan.unit_base = take(sequences * 4);
   }
   plan.bytes = at > 256 ? at : 256;
   return plan;
@@ -1094,20 +1469,26 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
   p.prefix = (int32_t)prefix_rows;
   p.chunk = gcd(cache->page_size, kStreamKeys);
   p.scale_log2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float)d)) * 1.4426950408889634f;
-  p.own_o = reinterpret_cast<float *>(ws + plan.own_o);
-  p.own_ml = reinterpret_cast<float2 *>(ws + plan.own_ml);
-  p.prefix_o = reinterpret_cast<float *>(ws + plan.prefix_o);
-  p.prefix_ml = reinterpret_cast<float2 *>(ws + plan.prefix_ml);
-  p.tile_sums = reinterpret_cast<int64_t *>(ws + plan.tile_sums);
-  p.stream_ctas = plan.stream_ctas;
-  p.own_splits = plan.own_splits;
-  p.prefix_splits = plan.prefix_splits;
+  p.stream_o = reinterpret_cast<float *>(ws + plan.stream_o);
+  p.stream_ml = reinterpret_cast<float2 *>(ws + plan.stream_ml);
+  p.stream_sums = reinterpret_cast<int64_t *>(ws + plan.stream_sums);
+  p.stream_rows = plan.stream_rows;
+  p.stream = plan.stream;
+  p.sms = plan.sms;
+  p.stream_prefix = plan.stream_prefix;
+  p.tile_o = reinterpret_cast<float *>(ws + plan.tile_o);
+  p.tile_ml = reinterpret_cast<float2 *>(ws + plan.tile_ml);
+  p.unit_sums = reinterpret_cast<int64_t *>(ws + plan.unit_sums);
+  p.unit_base = reinterpret_cast<int32_t *>(ws + plan.unit_base);
+  p.tile_slot_rows = plan.tile_slot_rows;
+  p.tile = plan.tile;
+  p.tile_own = plan.tile_own;
+  p.prefix_units = (int32_t)plan.prefix_units;
+  p.max_units = (int32_t)plan.max_units;
   p.tile_rows = plan.tile_rows;
   p.err = device_error_word();
-  const int64_t own_grid = plan.own_units * p.heads * plan.own_splits;
-  const int64_t prefix_grid = plan.prefix_units * p.heads * plan.prefix_splits, heads_all = p.rows * q_heads;
-  IPUC_CHECK_ARG(own_grid < (1ll << 31) && prefix_grid < (1ll << 31) && heads_all < (1ll << 31),
-                 "paged_attention: extent too large");
+  const int64_t tasks = p.rows * q_heads;
+  IPUC_CHECK_ARG(tasks < (1ll << 31) && plan.max_units < (1ll << 23), "paged_attention: extent too large");
   CUtensorMap tm_q, tm_k, tm_v;
   st = make_map_paged(&tm_k, cache->keys, d, cache->page_size, cache->heads, cache->pages, cache->row_stride,
                       cache->head_stride, cache->page_stride, p.chunk, 1);
@@ -1115,35 +1496,36 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
   st = make_map_paged(&tm_v, cache->values, d, cache->page_size, cache->heads, cache->pages, cache->row_stride,
                       cache->head_stride, cache->page_stride, p.chunk, 1);
   if (st != IPUC_OK) return st;
-  if (!plan.stream || prefix_rows > 0) {
+  if (plan.tile) {
     st = make_map_paged(&tm_q, q, d, p.group, cache->heads, p.rows, d, p.group * d, q_stride, p.group, p.tile_rows);
     if (st != IPUC_OK) return st;
   }
-  if (plan.stream) {
-    auto launch = [&](auto kernel, int bytes) -> ipuc_status {
-      IPUC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-      kernel<<<plan.stream_ctas, kStreamThreads, bytes, stream>>>(tm_k, tm_v, p);
-      return check_launch("paged_stream_kernel");
-    };
-    st = d > 64 ? launch(paged_stream_kernel<128>, stream_smem_bytes<128>())
-                : launch(paged_stream_kernel<64>, stream_smem_bytes<64>());
-    if (st != IPUC_OK) return st;
-  }
-  auto tiles = [&](auto kernel, int64_t grid, int32_t units, bool direct) -> ipuc_status {
-    IPUC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmem));
-    p.row_units = units;
-    p.direct = direct;
-    kernel<<<(unsigned)grid, kTileThreads, kTileSmem, stream>>>(tm_q, tm_k, tm_v, p);
-    return check_launch("paged_tile_kernel");
+  // The kernels after the first start early (programmatic dependent launch):
+  // the tile kernel beside the stream kernel, on the SMs that leaves it; the
+  // join waits for both.
+  auto launch = [&](auto kernel, dim3 grid, int threads, int bytes, bool first, auto... args) -> ipuc_status {
+    if (bytes) IPUC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = first ? 0 : 1;
+    IPUC_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    return check_launch("paged_attention");
   };
-  if (!plan.stream) {
-    st = tiles(paged_tile_kernel<false>, own_grid, (int32_t)plan.own_units, plan.own_direct);
-    if (st != IPUC_OK || plan.own_direct) return st;
-  }
-  if (prefix_rows > 0) {
-    st = tiles(paged_tile_kernel<true>, prefix_grid, (int32_t)plan.prefix_units, false);
+  if (plan.stream) {
+    st = d > 64 ? launch(paged_stream_kernel<128>, p.sms, kStreamThreads, stream_smem_bytes<128>(), true, tm_k, tm_v, p)
+                : launch(paged_stream_kernel<64>, p.sms, kStreamThreads, stream_smem_bytes<64>(), true, tm_k, tm_v, p);
     if (st != IPUC_OK) return st;
   }
-  paged_combine_kernel<<<(unsigned)((heads_all + 7) / 8), 256, 0, stream>>>(p);
-  return check_launch("paged_combine_kernel");
+  if (plan.tile) {
+    st = launch(paged_tile_kernel, p.sms, kTileThreads, kTileSmem, !plan.stream, tm_q, tm_k, tm_v, p);
+    if (st != IPUC_OK) return st;
+  }
+  return launch(paged_combine_kernel, dim3((unsigned)ceil_div(p.rows * p.group, 8), (unsigned)p.heads), 256, 0, false, p);
 }
