@@ -59,6 +59,31 @@ using namespace sm100;
 // Both factors cancel in O / l as long as every partial result has them.
 constexpr float kLazy = 8.0f, kShift = 4.0f;
 
+// What loading a unit's queries and storing its result costs, in key tiles:
+// measured 5-6 us against 2.5 for a tile of the tile kernel, 2 us against 1.2
+// of the stream kernel.  With 0, pieces of many short units ended last (long
+// batch: mean 141 us, last 180).
+constexpr int kUnitCost = 2;
+__device__ __forceinline__ int32_t unit_cost(int32_t tiles) { return tiles > 0 ? tiles + kUnitCost : 0; }
+
+// A place on a line: offset `x` in a unit of `n` key tiles, `left` to the
+// piece's end.  Tile i of the unit lies at x = kUnitCost + i.
+struct LinePlace {
+  int32_t x, n;
+  int64_t left;
+  __device__ __forceinline__ int32_t first() const { return max(0, x - kUnitCost); }
+  __device__ __forceinline__ int32_t end_x() const { return (int32_t)min((int64_t)unit_cost(n), x + left); }
+  // key tiles of this unit in this piece
+  __device__ __forceinline__ int32_t here() const { return max(0, end_x() - kUnitCost) - first(); }
+  // goes to the end of the unit or piece; true if the piece goes on in the next unit
+  __device__ __forceinline__ bool pass() {
+    const int32_t to = end_x();
+    left -= to - x;
+    x = to == unit_cost(n) ? 0 : to;
+    return left > 0;
+  }
+};
+
 struct PagedAttnParams {
   uint16_t *out;
   const uint16_t *q;
@@ -68,9 +93,10 @@ struct PagedAttnParams {
   int32_t q_heads, heads, group, head_dim, prefix;
   int32_t chunk;          // keys per TMA box: gcd(page_size, 64)
   float scale_log2;       // softmax scale * log2(e)
-  // Each kernel cuts a line of key tiles into equal pieces, one per CTA.  A
-  // unit (rows that read the same keys of one head) that a piece ends in has
-  // several partial results: unnormalised O (f32, head_dim wide) and (running
+  // Each kernel lays its units (rows that read the same keys of one head) on a
+  // line, a unit's length being its key tiles and kUnitCost more for its start
+  // and end, and cuts the line into equal pieces, one per CTA or worker.  A
+  // unit that a piece ends in has several partial results: unnormalised O (f32, head_dim wide) and (running
   // maximum in log2 units, sum of weights) per row, in slot (unit + CTA).
   float *stream_o, *tile_o;
   float2 *stream_ml, *tile_ml;
@@ -90,10 +116,28 @@ struct PagedAttnParams {
   uint32_t *err;
 };
 
+// Bounded wait.  Its slow path is one function for all call sites: code that a
+// kernel has not run yet comes from HBM, at a microsecond or more a stretch, so
+// the kernels here are kept small.
+__device__ __noinline__ bool wait_slow(uint64_t *bar, uint32_t parity, volatile int *abort, uint64_t limit_ns) {
+  return mbar_wait_bounded(bar, parity, abort, limit_ns);
+}
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *abort,
+                                     uint64_t limit_ns = 4000000000ull) {
+  return mbar_try_wait(bar, parity) || wait_slow(bar, parity, abort, limit_ns);
+}
+
 // Two f32 to packed f16 in one conversion.
 __device__ __forceinline__ uint32_t to_h2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Bits [from, to) of a word, for any from and to.
+__device__ __forceinline__ uint32_t bits_between(int32_t from, int32_t to) {
+  const uint32_t below_to = to >= 32 ? 0xffffffffu : to <= 0 ? 0u : (1u << to) - 1u;
+  const uint32_t below_from = from >= 32 ? 0xffffffffu : from <= 0 ? 0u : (1u << from) - 1u;
+  return below_to & ~below_from;
 }
 
 // Named barrier over `count` threads that says whether `pred` holds for any of them.
@@ -121,9 +165,11 @@ __device__ __forceinline__ int64_t block_sums(int32_t n, int64_t *scratch, Count
   const int32_t share = (n + kThreads - 1) / kThreads;
   const int32_t lo = min(n, (int32_t)threadIdx.x * share), hi = min(n, lo + share);
   int64_t mine = 0;
+#pragma unroll 1
   for (int32_t b = lo; b < hi; ++b) mine += count(b);
   int64_t sum = mine;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll 1
   for (int d = 1; d < 32; d <<= 1) {
     const int64_t x = __shfl_up_sync(0xffffffffu, sum, d);
     if (lane >= d) sum += x;
@@ -131,11 +177,13 @@ __device__ __forceinline__ int64_t block_sums(int32_t n, int64_t *scratch, Count
   if (lane == 31) scratch[warp] = sum;
   __syncthreads();
   int64_t before = 0, total = 0;
+#pragma unroll 1
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) before += scratch[w];
     total += scratch[w];
   }
   before += sum - mine;
+#pragma unroll 1
   for (int32_t b = lo; b < hi; ++b) {
     store(b, before);
     before += count(b);
@@ -143,18 +191,19 @@ __device__ __forceinline__ int64_t block_sums(int32_t n, int64_t *scratch, Count
   return total;
 }
 
-// Page coordinate of the chunk of keys at position `pos`: out of range (the
-// TMA then fills zeros) where the chunk has no key of [lo, hi) or its page id
-// is not one.
-__device__ __forceinline__ int32_t page_of(const PagedAttnParams &p, const int32_t *ids, int32_t pos, int32_t lo,
+// The page id of the chunk of keys at position `pos`, if the chunk has a key of
+// [lo, hi); checked_page makes a page coordinate of it, out of range (the TMA
+// then fills zeros) where the chunk has none or the id is not a page.  Two
+// steps, so that the load is in flight while the caller waits for a stage.
+__device__ __forceinline__ int32_t page_id(const PagedAttnParams &p, const int32_t *ids, int32_t pos, int32_t lo,
                                            int32_t hi) {
-  if (pos >= hi || pos + p.chunk <= lo) return p.paged.pages;
-  const int32_t id = ids[pos / p.paged.page_size];
-  if (id < 0 || id >= p.paged.pages) {
-    record_device_error(p.err, ERR_KERNEL_PAGED_ATTENTION | ERR_SITE_PAGE);
-    return p.paged.pages;
-  }
-  return id;
+  return pos < hi && pos + p.chunk > lo ? ids[pos / p.paged.page_size] : -1;
+}
+__device__ __forceinline__ int32_t checked_page(const PagedAttnParams &p, int32_t id, int32_t pos, int32_t lo,
+                                                int32_t hi) {
+  if (id >= 0 && id < p.paged.pages) return id;
+  if (pos < hi && pos + p.chunk > lo) record_device_error(p.err, ERR_KERNEL_PAGED_ATTENTION | ERR_SITE_PAGE);
+  return p.paged.pages;
 }
 
 // ---- single rows: the sequences' own parts ------------------------------------
@@ -196,11 +245,10 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A CTA's place on the line of key tiles: tile i of the n of unit (b, h), keys
-// [lo, hi); b = -1: the prefix.
+// A worker's place on the line: unit (b, h), keys [lo, hi); b = -1: the prefix.
 struct StreamWalk {
-  int32_t b, h, i, n, lo, hi;
-  int64_t left;
+  LinePlace at;
+  int32_t b, h, lo, hi;
 
   __device__ __forceinline__ static int32_t tiles(const PagedAttnParams &p, int32_t len) {
     return len > p.prefix ? (len + kStreamKeys - 1) / kStreamKeys - p.prefix / kStreamKeys : 0;
@@ -210,41 +258,38 @@ struct StreamWalk {
     if (b < 0) {
       lo = 0;
       hi = p.prefix;
-      n = (hi + kStreamKeys - 1) / kStreamKeys;
+      at.n = (hi + kStreamKeys - 1) / kStreamKeys;
     } else {
       lo = p.prefix;
       hi = checked_length(p, b, false);
-      n = tiles(p, hi);
+      at.n = tiles(p, hi);
     }
   }
-  __device__ __forceinline__ void step(const PagedAttnParams &p, int32_t count) {
-    left -= count;
-    i += count;
-    if (i < n || left <= 0) return;
-    i = 0;
+  __device__ __noinline__ void next(const PagedAttnParams &p) {
+    if (!at.pass()) return;
     if (++h < p.heads) return;
     h = 0;
+#pragma unroll 1
     do {
       if (b + 1 >= p.paged.sequences) {
-        left = 0;
+        at.left = 0;
         return;
       }
       enter(p, b + 1);
-    } while (n == 0);
+    } while (at.n == 0);
   }
 };
 
 // SMs that stream own parts while the others work on the prefix: so many that
-// both take the same time, at 55 GB/s an SM streaming (up to what saturates
-// HBM) and 2.5 us a key tile of two row tiles.  Every CTA of both kernels comes
-// to the same number.
-constexpr float kStreamBytesPerUs = 55e3f, kTileUs = 2.5f;
+// both take the same time, by the times per key tile and SM that were measured
+// with both kernels running (not more than saturate HBM).
 constexpr int kStreamSaturated = 112;
-__device__ __forceinline__ int32_t stream_sms(const PagedAttnParams &p, int64_t own_tiles) {
-  if (own_tiles == 0) return 0;
+__device__ __forceinline__ int32_t stream_sms(const PagedAttnParams &p, int64_t own_cost) {
+  if (own_cost == 0) return 0;
   if (p.prefix_units == 0) return p.sms;
-  const float stream = (float)own_tiles * p.heads * (2.0f * 64 * 2 * p.head_dim) / kStreamBytesPerUs;
-  const float tile = (float)p.prefix_units * p.heads * ((p.prefix + 127) / 128) * kTileUs;
+  const float stream = (float)own_cost * p.heads * (0.25f + 0.35f / 128 * p.head_dim);
+  const float tile = (float)p.prefix_units * p.heads * unit_cost((p.prefix + 127) / 128) *
+                     (p.rows > p.tile_rows ? 2.8f : 1.7f);
   const int32_t x = (int32_t)(p.sms * (stream / (stream + tile)) + 0.5f);
   return max(1, min(min(x, kStreamSaturated), p.sms - 1));
 }
@@ -271,7 +316,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   float *merge = reinterpret_cast<float *>(smem + kStreamWorkers * RING_BYTES) + worker * 4 * 16 * kMergeLd;
   smem += worker * RING_BYTES;
   if (threadIdx.x == 0) {
+#pragma unroll 1
     for (int w = 0; w < kStreamWorkers; ++w)
+#pragma unroll 1
       for (int i = 0; i < kStreamStages; ++i) {
         mbar_init(&all_full[w][i], 1);
         mbar_init(&all_empty[w][i], 4);
@@ -282,12 +329,12 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     tma_prefetch_desc(&tm_v);
   }
   griddep_launch_dependents();
-  auto count = [&](int32_t b) { return StreamWalk::tiles(p, checked_length(p, b, blockIdx.x == 0)); };
-  // Sums first, then this worker's piece [W c / C, W (c + 1) / C) of the line of W tiles.
+  auto count = [&](int32_t b) { return unit_cost(StreamWalk::tiles(p, checked_length(p, b, blockIdx.x == 0))); };
+  // Sums first, then this worker's piece [W c / C, W (c + 1) / C) of the line's W.
   const int64_t total = block_sums<kStreamThreads>(p.paged.sequences, scratch, count, [&](int32_t b, int64_t sum) {
     if (blockIdx.x == 0) p.stream_sums[b] = sum;
   });
-  const int64_t ahead = p.stream_prefix ? (int64_t)((p.prefix + kStreamKeys - 1) / kStreamKeys) * p.heads : 0;
+  const int64_t ahead = p.stream_prefix ? (int64_t)unit_cost((p.prefix + kStreamKeys - 1) / kStreamKeys) * p.heads : 0;
   const int64_t line = ahead + total * p.heads;
   const int64_t share = p.stream_prefix ? p.sms : stream_sms(p, total);
   const int64_t pieces = min(kStreamWorkers * share, line);  // no piece is empty
@@ -302,6 +349,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   __syncthreads();  // scratch is read before it is written again
   block_sums<kStreamThreads>(p.paged.sequences, scratch, count, [&](int32_t b, int64_t sum) {
     const int32_t n = count(b);
+#pragma unroll 1
     for (int w = 0; w < kStreamWorkers; ++w) {
       const int64_t at = start_of(w) - ahead - sum * p.heads;
       if (at >= 0 && at < (int64_t)n * p.heads) {
@@ -315,49 +363,62 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   const int64_t cta = piece_of(worker), start = start_of(worker);
   if (cta >= pieces) return;
   StreamWalk w;
-  w.left = line * (cta + 1) / pieces - start;
+  w.at.left = line * (cta + 1) / pieces - start;
   if (start < ahead) {
     w.enter(p, -1);
-    w.h = (int32_t)(start / w.n);
-    w.i = (int32_t)(start % w.n);
+    w.h = (int32_t)(start / unit_cost(w.at.n));
+    w.at.x = (int32_t)(start % unit_cost(w.at.n));
   } else {
     w.enter(p, first_unit[worker][0]);
     w.h = first_unit[worker][1];
-    w.i = first_unit[worker][2];
+    w.at.x = first_unit[worker][2];
   }
 
   if (warp == 4) {
-    // Producer: lane l issues boxes l, l + 32, ... of a tile: (K or V, half, chunk).
+    // Producer: lane l issues boxes l, l + 32, ... of a tile: (K or V, half,
+    // chunk).  The first one's page id is loaded a tile ahead.
     const int chunks = kStreamKeys / p.chunk, boxes = 2 * HALVES * chunks;
+    const int my_chunk = lane % chunks;
     bool ok = true;
     uint32_t t = 0;
-    for (; w.left > 0 && ok; ++t, w.step(p, 1)) {
-      const int st = t % kStreamStages;
-      const int32_t key0 = (w.lo / kStreamKeys + w.i) * kStreamKeys;
+#pragma unroll 1
+    while (w.at.left > 0 && ok) {
+      const int32_t count_here = w.at.here();
       const int32_t *ids = w.b < 0 ? p.prefix_pages : p.paged.page_table + w.b * p.paged.table_stride;
-      // this lane's first box's page is looked up before the stage is free
-      int32_t page = lane < boxes ? page_of(p, ids, key0 + (lane % chunks) * p.chunk, w.lo, w.hi) : 0;
-      if (!mbar_wait_bounded(&empty[st], ((t / kStreamStages) & 1) ^ 1, abort_flag)) {
-        ok = false;
-        break;
+      int32_t key0 = (w.lo / kStreamKeys + w.at.first()) * kStreamKeys;
+      int32_t id = count_here && lane < boxes ? page_id(p, ids, key0 + my_chunk * p.chunk, w.lo, w.hi) : -1;
+#pragma unroll 1
+      for (int32_t k = 0; k < count_here; ++k, ++t, key0 += kStreamKeys) {
+        const int st = t % kStreamStages;
+        const int32_t id_next = k + 1 < count_here && lane < boxes
+                                    ? page_id(p, ids, key0 + kStreamKeys + my_chunk * p.chunk, w.lo, w.hi)
+                                    : -1;
+        if (!wait(&empty[st], ((t / kStreamStages) & 1) ^ 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], 2 * TILE_BYTES);
+        __syncwarp();
+        uint8_t *base = smem + st * 2 * TILE_BYTES;
+#pragma unroll 1
+        for (int x = lane; x < boxes; x += 32) {
+          const int chunk = x % chunks, half = (x / chunks) % HALVES, v = x / (chunks * HALVES);
+          const int32_t pos = key0 + chunk * p.chunk;
+          if (x >= 32) id = page_id(p, ids, pos, w.lo, w.hi);
+          tma_load_4d(base + v * TILE_BYTES + half * HALF_BYTES + chunk * p.chunk * 128, v ? &tm_v : &tm_k, &full[st],
+                      half * 64, pos % p.paged.page_size, w.h, checked_page(p, id, pos, w.lo, w.hi));
+        }
+        id = id_next;
       }
-      if (lane == 0) mbar_arrive_expect_tx(&full[st], 2 * TILE_BYTES);
-      __syncwarp();
-      uint8_t *base = smem + st * 2 * TILE_BYTES;
-      for (int x = lane; x < boxes; x += 32) {
-        const int chunk = x % chunks, half = (x / chunks) % HALVES, v = x / (chunks * HALVES);
-        const int32_t pos = key0 + chunk * p.chunk;
-        if (x >= 32) page = page_of(p, ids, pos, w.lo, w.hi);
-        tma_load_4d(base + v * TILE_BYTES + half * HALF_BYTES + chunk * p.chunk * 128, v ? &tm_v : &tm_k, &full[st],
-                    half * 64, pos % p.paged.page_size, w.h, page);
-      }
+      w.next(p);
     }
     if (!ok) {
       if (lane == 0) record_device_error(p.err, ERR_KERNEL_PAGED_ATTENTION | ERR_SITE_PRODUCER);
       *abort_flag = 1;
       // nothing leaves while copies into its shared memory are in flight
+#pragma unroll 1
       for (uint32_t x = t > kStreamStages ? t - kStreamStages : 0; x < t; ++x)
-        mbar_wait_bounded(&full[x % kStreamStages], (x / kStreamStages) & 1, nullptr, 1000000000ull);
+        wait(&full[x % kStreamStages], (x / kStreamStages) & 1, nullptr, 1000000000ull);
     }
     return;
   }
@@ -367,7 +428,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   const int r0 = lane >> 2, r1 = r0 + 8, cq = (lane & 3) * 2;
   auto unit_rows = [&](const StreamWalk &u) { return u.b < 0 ? (int)p.rows * p.group : p.group; };
   auto load_q = [&](const StreamWalk &u, uint32_t (&a)[KS][4]) {
-    const int n = unit_rows(u);
+    const int n = u.at.left > 0 ? unit_rows(u) : 0;
     const uint16_t *base[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -382,8 +443,6 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         a[k][j] = row < n && col < p.head_dim ? *reinterpret_cast<const uint32_t *>(base[j & 1] + col) : 0u;
       }
   };
-  uint32_t q[KS][4];
-  load_q(w, q);
   // ldmatrix addresses: lane -> row lane % 8 of matrix lane / 8.  K matrices:
   // (keys 0-7, 8-15) x (two 16-byte column chunks); V: keys fastest.
   const int mi = lane >> 3, mr = lane & 7;
@@ -392,8 +451,80 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   const float c = p.scale_log2;
   bool ok = true;
   uint32_t t = 0;
-  while (w.left > 0) {
-    const int32_t count_here = (int32_t)min((int64_t)(w.n - w.i), w.left);
+  // A unit's queries load while the last one's results meet.
+  StreamWalk next = w;
+  int32_t count_here = 0;
+  float o[NT][4], m0, m1, l0, l1;
+#pragma unroll 1
+  for (;;) {
+    uint32_t q[KS][4];
+    load_q(next, q);
+    if (count_here) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+      l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+      if ((lane & 3) == 0) {
+        warp_m[warp][r0] = m0;
+        warp_m[warp][r1] = m1;
+        warp_l[warp][r0] = l0;
+        warp_l[warp][r1] = l1;
+      }
+      named_barrier_sync(1 + worker, 128);
+      const float t0 = fmaxf(fmaxf(warp_m[0][r0], warp_m[1][r0]), fmaxf(warp_m[2][r0], warp_m[3][r0]));
+      const float t1 = fmaxf(fmaxf(warp_m[0][r1], warp_m[1][r1]), fmaxf(warp_m[2][r1], warp_m[3][r1]));
+      const float a0 = m0 == -INFINITY ? 0.0f : ex2_approx((m0 - t0) * c);
+      const float a1 = m1 == -INFINITY ? 0.0f : ex2_approx((m1 - t1) * c);
+      const int orow = warp * 4 + (lane >> 3), ocol = (lane & 7) * 4;  // this thread's share of the sums
+      float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) top = fmaxf(top, warp_m[x][orow]);
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (warp_m[x][orow] != -INFINITY) sum += warp_l[x][orow] * ex2_approx((warp_m[x][orow] - top) * c);
+      const bool whole = p.prefix == 0 && count_here == w.at.n;
+      const int64_t unit = (int64_t)(w.b + p.stream_prefix) * p.heads + w.h;
+      const int64_t slot = (unit + cta) * p.stream_rows + orow;
+      const int rows_here = unit_rows(w);
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      if (!whole && orow < rows_here && ocol == 0) p.stream_ml[slot] = make_float2(top == -INFINITY ? top : top * c, sum);
+#pragma unroll
+      for (int round = 0; round < DP / 32; ++round) {
+        float *mine = merge + warp * 16 * kMergeLd;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float(&v)[4] = o[round * 4 + i];
+          *reinterpret_cast<float2 *>(mine + r0 * kMergeLd + i * 8 + cq) = make_float2(v[0] * a0, v[1] * a0);
+          *reinterpret_cast<float2 *>(mine + r1 * kMergeLd + i * 8 + cq) = make_float2(v[2] * a1, v[3] * a1);
+        }
+        named_barrier_sync(1 + worker, 128);
+        const int col = round * 32 + ocol;
+        if (orow < rows_here && col < p.head_dim) {
+          float4 r = *reinterpret_cast<const float4 *>(merge + orow * kMergeLd + ocol);
+#pragma unroll
+          for (int x = 1; x < 4; ++x) {
+            const float4 y = *reinterpret_cast<const float4 *>(merge + (x * 16 + orow) * kMergeLd + ocol);
+            r.x += y.x;
+            r.y += y.y;
+            r.z += y.z;
+            r.w += y.w;
+          }
+          if (whole) {
+            uint2 h;
+            h.x = to_h2(r.x * inv, r.y * inv);
+            h.y = to_h2(r.z * inv, r.w * inv);
+            const int64_t head = (int64_t)w.b * p.q_heads + w.h * p.group + orow;
+            *reinterpret_cast<uint2 *>(p.out + head * p.head_dim + col) = h;
+          } else {
+            *reinterpret_cast<float4 *>(p.stream_o + slot * p.head_dim + col) = r;
+          }
+        }
+        named_barrier_sync(1 + worker, 128);
+      }
+    }
+    if (next.at.left <= 0) break;
+    w = next;
+    count_here = w.at.here();
     // Keys a row attends to end at the unit's end, in the prefix perhaps before it.
     int32_t end0 = w.hi, end1 = w.hi, end = w.hi;
     if (w.b < 0) {
@@ -401,15 +532,17 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       if (r1 < (int)p.rows * p.group) end1 = min(w.hi, max(0, p.paged.lengths[r1 / p.group]));
       end = __reduce_min_sync(0xffffffffu, min(end0, end1));
     }
-    float o[NT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+    m0 = m1 = -INFINITY;
+    l0 = l1 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+#pragma unroll 1
     for (int32_t k = 0; k < count_here; ++k, ++t) {
       const int st = t % kStreamStages;
       // (a wait that ran out is not left early: the barriers below need every warp)
-      if (ok && !mbar_wait_bounded(&full[st], (t / kStreamStages) & 1, abort_flag)) ok = false;
+      if (ok && !wait(&full[st], (t / kStreamStages) & 1, abort_flag)) ok = false;
       const uint32_t ks = sbase + st * 2 * TILE_BYTES, vs = ks + TILE_BYTES;
-      const int32_t key0 = (w.lo / kStreamKeys + w.i + k) * kStreamKeys + warp * 16;
+      const int32_t key0 = (w.lo / kStreamKeys + w.at.first() + k) * kStreamKeys + warp * 16;
       float s[2][4] = {}, s2[2][4] = {};  // even and odd steps: two chains
 #pragma unroll
       for (int d = 0; d < KS; ++d) {
@@ -435,6 +568,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
             const int32_t key = key0 + x * 8 + cq + (j & 1);
             if (key < w.lo || key >= (j & 2 ? end1 : end0)) s[x][j] = -INFINITY;
           }
+#pragma unroll 1
         for (int x = lane; x < 16 * HALVES * 8; x += 32) {
           const int row = x / (HALVES * 8), half = (x >> 3) % HALVES;
           if (key0 + row < w.lo || key0 + row >= w.hi) {
@@ -490,77 +624,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[st]);
     }
-    // The next unit's queries load while this one's results meet.
-    StreamWalk next = w;
-    next.step(p, count_here);
-    uint32_t qn[KS][4];
-    if (next.left > 0) load_q(next, qn);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    if ((lane & 3) == 0) {
-      warp_m[warp][r0] = m0;
-      warp_m[warp][r1] = m1;
-      warp_l[warp][r0] = l0;
-      warp_l[warp][r1] = l1;
-    }
-    named_barrier_sync(1 + worker, 128);
-    const float t0 = fmaxf(fmaxf(warp_m[0][r0], warp_m[1][r0]), fmaxf(warp_m[2][r0], warp_m[3][r0]));
-    const float t1 = fmaxf(fmaxf(warp_m[0][r1], warp_m[1][r1]), fmaxf(warp_m[2][r1], warp_m[3][r1]));
-    const float a0 = m0 == -INFINITY ? 0.0f : ex2_approx((m0 - t0) * c);
-    const float a1 = m1 == -INFINITY ? 0.0f : ex2_approx((m1 - t1) * c);
-    const int orow = warp * 4 + (lane >> 3), ocol = (lane & 7) * 4;  // this thread's share of the sums
-    float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) top = fmaxf(top, warp_m[x][orow]);
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-      if (warp_m[x][orow] != -INFINITY) sum += warp_l[x][orow] * ex2_approx((warp_m[x][orow] - top) * c);
-    const bool whole = p.prefix == 0 && count_here == w.n;
-    const int64_t unit = (int64_t)(w.b + p.stream_prefix) * p.heads + w.h;
-    const int64_t slot = (unit + cta) * p.stream_rows + orow;
-    const int rows_here = unit_rows(w);
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (!whole && orow < rows_here && ocol == 0) p.stream_ml[slot] = make_float2(top == -INFINITY ? top : top * c, sum);
-#pragma unroll
-    for (int round = 0; round < DP / 32; ++round) {
-      float *mine = merge + warp * 16 * kMergeLd;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float(&v)[4] = o[round * 4 + i];
-        *reinterpret_cast<float2 *>(mine + r0 * kMergeLd + i * 8 + cq) = make_float2(v[0] * a0, v[1] * a0);
-        *reinterpret_cast<float2 *>(mine + r1 * kMergeLd + i * 8 + cq) = make_float2(v[2] * a1, v[3] * a1);
-      }
-      named_barrier_sync(1 + worker, 128);
-      const int col = round * 32 + ocol;
-      if (orow < rows_here && col < p.head_dim) {
-        float4 r = *reinterpret_cast<const float4 *>(merge + orow * kMergeLd + ocol);
-#pragma unroll
-        for (int x = 1; x < 4; ++x) {
-          const float4 y = *reinterpret_cast<const float4 *>(merge + (x * 16 + orow) * kMergeLd + ocol);
-          r.x += y.x;
-          r.y += y.y;
-          r.z += y.z;
-          r.w += y.w;
-        }
-        if (whole) {
-          uint2 h;
-          h.x = to_h2(r.x * inv, r.y * inv);
-          h.y = to_h2(r.z * inv, r.w * inv);
-          const int64_t head = (int64_t)w.b * p.q_heads + w.h * p.group + orow;
-          *reinterpret_cast<uint2 *>(p.out + head * p.head_dim + col) = h;
-        } else {
-          *reinterpret_cast<float4 *>(p.stream_o + slot * p.head_dim + col) = r;
-        }
-      }
-      named_barrier_sync(1 + worker, 128);
-    }
-    w = next;
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) q[k][j] = qn[k][j];
+    next.next(p);
   }
   if (!ok) {
     if (lane == 0) record_device_error(p.err, ERR_KERNEL_PAGED_ATTENTION | ERR_SITE_EPILOGUE);
@@ -591,16 +655,16 @@ __device__ __forceinline__ int32_t first_row(const PagedAttnParams &p, int32_t b
   return p.paged.row_offsets ? max(0, min(p.paged.row_offsets[b], (int32_t)p.rows)) : b;
 }
 
-// A CTA's place on the tile kernel's line: key tile i of the n of unit (row
-// unit, head h); `seq` < 0: the prefix, whose row units cover all rows.
+// A CTA's place on the tile kernel's line: unit (row unit, head h); `seq` < 0:
+// the prefix, whose row units cover all rows.
 struct TileWalk {
-  int32_t seq, j, h, i, n;   // row unit j of its sequence (or of the prefix)
+  LinePlace at;
+  int32_t seq, j, h;         // row unit j of its sequence (or of the prefix)
   int32_t unit;              // own part: row units before it
   int32_t rows, lo, hi;      // batch rows; keys [lo, hi)
   int64_t row0, pos0;        // first batch row and (own part) its position
-  int64_t left;
 
-  __device__ __forceinline__ void own(const PagedAttnParams &p, int32_t b, int32_t row_unit) {
+  __device__ __noinline__ void own(const PagedAttnParams &p, int32_t b, int32_t row_unit) {
     const int32_t begin = first_row(p, b), end = first_row(p, b + 1), per_unit = 2 * p.tile_rows;
     seq = b;
     j = row_unit;
@@ -609,7 +673,7 @@ struct TileWalk {
     pos0 = (int64_t)p.paged.lengths[b] - (end - begin) + (row0 - begin);
     lo = p.prefix;
     hi = (int32_t)max((int64_t)0, min((int64_t)checked_length(p, b, false), pos0 + rows));
-    n = rows > 0 && hi > lo ? (hi + kTileKeys - 1) / kTileKeys - lo / kTileKeys : 0;
+    at.n = rows > 0 && hi > lo ? (hi + kTileKeys - 1) / kTileKeys - lo / kTileKeys : 0;
   }
   __device__ __forceinline__ void prefix(const PagedAttnParams &p, int32_t row_unit) {
     const int32_t per_unit = 2 * p.tile_rows;
@@ -620,23 +684,17 @@ struct TileWalk {
     pos0 = 0;
     lo = 0;
     hi = p.prefix;
-    n = (hi + kTileKeys - 1) / kTileKeys;
+    at.n = (hi + kTileKeys - 1) / kTileKeys;
   }
   __device__ __forceinline__ static int32_t units(const PagedAttnParams &p, int32_t b) {
     const int32_t per_unit = 2 * p.tile_rows;
     return max(0, (first_row(p, b + 1) - first_row(p, b) + per_unit - 1) / per_unit);
   }
-  // Key tiles of this unit that are this CTA's.
-  __device__ __forceinline__ int32_t here() const { return (int32_t)min((int64_t)(n - i), left); }
   __device__ __forceinline__ int64_t slot_unit(const PagedAttnParams &p) const {
     return seq < 0 ? (int64_t)h * p.prefix_units + j : (int64_t)(p.prefix_units + unit) * p.heads + h;
   }
-  __device__ __forceinline__ void next(const PagedAttnParams &p) {
-    const int32_t count = here();
-    left -= count;
-    i += count;
-    if (i < n || left <= 0) return;
-    i = 0;
+  __device__ __noinline__ void next(const PagedAttnParams &p) {
+    if (!at.pass()) return;
     if (seq < 0) {  // units are in the order (head, row unit)
       if (++j < p.prefix_units) {
         prefix(p, j);
@@ -658,16 +716,18 @@ struct TileWalk {
     // the next row unit with keys
     ++unit;
     if (seq < 0) seq = 0;
+#pragma unroll 1
     for (;; ++unit) {
+#pragma unroll 1
       while (j >= units(p, seq)) {
         if (++seq >= p.paged.sequences) {
-          left = 0;
+          at.left = 0;
           return;
         }
         j = 0;
       }
       own(p, seq, j);
-      if (n > 0) return;
+      if (at.n > 0) return;
       ++j;
     }
   }
@@ -685,6 +745,19 @@ struct TileTask {
   // zero-filled by the TMA.
   int32_t fix_first, fix_last;
 };
+
+// S = Q K^T of one row tile (one function: a unit's first products run the code that the next ones use).
+__device__ __noinline__ void issue_scores(uint32_t d, uint64_t q_desc, uint64_t k_desc, int k_steps, uint64_t *full) {
+  constexpr uint32_t idesc = make_idesc(128, kTileKeys, 0, false, false);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    if (k < k_steps) {
+      const uint64_t step = (uint64_t)(((k >> 2) * kTileHalf + (k & 3) * 32) >> 4);
+      mma_f16_ss(d, q_desc + step, k_desc + step, idesc, k > 0 ? 1u : 0u);
+    }
+  }
+  mma_commit(full);
+}
 
 __global__ void __launch_bounds__(kTileThreads, 1)
     paged_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -707,6 +780,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1);
     mbar_init(&q_empty, 1);
+#pragma unroll 1
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&v_full[i], 1);
@@ -726,42 +800,45 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  // This CTA's piece of the line of W tiles, [W c / C, W (c + 1) / C).
+  // This CTA's piece of the line's W, [W c / C, W (c + 1) / C).
   const int64_t cta = blockIdx.x;
-  const int64_t ahead = (int64_t)p.prefix_units * p.heads * ((p.prefix + kTileKeys - 1) / kTileKeys);
-  // Row units (above 2^40) and key tiles of sequence b's own part, in one sum.
+  const int64_t ahead = (int64_t)p.prefix_units * p.heads * unit_cost((p.prefix + kTileKeys - 1) / kTileKeys);
+  // Row units (above 2^40) and the length of sequence b's own part per head, in one sum.
   auto count = [&](int32_t b) {
     const int32_t u = TileWalk::units(p, b);
     int64_t sum = (int64_t)u << 40;
     TileWalk w;
+#pragma unroll 1
     for (int32_t j = 0; j < u; ++j) {
       w.own(p, b, j);
-      sum += w.n;
+      sum += unit_cost(w.at.n);
     }
     return sum;
   };
   int64_t total = 0;
   int32_t share = p.sms;
   if (p.stream) {
-    const int64_t own_tiles = block_sums<kTileThreads>(
-        p.paged.sequences, scratch, [&](int32_t b) { return StreamWalk::tiles(p, checked_length(p, b, false)); },
+    const int64_t own_cost = block_sums<kTileThreads>(
+        p.paged.sequences, scratch, [&](int32_t b) { return unit_cost(StreamWalk::tiles(p, checked_length(p, b, false))); },
         [](int32_t, int64_t) {});
-    share -= stream_sms(p, own_tiles);
+    share -= stream_sms(p, own_cost);
   }
   if (p.tile_own) {
     if (cta == 0)
+#pragma unroll 1
       for (int32_t b = threadIdx.x; b < p.paged.sequences; b += kTileThreads) checked_length(p, b, true);
     total = block_sums<kTileThreads>(p.paged.sequences, scratch, count, [&](int32_t b, int64_t sum) {
       if (cta != 0) return;
       const int32_t base = (int32_t)(sum >> 40), u = TileWalk::units(p, b);
-      int64_t tiles = sum & ((1ll << 40) - 1);
+      int64_t cost = sum & ((1ll << 40) - 1);
       p.unit_base[b] = base;
       TileWalk w;
+#pragma unroll 1
       for (int32_t j = 0; j < u && base + j < p.max_units; ++j) {
-        p.unit_sums[base + j] = tiles;
+        p.unit_sums[base + j] = cost;
         w.own(p, b, j);
-        tiles += w.n;
-        p.unit_sums[base + j + 1] = tiles;
+        cost += unit_cost(w.at.n);
+        p.unit_sums[base + j + 1] = cost;
       }
     });
   }
@@ -780,10 +857,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   walk.unit = -1;
   if (start < ahead) {
     walk.prefix(p, 0);
-    const int64_t u = start / walk.n;
+    const int64_t u = start / unit_cost(walk.at.n);
     walk.h = (int32_t)(u / p.prefix_units);
     walk.prefix(p, (int32_t)(u % p.prefix_units));
-    walk.i = (int32_t)(start % walk.n);
+    walk.at.x = (int32_t)(start % unit_cost(walk.at.n));
   } else {
     __syncthreads();  // scratch is read before it is written again
     block_sums<kTileThreads>(p.paged.sequences, scratch, count, [&](int32_t b, int64_t sum) {
@@ -791,24 +868,25 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (at < 0 || at >= (count(b) & ((1ll << 40) - 1)) * p.heads) return;
       TileWalk w;
       int32_t j = 0;
+#pragma unroll 1
       for (;; ++j) {
         w.own(p, b, j);
-        if (at < (int64_t)w.n * p.heads) break;
-        at -= (int64_t)w.n * p.heads;
+        if (at < (int64_t)unit_cost(w.at.n) * p.heads) break;
+        at -= (int64_t)unit_cost(w.at.n) * p.heads;
       }
       found[0] = b;
       found[1] = j;
-      found[2] = (int32_t)(at / w.n);
-      found[3] = (int32_t)(at % w.n);
+      found[2] = (int32_t)(at / unit_cost(w.at.n));
+      found[3] = (int32_t)(at % unit_cost(w.at.n));
       found[4] = (int32_t)(sum >> 40) + j;
     });
     __syncthreads();
     walk.own(p, found[0], found[1]);
     walk.h = found[2];
-    walk.i = found[3];
+    walk.at.x = found[3];
     walk.unit = found[4];
   }
-  walk.left = line * (cta + 1) / ctas - start;
+  walk.at.left = line * (cta + 1) / ctas - start;
   const int halves = p.head_dim > 64 ? 2 : 1, k_steps = (p.head_dim + 15) / 16;
 
   if (warp == 1) {
@@ -825,14 +903,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     uint32_t unit = 0, k_issued = 0, v_issued = 0, q_issued = 0;
     // Tasks are written two ahead of the last reader at most; after the last comes one with n = 0.
     auto publish = [&](const TileTask &task, uint32_t index) {
-      const bool free = mbar_wait_bounded(&task_empty[index & 1], ((index >> 1) & 1) ^ 1, abort_flag);
+      const bool free = wait(&task_empty[index & 1], ((index >> 1) & 1) ^ 1, abort_flag);
       if (free && lane == 0) {
         tasks[index & 1] = task;
         mbar_arrive(&task_full[index & 1]);
       }
       return free;
     };
-    for (; walk.left > 0 && ok; walk.next(p), ++unit) {
+#pragma unroll 1
+    for (; walk.at.left > 0 && ok; walk.next(p)) {
+      if (walk.at.here() == 0) continue;  // the piece ends in front of the unit's first tile
       TileTask task;
       task.row0 = walk.row0;
       task.pos0 = walk.pos0;
@@ -841,11 +921,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       task.lo = walk.lo;
       task.hi = walk.hi;
       task.h = walk.h;
-      task.n = walk.here();
-      task.first = walk.lo / kTileKeys + walk.i;
+      task.n = walk.at.here();
+      task.first = walk.lo / kTileKeys + walk.at.first();
       task.tiles = walk.rows > p.tile_rows ? 2 : 1;
       task.prefix = walk.seq < 0;
-      task.direct = p.prefix == 0 && task.n == walk.n;
+      task.direct = p.prefix == 0 && task.n == walk.at.n;
       // (max_units holds for sorted row offsets; others write no partials past it)
       task.store = walk.unit < p.max_units;
       task.fix_first = task.first * kTileKeys < walk.lo && walk.lo % p.chunk != 0;
@@ -855,20 +935,29 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         break;
       }
       const int32_t *ids = walk.seq < 0 ? p.prefix_pages : p.paged.page_table + walk.seq * p.paged.table_stride;
+      int32_t id = 0;  // of this lane's first chunk, loaded a tile ahead
       auto load = [&](uint8_t *base, const CUtensorMap *map, uint64_t *bar, int32_t key0) {
         if (lane == 0) mbar_arrive_expect_tx(bar, halves * kTileHalf);
         __syncwarp();
+#pragma unroll 1
         for (int i = lane; i < boxes; i += 32) {
           const int chunk = i % chunks, half = i / chunks;
           const int32_t pos = key0 + chunk * p.chunk;
+          const int32_t page = i < 32 ? id : page_id(p, ids, pos, walk.lo, walk.hi);
           tma_load_4d(base + half * kTileHalf + chunk * p.chunk * 128, map, bar, half * 64, pos % p.paged.page_size,
-                      walk.h, page_of(p, ids, pos, walk.lo, walk.hi));
+                      walk.h, checked_page(p, page, pos, walk.lo, walk.hi));
         }
       };
+      auto first_id = [&](int32_t key0) {
+        return lane < boxes ? page_id(p, ids, key0 + (lane % chunks) * p.chunk, walk.lo, walk.hi) : -1;
+      };
+      id = first_id(task.first * kTileKeys);
+#pragma unroll 1
       for (int32_t j = 0; j < task.n; ++j) {
         const int st = k_issued & 1;
         const int32_t key0 = (task.first + j) * kTileKeys;
-        if (!mbar_wait_bounded(&k_empty[st], ((k_issued >> 1) & 1) ^ 1, abort_flag)) {
+        const int32_t id_next = j + 1 < task.n ? first_id(key0 + kTileKeys) : -1;
+        if (!wait(&k_empty[st], ((k_issued >> 1) & 1) ^ 1, abort_flag)) {
           ok = false;
           break;
         }
@@ -876,30 +965,33 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         ++k_issued;
         if (j == 0) {
           // Q's buffer: the previous unit's S products are done
-          if (!mbar_wait_bounded(&q_empty, (unit & 1) ^ 1, abort_flag)) {
+          if (!wait(&q_empty, (unit & 1) ^ 1, abort_flag)) {
             ok = false;
             break;
           }
           if (lane == 0) {
             mbar_arrive_expect_tx(&q_full, task.tiles * halves * p.tile_rows * p.group * 128);
+#pragma unroll 1
             for (int t = 0; t < task.tiles; ++t)
+#pragma unroll 1
               for (int half = 0; half < halves; ++half)
                 tma_load_4d(s_q + t * kTileBytes + half * kTileHalf, &tm_q, &q_full, half * 64, 0, walk.h,
                             (int32_t)walk.row0 + t * p.tile_rows);
           }
           ++q_issued;
         }
-        if (!mbar_wait_bounded(&v_empty[st], ((v_issued >> 1) & 1) ^ 1, abort_flag)) {
+        if (!wait(&v_empty[st], ((v_issued >> 1) & 1) ^ 1, abort_flag)) {
           ok = false;
           break;
         }
         load(s_v + st * kTileBytes, &tm_v, &v_full[st], key0);
         ++v_issued;
         if ((task.fix_first && j == 0) || (task.fix_last && j == task.n - 1)) {
-          if (!mbar_wait_bounded(&v_full[st], ((v_issued - 1) >> 1) & 1, abort_flag)) {
+          if (!wait(&v_full[st], ((v_issued - 1) >> 1) & 1, abort_flag)) {
             ok = false;
             break;
           }
+#pragma unroll 1
           for (int i = lane; i < kTileKeys * halves * 8; i += 32) {
             const int row = i / (halves * 8), half = (i >> 3) % halves;
             if (key0 + row < walk.lo || key0 + row >= walk.hi)
@@ -910,7 +1002,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&v_fixed[st]);
         }
+        id = id_next;
       }
+      ++unit;
     }
     if (ok) {
       TileTask done = {};
@@ -920,29 +1014,23 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (lane == 0) record_device_error(p.err, ERR_KERNEL_PAGED_ATTENTION | ERR_SITE_PRODUCER);
       *abort_flag = 1;
       // nothing leaves while copies into its shared memory are in flight
-      if (q_issued) mbar_wait_bounded(&q_full, (q_issued - 1) & 1, nullptr, 1000000000ull);
+      if (q_issued) wait(&q_full, (q_issued - 1) & 1, nullptr, 1000000000ull);
+#pragma unroll 1
       for (uint32_t i = k_issued > 2 ? k_issued - 2 : 0; i < k_issued; ++i)
-        mbar_wait_bounded(&k_full[i & 1], (i >> 1) & 1, nullptr, 1000000000ull);
+        wait(&k_full[i & 1], (i >> 1) & 1, nullptr, 1000000000ull);
+#pragma unroll 1
       for (uint32_t i = v_issued > 2 ? v_issued - 2 : 0; i < v_issued; ++i)
-        mbar_wait_bounded(&v_full[i & 1], (i >> 1) & 1, nullptr, 1000000000ull);
+        wait(&v_full[i & 1], (i >> 1) & 1, nullptr, 1000000000ull);
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      const uint32_t idesc_s = make_idesc(128, kTileKeys, 0, false, false);
       const uint32_t idesc_o = make_idesc(128, k_steps * 16, 0, false, true);  // V: head dims contiguous
       const uint64_t q_desc = make_smem_desc(smem_u32(s_q), 16, 1024, kSwizzle128B);
       const uint64_t k_desc = make_smem_desc(smem_u32(s_k), 16, 1024, kSwizzle128B);
       const uint64_t v_desc = make_smem_desc(smem_u32(s_v), kTileHalf, 1024, kSwizzle128B);
       auto issue_s = [&](int t, int st) {
-        const uint64_t qd = q_desc + (uint64_t)(t * (kTileBytes >> 4)), kd = k_desc + (uint64_t)(st * (kTileBytes >> 4));
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (k < k_steps) {
-            const uint64_t step = (uint64_t)(((k >> 2) * kTileHalf + (k & 3) * 32) >> 4);
-            mma_f16_ss(tmem + t * 128, qd + step, kd + step, idesc_s, k > 0 ? 1u : 0u);
-          }
-        }
-        mma_commit(&s_full[t]);
+        issue_scores(tmem + t * 128, q_desc + (uint64_t)(t * (kTileBytes >> 4)), k_desc + (uint64_t)(st * (kTileBytes >> 4)),
+                     k_steps, &s_full[t]);
       };
       // Per key tile j: PV_t(j) as soon as P_t(j) is there, then S_t(j + 1)
       // behind it.  A unit's first S products queue behind the last unit's last
@@ -950,8 +1038,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       bool ok = true;
       uint32_t unit = 0, g = 0;          // units begun, key tiles done
       uint32_t p_count[2] = {0, 0}, o_count[2] = {0, 0}, fixes[2] = {0, 0};
+#pragma unroll 1
       for (;; ++unit) {
-        ok = mbar_wait_bounded(&task_full[unit & 1], (unit >> 1) & 1, abort_flag);
+        ok = wait(&task_full[unit & 1], (unit >> 1) & 1, abort_flag);
         if (!ok) break;
         const TileTask &task = tasks[unit & 1];
         const int tiles = task.tiles;
@@ -959,22 +1048,25 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const bool fix_first = task.fix_first, fix_last = task.fix_last;
         mbar_arrive(&task_empty[unit & 1]);
         if (n == 0) break;
-        ok = mbar_wait_bounded(&k_full[g & 1], (g >> 1) & 1, abort_flag) && mbar_wait_bounded(&q_full, unit & 1, abort_flag);
+        ok = wait(&k_full[g & 1], (g >> 1) & 1, abort_flag) && wait(&q_full, unit & 1, abort_flag);
         if (!ok) break;
+#pragma unroll 1
         for (int t = 0; t < tiles; ++t) issue_s(t, g & 1);
         if (n == 1) mma_commit(&q_empty);
+#pragma unroll 1
         for (int32_t j = 0; j < n && ok; ++j, ++g) {
           const int st = g & 1;
           const bool more = j + 1 < n;
           const uint64_t vd = v_desc + (uint64_t)(st * (kTileBytes >> 4));
           if ((fix_first && j == 0) || (fix_last && !more))
-            ok = mbar_wait_bounded(&v_fixed[st], fixes[st]++ & 1, abort_flag);
+            ok = wait(&v_fixed[st], fixes[st]++ & 1, abort_flag);
           else
-            ok = mbar_wait_bounded(&v_full[st], (g >> 1) & 1, abort_flag);
+            ok = wait(&v_full[st], (g >> 1) & 1, abort_flag);
+#pragma unroll 1
           for (int t = 0; t < tiles && ok; ++t) {
-            ok = mbar_wait_bounded(&p_ready[t], p_count[t]++ & 1, abort_flag);
+            ok = wait(&p_ready[t], p_count[t]++ & 1, abort_flag);
             // the last unit's O_t has been read out before this one's first PV_t
-            if (ok && j == 0 && o_count[t]) ok = mbar_wait_bounded(&o_empty[t], (o_count[t] - 1) & 1, abort_flag);
+            if (ok && j == 0 && o_count[t]) ok = wait(&o_empty[t], (o_count[t] - 1) & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
@@ -984,7 +1076,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (t == 0) {
               // K's stage was last read by the S products that P_t(j) came from
               mma_commit(&k_empty[st]);
-              if (more && !mbar_wait_bounded(&k_full[st ^ 1], ((g + 1) >> 1) & 1, abort_flag)) {
+              if (more && !wait(&k_full[st ^ 1], ((g + 1) >> 1) & 1, abort_flag)) {
                 ok = false;
                 break;
               }
@@ -996,6 +1088,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (ok && j + 2 == n) mma_commit(&q_empty);
         }
         if (!ok) break;
+#pragma unroll 1
         for (int t = 0; t < tiles; ++t) ++o_count[t];
       }
       if (!ok) {
@@ -1014,9 +1107,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const bool in_tile = row < p.tile_rows * p.group;
     bool ok = true;
     uint32_t g = 0, unit = 0;  // key tiles and units of this row tile so far
+#pragma unroll 1
     for (uint32_t index = 0;; ++index) {
       // (the two warps of a lane quarter go on or stop together: they meet at barriers below)
-      const bool late = ok && !mbar_wait_bounded(&task_full[index & 1], (index >> 1) & 1, abort_flag);
+      const bool late = ok && !wait(&task_full[index & 1], (index >> 1) & 1, abort_flag);
       if (barrier_any(bar_id, 64, late || !ok)) {
         ok = false;
         break;
@@ -1047,9 +1141,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&task_empty[index & 1]);
       float m = -INFINITY, l = 0.0f;
+#pragma unroll 1
       for (int32_t j = 0; j < n; ++j, ++g) {
         // (a wait that ran out is not left early: the barriers below need every warp)
-        if (ok && !mbar_wait_bounded(&s_full[t], g & 1, abort_flag)) ok = false;
+        if (ok && !wait(&s_full[t], g & 1, abort_flag)) ok = false;
         tc_fence_after();
         const int32_t key0 = (first + j) * kTileKeys + half * 64;
         uint32_t a[32], b[32];
@@ -1059,10 +1154,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         tmem_regs_fence(b);
         const int from = lo - key0, to = limit - key0;
         if (__any_sync(0xffffffffu, from > 0 || to < 64)) {
+          const uint32_t keep0 = bits_between(from, to), keep1 = bits_between(from - 32, to - 32);
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            if (i < from || i >= to) a[i] = __float_as_uint(-INFINITY);
-            if (i + 32 < from || i + 32 >= to) b[i] = __float_as_uint(-INFINITY);
+            if (!(keep0 >> i & 1u)) a[i] = __float_as_uint(-INFINITY);
+            if (!(keep1 >> i & 1u)) b[i] = __float_as_uint(-INFINITY);
           }
         }
         float mx = -INFINITY, mx1 = -INFINITY;
@@ -1137,7 +1233,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       x_sum[t][half][row] = l;
       named_barrier_sync(bar_id, 64);
       l += x_sum[t][half ^ 1][row];
-      if (ok && !mbar_wait_bounded(&o_final[t], unit & 1, abort_flag)) ok = false;
+      if (ok && !wait(&o_final[t], unit & 1, abort_flag)) ok = false;
       ++unit;
       tc_fence_after();
       if (row_ok && !direct && half == 0) p.tile_ml[slot * p.tile_slot_rows + slot_row] = make_float2(m == -INFINITY ? m : m * c, l);
@@ -1202,28 +1298,26 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 // group), a thread four dims of one of them: so 16-byte reads are neighbours
 // row by row (tile slots) or dim by dim (stream slots).  A row's partials are
 // the pieces of its prefix unit and those of its own unit, both runs of slots.
-template <int32_t N>
-struct Number {
-  static constexpr int32_t value = N;
-};
-
 struct Pieces {
   int64_t slot;    // of the first
   int32_t count, row;
 };
-// Pieces of unit `unit`, tiles [first, first + n) of a line of `line` tiles:
-// CTA c has [line c / C, line (c + 1) / C), so tile t is c = ((t + 1) C - 1) / line's.
-__device__ __forceinline__ Pieces pieces_of(int64_t line, int64_t c, int64_t first, int64_t n, int64_t unit,
-                                            int32_t row) {
+// Pieces of unit `unit`, at [first, first + cost) of a line of length `line`:
+// piece c of C is [line c / C, line (c + 1) / C), so place t is in c = ((t + 1) C
+// - 1) / line, and the unit's tiles are its places from kUnitCost on.
+__device__ __forceinline__ Pieces pieces_of(int64_t line, int64_t c, int64_t first, int64_t cost,
+                                            int64_t unit, int32_t row) {
   Pieces r = {0, 0, row};
-  if (n <= 0) return r;
+  if (cost <= 0) return r;
+  const int64_t last = first + cost;
+  first += kUnitCost;
   int32_t c0, c1;
   if (line * c < (1ll << 31)) {  // (32-bit divisions: a quarter of the time)
     c0 = (int32_t)(((uint32_t)(first + 1) * (uint32_t)c - 1) / (uint32_t)line);
-    c1 = (int32_t)(((uint32_t)(first + n) * (uint32_t)c - 1) / (uint32_t)line);
+    c1 = (int32_t)(((uint32_t)last * (uint32_t)c - 1) / (uint32_t)line);
   } else {
     c0 = (int32_t)(((first + 1) * c - 1) / line);
-    c1 = (int32_t)(((first + n) * c - 1) / line);
+    c1 = (int32_t)((last * c - 1) / line);
   }
   // (in bounds whatever the sums of unsorted row offsets are)
   c0 = max(0, min(c0, (int32_t)c - 1));
@@ -1237,7 +1331,7 @@ __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_cons
   const int32_t dim = (threadIdx.x >> 3) * 4;
   const uint32_t index = blockIdx.x * 8 + (threadIdx.x & 7), row = index / (uint32_t)p.group;
   const int32_t kv = blockIdx.y, in_group = (int32_t)(index - row * (uint32_t)p.group);
-  const int32_t stream_keys = p.stream_prefix ? (p.prefix + kStreamKeys - 1) / kStreamKeys : 0;
+  const int32_t stream_cost = p.stream_prefix ? unit_cost((p.prefix + kStreamKeys - 1) / kStreamKeys) : 0;
   __shared__ Pieces shared_pieces[2][8];  // own, prefix
   griddep_wait();
   // One thread per row and kind finds the pieces.
@@ -1247,17 +1341,17 @@ __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_cons
     PagedRow where;
     if (row < p.rows && paged_row(p.paged, row, where)) {
       r.count = 0;
-      const int32_t tile_keys = (p.prefix + kTileKeys - 1) / kTileKeys, per_unit = 2 * p.tile_rows;
-      if (prefix && stream_keys) {
-        const int64_t line = (int64_t)stream_keys * p.heads + p.stream_sums[p.paged.sequences] * p.heads;
-        r = pieces_of(line, p.stream_sums[p.paged.sequences + 1], (int64_t)kv * stream_keys, stream_keys, kv, (int32_t)index);
+      const int32_t tile_cost = unit_cost((p.prefix + kTileKeys - 1) / kTileKeys), per_unit = 2 * p.tile_rows;
+      if (prefix && stream_cost) {
+        const int64_t line = (int64_t)stream_cost * p.heads + p.stream_sums[p.paged.sequences] * p.heads;
+        r = pieces_of(line, p.stream_sums[p.paged.sequences + 1], (int64_t)kv * stream_cost, stream_cost, kv, (int32_t)index);
       } else if (prefix && p.prefix_units) {
         const int32_t unit = kv * p.prefix_units + (int32_t)row / per_unit;
-        r = pieces_of(p.unit_sums[p.max_units + 1], p.unit_sums[p.max_units + 2], (int64_t)unit * tile_keys, tile_keys, unit,
+        r = pieces_of(p.unit_sums[p.max_units + 1], p.unit_sums[p.max_units + 2], (int64_t)unit * tile_cost, tile_cost, unit,
                       (int32_t)row % per_unit * p.group + in_group);
       } else if (!prefix && p.stream) {
         const int64_t before = p.stream_sums[row], n = p.stream_sums[row + 1] - before;
-        const int64_t ahead = (int64_t)stream_keys * p.heads, line = ahead + p.stream_sums[p.paged.sequences] * p.heads;
+        const int64_t ahead = (int64_t)stream_cost * p.heads, line = ahead + p.stream_sums[p.paged.sequences] * p.heads;
         r = pieces_of(line, p.stream_sums[p.paged.sequences + 1], ahead + before * p.heads + kv * n, n,
                       (int64_t)((int32_t)row + p.stream_prefix) * p.heads + kv, in_group);
       } else if (!prefix && p.tile_own) {
@@ -1266,7 +1360,7 @@ __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_cons
         if (unit < p.max_units) {
           const int64_t before = p.unit_sums[unit], n = p.unit_sums[unit + 1] - before;
           r = pieces_of(p.unit_sums[p.max_units + 1], p.unit_sums[p.max_units + 2],
-                        ((int64_t)p.prefix_units * tile_keys + before) * p.heads + kv * n, n,
+                        ((int64_t)p.prefix_units * tile_cost + before) * p.heads + kv * n, n,
                         (int64_t)(p.prefix_units + unit) * p.heads + kv, place % per_unit * p.group + in_group);
         }
       }
@@ -1279,14 +1373,15 @@ __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_cons
   if (p.prefix == 0 && own.count == 1) return;  // the whole unit was one CTA's, which wrote the result
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float l = 0.0f, top = -INFINITY;
-  // `n` partials' loads are issued before the first is used, with no branch between them.
-  auto join = [&](const Pieces &r, bool stream, auto n) {
-    constexpr int32_t N = decltype(n)::value;
+  // Four partials' loads are issued before the first is used, with no branch between them.
+  auto join = [&](const Pieces &r, bool stream) {
+    constexpr int32_t N = 4;
     const int32_t rows = stream ? p.stream_rows : p.tile_slot_rows;
     const float2 *ml = (stream ? p.stream_ml : p.tile_ml) + r.slot * rows + r.row;
     const float *part = stream ? p.stream_o + (r.slot * rows + r.row) * p.head_dim + dim
                                : p.tile_o + ((r.slot * (p.head_dim >> 2) + (dim >> 2)) * rows + r.row) * 4;
     const int64_t step = (int64_t)rows * p.head_dim;
+#pragma unroll 1
     for (int32_t i = 0; i < r.count; i += N) {
       float2 s[N];
       float4 v[N];
@@ -1322,9 +1417,8 @@ __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_cons
       }
     }
   };
-  if (pre.count > 2) join(pre, stream_keys != 0, Number<4>());
-  else join(pre, stream_keys != 0, Number<2>());
-  join(own, p.stream != 0, Number<2>());
+#pragma unroll 1
+  for (int kind = 0; kind < 2; ++kind) join(kind ? own : pre, kind ? p.stream != 0 : stream_cost != 0);
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint2 v;
   v.x = to_h2(o.x * inv, o.y * inv);
