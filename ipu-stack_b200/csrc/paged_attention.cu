@@ -108,7 +108,8 @@ struct PagedAttnParams {
   int32_t *unit_base;
   int32_t sms;                     // CTAs of each kernel
   int32_t stream, tile;            // which of the two run
-  int32_t stream_prefix;  // the stream kernel takes the prefix too
+  int32_t join_rows;               // rows of a block of the join: 8 or kJoinRows
+  int32_t stream_prefix;  // the stream kernel takes the prefix too, for so many groups of 16 rows; or 0
   int32_t tile_own;       // the tile kernel takes the own parts, in at most max_units row units
   int32_t max_units;
   int32_t prefix_units;   // tile kernel: row units of the prefix
@@ -158,15 +159,25 @@ __device__ __forceinline__ int32_t checked_length(const PagedAttnParams &p, int3
   return n < 0 ? 0 : min(n, max(cap, p.prefix));
 }
 
-// Exclusive sums of count(b) over the block's threads' contiguous shares of
-// [0, n): returns the total; store(b, sum before b) is called for every b.
-template <int kThreads, typename Count, typename Store>
-__device__ __forceinline__ int64_t block_sums(int32_t n, int64_t *scratch, Count count, Store store) {
-  const int32_t share = (n + kThreads - 1) / kThreads;
-  const int32_t lo = min(n, (int32_t)threadIdx.x * share), hi = min(n, lo + share);
+// A thread's contiguous share of [0, n) in a block of kThreads.
+template <int kThreads>
+struct Share {
+  int32_t lo, hi;
+  __device__ __forceinline__ explicit Share(int32_t n) {
+    const int32_t size = (n + kThreads - 1) / kThreads;
+    lo = min(n, (int32_t)threadIdx.x * size);
+    hi = min(n, lo + size);
+  }
+};
+
+// Sum of count(b) over [0, n) by the whole block; `before` becomes the sum in
+// front of this thread's share.
+template <int kThreads, typename Count>
+__device__ __forceinline__ int64_t block_sum(int32_t n, int64_t *scratch, Count count, int64_t &before) {
+  const Share<kThreads> share(n);
   int64_t mine = 0;
 #pragma unroll 1
-  for (int32_t b = lo; b < hi; ++b) mine += count(b);
+  for (int32_t b = share.lo; b < share.hi; ++b) mine += count(b);
   int64_t sum = mine;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll 1
@@ -176,17 +187,12 @@ __device__ __forceinline__ int64_t block_sums(int32_t n, int64_t *scratch, Count
   }
   if (lane == 31) scratch[warp] = sum;
   __syncthreads();
-  int64_t before = 0, total = 0;
+  int64_t total = 0;
+  before = sum - mine;
 #pragma unroll 1
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) before += scratch[w];
     total += scratch[w];
-  }
-  before += sum - mine;
-#pragma unroll 1
-  for (int32_t b = lo; b < hi; ++b) {
-    store(b, before);
-    before += count(b);
   }
   return total;
 }
@@ -213,8 +219,9 @@ __device__ __forceinline__ int32_t checked_page(const PagedAttnParams &p, int32_
 // and K and V are streamed once: HBM-bound.  The key tiles (64 keys, at
 // absolute multiples of 64) of all (sequence, head) units form one line that
 // is cut into equal pieces, one per CTA, so ragged lengths leave no CTA idle.
-// When all rows of the call fit one m16 tile, the shared prefix is on the line
-// too, as a first unit per head.
+// When the call has so few rows that the tile kernel's start would cost more,
+// the shared prefix is on the line too, in front, as a unit per head and group
+// of 16 rows (the later groups' reads of it come from L2).
 // A CTA is two workers with a piece each: a producer warp fills a ring of
 // tiles by TMA, box by box of gcd(page_size, 64) keys; four warps take 16 keys
 // of every tile each, with a running maximum, sum and O of their own, and meet
@@ -245,10 +252,11 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A worker's place on the line: unit (b, h), keys [lo, hi); b = -1: the prefix.
+// A worker's place on the line: unit (b, h), keys [lo, hi); b = -1: the prefix,
+// for rows [16 rows16, 16 rows16 + 16) of the call.
 struct StreamWalk {
   LinePlace at;
-  int32_t b, h, lo, hi;
+  int32_t b, h, rows16, lo, hi;
 
   __device__ __forceinline__ static int32_t tiles(const PagedAttnParams &p, int32_t len) {
     return len > p.prefix ? (len + kStreamKeys - 1) / kStreamKeys - p.prefix / kStreamKeys : 0;
@@ -267,6 +275,8 @@ struct StreamWalk {
   }
   __device__ __noinline__ void next(const PagedAttnParams &p) {
     if (!at.pass()) return;
+    if (b < 0 && ++rows16 < p.stream_prefix) return;
+    rows16 = 0;
     if (++h < p.heads) return;
     h = 0;
 #pragma unroll 1
@@ -328,47 +338,61 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  griddep_launch_dependents();
   auto count = [&](int32_t b) { return unit_cost(StreamWalk::tiles(p, checked_length(p, b, blockIdx.x == 0))); };
   // Sums first, then this worker's piece [W c / C, W (c + 1) / C) of the line's W.
-  const int64_t total = block_sums<kStreamThreads>(p.paged.sequences, scratch, count, [&](int32_t b, int64_t sum) {
-    if (blockIdx.x == 0) p.stream_sums[b] = sum;
-  });
-  const int64_t ahead = p.stream_prefix ? (int64_t)unit_cost((p.prefix + kStreamKeys - 1) / kStreamKeys) * p.heads : 0;
+  int64_t before;
+  const int64_t total = block_sum<kStreamThreads>(p.paged.sequences, scratch, count, before);
+  const int64_t ahead = (int64_t)unit_cost((p.prefix + kStreamKeys - 1) / kStreamKeys) * p.stream_prefix * p.heads;
   const int64_t line = ahead + total * p.heads;
-  const int64_t share = p.stream_prefix ? p.sms : stream_sms(p, total);
-  const int64_t pieces = min(kStreamWorkers * share, line);  // no piece is empty
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    p.stream_sums[p.paged.sequences] = total;
-    p.stream_sums[p.paged.sequences + 1] = pieces;
-  }
-  if ((int64_t)blockIdx.x >= share || blockIdx.x >= pieces) return;
-  // Worker w of CTA c has piece w * share + c: few pieces spread over many SMs.
-  auto piece_of = [&](int w) { return w * share + (int64_t)blockIdx.x; };
+  const int64_t sms = p.stream_prefix ? p.sms : stream_sms(p, total);
+  const int64_t pieces = min(kStreamWorkers * sms, line);  // no piece is empty
+  // Worker w of CTA c has piece w * sms + c: few pieces spread over many SMs.
+  auto piece_of = [&](int w) { return w * sms + (int64_t)blockIdx.x; };
   auto start_of = [&](int w) { return line * piece_of(w) / pieces; };
-  __syncthreads();  // scratch is read before it is written again
-  block_sums<kStreamThreads>(p.paged.sequences, scratch, count, [&](int32_t b, int64_t sum) {
+  const bool idle = (int64_t)blockIdx.x >= min(sms, pieces);
+  if (blockIdx.x == 0) {
+    const Share<kStreamThreads> mine(p.paged.sequences);
+    int64_t sum = before;
+#pragma unroll 1
+    for (int32_t b = mine.lo; b < mine.hi; ++b) {
+      p.stream_sums[b] = sum;
+      sum += count(b);
+    }
+    if (threadIdx.x == 0) {
+      p.stream_sums[p.paged.sequences] = total;
+      p.stream_sums[p.paged.sequences + 1] = pieces;
+    }
+    if (idle) griddep_wait();  // (see the end)
+  }
+  if (idle) return;
+  const Share<kStreamThreads> mine(p.paged.sequences);
+#pragma unroll 1
+  for (int32_t b = mine.lo; b < mine.hi; ++b) {
     const int32_t n = count(b);
 #pragma unroll 1
     for (int w = 0; w < kStreamWorkers; ++w) {
-      const int64_t at = start_of(w) - ahead - sum * p.heads;
+      const int64_t at = start_of(w) - ahead - before * p.heads;
       if (at >= 0 && at < (int64_t)n * p.heads) {
         first_unit[w][0] = b;
         first_unit[w][1] = (int32_t)(at / n);
         first_unit[w][2] = (int32_t)(at % n);
       }
     }
-  });
+    before += n;
+  }
   __syncthreads();  // (the barriers' initialisation too)
   const int64_t cta = piece_of(worker), start = start_of(worker);
-  if (cta >= pieces) return;
+  if (cta >= pieces) return;  // (a second worker)
   StreamWalk w;
   w.at.left = line * (cta + 1) / pieces - start;
   if (start < ahead) {
     w.enter(p, -1);
-    w.h = (int32_t)(start / unit_cost(w.at.n));
+    const int32_t unit = (int32_t)(start / unit_cost(w.at.n));
+    w.h = unit / p.stream_prefix;
+    w.rows16 = unit % p.stream_prefix;
     w.at.x = (int32_t)(start % unit_cost(w.at.n));
   } else {
+    w.rows16 = 0;
     w.enter(p, first_unit[worker][0]);
     w.h = first_unit[worker][1];
     w.at.x = first_unit[worker][2];
@@ -426,13 +450,13 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   // Consumers.  A fragments: rows lane / 4 and lane / 4 + 8 of the unit: the
   // group's heads, or (prefix) those of all rows of the call.
   const int r0 = lane >> 2, r1 = r0 + 8, cq = (lane & 3) * 2;
-  auto unit_rows = [&](const StreamWalk &u) { return u.b < 0 ? (int)p.rows * p.group : p.group; };
+  auto unit_rows = [&](const StreamWalk &u) { return u.b < 0 ? min(16, (int)p.rows * p.group - u.rows16 * 16) : p.group; };
   auto load_q = [&](const StreamWalk &u, uint32_t (&a)[KS][4]) {
     const int n = u.at.left > 0 ? unit_rows(u) : 0;
     const uint16_t *base[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      const int row = x ? r1 : r0, token = row / p.group;
+      const int row = u.rows16 * 16 + (x ? r1 : r0), token = row / p.group;
       base[x] = p.q + (u.b < 0 ? token : u.b) * p.q_stride + (u.h * p.group + row - token * p.group) * p.head_dim;
     }
 #pragma unroll
@@ -483,7 +507,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       for (int x = 0; x < 4; ++x)
         if (warp_m[x][orow] != -INFINITY) sum += warp_l[x][orow] * ex2_approx((warp_m[x][orow] - top) * c);
       const bool whole = p.prefix == 0 && count_here == w.at.n;
-      const int64_t unit = (int64_t)(w.b + p.stream_prefix) * p.heads + w.h;
+      const int64_t unit = w.b < 0 ? w.h * p.stream_prefix + w.rows16 : (int64_t)(w.b + p.stream_prefix) * p.heads + w.h;
       const int64_t slot = (unit + cta) * p.stream_rows + orow;
       const int rows_here = unit_rows(w);
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -528,8 +552,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     // Keys a row attends to end at the unit's end, in the prefix perhaps before it.
     int32_t end0 = w.hi, end1 = w.hi, end = w.hi;
     if (w.b < 0) {
-      if (r0 < (int)p.rows * p.group) end0 = min(w.hi, max(0, p.paged.lengths[r0 / p.group]));
-      if (r1 < (int)p.rows * p.group) end1 = min(w.hi, max(0, p.paged.lengths[r1 / p.group]));
+      const int n = (int)p.rows * p.group, s0 = w.rows16 * 16 + r0, s1 = s0 + 8;
+      if (s0 < n) end0 = min(w.hi, max(0, p.paged.lengths[s0 / p.group]));
+      if (s1 < n) end1 = min(w.hi, max(0, p.paged.lengths[s1 / p.group]));
       end = __reduce_min_sync(0xffffffffu, min(end0, end1));
     }
     m0 = m1 = -INFINITY;
@@ -630,6 +655,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     if (lane == 0) record_device_error(p.err, ERR_KERNEL_PAGED_ATTENTION | ERR_SITE_EPILOGUE);
     *abort_flag = 1;
   }
+  // What follows waits for this grid, so it ends after the tile kernel, beside
+  // which it runs.
+  if (blockIdx.x == 0) griddep_wait();
 }
 
 // ---- many rows: tiles of 128 on the tensor cores --------------------------------
@@ -664,6 +692,12 @@ struct TileWalk {
   int32_t rows, lo, hi;      // batch rows; keys [lo, hi)
   int64_t row0, pos0;        // first batch row and (own part) its position
 
+  // Key tiles of row unit j of a sequence with rows [begin, end), the first at position `pos`.
+  __device__ __forceinline__ static int32_t own_tiles(const PagedAttnParams &p, int32_t begin, int32_t end, int64_t pos,
+                                                      int32_t len, int32_t j) {
+    const int64_t to = min((int64_t)len, pos + min((int64_t)(end - begin), (int64_t)(j + 1) * 2 * p.tile_rows));
+    return to > p.prefix ? (int32_t)((to + kTileKeys - 1) / kTileKeys) - p.prefix / kTileKeys : 0;
+  }
   __device__ __noinline__ void own(const PagedAttnParams &p, int32_t b, int32_t row_unit) {
     const int32_t begin = first_row(p, b), end = first_row(p, b + 1), per_unit = 2 * p.tile_rows;
     seq = b;
@@ -672,8 +706,9 @@ struct TileWalk {
     rows = (int32_t)max((int64_t)0, min((int64_t)per_unit, end - row0));
     pos0 = (int64_t)p.paged.lengths[b] - (end - begin) + (row0 - begin);
     lo = p.prefix;
-    hi = (int32_t)max((int64_t)0, min((int64_t)checked_length(p, b, false), pos0 + rows));
-    at.n = rows > 0 && hi > lo ? (hi + kTileKeys - 1) / kTileKeys - lo / kTileKeys : 0;
+    const int32_t len = checked_length(p, b, false);
+    hi = (int32_t)max((int64_t)0, min((int64_t)len, pos0 + rows));
+    at.n = own_tiles(p, begin, end, pos0 - (row0 - begin), len, j);
   }
   __device__ __forceinline__ void prefix(const PagedAttnParams &p, int32_t row_unit) {
     const int32_t per_unit = 2 * p.tile_rows;
@@ -804,55 +839,63 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int64_t cta = blockIdx.x;
   const int64_t ahead = (int64_t)p.prefix_units * p.heads * unit_cost((p.prefix + kTileKeys - 1) / kTileKeys);
   // Row units (above 2^40) and the length of sequence b's own part per head, in one sum.
+  constexpr int64_t kLength = (1ll << 40) - 1;
   auto count = [&](int32_t b) {
-    const int32_t u = TileWalk::units(p, b);
+    const int32_t begin = first_row(p, b), end = first_row(p, b + 1), u = TileWalk::units(p, b);
+    const int32_t len = checked_length(p, b, cta == 0);
+    const int64_t pos0 = (int64_t)p.paged.lengths[b] - (end - begin);
     int64_t sum = (int64_t)u << 40;
-    TileWalk w;
 #pragma unroll 1
-    for (int32_t j = 0; j < u; ++j) {
-      w.own(p, b, j);
-      sum += unit_cost(w.at.n);
-    }
+    for (int32_t j = 0; j < u; ++j) sum += unit_cost(TileWalk::own_tiles(p, begin, end, pos0, len, j));
     return sum;
   };
-  int64_t total = 0;
-  int32_t share = p.sms;
-  if (p.stream) {
-    const int64_t own_cost = block_sums<kTileThreads>(
-        p.paged.sequences, scratch, [&](int32_t b) { return unit_cost(StreamWalk::tiles(p, checked_length(p, b, false))); },
-        [](int32_t, int64_t) {});
-    share -= stream_sms(p, own_cost);
-  }
-  if (p.tile_own) {
-    if (cta == 0)
+  int64_t total = 0, before = 0;
+  int32_t sms = p.sms;
+  if (p.stream)
+    sms -= stream_sms(p, block_sum<kTileThreads>(
+                             p.paged.sequences, scratch,
+                             [&](int32_t b) { return unit_cost(StreamWalk::tiles(p, checked_length(p, b, false))); },
+                             before));
+  if (p.tile_own) total = block_sum<kTileThreads>(p.paged.sequences, scratch, count, before);
+  const int64_t line = ahead + (total & kLength) * p.heads, ctas = min((int64_t)sms, line);
+  const bool idle = cta >= ctas;  // no piece is empty
+  const int64_t start = idle ? -1 : line * cta / ctas;
+  griddep_launch_dependents();
+  if (p.tile_own && (!idle || cta == 0)) {
+    const Share<kTileThreads> mine(p.paged.sequences);
 #pragma unroll 1
-      for (int32_t b = threadIdx.x; b < p.paged.sequences; b += kTileThreads) checked_length(p, b, true);
-    total = block_sums<kTileThreads>(p.paged.sequences, scratch, count, [&](int32_t b, int64_t sum) {
-      if (cta != 0) return;
-      const int32_t base = (int32_t)(sum >> 40), u = TileWalk::units(p, b);
-      int64_t cost = sum & ((1ll << 40) - 1);
-      p.unit_base[b] = base;
-      TileWalk w;
+    for (int32_t b = mine.lo; b < mine.hi; ++b) {
+      const int32_t begin = first_row(p, b), end = first_row(p, b + 1), u = TileWalk::units(p, b);
+      const int32_t base = (int32_t)(before >> 40), len = checked_length(p, b, false);
+      const int64_t pos0 = (int64_t)p.paged.lengths[b] - (end - begin);
+      int64_t cost = before & kLength;
+      if (cta == 0) p.unit_base[b] = base;
 #pragma unroll 1
-      for (int32_t j = 0; j < u && base + j < p.max_units; ++j) {
-        p.unit_sums[base + j] = cost;
-        w.own(p, b, j);
-        cost += unit_cost(w.at.n);
-        p.unit_sums[base + j + 1] = cost;
+      for (int32_t j = 0; j < u; ++j) {
+        const int32_t n = unit_cost(TileWalk::own_tiles(p, begin, end, pos0, len, j));
+        const int64_t at = start - ahead - cost * p.heads;
+        if (at >= 0 && at < (int64_t)n * p.heads) {
+          found[0] = b;
+          found[1] = j;
+          found[2] = (int32_t)(at / n);
+          found[3] = (int32_t)(at % n);
+          found[4] = base + j;
+        }
+        if (cta == 0 && base + j < p.max_units) {
+          p.unit_sums[base + j] = cost;
+          p.unit_sums[base + j + 1] = cost + n;
+        }
+        cost += n;
       }
-    });
+      before = ((before >> 40) + u) << 40 | cost;
+    }
   }
-  const int64_t line = ahead + (total & ((1ll << 40) - 1)) * p.heads, ctas = min((int64_t)share, line);
   if (cta == 0 && threadIdx.x == 0) {
     p.unit_sums[p.max_units + 1] = line;
     p.unit_sums[p.max_units + 2] = ctas;
   }
-  griddep_launch_dependents();
-  if (cta >= ctas) {  // no piece is empty
-    if (cta == 0) griddep_wait();
-    return;
-  }
-  const int64_t start = line * cta / ctas;
+  if (idle) return;
+  __syncthreads();
   TileWalk walk;
   walk.unit = -1;
   if (start < ahead) {
@@ -862,25 +905,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     walk.prefix(p, (int32_t)(u % p.prefix_units));
     walk.at.x = (int32_t)(start % unit_cost(walk.at.n));
   } else {
-    __syncthreads();  // scratch is read before it is written again
-    block_sums<kTileThreads>(p.paged.sequences, scratch, count, [&](int32_t b, int64_t sum) {
-      int64_t at = start - ahead - (sum & ((1ll << 40) - 1)) * p.heads;
-      if (at < 0 || at >= (count(b) & ((1ll << 40) - 1)) * p.heads) return;
-      TileWalk w;
-      int32_t j = 0;
-#pragma unroll 1
-      for (;; ++j) {
-        w.own(p, b, j);
-        if (at < (int64_t)unit_cost(w.at.n) * p.heads) break;
-        at -= (int64_t)unit_cost(w.at.n) * p.heads;
-      }
-      found[0] = b;
-      found[1] = j;
-      found[2] = (int32_t)(at / unit_cost(w.at.n));
-      found[3] = (int32_t)(at % unit_cost(w.at.n));
-      found[4] = (int32_t)(sum >> 40) + j;
-    });
-    __syncthreads();
     walk.own(p, found[0], found[1]);
     walk.h = found[2];
     walk.at.x = found[3];
@@ -1288,8 +1312,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  // The join waits for this grid alone: it ends after the stream kernel's, with which it runs.
-  if (cta == 0) griddep_wait();
 }
 
 // ---- the partial results' sum -----------------------------------------------------
@@ -1327,31 +1349,34 @@ __device__ __forceinline__ Pieces pieces_of(int64_t line, int64_t c, int64_t fir
   return r;
 }
 
+constexpr int kJoinRows = 32;
 __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_constant__ PagedAttnParams p) {
-  const int32_t dim = (threadIdx.x >> 3) * 4;
-  const uint32_t index = blockIdx.x * 8 + (threadIdx.x & 7), row = index / (uint32_t)p.group;
-  const int32_t kv = blockIdx.y, in_group = (int32_t)(index - row * (uint32_t)p.group);
+  const int32_t dim = (threadIdx.x >> 3) * 4, kv = blockIdx.y;
   const int32_t stream_cost = p.stream_prefix ? unit_cost((p.prefix + kStreamKeys - 1) / kStreamKeys) : 0;
-  __shared__ Pieces shared_pieces[2][8];  // own, prefix
-  griddep_wait();
+  __shared__ Pieces shared_pieces[2][kJoinRows];  // own, prefix
   // One thread per row and kind finds the pieces.
-  if ((threadIdx.x & 31) < 8 && threadIdx.x < 64) {
-    const bool prefix = threadIdx.x >= 32;
+  if (threadIdx.x < 2 * kJoinRows && (int32_t)(threadIdx.x % kJoinRows) < p.join_rows) {
+    const bool prefix = threadIdx.x >= kJoinRows;
+    const uint32_t index = blockIdx.x * p.join_rows + threadIdx.x % kJoinRows, row = index / (uint32_t)p.group;
+    const int32_t in_group = (int32_t)(index - row * (uint32_t)p.group);
     Pieces r = {0, -1, 0};
     PagedRow where;
     if (row < p.rows && paged_row(p.paged, row, where)) {
       r.count = 0;
       const int32_t tile_cost = unit_cost((p.prefix + kTileKeys - 1) / kTileKeys), per_unit = 2 * p.tile_rows;
       if (prefix && stream_cost) {
-        const int64_t line = (int64_t)stream_cost * p.heads + p.stream_sums[p.paged.sequences] * p.heads;
-        r = pieces_of(line, p.stream_sums[p.paged.sequences + 1], (int64_t)kv * stream_cost, stream_cost, kv, (int32_t)index);
+        const int64_t line = ((int64_t)stream_cost * p.stream_prefix + p.stream_sums[p.paged.sequences]) * p.heads;
+        const int32_t unit = kv * p.stream_prefix + (int32_t)index / 16;
+        r = pieces_of(line, p.stream_sums[p.paged.sequences + 1], (int64_t)unit * stream_cost, stream_cost, unit,
+                      (int32_t)index % 16);
       } else if (prefix && p.prefix_units) {
         const int32_t unit = kv * p.prefix_units + (int32_t)row / per_unit;
         r = pieces_of(p.unit_sums[p.max_units + 1], p.unit_sums[p.max_units + 2], (int64_t)unit * tile_cost, tile_cost, unit,
                       (int32_t)row % per_unit * p.group + in_group);
       } else if (!prefix && p.stream) {
         const int64_t before = p.stream_sums[row], n = p.stream_sums[row + 1] - before;
-        const int64_t ahead = (int64_t)stream_cost * p.heads, line = ahead + p.stream_sums[p.paged.sequences] * p.heads;
+        const int64_t ahead = (int64_t)stream_cost * p.stream_prefix * p.heads;
+        const int64_t line = ahead + p.stream_sums[p.paged.sequences] * p.heads;
         r = pieces_of(line, p.stream_sums[p.paged.sequences + 1], ahead + before * p.heads + kv * n, n,
                       (int64_t)((int32_t)row + p.stream_prefix) * p.heads + kv, in_group);
       } else if (!prefix && p.tile_own) {
@@ -1365,38 +1390,48 @@ __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_cons
         }
       }
     }
-    shared_pieces[prefix][threadIdx.x & 7] = r;
+    shared_pieces[prefix][threadIdx.x % kJoinRows] = r;
   }
   __syncthreads();
-  const Pieces own = shared_pieces[0][threadIdx.x & 7], pre = shared_pieces[1][threadIdx.x & 7];
-  if (own.count < 0 || dim >= p.head_dim) return;  // padding
-  if (p.prefix == 0 && own.count == 1) return;  // the whole unit was one CTA's, which wrote the result
-  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float l = 0.0f, top = -INFINITY;
-  // Four partials' loads are issued before the first is used, with no branch between them.
-  auto join = [&](const Pieces &r, bool stream) {
-    constexpr int32_t N = 4;
-    const int32_t rows = stream ? p.stream_rows : p.tile_slot_rows;
-    const float2 *ml = (stream ? p.stream_ml : p.tile_ml) + r.slot * rows + r.row;
-    const float *part = stream ? p.stream_o + (r.slot * rows + r.row) * p.head_dim + dim
-                               : p.tile_o + ((r.slot * (p.head_dim >> 2) + (dim >> 2)) * rows + r.row) * 4;
-    const int64_t step = (int64_t)rows * p.head_dim;
+  if (dim >= p.head_dim) return;
 #pragma unroll 1
-    for (int32_t i = 0; i < r.count; i += N) {
-      float2 s[N];
-      float4 v[N];
+  for (int32_t sub = threadIdx.x & 7; sub < p.join_rows; sub += 8) {
+    const Pieces own = shared_pieces[0][sub], pre = shared_pieces[1][sub];
+    if (own.count < 0) continue;  // padding
+    if (p.prefix == 0 && own.count == 1) continue;  // the whole unit was one CTA's, which wrote the result
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float l = 0.0f, top = -INFINITY;
+    // Four partials' loads are issued before the first is used, with no branch between them.
+    const bool pre_stream = stream_cost != 0, own_stream = p.stream != 0;
+    const int32_t pre_rows = pre_stream ? p.stream_rows : p.tile_slot_rows, own_rows = own_stream ? p.stream_rows : p.tile_slot_rows;
+    auto ml_of = [&](const Pieces &r, bool stream, int32_t rows) {
+      return (stream ? p.stream_ml : p.tile_ml) + r.slot * rows + r.row;
+    };
+    auto part_of = [&](const Pieces &r, bool stream, int32_t rows) {
+      return stream ? p.stream_o + (r.slot * rows + r.row) * p.head_dim + dim
+                    : p.tile_o + ((r.slot * (p.head_dim >> 2) + (dim >> 2)) * rows + r.row) * 4;
+    };
+    const float2 *pre_ml = ml_of(pre, pre_stream, pre_rows), *own_ml = ml_of(own, own_stream, own_rows) - (int64_t)pre.count * own_rows;
+    const int64_t pre_step = (int64_t)pre_rows * p.head_dim, own_step = (int64_t)own_rows * p.head_dim;
+    const float *pre_part = part_of(pre, pre_stream, pre_rows), *own_part = part_of(own, own_stream, own_rows) - pre.count * own_step;
+    const int32_t count = pre.count + own.count;
+#pragma unroll 1
+    for (int32_t i = 0; i < count; i += 4) {
+      float2 s[4];
+      float4 v[4];
       float t = top;
 #pragma unroll
-      for (int32_t x = 0; x < N; ++x) {
+      for (int32_t x = 0; x < 4; ++x) {
         s[x] = make_float2(-INFINITY, 0.0f);
         v[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (i + x < r.count) {
-          s[x] = ml[(int64_t)(i + x) * rows];
-          v[x] = *reinterpret_cast<const float4 *>(part + (i + x) * step);
+        if (i + x < count) {
+          const bool first = i + x < pre.count;
+          s[x] = first ? pre_ml[(int64_t)(i + x) * pre_rows] : own_ml[(int64_t)(i + x) * own_rows];
+          v[x] = *reinterpret_cast<const float4 *>(first ? pre_part + (i + x) * pre_step : own_part + (i + x) * own_step);
         }
       }
 #pragma unroll
-      for (int32_t x = 0; x < N; ++x) t = fmaxf(t, s[x].x);
+      for (int32_t x = 0; x < 4; ++x) t = fmaxf(t, s[x].x);
       if (t == -INFINITY) continue;  // no keys
       const float a = ex2_approx(top - t);
       top = t;
@@ -1406,7 +1441,7 @@ __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_cons
       o.z *= a;
       o.w *= a;
 #pragma unroll
-      for (int32_t x = 0; x < N; ++x) {
+      for (int32_t x = 0; x < 4; ++x) {
         if (s[x].x == -INFINITY) continue;  // (its O was not written)
         const float w = ex2_approx(s[x].x - t);
         l = fmaf(s[x].y, w, l);
@@ -1416,14 +1451,14 @@ __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_cons
         o.w = fmaf(v[x].w, w, o.w);
       }
     }
-  };
-#pragma unroll 1
-  for (int kind = 0; kind < 2; ++kind) join(kind ? own : pre, kind ? p.stream != 0 : stream_cost != 0);
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint2 v;
-  v.x = to_h2(o.x * inv, o.y * inv);
-  v.y = to_h2(o.z * inv, o.w * inv);
-  *reinterpret_cast<uint2 *>(p.out + ((int64_t)row * p.q_heads + kv * p.group + in_group) * p.head_dim + dim) = v;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint2 v;
+    v.x = to_h2(o.x * inv, o.y * inv);
+    v.y = to_h2(o.z * inv, o.w * inv);
+    const uint32_t index = blockIdx.x * p.join_rows + sub, row = index / (uint32_t)p.group;
+    const int32_t in_group = (int32_t)(index - row * (uint32_t)p.group);
+    *reinterpret_cast<uint2 *>(p.out + ((int64_t)row * p.q_heads + kv * p.group + in_group) * p.head_dim + dim) = v;
+  }
 }
 
 // ---- host ---------------------------------------------------------------------------
@@ -1432,7 +1467,8 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // How a call is cut up, from sizes the host knows, and its workspace.
 struct PagedPlan {
-  bool stream, stream_prefix;  // the stream kernel takes single rows, and their prefix if all fit one m16 tile
+  bool stream;                 // the stream kernel takes single rows
+  int32_t stream_prefix;       // and their prefix, for so many groups of 16 rows
   bool tile, tile_own;         // the tile kernel runs; takes the own parts
   int32_t sms, stream_rows, tile_rows, tile_slot_rows;
   int64_t prefix_units, max_units;
@@ -1446,10 +1482,16 @@ PagedPlan paged_plan(int64_t rows, int64_t sequences, int64_t q_heads, int64_t h
   plan.sms = sm_count();
   plan.stream = !ragged && group <= 16;
   plan.tile_own = !plan.stream;
-  plan.stream_prefix = plan.stream && prefix_rows > 0 && rows * group <= 16;
+  // The stream kernel takes the prefix too where its extra time, 0.6 us a key
+  // tile and SM, is below the tile kernel's start (23 rows of 16 heads behind
+  // 729 positions: XX against 27 us).
+  const int64_t groups = ceil_div(rows * group, 16);
+  if (plan.stream && prefix_rows > 0 && groups * heads * ceil_div(prefix_rows, kStreamKeys) * 0.6 < plan.sms * 8.0)
+    plan.stream_prefix = (int32_t)groups;
+  if (plan.stream && prefix_rows > 0 && groups == 1) plan.stream_prefix = 1;
   plan.tile_rows = (int32_t)(kTileRows / group);
   plan.tile_slot_rows = (int32_t)(2 * plan.tile_rows * group);
-  plan.stream_rows = (int32_t)(plan.stream_prefix ? rows * group : group);
+  plan.stream_rows = (int32_t)(plan.stream_prefix ? 16 : group);
   const int64_t per_unit = 2 * plan.tile_rows;
   uint64_t at = 0;
   auto take = [&](uint64_t bytes) {
@@ -1459,7 +1501,7 @@ PagedPlan paged_plan(int64_t rows, int64_t sequences, int64_t q_heads, int64_t h
   };
   if (plan.stream) {
     const int64_t slots =
-        ((sequences + (plan.stream_prefix ? 1 : 0)) * heads + kStreamWorkers * plan.sms) * plan.stream_rows;
+        ((sequences + plan.stream_prefix) * heads + kStreamWorkers * plan.sms) * plan.stream_rows;
     plan.stream_o = take(slots * head_dim * 4);
     plan.stream_ml = take(slots * 8);
     plan.stream_sums = take((sequences + 2) * 8);
@@ -1594,10 +1636,10 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
     st = make_map_paged(&tm_q, q, d, p.group, cache->heads, p.rows, d, p.group * d, q_stride, p.group, p.tile_rows);
     if (st != IPUC_OK) return st;
   }
-  // The kernels after the first start early (programmatic dependent launch):
-  // the tile kernel beside the stream kernel, on the SMs that leaves it; the
-  // join waits for both.
-  auto launch = [&](auto kernel, dim3 grid, int threads, int bytes, bool first, auto... args) -> ipuc_status {
+  // The stream kernel runs beside the tile kernel, whose start takes longer, on
+  // the SMs that leaves it (programmatic dependent launch).  The join is an
+  // ordinary launch: an early one measured 3.5 us slower for few rows.
+  auto launch = [&](auto kernel, dim3 grid, int threads, int bytes, bool beside, auto... args) -> ipuc_status {
     if (bytes) IPUC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
@@ -1608,18 +1650,21 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = first ? 0 : 1;
+    cfg.numAttrs = beside ? 1 : 0;
     IPUC_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
     return check_launch("paged_attention");
   };
-  if (plan.stream) {
-    st = d > 64 ? launch(paged_stream_kernel<128>, p.sms, kStreamThreads, stream_smem_bytes<128>(), true, tm_k, tm_v, p)
-                : launch(paged_stream_kernel<64>, p.sms, kStreamThreads, stream_smem_bytes<64>(), true, tm_k, tm_v, p);
-    if (st != IPUC_OK) return st;
-  }
   if (plan.tile) {
-    st = launch(paged_tile_kernel, p.sms, kTileThreads, kTileSmem, !plan.stream, tm_q, tm_k, tm_v, p);
+    st = launch(paged_tile_kernel, p.sms, kTileThreads, kTileSmem, false, tm_q, tm_k, tm_v, p);
     if (st != IPUC_OK) return st;
   }
-  return launch(paged_combine_kernel, dim3((unsigned)ceil_div(p.rows * p.group, 8), (unsigned)p.heads), 256, 0, false, p);
+  if (plan.stream) {
+    st = d > 64 ? launch(paged_stream_kernel<128>, p.sms, kStreamThreads, stream_smem_bytes<128>(), plan.tile, tm_k, tm_v, p)
+                : launch(paged_stream_kernel<64>, p.sms, kStreamThreads, stream_smem_bytes<64>(), plan.tile, tm_k, tm_v, p);
+    if (st != IPUC_OK) return st;
+  }
+  // Few rows: many small blocks; more than fill the GPU: fewer, which find their pieces at once.
+  p.join_rows = p.rows * q_heads >= 8 * 4 * (int64_t)p.sms ? kJoinRows : 8;
+  return launch(paged_combine_kernel, dim3((unsigned)ceil_div(p.rows * p.group, p.join_rows), (unsigned)p.heads), 256, 0,
+                false, p);
 }
