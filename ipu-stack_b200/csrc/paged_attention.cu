@@ -92,6 +92,7 @@ struct PagedAttnParams {
   int64_t q_stride, rows;
   int32_t q_heads, heads, group, head_dim, prefix;
   int32_t chunk;          // keys per TMA box: gcd(page_size, 64)
+  int32_t pitch, stages;  // stream kernel: bytes from key to key in shared memory, ring stages
   float scale_log2;       // softmax scale * log2(e)
   // Each kernel lays its units (rows that read the same keys of one head) on a
   // line, a unit's length being its key tiles and kUnitCost more for its start
@@ -226,11 +227,26 @@ __device__ __forceinline__ int32_t checked_page(const PagedAttnParams &p, int32_
 // tiles by TMA, box by box of gcd(page_size, 64) keys; four warps take 16 keys
 // of every tile each, with a running maximum, sum and O of their own, and meet
 // once per unit.
-constexpr int kStreamKeys = 64, kStreamStages = 3, kStreamWorkers = 2, kStreamThreads = kStreamWorkers * 160, kMergeLd = 36;
+// K and V rows lie `pitch` bytes apart in shared memory, an odd multiple of 16
+// where the boxes' 128-byte alignment allows it: then ldmatrix's eight rows meet
+// no bank twice, without a swizzle, and a row is one box whatever head_dim is
+// (in swizzled halves of 64 elements, heads of 72 held 16 KB a tile for 9 KB of
+// keys and ran at 0.52 of HBM).  The ring has as many stages as fit.
+constexpr int kStreamKeys = 64, kStreamWorkers = 2, kStreamThreads = kStreamWorkers * 160, kMergeLd = 36;
+constexpr int kStreamStages = 8;  // at most
+constexpr int kMergeBytes = 4 * 16 * kMergeLd * 4, kStreamRingBytes = 105600;
 
-template <int DP>
-constexpr int stream_smem_bytes() {
-  return kStreamWorkers * (kStreamStages * 2 * kStreamKeys * DP * 2 + 4 * 16 * kMergeLd * 4) + 1024;
+struct StreamShape {
+  int32_t pitch, stages, bytes;  // bytes: dynamic shared memory
+};
+StreamShape stream_shape(int32_t padded_dim, int32_t chunk) {
+  StreamShape r;
+  const int32_t align = 128 / (chunk < 8 ? chunk : 8);
+  r.pitch = (padded_dim * 2 + 16 + align - 1) / align * align;
+  const int32_t stage = 2 * kStreamKeys * r.pitch;
+  r.stages = kStreamRingBytes / stage < kStreamStages ? kStreamRingBytes / stage : kStreamStages;
+  r.bytes = kStreamWorkers * (r.stages * stage + kMergeBytes) + 1024;
+  return r;
 }
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
@@ -308,11 +324,10 @@ template <int DP>
 __global__ void __launch_bounds__(kStreamThreads, 1)
     paged_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const __grid_constant__ PagedAttnParams p) {
-  constexpr int HALVES = DP / 64, KS = DP / 16, NT = DP / 8;
-  constexpr int HALF_BYTES = kStreamKeys * 128, TILE_BYTES = HALVES * HALF_BYTES;  // K or V of a tile
+  constexpr int KS = DP / 16, NT = DP / 8;
+  const int tile_bytes = kStreamKeys * p.pitch, ring_bytes = p.stages * 2 * tile_bytes;  // K or V of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  constexpr int RING_BYTES = kStreamStages * 2 * TILE_BYTES;
   __shared__ uint64_t all_full[kStreamWorkers][kStreamStages], all_empty[kStreamWorkers][kStreamStages];
   __shared__ int64_t scratch[kStreamThreads / 32];
   __shared__ int32_t first_unit[kStreamWorkers][3];
@@ -323,13 +338,13 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   const int worker = threadIdx.x / 160, warp = (threadIdx.x >> 5) % 5, lane = threadIdx.x & 31;
   uint64_t *full = all_full[worker], *empty = all_empty[worker];
   float(&warp_m)[4][16] = all_m[worker], (&warp_l)[4][16] = all_l[worker];
-  float *merge = reinterpret_cast<float *>(smem + kStreamWorkers * RING_BYTES) + worker * 4 * 16 * kMergeLd;
-  smem += worker * RING_BYTES;
+  float *merge = reinterpret_cast<float *>(smem + kStreamWorkers * ring_bytes + worker * kMergeBytes);
+  smem += worker * ring_bytes;
   if (threadIdx.x == 0) {
 #pragma unroll 1
     for (int w = 0; w < kStreamWorkers; ++w)
 #pragma unroll 1
-      for (int i = 0; i < kStreamStages; ++i) {
+      for (int i = 0; i < p.stages; ++i) {
         mbar_init(&all_full[w][i], 1);
         mbar_init(&all_empty[w][i], 4);
       }
@@ -399,12 +414,13 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   }
 
   if (warp == 4) {
-    // Producer: lane l issues boxes l, l + 32, ... of a tile: (K or V, half,
-    // chunk).  The first one's page id is loaded a tile ahead.
-    const int chunks = kStreamKeys / p.chunk, boxes = 2 * HALVES * chunks;
+    // Producer: lane l issues boxes l, l + 32, ... of a tile: (K or V, chunk).
+    // The first one's page id is loaded a tile ahead.
+    const int chunks = kStreamKeys / p.chunk, boxes = 2 * chunks;
     const int my_chunk = lane % chunks;
     bool ok = true;
-    uint32_t t = 0;
+    int st = 0, filled = 0;
+    uint32_t phase = 0;  // of the stage's barriers
 #pragma unroll 1
     while (w.at.left > 0 && ok) {
       const int32_t count_here = w.at.here();
@@ -412,37 +428,41 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       int32_t key0 = (w.lo / kStreamKeys + w.at.first()) * kStreamKeys;
       int32_t id = count_here && lane < boxes ? page_id(p, ids, key0 + my_chunk * p.chunk, w.lo, w.hi) : -1;
 #pragma unroll 1
-      for (int32_t k = 0; k < count_here; ++k, ++t, key0 += kStreamKeys) {
-        const int st = t % kStreamStages;
+      for (int32_t k = 0; k < count_here; ++k, key0 += kStreamKeys) {
         const int32_t id_next = k + 1 < count_here && lane < boxes
                                     ? page_id(p, ids, key0 + kStreamKeys + my_chunk * p.chunk, w.lo, w.hi)
                                     : -1;
-        if (!wait(&empty[st], ((t / kStreamStages) & 1) ^ 1, abort_flag)) {
+        if (!wait(&empty[st], phase ^ 1, abort_flag)) {
           ok = false;
           break;
         }
-        if (lane == 0) mbar_arrive_expect_tx(&full[st], 2 * TILE_BYTES);
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], 2 * tile_bytes);
         __syncwarp();
-        uint8_t *base = smem + st * 2 * TILE_BYTES;
+        uint8_t *base = smem + st * 2 * tile_bytes;
 #pragma unroll 1
         for (int x = lane; x < boxes; x += 32) {
-          const int chunk = x % chunks, half = (x / chunks) % HALVES, v = x / (chunks * HALVES);
+          const int chunk = x % chunks, v = x / chunks;
           const int32_t pos = key0 + chunk * p.chunk;
           if (x >= 32) id = page_id(p, ids, pos, w.lo, w.hi);
-          tma_load_4d(base + v * TILE_BYTES + half * HALF_BYTES + chunk * p.chunk * 128, v ? &tm_v : &tm_k, &full[st],
-                      half * 64, pos % p.paged.page_size, w.h, checked_page(p, id, pos, w.lo, w.hi));
+          tma_load_4d(base + v * tile_bytes + chunk * p.chunk * p.pitch, v ? &tm_v : &tm_k, &full[st], 0,
+                      pos % p.paged.page_size, w.h, checked_page(p, id, pos, w.lo, w.hi));
         }
         id = id_next;
+        if (filled < p.stages) ++filled;
+        if (++st == p.stages) {
+          st = 0;
+          phase ^= 1;
+        }
       }
       w.next(p);
     }
     if (!ok) {
       if (lane == 0) record_device_error(p.err, ERR_KERNEL_PAGED_ATTENTION | ERR_SITE_PRODUCER);
       *abort_flag = 1;
-      // nothing leaves while copies into its shared memory are in flight
+      // nothing leaves while copies into its shared memory are in flight: the
+      // stages from st on were last filled in the other phase
 #pragma unroll 1
-      for (uint32_t x = t > kStreamStages ? t - kStreamStages : 0; x < t; ++x)
-        wait(&full[x % kStreamStages], (x / kStreamStages) & 1, nullptr, 1000000000ull);
+      for (int x = 0; x < filled; ++x) wait(&full[x], x < st ? phase : phase ^ 1, nullptr, 1000000000ull);
     }
     return;
   }
@@ -471,10 +491,11 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   // (keys 0-7, 8-15) x (two 16-byte column chunks); V: keys fastest.
   const int mi = lane >> 3, mr = lane & 7;
   const uint32_t k_row = warp * 16 + (mi >> 1) * 8 + mr, v_row = warp * 16 + (mi & 1) * 8 + mr;
-  const uint32_t sbase = smem_u32(smem);
+  const uint32_t sbase = smem_u32(smem), pitch = p.pitch;
   const float c = p.scale_log2;
   bool ok = true;
-  uint32_t t = 0;
+  int st = 0;
+  uint32_t phase = 0;
   // A unit's queries load while the last one's results meet.
   StreamWalk next = w;
   int32_t count_here = 0;
@@ -513,10 +534,11 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       if (!whole && orow < rows_here && ocol == 0) p.stream_ml[slot] = make_float2(top == -INFINITY ? top : top * c, sum);
 #pragma unroll
-      for (int round = 0; round < DP / 32; ++round) {
+      for (int round = 0; round < (DP + 31) / 32; ++round) {
         float *mine = merge + warp * 16 * kMergeLd;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+          if (round * 4 + i >= NT) continue;
           const float(&v)[4] = o[round * 4 + i];
           *reinterpret_cast<float2 *>(mine + r0 * kMergeLd + i * 8 + cq) = make_float2(v[0] * a0, v[1] * a0);
           *reinterpret_cast<float2 *>(mine + r1 * kMergeLd + i * 8 + cq) = make_float2(v[2] * a1, v[3] * a1);
@@ -562,18 +584,16 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 #pragma unroll
     for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 #pragma unroll 1
-    for (int32_t k = 0; k < count_here; ++k, ++t) {
-      const int st = t % kStreamStages;
+    for (int32_t k = 0; k < count_here; ++k) {
       // (a wait that ran out is not left early: the barriers below need every warp)
-      if (ok && !wait(&full[st], (t / kStreamStages) & 1, abort_flag)) ok = false;
-      const uint32_t ks = sbase + st * 2 * TILE_BYTES, vs = ks + TILE_BYTES;
+      if (ok && !wait(&full[st], phase, abort_flag)) ok = false;
+      const uint32_t ks = sbase + st * 2 * tile_bytes, vs = ks + tile_bytes;
       const int32_t key0 = (w.lo / kStreamKeys + w.at.first() + k) * kStreamKeys + warp * 16;
       float s[2][4] = {}, s2[2][4] = {};  // even and odd steps: two chains
 #pragma unroll
       for (int d = 0; d < KS; ++d) {
         uint32_t b[4];
-        const uint32_t chunk = (d * 2 + (mi & 1)) & 7;
-        ldmatrix_x4(ks + (d >> 2) * HALF_BYTES + k_row * 128 + ((chunk ^ (k_row & 7)) << 4), b);
+        ldmatrix_x4(ks + k_row * pitch + (d * 2 + (mi & 1)) * 16, b);
         mma_16816(d & 1 ? s2[0] : s[0], q[d], b[0], b[1]);
         mma_16816(d & 1 ? s2[1] : s[1], q[d], b[2], b[3]);
       }
@@ -594,10 +614,10 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
             if (key < w.lo || key >= (j & 2 ? end1 : end0)) s[x][j] = -INFINITY;
           }
 #pragma unroll 1
-        for (int x = lane; x < 16 * HALVES * 8; x += 32) {
-          const int row = x / (HALVES * 8), half = (x >> 3) % HALVES;
+        for (int x = lane; x < 16 * NT; x += 32) {
+          const int row = x / NT;
           if (key0 + row < w.lo || key0 + row >= w.hi) {
-            const uint32_t at = vs + half * HALF_BYTES + (warp * 16 + row) * 128 + (x & 7) * 16;
+            const uint32_t at = vs + (warp * 16 + row) * pitch + x % NT * 16;
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
           }
         }
@@ -641,13 +661,16 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 #pragma unroll
       for (int d = 0; d < NT; d += 2) {
         uint32_t b[4];
-        const uint32_t chunk = (d + (mi >> 1)) & 7;
-        ldmatrix_x4_trans(vs + (d >> 3) * HALF_BYTES + v_row * 128 + ((chunk ^ (v_row & 7)) << 4), b);
+        ldmatrix_x4_trans(vs + v_row * pitch + (d + (mi >> 1)) * 16, b);
         mma_16816(o[d], a, b[0], b[1]);
         mma_16816(o[d + 1], a, b[2], b[3]);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[st]);
+      if (++st == p.stages) {
+        st = 0;
+        phase ^= 1;
+      }
     }
     next.next(p);
   }
@@ -1532,16 +1555,17 @@ int32_t gcd(int32_t a, int32_t b) {
   return a;
 }
 
-// 4-D tile map (head_dim, d1, d2, d3) with box {64, b1, 1, b3}, 128-byte swizzle, zero fill.
+// 4-D tile map (head_dim, d1, d2, d3) with box {b0, b1, 1, b3}, zero fill, 128-byte swizzle for b0 = 64.
 ipuc_status make_map_paged(CUtensorMap *map, const void *base, int64_t head_dim, int64_t d1, int64_t d2, int64_t d3,
-                           int64_t s1, int64_t s2, int64_t s3, int32_t b1, int32_t b3) {
+                           int64_t s1, int64_t s2, int64_t s3, int32_t b0, int32_t b1, int32_t b3) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return fail(IPUC_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
   const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)d1, (cuuint64_t)d2, (cuuint64_t)d3};
   const cuuint64_t strides[3] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2, (cuuint64_t)s3 * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)b1, 1, (cuuint32_t)b3}, ones[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {(cuuint32_t)b0, (cuuint32_t)b1, 1, (cuuint32_t)b3}, ones[4] = {1, 1, 1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(base), dims, strides, box, ones,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, b0 == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(IPUC_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled failed");
   return IPUC_OK;
@@ -1626,16 +1650,10 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
   const int64_t tasks = p.rows * q_heads;
   IPUC_CHECK_ARG(tasks < (1ll << 31) && plan.max_units < (1ll << 23), "paged_attention: extent too large");
   CUtensorMap tm_q, tm_k, tm_v;
-  st = make_map_paged(&tm_k, cache->keys, d, cache->page_size, cache->heads, cache->pages, cache->row_stride,
-                      cache->head_stride, cache->page_stride, p.chunk, 1);
-  if (st != IPUC_OK) return st;
-  st = make_map_paged(&tm_v, cache->values, d, cache->page_size, cache->heads, cache->pages, cache->row_stride,
-                      cache->head_stride, cache->page_stride, p.chunk, 1);
-  if (st != IPUC_OK) return st;
-  if (plan.tile) {
-    st = make_map_paged(&tm_q, q, d, p.group, cache->heads, p.rows, d, p.group * d, q_stride, p.group, p.tile_rows);
-    if (st != IPUC_OK) return st;
-  }
+  auto cache_map = [&](CUtensorMap *map, const void *base, int32_t box) {
+    return make_map_paged(map, base, d, cache->page_size, cache->heads, cache->pages, cache->row_stride,
+                          cache->head_stride, cache->page_stride, box, p.chunk, 1);
+  };
   // The stream kernel runs beside the tile kernel, whose start takes longer, on
   // the SMs that leaves it (programmatic dependent launch).  The join is an
   // ordinary launch: an early one measured 3.5 us slower for few rows.
@@ -1655,12 +1673,27 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
     return check_launch("paged_attention");
   };
   if (plan.tile) {
-    st = launch(paged_tile_kernel, p.sms, kTileThreads, kTileSmem, false, tm_q, tm_k, tm_v, p);
+    st = make_map_paged(&tm_q, q, d, p.group, cache->heads, p.rows, d, p.group * d, q_stride, 64, p.group, p.tile_rows);
+    if (st == IPUC_OK) st = cache_map(&tm_k, cache->keys, 64);
+    if (st == IPUC_OK) st = cache_map(&tm_v, cache->values, 64);
+    if (st == IPUC_OK) st = launch(paged_tile_kernel, p.sms, kTileThreads, kTileSmem, false, tm_q, tm_k, tm_v, p);
     if (st != IPUC_OK) return st;
   }
   if (plan.stream) {
-    st = d > 64 ? launch(paged_stream_kernel<128>, p.sms, kStreamThreads, stream_smem_bytes<128>(), plan.tile, tm_k, tm_v, p)
-                : launch(paged_stream_kernel<64>, p.sms, kStreamThreads, stream_smem_bytes<64>(), plan.tile, tm_k, tm_v, p);
+    const int32_t padded = d <= 64 ? 64 : d <= 80 ? 80 : d <= 96 ? 96 : 128;
+    const StreamShape shape = stream_shape(padded, p.chunk);
+    p.pitch = shape.pitch;
+    p.stages = shape.stages;
+    st = cache_map(&tm_k, cache->keys, shape.pitch / 2);
+    if (st == IPUC_OK) st = cache_map(&tm_v, cache->values, shape.pitch / 2);
+    if (st != IPUC_OK) return st;
+    auto stream_kernel = [&](auto kernel) {
+      return launch(kernel, p.sms, kStreamThreads, shape.bytes, plan.tile, tm_k, tm_v, p);
+    };
+    st = padded == 64   ? stream_kernel(paged_stream_kernel<64>)
+         : padded == 80 ? stream_kernel(paged_stream_kernel<80>)
+         : padded == 96 ? stream_kernel(paged_stream_kernel<96>)
+                        : stream_kernel(paged_stream_kernel<128>);
     if (st != IPUC_OK) return st;
   }
   // Few rows: many small blocks; more than fill the GPU: fewer, which find their pieces at once.

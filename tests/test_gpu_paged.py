@@ -305,6 +305,10 @@ DECODE = [
     ([129, 700, 200], 129, 64, 2, 8, 128), ([600] * 9 + [513], 512, 64, 2, 5, 128), ([1100, 1024, 3], 1024, 128, 1, 6, 72),
     ([20, 30], 100, 16, 2, 4, 64), ([400] * 40, 399, 16, 1, 4, 80), ([300] * 70, 256, 64, 2, 4, 128),
     ([9, 8, 7], 5, 16, 1, 1, 128), ([2000, 50], 0, 256, 2, 4, 128), ([700] * 3, 640, 256, 1, 7, 64),
+    # page sizes that are no power of two, or shorter than a box of eight rows
+    ([50, 7, 0], 0, 1, 2, 4, 72), ([50, 47, 90], 40, 1, 1, 4, 128), ([77, 130], 0, 2, 1, 2, 64), ([77, 130], 60, 4, 2, 8, 128),
+    ([90, 33], 0, 12, 1, 4, 96), ([300, 33], 25, 24, 1, 4, 128), ([200, 333], 100, 48, 2, 3, 80), ([500] * 40, 410, 100, 1, 4, 128),
+    ([260] * 33, 255, 1, 1, 4, 64),
 ]
 
 
@@ -320,6 +324,7 @@ RAGGED = [
     ([600, 530], [70, 18], 512, 64, 2, 4, 128, 2), ([4, 200], [6, 150], 0, 32, 1, 3, 64, 0),
     ([700], [129], 300, 128, 1, 1, 96, 0), ([64, 10, 90], [40, 10, 80], 50, 16, 1, 5, 128, 0),
     ([129, 1, 128], [129, 1, 128], 0, 16, 1, 24, 64, 0), ([40, 41], [1, 1], 16, 8, 1, 128, 128, 0),
+    ([60, 41], [9, 30], 0, 1, 1, 4, 128, 0), ([200, 141], [70, 30], 100, 20, 1, 4, 72, 1), ([300, 290], [7, 9], 280, 2, 2, 2, 64, 0),
 ]
 
 
