@@ -92,7 +92,7 @@ struct PagedAttnParams {
   int64_t q_stride, rows;
   int32_t q_heads, heads, group, head_dim, prefix;
   int32_t chunk;          // keys per TMA box: gcd(page_size, 64)
-  int32_t pitch, stages;  // stream kernel: bytes from key to key in shared memory, ring stages
+  int32_t pitch, stages;  // stream kernel: bytes of a key in shared memory, ring stages
   float scale_log2;       // softmax scale * log2(e)
   // Each kernel lays its units (rows that read the same keys of one head) on a
   // line, a unit's length being its key tiles and kUnitCost more for its start
@@ -227,11 +227,13 @@ __device__ __forceinline__ int32_t checked_page(const PagedAttnParams &p, int32_
 // tiles by TMA, box by box of gcd(page_size, 64) keys; four warps take 16 keys
 // of every tile each, with a running maximum, sum and O of their own, and meet
 // once per unit.
-// K and V rows lie `pitch` bytes apart in shared memory, an odd multiple of 16
-// where the boxes' 128-byte alignment allows it: then ldmatrix's eight rows meet
-// no bank twice, without a swizzle, and a row is one box whatever head_dim is
-// (in swizzled halves of 64 elements, heads of 72 held 16 KB a tile for 9 KB of
-// keys and ran at 0.52 of HBM).  The ring has as many stages as fit.
+// Two layouts of K and V in shared memory.  Heads of 64 and 128 lie in halves
+// of 64 elements with the 128-byte swizzle.  Others would waste up to half of
+// that (72 elements: 9 KB of keys in 16, 0.52 of HBM): their rows are single
+// boxes, unswizzled, `pitch` bytes apart, an odd multiple of 16 where the
+// boxes' 128-byte alignment allows it, so that ldmatrix's eight rows meet no
+// bank twice (heads of 72: 170 -> 113 us; heads of 128 lose by it, the rows
+// start inside 128-byte lines: 58 -> 66 us).  The ring has as many stages as fit.
 constexpr int kStreamKeys = 64, kStreamWorkers = 2, kStreamThreads = kStreamWorkers * 160, kMergeLd = 36;
 constexpr int kStreamStages = 8;  // at most
 constexpr int kMergeBytes = 4 * 16 * kMergeLd * 4, kStreamRingBytes = 105600;
@@ -239,10 +241,11 @@ constexpr int kMergeBytes = 4 * 16 * kMergeLd * 4, kStreamRingBytes = 105600;
 struct StreamShape {
   int32_t pitch, stages, bytes;  // bytes: dynamic shared memory
 };
+constexpr bool stream_swizzled(int padded_dim) { return padded_dim % 64 == 0; }
 StreamShape stream_shape(int32_t padded_dim, int32_t chunk) {
   StreamShape r;
   const int32_t align = 128 / (chunk < 8 ? chunk : 8);
-  r.pitch = (padded_dim * 2 + 16 + align - 1) / align * align;
+  r.pitch = stream_swizzled(padded_dim) ? padded_dim * 2 : (padded_dim * 2 + 16 + align - 1) / align * align;
   const int32_t stage = 2 * kStreamKeys * r.pitch;
   r.stages = kStreamRingBytes / stage < kStreamStages ? kStreamRingBytes / stage : kStreamStages;
   r.bytes = kStreamWorkers * (r.stages * stage + kMergeBytes) + 1024;
@@ -324,7 +327,7 @@ template <int DP>
 __global__ void __launch_bounds__(kStreamThreads, 1)
     paged_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const __grid_constant__ PagedAttnParams p) {
-  constexpr int KS = DP / 16, NT = DP / 8;
+  constexpr int KS = DP / 16, NT = DP / 8, HALVES = stream_swizzled(DP) ? DP / 64 : 1, HALF_BYTES = kStreamKeys * 128;
   const int tile_bytes = kStreamKeys * p.pitch, ring_bytes = p.stages * 2 * tile_bytes;  // K or V of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -414,9 +417,10 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   }
 
   if (warp == 4) {
-    // Producer: lane l issues boxes l, l + 32, ... of a tile: (K or V, chunk).
-    // The first one's page id is loaded a tile ahead.
-    const int chunks = kStreamKeys / p.chunk, boxes = 2 * chunks;
+    // Producer: lane l issues boxes l, l + 32, ... of a tile: (K or V, half,
+    // chunk).  The first one's page id is loaded a tile ahead.
+    const int chunks = kStreamKeys / p.chunk, boxes = 2 * HALVES * chunks;
+    const int chunk_bytes = p.chunk * (stream_swizzled(DP) ? 128 : p.pitch);
     const int my_chunk = lane % chunks;
     bool ok = true;
     int st = 0, filled = 0;
@@ -441,11 +445,11 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         uint8_t *base = smem + st * 2 * tile_bytes;
 #pragma unroll 1
         for (int x = lane; x < boxes; x += 32) {
-          const int chunk = x % chunks, v = x / chunks;
+          const int chunk = x % chunks, half = x / chunks % HALVES, v = x / (chunks * HALVES);
           const int32_t pos = key0 + chunk * p.chunk;
           if (x >= 32) id = page_id(p, ids, pos, w.lo, w.hi);
-          tma_load_4d(base + v * tile_bytes + chunk * p.chunk * p.pitch, v ? &tm_v : &tm_k, &full[st], 0,
-                      pos % p.paged.page_size, w.h, checked_page(p, id, pos, w.lo, w.hi));
+          tma_load_4d(base + v * tile_bytes + half * HALF_BYTES + chunk * chunk_bytes, v ? &tm_v : &tm_k, &full[st],
+                      half * 64, pos % p.paged.page_size, w.h, checked_page(p, id, pos, w.lo, w.hi));
         }
         id = id_next;
         if (filled < p.stages) ++filled;
@@ -492,6 +496,10 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   const int mi = lane >> 3, mr = lane & 7;
   const uint32_t k_row = warp * 16 + (mi >> 1) * 8 + mr, v_row = warp * 16 + (mi & 1) * 8 + mr;
   const uint32_t sbase = smem_u32(smem), pitch = p.pitch;
+  // 16-byte column `col` of key `row` of a K or V tile
+  auto place = [&](uint32_t row, uint32_t col) {
+    return stream_swizzled(DP) ? (col >> 3) * HALF_BYTES + row * 128 + (((col & 7) ^ (row & 7)) << 4) : row * pitch + col * 16;
+  };
   const float c = p.scale_log2;
   bool ok = true;
   int st = 0;
@@ -593,7 +601,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 #pragma unroll
       for (int d = 0; d < KS; ++d) {
         uint32_t b[4];
-        ldmatrix_x4(ks + k_row * pitch + (d * 2 + (mi & 1)) * 16, b);
+        ldmatrix_x4(ks + place(k_row, d * 2 + (mi & 1)), b);
         mma_16816(d & 1 ? s2[0] : s[0], q[d], b[0], b[1]);
         mma_16816(d & 1 ? s2[1] : s[1], q[d], b[2], b[3]);
       }
@@ -617,7 +625,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         for (int x = lane; x < 16 * NT; x += 32) {
           const int row = x / NT;
           if (key0 + row < w.lo || key0 + row >= w.hi) {
-            const uint32_t at = vs + (warp * 16 + row) * pitch + x % NT * 16;
+            const uint32_t at = vs + place(warp * 16 + row, x % NT);
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
           }
         }
@@ -661,7 +669,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 #pragma unroll
       for (int d = 0; d < NT; d += 2) {
         uint32_t b[4];
-        ldmatrix_x4_trans(vs + v_row * pitch + (d + (mi >> 1)) * 16, b);
+        ldmatrix_x4_trans(vs + place(v_row, d + (mi >> 1)), b);
         mma_16816(o[d], a, b[0], b[1]);
         mma_16816(o[d + 1], a, b[2], b[3]);
       }
@@ -1684,9 +1692,12 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
     const StreamShape shape = stream_shape(padded, p.chunk);
     p.pitch = shape.pitch;
     p.stages = shape.stages;
-    st = cache_map(&tm_k, cache->keys, shape.pitch / 2);
-    if (st == IPUC_OK) st = cache_map(&tm_v, cache->values, shape.pitch / 2);
-    if (st != IPUC_OK) return st;
+    const int32_t box = stream_swizzled(padded) ? 64 : shape.pitch / 2;
+    if (!plan.tile || box != 64) {  // (else they are there)
+      st = cache_map(&tm_k, cache->keys, box);
+      if (st == IPUC_OK) st = cache_map(&tm_v, cache->values, box);
+      if (st != IPUC_OK) return st;
+    }
     auto stream_kernel = [&](auto kernel) {
       return launch(kernel, p.sms, kStreamThreads, shape.bytes, plan.tile, tm_k, tm_v, p);
     };
