@@ -706,6 +706,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 //   warps 2-17  softmax: two warps per lane quarter of a tile, 64 keys each
 // so the tensor core works on one tile while the other's softmax runs, and a
 // unit's Q and first K tile load while the last unit's results are stored.
+// A unit whose rows fill one row tile only has it twice, for even and for odd
+// key tiles (`dual`), and joins both at its end: each row's two O lie in the same
+// TMEM lane.
 constexpr int kTileRows = 128, kTileKeys = 128;
 constexpr int kTileBytes = 128 * 128 * 2, kTileHalf = kTileBytes / 2;
 constexpr int kTileThreads = 576, kTileSmem = 6 * kTileBytes + 1024;
@@ -804,7 +807,7 @@ struct TileWalk {
 struct TileTask {
   int64_t row0, pos0, slot;
   int32_t rows, lo, hi, h, first, n;  // key tiles [first, first + n); n = 0: the piece is done
-  int32_t tiles;                      // row tiles in use
+  int32_t dual;                       // one row tile, for even and odd key tiles
   int32_t prefix, direct, store;
   // V rows outside [lo, hi) of a chunk that has both kinds may hold anything
   // and are zeroed in shared memory (0 * NaN is NaN); whole chunks outside are
@@ -812,17 +815,45 @@ struct TileTask {
   int32_t fix_first, fix_last;
 };
 
-// S = Q K^T of one row tile (one function: a unit's first products run the code that the next ones use).
-__device__ __noinline__ void issue_scores(uint32_t d, uint64_t q_desc, uint64_t k_desc, int k_steps, uint64_t *full) {
+// The MMA warp runs as a whole and one elected lane issues: in code that only
+// one lane reaches, the compiler moves every descriptor from a thread's to a
+// uniform register before each MMA, which took 95 cycles an MMA (64 is what the
+// tensor core needs) and bound the kernel.  Loop bounds and flags go through
+// uniform() and all() so that it knows them to be the same in all lanes.
+__device__ __forceinline__ int32_t uniform(int32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ bool all(bool x) { return __all_sync(0xffffffffu, x); }
+template <bool kAccumulate>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+  asm volatile(
+      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "n"(kAccumulate ? 1 : 0)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t *bar) {
+  asm volatile(
+      "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
+      : "memory");
+}
+
+// S = Q K^T of one row tile, K steps of 16 head dims.
+template <int K>
+__device__ __forceinline__ void issue_scores(uint32_t d, uint64_t q_desc, uint64_t k_desc) {
   constexpr uint32_t idesc = make_idesc(128, kTileKeys, 0, false, false);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    if (k < k_steps) {
-      const uint64_t step = (uint64_t)(((k >> 2) * kTileHalf + (k & 3) * 32) >> 4);
-      mma_f16_ss(d, q_desc + step, k_desc + step, idesc, k > 0 ? 1u : 0u);
-    }
+  for (int k = 0; k < K; ++k) {
+    const uint64_t step = (uint64_t)(((k >> 2) * kTileHalf + (k & 3) * 32) >> 4);
+    if (k) mma_ss<true>(d, q_desc + step, k_desc + step, idesc);
+    else mma_ss<false>(d, q_desc + step, k_desc + step, idesc);
   }
-  mma_commit(full);
 }
 
 __global__ void __launch_bounds__(kTileThreads, 1)
@@ -841,7 +872,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __shared__ uint64_t task_full[2], task_empty[2];
   __shared__ TileTask tasks[2];
   volatile int *abort_flag = &aborted;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1);
@@ -856,7 +887,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       mbar_init(&s_full[i], 1);
       mbar_init(&p_ready[i], 8);
       mbar_init(&o_final[i], 1);
-      mbar_init(&o_empty[i], 8);
+      mbar_init(&o_empty[i], 16);
       mbar_init(&task_full[i], 1);
       mbar_init(&task_empty[i], 17);  // the MMA thread and 16 softmax warps
     }
@@ -951,9 +982,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;  // S_t at column t * 128, O_t at 256 + t * 128
+  const uint32_t tmem = uniform(tmem_slot);  // S_t at column t * 128, O_t at 256 + t * 128
   if (warp == 0) {
+    // Lane l issues boxes l, l + 32, ... of a tile: (half, chunk).  Where the
+    // first one comes from is known before the stage is free: the softmax
+    // warps leave this one little of its scheduler, and every instruction
+    // between a free stage and its load lengthens the chain.
     const int chunks = kTileKeys / p.chunk, boxes = halves * chunks;
+    const int my_chunk = lane % chunks, my_half = lane / chunks;
+    const int my_offset = my_half * kTileHalf + my_chunk * p.chunk * 128;
     bool ok = true;
     uint32_t unit = 0, k_issued = 0, v_issued = 0, q_issued = 0;
     // Tasks are written two ahead of the last reader at most; after the last comes one with n = 0.
@@ -978,7 +1015,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       task.h = walk.h;
       task.n = walk.at.here();
       task.first = walk.lo / kTileKeys + walk.at.first();
-      task.tiles = walk.rows > p.tile_rows ? 2 : 1;
+      task.dual = walk.rows <= p.tile_rows;
       task.prefix = walk.seq < 0;
       task.direct = p.prefix == 0 && task.n == walk.at.n;
       // (max_units holds for sorted row offsets; others write no partials past it)
@@ -990,74 +1027,79 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         break;
       }
       const int32_t *ids = walk.seq < 0 ? p.prefix_pages : p.paged.page_table + walk.seq * p.paged.table_stride;
-      int32_t id = 0;  // of this lane's first chunk, loaded a tile ahead
-      auto load = [&](uint8_t *base, const CUtensorMap *map, uint64_t *bar, int32_t key0) {
+      // K runs a tile ahead of V: its stages are free earlier.
+      int32_t id = -1, slot = 0, page = 0;  // of the next K tile
+      int32_t v_slot = 0, v_page = 0;       // of the next V tile
+      auto look = [&](int32_t key0) {
+        const int32_t pos = key0 + my_chunk * p.chunk;
+        id = lane < boxes ? page_id(p, ids, pos, walk.lo, walk.hi) : -1;
+        slot = pos % p.paged.page_size;
+      };
+      auto load = [&](uint8_t *base, const CUtensorMap *map, uint64_t *bar, int32_t key0, int32_t from_slot, int32_t from_page) {
         if (lane == 0) mbar_arrive_expect_tx(bar, halves * kTileHalf);
         __syncwarp();
+        if (lane < boxes) tma_load_4d(base + my_offset, map, bar, my_half * 64, from_slot, walk.h, from_page);
 #pragma unroll 1
-        for (int i = lane; i < boxes; i += 32) {
+        for (int i = lane + 32; i < boxes; i += 32) {
           const int chunk = i % chunks, half = i / chunks;
           const int32_t pos = key0 + chunk * p.chunk;
-          const int32_t page = i < 32 ? id : page_id(p, ids, pos, walk.lo, walk.hi);
           tma_load_4d(base + half * kTileHalf + chunk * p.chunk * 128, map, bar, half * 64, pos % p.paged.page_size,
-                      walk.h, checked_page(p, page, pos, walk.lo, walk.hi));
+                      walk.h, checked_page(p, page_id(p, ids, pos, walk.lo, walk.hi), pos, walk.lo, walk.hi));
         }
       };
-      auto first_id = [&](int32_t key0) {
-        return lane < boxes ? page_id(p, ids, key0 + (lane % chunks) * p.chunk, walk.lo, walk.hi) : -1;
-      };
-      id = first_id(task.first * kTileKeys);
+      look(task.first * kTileKeys);
 #pragma unroll 1
-      for (int32_t j = 0; j < task.n; ++j) {
-        const int st = k_issued & 1;
-        const int32_t key0 = (task.first + j) * kTileKeys;
-        const int32_t id_next = j + 1 < task.n ? first_id(key0 + kTileKeys) : -1;
-        if (!wait(&k_empty[st], ((k_issued >> 1) & 1) ^ 1, abort_flag)) {
-          ok = false;
-          break;
-        }
-        load(s_k + st * kTileBytes, &tm_k, &k_full[st], key0);
-        ++k_issued;
-        if (j == 0) {
-          // Q's buffer: the previous unit's S products are done
-          if (!wait(&q_empty, (unit & 1) ^ 1, abort_flag)) {
-            ok = false;
-            break;
-          }
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&q_full, task.tiles * halves * p.tile_rows * p.group * 128);
+      for (int32_t j = 0; j <= task.n && ok; ++j) {
+        if (j < task.n) {
+          const int st = k_issued & 1;
+          const int32_t key0 = (task.first + j) * kTileKeys;
+          page = lane < boxes ? checked_page(p, id, key0 + my_chunk * p.chunk, walk.lo, walk.hi) : 0;
+          ok = wait(&k_empty[st], ((k_issued >> 1) & 1) ^ 1, abort_flag);
+          if (!ok) break;
+          load(s_k + st * kTileBytes, &tm_k, &k_full[st], key0, slot, page);
+          ++k_issued;
+          if (j == 0) {
+            // Q's buffer: the previous unit's S products are done
+            ok = wait(&q_empty, (unit & 1) ^ 1, abort_flag);
+            if (!ok) break;
+            if (lane == 0) {
+              const int tiles = task.dual ? 1 : 2;
+              mbar_arrive_expect_tx(&q_full, tiles * halves * p.tile_rows * p.group * 128);
 #pragma unroll 1
-            for (int t = 0; t < task.tiles; ++t)
+              for (int t = 0; t < tiles; ++t)
 #pragma unroll 1
-              for (int half = 0; half < halves; ++half)
-                tma_load_4d(s_q + t * kTileBytes + half * kTileHalf, &tm_q, &q_full, half * 64, 0, walk.h,
-                            (int32_t)walk.row0 + t * p.tile_rows);
+                for (int half = 0; half < halves; ++half)
+                  tma_load_4d(s_q + t * kTileBytes + half * kTileHalf, &tm_q, &q_full, half * 64, 0, walk.h,
+                              (int32_t)walk.row0 + t * p.tile_rows);
+            }
+            ++q_issued;
           }
-          ++q_issued;
         }
-        if (!wait(&v_empty[st], ((v_issued >> 1) & 1) ^ 1, abort_flag)) {
-          ok = false;
-          break;
-        }
-        load(s_v + st * kTileBytes, &tm_v, &v_full[st], key0);
-        ++v_issued;
-        if ((task.fix_first && j == 0) || (task.fix_last && j == task.n - 1)) {
-          if (!wait(&v_full[st], ((v_issued - 1) >> 1) & 1, abort_flag)) {
-            ok = false;
-            break;
-          }
+        if (j > 0) {
+          const int st = v_issued & 1;
+          const int32_t key0 = (task.first + j - 1) * kTileKeys;
+          ok = wait(&v_empty[st], ((v_issued >> 1) & 1) ^ 1, abort_flag);
+          if (!ok) break;
+          load(s_v + st * kTileBytes, &tm_v, &v_full[st], key0, v_slot, v_page);
+          ++v_issued;
+          if ((task.fix_first && j == 1) || (task.fix_last && j == task.n)) {
+            ok = wait(&v_full[st], ((v_issued - 1) >> 1) & 1, abort_flag);
+            if (!ok) break;
 #pragma unroll 1
-          for (int i = lane; i < kTileKeys * halves * 8; i += 32) {
-            const int row = i / (halves * 8), half = (i >> 3) % halves;
-            if (key0 + row < walk.lo || key0 + row >= walk.hi)
-              *reinterpret_cast<uint4 *>(s_v + st * kTileBytes + half * kTileHalf + row * 128 + (i & 7) * 16) =
-                  make_uint4(0u, 0u, 0u, 0u);
+            for (int i = lane; i < kTileKeys * halves * 8; i += 32) {
+              const int row = i / (halves * 8), half = (i >> 3) % halves;
+              if (key0 + row < walk.lo || key0 + row >= walk.hi)
+                *reinterpret_cast<uint4 *>(s_v + st * kTileBytes + half * kTileHalf + row * 128 + (i & 7) * 16) =
+                    make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&v_fixed[st]);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&v_fixed[st]);
         }
-        id = id_next;
+        v_slot = slot;
+        v_page = page;
+        if (j + 1 < task.n) look((task.first + j + 1) * kTileKeys);
       }
       ++unit;
     }
@@ -1078,78 +1120,94 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         wait(&v_full[i & 1], (i >> 1) & 1, nullptr, 1000000000ull);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc_o = make_idesc(128, k_steps * 16, 0, false, true);  // V: head dims contiguous
-      const uint64_t q_desc = make_smem_desc(smem_u32(s_q), 16, 1024, kSwizzle128B);
-      const uint64_t k_desc = make_smem_desc(smem_u32(s_k), 16, 1024, kSwizzle128B);
-      const uint64_t v_desc = make_smem_desc(smem_u32(s_v), kTileHalf, 1024, kSwizzle128B);
-      auto issue_s = [&](int t, int st) {
-        issue_scores(tmem + t * 128, q_desc + (uint64_t)(t * (kTileBytes >> 4)), k_desc + (uint64_t)(st * (kTileBytes >> 4)),
-                     k_steps, &s_full[t]);
-      };
-      // Per key tile j: PV_t(j) as soon as P_t(j) is there, then S_t(j + 1)
-      // behind it.  A unit's first S products queue behind the last unit's last
-      // PV products, so its S tiles (which held the last P) are free by then.
-      bool ok = true;
-      uint32_t unit = 0, g = 0;          // units begun, key tiles done
-      uint32_t p_count[2] = {0, 0}, o_count[2] = {0, 0}, fixes[2] = {0, 0};
+    const uint32_t idesc_o = make_idesc(128, k_steps * 16, 0, false, true);  // V: head dims contiguous
+    const uint64_t q_desc = make_smem_desc(smem_u32(s_q), 16, 1024, kSwizzle128B);
+    const uint64_t k_desc = make_smem_desc(smem_u32(s_k), 16, 1024, kSwizzle128B);
+    const uint64_t v_desc = make_smem_desc(smem_u32(s_v), kTileHalf, 1024, kSwizzle128B);
+    auto issue_s = [&](int t, int q_tile, int st) {
+      const uint32_t d = tmem + t * 128;
+      const uint64_t qd = q_desc + (uint64_t)(q_tile * (kTileBytes >> 4)), kd = k_desc + (uint64_t)(st * (kTileBytes >> 4));
+      if (k_steps > 4) issue_scores<8>(d, qd, kd);  // (columns from head_dim on are zero)
+      else issue_scores<4>(d, qd, kd);
+      commit(&s_full[t]);
+    };
+    // Per key tile j and row tile t that takes it: PV_t(j) as soon as P_t(j) is
+    // there, then t's next S product behind it.  A stage of K is released
+    // behind its last S product, one of V behind its last PV product.  A
+    // unit's first S products queue behind the last unit's last PV products,
+    // so its S tiles (which held the last P) are free by then.
+    bool ok = true;
+    uint32_t unit = 0, g = 0;  // units begun, key tiles of the units before
+    uint32_t p_count[2] = {0, 0}, fixes[2] = {0, 0};
+    auto there = [&](uint64_t *bar, uint32_t parity) { return all(wait(bar, parity & 1, abort_flag)); };
+    auto k_there = [&](uint32_t i) { return there(&k_full[i & 1], i >> 1); };
 #pragma unroll 1
-      for (;; ++unit) {
-        ok = wait(&task_full[unit & 1], (unit >> 1) & 1, abort_flag);
-        if (!ok) break;
-        const TileTask &task = tasks[unit & 1];
-        const int tiles = task.tiles;
-        const int32_t n = task.n;
-        const bool fix_first = task.fix_first, fix_last = task.fix_last;
-        mbar_arrive(&task_empty[unit & 1]);
-        if (n == 0) break;
-        ok = wait(&k_full[g & 1], (g >> 1) & 1, abort_flag) && wait(&q_full, unit & 1, abort_flag);
-        if (!ok) break;
+    for (;; ++unit) {
+      ok = there(&task_full[unit & 1], unit >> 1);
+      if (!ok) break;
+      const TileTask &task = tasks[unit & 1];
+      const int32_t n = uniform(task.n), flags = uniform(task.fix_first | task.fix_last << 1 | task.dual << 2);
+      const bool fix_first = flags & 1, fix_last = flags & 2, dual = flags & 4;
+      if (lane == 0) mbar_arrive(&task_empty[unit & 1]);
+      __syncwarp();
+      if (n == 0) break;
+      const int32_t step = dual ? 2 : 1;  // key tiles from a row tile's one to its next
+      ok = k_there(g) && there(&q_full, unit);
+      if (!ok) break;
 #pragma unroll 1
-        for (int t = 0; t < tiles; ++t) issue_s(t, g & 1);
-        if (n == 1) mma_commit(&q_empty);
-#pragma unroll 1
-        for (int32_t j = 0; j < n && ok; ++j, ++g) {
-          const int st = g & 1;
-          const bool more = j + 1 < n;
-          const uint64_t vd = v_desc + (uint64_t)(st * (kTileBytes >> 4));
-          if ((fix_first && j == 0) || (fix_last && !more))
-            ok = wait(&v_fixed[st], fixes[st]++ & 1, abort_flag);
-          else
-            ok = wait(&v_full[st], (g >> 1) & 1, abort_flag);
-#pragma unroll 1
-          for (int t = 0; t < tiles && ok; ++t) {
-            ok = wait(&p_ready[t], p_count[t]++ & 1, abort_flag);
-            // the last unit's O_t has been read out before this one's first PV_t
-            if (ok && j == 0 && o_count[t]) ok = wait(&o_empty[t], (o_count[t] - 1) & 1, abort_flag);
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll
-            for (int k = 0; k < kTileKeys / 16; ++k)
-              mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, vd + (uint64_t)((k * 2048) >> 4), idesc_o,
-                         j > 0 || k > 0 ? 1u : 0u);
-            if (t == 0) {
-              // K's stage was last read by the S products that P_t(j) came from
-              mma_commit(&k_empty[st]);
-              if (more && !wait(&k_full[st ^ 1], ((g + 1) >> 1) & 1, abort_flag)) {
-                ok = false;
-                break;
-              }
-            }
-            if (t == tiles - 1) mma_commit(&v_empty[st]);
-            if (more) issue_s(t, st ^ 1);
-            else mma_commit(&o_final[t]);
-          }
-          if (ok && j + 2 == n) mma_commit(&q_empty);
+      for (int t = 0; t < 2; ++t) {
+        if (dual && t == 1) {
+          if (n == 1) break;
+          ok = k_there(g + 1);
+          if (!ok) break;
         }
-        if (!ok) break;
+        const int st = dual ? (g + t) & 1 : g & 1;
+        issue_s(t, dual ? 0 : t, st);
+        if (dual || t == 1) commit(&k_empty[st]);
+      }
+      if (!ok) break;
+      if (n <= step) commit(&q_empty);
 #pragma unroll 1
-        for (int t = 0; t < tiles; ++t) ++o_count[t];
+      for (int32_t j = 0; j < n && ok; ++j) {
+        const uint32_t i = g + j;
+        const int st = i & 1;
+        const bool more = j + step < n;
+        const uint64_t vd = v_desc + (uint64_t)(st * (kTileBytes >> 4));
+        if ((fix_first && j == 0) || (fix_last && j == n - 1)) ok = there(&v_fixed[st], fixes[st]++);
+        else ok = there(&v_full[st], i >> 1);
+#pragma unroll 1
+        for (int x = dual ? 1 : 0; x < 2 && ok; ++x) {
+          const int t = dual ? j & 1 : x;
+          ok = there(&p_ready[t], p_count[t]++);
+          // the last unit's O_t has been read out before this one's first PV_t
+          if (ok && j < step && unit) ok = there(&o_empty[t], unit - 1);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < kTileKeys / 16; ++k)
+            mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, vd + (uint64_t)((k * 2048) >> 4), idesc_o,
+                   j >= step || k > 0 ? 1u : 0u);
+          if (x == 1) commit(&v_empty[st]);
+          if (!more) {
+            commit(&o_final[t]);
+            continue;
+          }
+          const int next = (i + step) & 1;
+          if (dual || t == 0) {
+            ok = k_there(i + step);
+            if (!ok) break;
+          }
+          issue_s(t, dual ? 0 : t, next);
+          if (x == 1) commit(&k_empty[next]);
+        }
+        if (ok && j + step == n - 1) commit(&q_empty);
       }
-      if (!ok) {
-        record_device_error(p.err, ERR_KERNEL_PAGED_ATTENTION | ERR_SITE_MMA);
-        *abort_flag = 1;
-      }
+      if (!ok) break;
+      g += n;
+    }
+    if (!ok) {
+      if (lane == 0) record_device_error(p.err, ERR_KERNEL_PAGED_ATTENTION | ERR_SITE_MMA);
+      *abort_flag = 1;
     }
   } else {
     const int sw = warp - 2, t = sw >> 3, half = (sw >> 2) & 1, quarter = warp & 3;
@@ -1158,33 +1216,30 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_col = tmem + lane_off + t * 128, o_col = tmem + lane_off + 256 + t * 128 + half * 64;
     const float c = p.scale_log2;
-    const int32_t local = t * p.tile_rows + row / p.group;  // batch row within a unit
     const bool in_tile = row < p.tile_rows * p.group;
     bool ok = true;
-    uint32_t g = 0, unit = 0;  // key tiles and units of this row tile so far
+    uint32_t g = 0, units[2] = {0, 0};  // key tiles of this row tile so far; units that have had PV_0 and PV_1
 #pragma unroll 1
     for (uint32_t index = 0;; ++index) {
-      // (the two warps of a lane quarter go on or stop together: they meet at barriers below)
+      // (the four warps of a lane quarter go on or stop together: they meet at barriers below)
       const bool late = ok && !wait(&task_full[index & 1], (index >> 1) & 1, abort_flag);
-      if (barrier_any(bar_id, 64, late || !ok)) {
+      if (barrier_any(9 + quarter, 128, late || !ok)) {
         ok = false;
         break;
       }
       const TileTask &task = tasks[index & 1];
-      const int32_t n = task.n;
-      if (n == 0) break;
-      if (t >= task.tiles) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&task_empty[index & 1]);
-        continue;
-      }
+      if (task.n == 0) break;
+      // This row tile's key tiles: all, or every second from t on.
+      const bool dual = task.dual, both = !dual || task.n > 1;
+      const int32_t n = dual ? (task.n - t + 1) >> 1 : task.n, step = dual ? 2 : 1;
+      const int32_t row_tile = dual ? 0 : t, local = row_tile * p.tile_rows + row / p.group;  // batch row within the unit
       // This row's keys: [lo, limit).
       const bool row_ok = in_tile && local < task.rows && task.store;
       const int64_t token = task.row0 + local;
-      const int32_t lo = task.lo, first = task.first;
+      const int32_t lo = task.lo, first = task.first + (dual ? t : 0);
       const bool direct = task.direct;
       const int64_t head = token * p.q_heads + task.h * p.group + row % p.group;
-      const int32_t slot_row = t * p.tile_rows * p.group + row;
+      const int32_t slot_row = row_tile * p.tile_rows * p.group + row;
       const int64_t slot = task.slot;
       int32_t limit = 0;
       if (row_ok) {
@@ -1201,7 +1256,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         // (a wait that ran out is not left early: the barriers below need every warp)
         if (ok && !wait(&s_full[t], g & 1, abort_flag)) ok = false;
         tc_fence_after();
-        const int32_t key0 = (first + j) * kTileKeys + half * 64;
+        const int32_t key0 = (first + j * step) * kTileKeys + half * 64;
         uint32_t a[32], b[32];
         tmem_ld_32x32b_x32(s_col + half * 64, a);
         tmem_ld_32x32b_x32(s_col + half * 64 + 32, b);
@@ -1288,24 +1343,59 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       x_sum[t][half][row] = l;
       named_barrier_sync(bar_id, 64);
       l += x_sum[t][half ^ 1][row];
-      if (ok && !wait(&o_final[t], unit & 1, abort_flag)) ok = false;
-      ++unit;
+      if (ok && (t == 0 || dual) && !wait(&o_final[0], units[0] & 1, abort_flag)) ok = false;
+      if (ok && both && (t == 1 || dual) && !wait(&o_final[1], units[1] & 1, abort_flag)) ok = false;
+      ++units[0];
+      if (both) ++units[1];
       tc_fence_after();
-      if (row_ok && !direct && half == 0) p.tile_ml[slot * p.tile_slot_rows + slot_row] = make_float2(m == -INFINITY ? m : m * c, l);
+      // A thread stores 64 columns of its row's O, or (dual) 32 of the sum of its
+      // two O: columns half * 64 + t * 32 on.
+      float own = 1.0f, other = 0.0f;  // (dual) weights of O_t and of the other
+      if (dual) {
+        if (half == 0) {
+          x_max[t][0][row] = m;
+          x_max[t][1][row] = l;
+        }
+        named_barrier_sync(9 + quarter, 128);
+        const float m2 = x_max[t ^ 1][0][row], l2 = x_max[t ^ 1][1][row], top = fmaxf(m, m2);
+        own = m == -INFINITY ? 0.0f : ex2_approx((m - top) * c);
+        other = m2 == -INFINITY ? 0.0f : ex2_approx((m2 - top) * c);
+        l = l * own + l2 * other;
+        m = top;
+        named_barrier_sync(9 + quarter, 128);  // read before the next unit's maxima are written
+      }
+      if (row_ok && !direct && half == 0 && (!dual || t == 0))
+        p.tile_ml[slot * p.tile_slot_rows + slot_row] = make_float2(m == -INFINITY ? m : m * c, l);
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
       for (int ch = 0; ch < 2; ++ch) {
+        const int32_t at = dual ? t * 32 : ch * 32;  // column in this thread's half
         uint32_t r[32];
-        tmem_ld_32x32b_x32(o_col + ch * 32, r);
-        tmem_wait_ld(r);
-        if (ch == 1) {
-          // O_t is read out: the next unit's first PV may overwrite it
+        if (!dual || ch == 0) {
+          tmem_ld_32x32b_x32(o_col + at, r);
+          tmem_wait_ld(r);
+        }
+        if (dual && ch == 0) {
+          // (O_1 is not there after a single key tile; its weight is 0)
+          uint32_t r2[32];
+          tmem_ld_32x32b_x32(o_col + at + (t ? -128 : 128), r2);
+          tmem_wait_ld(r2);
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            r[i] = __float_as_uint((own != 0.0f ? __uint_as_float(r[i]) * own : 0.0f) +
+                                   (other != 0.0f ? __uint_as_float(r2[i]) * other : 0.0f));
+        }
+        if (ch == (dual ? 0 : 1)) {
+          // read out: the next unit's first PV products may overwrite it
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&o_empty[t]);
+          if (lane == 0) {
+            mbar_arrive(&o_empty[t]);
+            mbar_arrive(&o_empty[dual ? t ^ 1 : t]);
+          }
         }
-        const int col0 = half * 64 + ch * 32;
-        if (!row_ok) continue;
+        const int col0 = half * 64 + at;
+        if (!row_ok || (dual && ch == 1)) continue;
         if (direct) {
           // (a row without keys: O is 0 * V, which a non-finite V of another row's keys makes NaN)
           uint16_t *o = p.out + head * p.head_dim + col0;
@@ -1326,8 +1416,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
             if (col0 + i >= p.head_dim) break;
-            *reinterpret_cast<float4 *>(o + (int64_t)i * p.tile_slot_rows) = make_float4(__uint_as_float(r[i]), __uint_as_float(r[i + 1]),
-                                                             __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
+            *reinterpret_cast<float4 *>(o + (int64_t)i * p.tile_slot_rows) =
+                make_float4(__uint_as_float(r[i]), __uint_as_float(r[i + 1]), __uint_as_float(r[i + 2]),
+                            __uint_as_float(r[i + 3]));
           }
         }
       }
