@@ -234,9 +234,14 @@ __device__ __forceinline__ int32_t checked_page(const PagedAttnParams &p, int32_
 // boxes' 128-byte alignment allows it, so that ldmatrix's eight rows meet no
 // bank twice (heads of 72: 170 -> 113 us; heads of 128 lose by it, the rows
 // start inside 128-byte lines: 58 -> 66 us).  The ring has as many stages as fit.
-constexpr int kStreamKeys = 64, kStreamWorkers = 2, kStreamThreads = kStreamWorkers * 160, kMergeLd = 36;
+template <int N>
+struct Number {
+  static constexpr int value = N;
+};
+constexpr int kStreamKeys = 64, kStreamWorkers = 2, kStreamThreads = kStreamWorkers * 160;
 constexpr int kStreamStages = 8;  // at most
-constexpr int kMergeBytes = 4 * 16 * kMergeLd * 4, kStreamRingBytes = 105600;
+constexpr int kMergeBytes = 4 * 16 * 20 * 4, kStreamRingBytes = 98304;
+constexpr int kQueryLd = 136, kQueryBytes = 16 * kQueryLd * 2;  // a unit's 16 query rows, an odd multiple of 16 bytes apart
 
 struct StreamShape {
   int32_t pitch, stages, bytes;  // bytes: dynamic shared memory
@@ -248,7 +253,7 @@ StreamShape stream_shape(int32_t padded_dim, int32_t chunk) {
   r.pitch = stream_swizzled(padded_dim) ? padded_dim * 2 : (padded_dim * 2 + 16 + align - 1) / align * align;
   const int32_t stage = 2 * kStreamKeys * r.pitch;
   r.stages = kStreamRingBytes / stage < kStreamStages ? kStreamRingBytes / stage : kStreamStages;
-  r.bytes = kStreamWorkers * (r.stages * stage + kMergeBytes) + 1024;
+  r.bytes = kStreamWorkers * (r.stages * stage + kMergeBytes + 2 * kQueryBytes) + 1024;
   return r;
 }
 
@@ -263,6 +268,14 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&r)[4
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr)
                : "memory");
+}
+// 16 bytes to shared memory, of which `bytes` are read and the rest zeros.
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// This thread's arrival on the barrier, once its cp.async so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -323,6 +336,14 @@ __device__ __forceinline__ int32_t stream_sms(const PagedAttnParams &p, int64_t 
   return max(1, min(min(x, kStreamSaturated), p.sms - 1));
 }
 
+// One unit's share of a worker's piece, as the producer hands it to the others.
+struct StreamTask {
+  int64_t slot, head;        // of the partial result; (whole) output head of row 0
+  int32_t n, key0, lo, hi;   // key tiles from position key0 on, keys [lo, hi); n = 0: the piece is done
+  int32_t rows, whole;       // rows of the unit; the result is final
+  int32_t prefix, row0;      // the prefix: first row (token, head of the group) of the unit
+};
+
 template <int DP>
 __global__ void __launch_bounds__(kStreamThreads, 1)
     paged_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -332,6 +353,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t all_full[kStreamWorkers][kStreamStages], all_empty[kStreamWorkers][kStreamStages];
+  __shared__ uint64_t all_unit_full[kStreamWorkers][2], all_unit_empty[kStreamWorkers][2];  // queries and task
+  __shared__ StreamTask all_tasks[kStreamWorkers][2];
   __shared__ int64_t scratch[kStreamThreads / 32];
   __shared__ int32_t first_unit[kStreamWorkers][3];
   __shared__ float all_m[kStreamWorkers][4][16], all_l[kStreamWorkers][4][16];
@@ -340,17 +363,26 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 
   const int worker = threadIdx.x / 160, warp = (threadIdx.x >> 5) % 5, lane = threadIdx.x & 31;
   uint64_t *full = all_full[worker], *empty = all_empty[worker];
+  uint64_t *unit_full = all_unit_full[worker], *unit_empty = all_unit_empty[worker];
+  StreamTask *tasks = all_tasks[worker];
   float(&warp_m)[4][16] = all_m[worker], (&warp_l)[4][16] = all_l[worker];
   float *merge = reinterpret_cast<float *>(smem + kStreamWorkers * ring_bytes + worker * kMergeBytes);
+  uint8_t *queries = smem + kStreamWorkers * (ring_bytes + kMergeBytes) + worker * 2 * kQueryBytes;
   smem += worker * ring_bytes;
   if (threadIdx.x == 0) {
 #pragma unroll 1
-    for (int w = 0; w < kStreamWorkers; ++w)
+    for (int w = 0; w < kStreamWorkers; ++w) {
 #pragma unroll 1
       for (int i = 0; i < p.stages; ++i) {
         mbar_init(&all_full[w][i], 1);
         mbar_init(&all_empty[w][i], 4);
       }
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&all_unit_full[w][i], 33);  // the task, and the queries from each lane
+        mbar_init(&all_unit_empty[w][i], 4);
+      }
+    }
     aborted = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tm_k);
@@ -425,12 +457,54 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     bool ok = true;
     int st = 0, filled = 0;
     uint32_t phase = 0;  // of the stage's barriers
+    uint32_t unit = 0;
+    // Hands out the next task and its query rows: the group's heads, or (prefix)
+    // those of 16 rows of the call; zeros behind them and behind head_dim.
+    auto publish = [&](int32_t n) {
+      const uint32_t buffer = unit & 1;
+      if (!wait(&unit_empty[buffer], ((unit >> 1) & 1) ^ 1, abort_flag)) return false;
+      ++unit;
+      const int32_t row0 = w.b < 0 ? w.rows16 * 16 : 0;
+      const int32_t rows = w.b < 0 ? min(16, (int32_t)p.rows * p.group - row0) : p.group;
+      if (n) {
 #pragma unroll 1
-    while (w.at.left > 0 && ok) {
+        for (int x = lane; x < 16 * (DP / 8); x += 32) {
+          const int r = x / (DP / 8), col = x % (DP / 8) * 8, token = (row0 + r) / p.group;
+          const bool there = r < rows && col < p.head_dim;
+          const uint16_t *src = p.q + (w.b < 0 ? token : w.b) * p.q_stride +
+                                (w.h * p.group + row0 + r - token * p.group) * p.head_dim + col;
+          cp_async_16(smem_u32(queries) + buffer * kQueryBytes + (r * kQueryLd + col) * 2, there ? src : p.q, there ? 16 : 0);
+        }
+      }
+      if (lane == 0) {
+        StreamTask &task = tasks[buffer];
+        const int64_t at = w.b < 0 ? w.h * p.stream_prefix + w.rows16 : (int64_t)(w.b + p.stream_prefix) * p.heads + w.h;
+        task.slot = (at + cta) * p.stream_rows;
+        task.head = (int64_t)w.b * p.q_heads + w.h * p.group;
+        task.n = n;
+        task.key0 = (w.lo / kStreamKeys + w.at.first()) * kStreamKeys;
+        task.lo = w.lo;
+        task.hi = w.hi;
+        task.rows = rows;
+        task.whole = p.prefix == 0 && n == w.at.n;
+        task.prefix = w.b < 0;
+        task.row0 = row0;
+        mbar_arrive(&unit_full[buffer]);
+      }
+      cp_async_arrive(&unit_full[buffer]);
+      return true;
+    };
+#pragma unroll 1
+    for (; w.at.left > 0 && ok; w.next(p)) {
       const int32_t count_here = w.at.here();
+      if (count_here == 0) continue;  // the piece ends in front of the unit's first tile
+      if (!publish(count_here)) {
+        ok = false;
+        break;
+      }
       const int32_t *ids = w.b < 0 ? p.prefix_pages : p.paged.page_table + w.b * p.paged.table_stride;
       int32_t key0 = (w.lo / kStreamKeys + w.at.first()) * kStreamKeys;
-      int32_t id = count_here && lane < boxes ? page_id(p, ids, key0 + my_chunk * p.chunk, w.lo, w.hi) : -1;
+      int32_t id = lane < boxes ? page_id(p, ids, key0 + my_chunk * p.chunk, w.lo, w.hi) : -1;
 #pragma unroll 1
       for (int32_t k = 0; k < count_here; ++k, key0 += kStreamKeys) {
         const int32_t id_next = k + 1 < count_here && lane < boxes
@@ -458,8 +532,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
           phase ^= 1;
         }
       }
-      w.next(p);
     }
+    if (ok) ok = publish(0);
     if (!ok) {
       if (lane == 0) record_device_error(p.err, ERR_KERNEL_PAGED_ATTENTION | ERR_SITE_PRODUCER);
       *abort_flag = 1;
@@ -467,34 +541,19 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       // stages from st on were last filled in the other phase
 #pragma unroll 1
       for (int x = 0; x < filled; ++x) wait(&full[x], x < st ? phase : phase ^ 1, nullptr, 1000000000ull);
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
     return;
   }
 
-  // Consumers.  A fragments: rows lane / 4 and lane / 4 + 8 of the unit: the
-  // group's heads, or (prefix) those of all rows of the call.
+  // Consumers.  Fragments: rows lane / 4 and lane / 4 + 8 of the unit.
   const int r0 = lane >> 2, r1 = r0 + 8, cq = (lane & 3) * 2;
-  auto unit_rows = [&](const StreamWalk &u) { return u.b < 0 ? min(16, (int)p.rows * p.group - u.rows16 * 16) : p.group; };
-  auto load_q = [&](const StreamWalk &u, uint32_t (&a)[KS][4]) {
-    const int n = u.at.left > 0 ? unit_rows(u) : 0;
-    const uint16_t *base[2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int row = u.rows16 * 16 + (x ? r1 : r0), token = row / p.group;
-      base[x] = p.q + (u.b < 0 ? token : u.b) * p.q_stride + (u.h * p.group + row - token * p.group) * p.head_dim;
-    }
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int row = j & 1 ? r1 : r0, col = k * 16 + cq + (j & 2 ? 8 : 0);
-        a[k][j] = row < n && col < p.head_dim ? *reinterpret_cast<const uint32_t *>(base[j & 1] + col) : 0u;
-      }
-  };
   // ldmatrix addresses: lane -> row lane % 8 of matrix lane / 8.  K matrices:
   // (keys 0-7, 8-15) x (two 16-byte column chunks); V: keys fastest.
   const int mi = lane >> 3, mr = lane & 7;
   const uint32_t k_row = warp * 16 + (mi >> 1) * 8 + mr, v_row = warp * 16 + (mi & 1) * 8 + mr;
+  // Q: (rows 0-7, 8-15) x (two 16-byte column chunks).
+  const uint32_t q_at = smem_u32(queries) + (((mi & 1) * 8 + mr) * kQueryLd + (mi >> 1) * 8) * 2;
   const uint32_t sbase = smem_u32(smem), pitch = p.pitch;
   // 16-byte column `col` of key `row` of a K or V tile
   auto place = [&](uint32_t row, uint32_t col) {
@@ -504,91 +563,34 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   bool ok = true;
   int st = 0;
   uint32_t phase = 0;
-  // A unit's queries load while the last one's results meet.
-  StreamWalk next = w;
-  int32_t count_here = 0;
-  float o[NT][4], m0, m1, l0, l1;
 #pragma unroll 1
-  for (;;) {
-    uint32_t q[KS][4];
-    load_q(next, q);
-    if (count_here) {
-      l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-      l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-      if ((lane & 3) == 0) {
-        warp_m[warp][r0] = m0;
-        warp_m[warp][r1] = m1;
-        warp_l[warp][r0] = l0;
-        warp_l[warp][r1] = l1;
-      }
-      named_barrier_sync(1 + worker, 128);
-      const float t0 = fmaxf(fmaxf(warp_m[0][r0], warp_m[1][r0]), fmaxf(warp_m[2][r0], warp_m[3][r0]));
-      const float t1 = fmaxf(fmaxf(warp_m[0][r1], warp_m[1][r1]), fmaxf(warp_m[2][r1], warp_m[3][r1]));
-      const float a0 = m0 == -INFINITY ? 0.0f : ex2_approx((m0 - t0) * c);
-      const float a1 = m1 == -INFINITY ? 0.0f : ex2_approx((m1 - t1) * c);
-      const int orow = warp * 4 + (lane >> 3), ocol = (lane & 7) * 4;  // this thread's share of the sums
-      float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) top = fmaxf(top, warp_m[x][orow]);
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        if (warp_m[x][orow] != -INFINITY) sum += warp_l[x][orow] * ex2_approx((warp_m[x][orow] - top) * c);
-      const bool whole = p.prefix == 0 && count_here == w.at.n;
-      const int64_t unit = w.b < 0 ? w.h * p.stream_prefix + w.rows16 : (int64_t)(w.b + p.stream_prefix) * p.heads + w.h;
-      const int64_t slot = (unit + cta) * p.stream_rows + orow;
-      const int rows_here = unit_rows(w);
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      if (!whole && orow < rows_here && ocol == 0) p.stream_ml[slot] = make_float2(top == -INFINITY ? top : top * c, sum);
-#pragma unroll
-      for (int round = 0; round < (DP + 31) / 32; ++round) {
-        float *mine = merge + warp * 16 * kMergeLd;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (round * 4 + i >= NT) continue;
-          const float(&v)[4] = o[round * 4 + i];
-          *reinterpret_cast<float2 *>(mine + r0 * kMergeLd + i * 8 + cq) = make_float2(v[0] * a0, v[1] * a0);
-          *reinterpret_cast<float2 *>(mine + r1 * kMergeLd + i * 8 + cq) = make_float2(v[2] * a1, v[3] * a1);
-        }
-        named_barrier_sync(1 + worker, 128);
-        const int col = round * 32 + ocol;
-        if (orow < rows_here && col < p.head_dim) {
-          float4 r = *reinterpret_cast<const float4 *>(merge + orow * kMergeLd + ocol);
-#pragma unroll
-          for (int x = 1; x < 4; ++x) {
-            const float4 y = *reinterpret_cast<const float4 *>(merge + (x * 16 + orow) * kMergeLd + ocol);
-            r.x += y.x;
-            r.y += y.y;
-            r.z += y.z;
-            r.w += y.w;
-          }
-          if (whole) {
-            uint2 h;
-            h.x = to_h2(r.x * inv, r.y * inv);
-            h.y = to_h2(r.z * inv, r.w * inv);
-            const int64_t head = (int64_t)w.b * p.q_heads + w.h * p.group + orow;
-            *reinterpret_cast<uint2 *>(p.out + head * p.head_dim + col) = h;
-          } else {
-            *reinterpret_cast<float4 *>(p.stream_o + slot * p.head_dim + col) = r;
-          }
-        }
-        named_barrier_sync(1 + worker, 128);
-      }
+  for (uint32_t unit = 0;; ++unit) {
+    // (the four warps go on or stop together: they meet at barriers below)
+    const bool late = !wait(&unit_full[unit & 1], (unit >> 1) & 1, abort_flag);
+    if (barrier_any(1 + worker, 128, late || !ok)) {
+      ok = false;
+      break;
     }
-    if (next.at.left <= 0) break;
-    w = next;
-    count_here = w.at.here();
+    const StreamTask &task = tasks[unit & 1];
+    const int32_t count_here = task.n, lo = task.lo, hi = task.hi, first_key = task.key0 + warp * 16;
+    const int32_t rows_here = task.rows;
+    const bool whole = task.whole, prefix = task.prefix;
+    const int64_t slot0 = task.slot, head0 = task.head;
+    const int32_t row0 = task.row0;
+    uint32_t q[KS][4];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) ldmatrix_x4(q_at + (unit & 1) * kQueryBytes + k * 32, q[k]);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&unit_empty[unit & 1]);
+    if (count_here == 0) break;
     // Keys a row attends to end at the unit's end, in the prefix perhaps before it.
-    int32_t end0 = w.hi, end1 = w.hi, end = w.hi;
-    if (w.b < 0) {
-      const int n = (int)p.rows * p.group, s0 = w.rows16 * 16 + r0, s1 = s0 + 8;
-      if (s0 < n) end0 = min(w.hi, max(0, p.paged.lengths[s0 / p.group]));
-      if (s1 < n) end1 = min(w.hi, max(0, p.paged.lengths[s1 / p.group]));
+    int32_t end0 = hi, end1 = hi, end = hi;
+    if (prefix) {
+      if (r0 < rows_here) end0 = min(hi, max(0, p.paged.lengths[(row0 + r0) / p.group]));
+      if (r1 < rows_here) end1 = min(hi, max(0, p.paged.lengths[(row0 + r1) / p.group]));
       end = __reduce_min_sync(0xffffffffu, min(end0, end1));
     }
-    m0 = m1 = -INFINITY;
-    l0 = l1 = 0.0f;
+    float o[NT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 #pragma unroll 1
@@ -596,7 +598,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       // (a wait that ran out is not left early: the barriers below need every warp)
       if (ok && !wait(&full[st], phase, abort_flag)) ok = false;
       const uint32_t ks = sbase + st * 2 * tile_bytes, vs = ks + tile_bytes;
-      const int32_t key0 = (w.lo / kStreamKeys + w.at.first() + k) * kStreamKeys + warp * 16;
+      const int32_t key0 = first_key + k * kStreamKeys;
       float s[2][4] = {}, s2[2][4] = {};  // even and odd steps: two chains
 #pragma unroll
       for (int d = 0; d < KS; ++d) {
@@ -610,7 +612,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         s[0][j] += s2[0][j];
         s[1][j] += s2[1][j];
       }
-      if (key0 < w.lo || key0 + 16 > end) {
+      if (key0 < lo || key0 + 16 > end) {
         // The unit's first or last tile: scores of keys that are not its own
         // are dropped, and the warp's V rows of such keys, which may hold
         // anything, are zeroed (0 * NaN is NaN).
@@ -619,12 +621,12 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int32_t key = key0 + x * 8 + cq + (j & 1);
-            if (key < w.lo || key >= (j & 2 ? end1 : end0)) s[x][j] = -INFINITY;
+            if (key < lo || key >= (j & 2 ? end1 : end0)) s[x][j] = -INFINITY;
           }
 #pragma unroll 1
         for (int x = lane; x < 16 * NT; x += 32) {
           const int row = x / NT;
-          if (key0 + row < w.lo || key0 + row >= w.hi) {
+          if (key0 + row < lo || key0 + row >= hi) {
             const uint32_t at = vs + place(warp * 16 + row, x % NT);
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
           }
@@ -680,7 +682,73 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         phase ^= 1;
       }
     }
-    next.next(p);
+    // The four warps' results meet: the weights of their maxima, then O in as
+    // many rounds as shared memory needs for the unit's rows.
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    if ((lane & 3) == 0) {
+      warp_m[warp][r0] = m0;
+      warp_m[warp][r1] = m1;
+      warp_l[warp][r0] = l0;
+      warp_l[warp][r1] = l1;
+    }
+    named_barrier_sync(1 + worker, 128);
+    auto weight = [&](float m, int row) {
+      const float t = fmaxf(fmaxf(warp_m[0][row], warp_m[1][row]), fmaxf(warp_m[2][row], warp_m[3][row]));
+      return m == -INFINITY ? 0.0f : ex2_approx((m - t) * c);
+    };
+    const float a0 = weight(m0, r0), a1 = weight(m1, r1);
+    auto meet = [&](auto per_round) {
+      constexpr int NI = decltype(per_round)::value, ROWS = 32 / NI, LD = NI * 8 + 4;  // n8 tiles a round; rows
+      const int orow = (warp * 32 + lane) / (NI * 2), ocol = (lane % (NI * 2)) * 4;   // this thread's share of the sums
+      float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) top = fmaxf(top, warp_m[x][orow & 15]);
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (warp_m[x][orow & 15] != -INFINITY) sum += warp_l[x][orow & 15] * ex2_approx((warp_m[x][orow & 15] - top) * c);
+      const int64_t slot = slot0 + orow;
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      if (!whole && orow < rows_here && ocol == 0) p.stream_ml[slot] = make_float2(top == -INFINITY ? top : top * c, sum);
+#pragma unroll
+      for (int round = 0; round < (NT + NI - 1) / NI; ++round) {
+        if (round) named_barrier_sync(1 + worker, 128);
+        float *mine = merge + warp * ROWS * LD;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          if (round * NI + i >= NT) continue;
+          const float(&v)[4] = o[round * NI + i];
+          if (r0 < ROWS) *reinterpret_cast<float2 *>(mine + r0 * LD + i * 8 + cq) = make_float2(v[0] * a0, v[1] * a0);
+          if (ROWS == 16) *reinterpret_cast<float2 *>(mine + r1 * LD + i * 8 + cq) = make_float2(v[2] * a1, v[3] * a1);
+        }
+        named_barrier_sync(1 + worker, 128);
+        const int col = round * NI * 8 + ocol;
+        if (orow < rows_here && col < p.head_dim) {
+          float4 r = *reinterpret_cast<const float4 *>(merge + orow * LD + ocol);
+#pragma unroll
+          for (int x = 1; x < 4; ++x) {
+            const float4 y = *reinterpret_cast<const float4 *>(merge + (x * ROWS + orow) * LD + ocol);
+            r.x += y.x;
+            r.y += y.y;
+            r.z += y.z;
+            r.w += y.w;
+          }
+          if (whole) {
+            uint2 h;
+            h.x = to_h2(r.x * inv, r.y * inv);
+            h.y = to_h2(r.z * inv, r.w * inv);
+            *reinterpret_cast<uint2 *>(p.out + (head0 + orow) * p.head_dim + col) = h;
+          } else {
+            *reinterpret_cast<float4 *>(p.stream_o + slot * p.head_dim + col) = r;
+          }
+        }
+      }
+    };
+    if (rows_here <= 4) meet(Number<8>());
+    else if (rows_here <= 8) meet(Number<4>());
+    else meet(Number<2>());
   }
   if (!ok) {
     if (lane == 0) record_device_error(p.err, ERR_KERNEL_PAGED_ATTENTION | ERR_SITE_EPILOGUE);
