@@ -323,17 +323,24 @@ struct StreamWalk {
 };
 
 // SMs that stream own parts while the others work on the prefix: so many that
-// both take the same time, by the times per key tile and SM that were measured
-// with both kernels running (not more than saturate HBM).
+// both end together, by what was measured with both kernels running: a start of
+// 8 us and 0.6 us a key tile and SM (heads of 128) against 13 us and 2.15 us a
+// key tile (a row tile alone: 1.5).  More than kStreamSaturated saturate HBM.
 constexpr int kStreamSaturated = 112;
 __device__ __forceinline__ int32_t stream_sms(const PagedAttnParams &p, int64_t own_cost) {
   if (own_cost == 0) return 0;
   if (p.prefix_units == 0) return p.sms;
   const float stream = (float)own_cost * p.heads * (0.25f + 0.35f / 128 * p.head_dim);
   const float tile = (float)p.prefix_units * p.heads * unit_cost((p.prefix + 127) / 128) *
-                     (p.rows > p.tile_rows ? 2.8f : 1.7f);
-  const int32_t x = (int32_t)(p.sms * (stream / (stream + tile)) + 0.5f);
-  return max(1, min(min(x, kStreamSaturated), p.sms - 1));
+                     (p.rows > p.tile_rows ? 2.15f : 1.5f);
+  int32_t lo = 1, hi = min(kStreamSaturated, p.sms - 1);
+#pragma unroll 1
+  while (lo < hi) {
+    const int32_t x = (lo + hi) >> 1;
+    if (8.0f + __fdividef(stream, (float)x) > 13.0f + __fdividef(tile, (float)(p.sms - x))) lo = x + 1;
+    else hi = x;
+  }
+  return lo;
 }
 
 // One unit's share of a worker's piece, as the producer hands it to the others.
