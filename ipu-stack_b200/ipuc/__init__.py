@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libipuc.so")
@@ -474,6 +475,13 @@ class _PagedBatch(ctypes.Structure):
                 ("sequences", _i32), ("max_pages", _i32)]
 
 
+# The same three as bytes: packing costs a third of filling a ctypes structure,
+# and a decode step makes them for every layer.
+_pack_rotary = struct.Struct("@Pqii").pack
+_pack_cache = struct.Struct("@PPqiii4xqqq").pack
+_pack_batch = struct.Struct("@PPPqqii").pack
+
+
 def _refuse(fn, text):
     raise IpucError(fn, ERR_INVALID_ARGUMENT, f"{fn[5:]}: {text}")
 
@@ -508,12 +516,12 @@ def _want(fn, name, t, device, dtype, ndim):
     """Shape and strides of `t`, a CUDA tensor of the current device with this type and rank."""
     if not isinstance(t, _torch.Tensor) or t.dtype is not dtype:
         _refuse(fn, f"{name} has the wrong type")
-    shape = t.shape
-    if len(shape) != ndim:
+    stride = t.stride()
+    if len(stride) != ndim:
         _refuse(fn, f"{name} must have {ndim} dimensions")
     if t.get_device() != device:
         _refuse(fn, f"{name} is not on the current device")
-    return shape, t.stride()
+    return t.shape, stride
 
 
 def _vector(fn, name, t, device, dtype, size):
@@ -549,9 +557,9 @@ def rotary_table(out, base=10000.0, scaling=ROTARY_SCALE_NONE, factor=1.0, low=1
                  magnitude=1.0, stream=None):
     """Fills out (f32 [positions, rotary_dim]) with the cosines and sines of every position; see ipuc_rotary_scaling."""
     fn, (_, device) = "ipuc_rotary_table", _device()
-    spec = Rotary(out).spec
+    Rotary(out)  # its checks
     s = _RotaryScaling(scaling, base, factor, low, high, original, magnitude)
-    call(fn, spec.table, spec.positions, spec.rotary_dim, ctypes.byref(s), _stream_on(device, stream))
+    call(fn, out.data_ptr(), *out.shape, ctypes.byref(s), _stream_on(device, stream))
 
 
 class Rotary:
@@ -563,8 +571,7 @@ class Rotary:
         if stride[1] != 1 or (positions > 1 and stride[0] != columns):
             _refuse(fn, "table must be dense")
         self.table = table
-        self.spec = _Rotary(table.data_ptr(), positions, columns, layout)
-        self._ref = ctypes.byref(self.spec)
+        self._spec = _pack_rotary(table.data_ptr(), positions, columns, layout)
 
 
 def rotary_f16(out, x, rotary, positions=None, stream=None):
@@ -574,7 +581,7 @@ def rotary_f16(out, x, rotary, positions=None, stream=None):
     shape, xs = _token_rows(fn, "x", x, device, dtype)
     _, os_ = _token_rows(fn, "out", out, device, torch.float16, shape)
     at = None if positions is None else _vector(fn, "positions", positions, device, torch.int32, shape[0])
-    call(fn, out.data_ptr(), os_, x.data_ptr(), xs, precision, *shape, None if rotary is None else rotary._ref, at,
+    call(fn, out.data_ptr(), os_, x.data_ptr(), xs, precision, *shape, None if rotary is None else rotary._spec, at,
          _stream_on(device, stream))
 
 
@@ -594,7 +601,7 @@ def qk_norm_rotary_f16(q_out, k_out, q, k, q_weight=None, k_weight=None, eps=1e-
     wk = None if k_weight is None else _vector(fn, "k_weight", k_weight, device, torch.float16, d)
     at = None if positions is None else _vector(fn, "positions", positions, device, torch.int32, tokens)
     call(fn, q_out.data_ptr(), qos, k_out.data_ptr(), kos, q.data_ptr(), qs, k.data_ptr(), ks, precision, wq, wk, eps,
-         tokens, q_heads, k_heads, d, None if rotary is None else rotary._ref, at, _stream_on(device, stream))
+         tokens, q_heads, k_heads, d, None if rotary is None else rotary._spec, at, _stream_on(device, stream))
 
 
 class PagedCache:
@@ -610,11 +617,16 @@ class PagedCache:
         if d > 1 and stride[3] != 1:
             _refuse(fn, "head_dim must be dense")
         # a dimension of one element has no meaningful stride
-        page_stride, head_stride, row_stride = [s if n > 1 else max(s, d) for s, n in zip(stride, shape[:3])]
-        self.keys, self.values = keys, values
-        self.spec = _PagedCache(keys.data_ptr(), values.data_ptr(), pages, page_size, heads, d, page_stride,
-                                head_stride, row_stride)
-        self._ref = ctypes.byref(self.spec)
+        page_stride, head_stride, row_stride, _ = stride
+        if pages == 1:
+            page_stride = max(page_stride, d)
+        if heads == 1:
+            head_stride = max(head_stride, d)
+        if page_size == 1:
+            row_stride = max(row_stride, d)
+        self.keys, self.values, self.heads, self.page_size, self.head_dim = keys, values, heads, page_size, d
+        self._spec = _pack_cache(keys.data_ptr(), values.data_ptr(), pages, page_size, heads, d, page_stride,
+                                 head_stride, row_stride)
 
 
 class PagedBatch:
@@ -630,13 +642,11 @@ class PagedBatch:
         at = _vector(fn, "lengths", lengths, device, torch.int32, n)
         offsets = None if row_offsets is None else _vector(fn, "row_offsets", row_offsets, device, torch.int32, n + 1)
         self._keep = (page_table, lengths, row_offsets)
-        self.spec = _PagedBatch(page_table.data_ptr(), at, offsets, stride[0] if n > 1 else width, 0, n, width)
+        self._spec = (page_table.data_ptr(), at, offsets, stride[0] if n > 1 else width, n, width)
 
     def _with_rows(self, rows):
-        # a struct of its own for each call: two threads may use one batch
-        s = self.spec
-        return ctypes.byref(_PagedBatch(s.page_table, s.lengths, s.row_offsets, s.table_stride, rows, s.sequences,
-                                        s.max_pages))
+        table, lengths, offsets, stride, n, width = self._spec
+        return _pack_batch(table, lengths, offsets or 0, stride, rows, n, width)
 
 
 def paged_append_f16(cache, batch, k, v, rotary=None, stream=None):
@@ -644,11 +654,11 @@ def paged_append_f16(cache, batch, k, v, rotary=None, stream=None):
     fn, (_, device) = "ipuc_paged_append_f16", _device()
     dtype, precision = _precision(fn, "k", k)
     rows = k.shape[0] if k.dim() else 0
-    shape = (rows, cache.spec.heads, cache.spec.head_dim)
+    shape = (rows, cache.heads, cache.head_dim)
     _, ks = _token_rows(fn, "k", k, device, dtype, shape)
     _, vs = _token_rows(fn, "v", v, device, dtype, shape)
-    call(fn, cache._ref, batch._with_rows(rows), k.data_ptr(), ks, v.data_ptr(), vs, precision,
-         None if rotary is None else rotary._ref, _stream_on(device, stream))
+    call(fn, cache._spec, batch._with_rows(rows), k.data_ptr(), ks, v.data_ptr(), vs, precision,
+         None if rotary is None else rotary._spec, _stream_on(device, stream))
 
 
 def paged_attention_workspace_bytes(rows, sequences, q_heads, heads, head_dim, prefix_rows=0, ragged=False) -> int:
@@ -666,19 +676,19 @@ def paged_attention_f16(out, q, cache, batch, workspace, prefix_rows=0, prefix_p
     _, os_ = _token_rows(fn, "out", out, device, torch.float16, shape)
     if os_ != heads * d:
         _refuse(fn, "out must be dense")
-    if d != cache.spec.head_dim:
+    if d != cache.head_dim:
         _refuse(fn, "rows must have the cache's head_dim")
     at = None
     if prefix_rows:
         if prefix_pages is None:
             _refuse(fn, "prefix_rows without prefix_pages")
         (n,), stride = _want(fn, "prefix_pages", prefix_pages, device, torch.int32, 1)
-        if n * cache.spec.page_size < prefix_rows or (n > 1 and stride[0] != 1):
+        if n * cache.page_size < prefix_rows or (n > 1 and stride[0] != 1):
             _refuse(fn, "prefix_pages must be dense and hold prefix_rows")
         at = prefix_pages.data_ptr()
     if workspace is not None and workspace.get_device() != device:
         _refuse(fn, "workspace is not on the current device")
-    call(fn, out.data_ptr(), q.data_ptr(), qs, heads, cache._ref, batch._with_rows(rows), prefix_rows, at, scale,
+    call(fn, out.data_ptr(), q.data_ptr(), qs, heads, cache._spec, batch._with_rows(rows), prefix_rows, at, scale,
          _ptr(workspace), workspace.numel() * workspace.element_size() if workspace is not None else 0,
          _stream_on(device, stream))
 

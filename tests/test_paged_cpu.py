@@ -156,3 +156,13 @@ def test_restatement_of_rotation_keeps_lengths_and_relative_angles():
         assert torch.allclose(y.norm(dim=-1), x.norm(dim=-1))
         dots = torch.einsum("nhd,mhd->nm", y, y)
         assert torch.allclose(dots[1:, 1:], dots[:-1, :-1])   # only the distance matters
+
+
+def test_packed_descriptors_have_the_c_layout():
+    """What the wrappers pack is, byte for byte, the structure of the header."""
+    r = ipuc._Rotary(1 << 40, 5, 64, 1)
+    c = ipuc._PagedCache(1 << 40, 1 << 41, 1 << 33, 16, 3, 128, 1 << 35, 1 << 34, 7)
+    b = ipuc._PagedBatch(1 << 40, 1 << 41, None, 1 << 33, 9, 4, 5)
+    assert bytes(r) == ipuc._pack_rotary(1 << 40, 5, 64, 1)
+    assert bytes(c) == ipuc._pack_cache(1 << 40, 1 << 41, 1 << 33, 16, 3, 128, 1 << 35, 1 << 34, 7)
+    assert bytes(b) == ipuc._pack_batch(1 << 40, 1 << 41, 0, 1 << 33, 9, 4, 5)
