@@ -153,6 +153,12 @@ __device__ __forceinline__ bool barrier_any(uint32_t id, uint32_t count, bool pr
   return r != 0;
 }
 
+// What the f16 pair `h` of two f32 leaves of them.
+__device__ __forceinline__ uint32_t rest_h2(float lo, float hi, uint32_t h) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+  return to_h2(lo - f.x, hi - f.y);
+}
+
 // Length of sequence b as far as its table row can hold it.
 __device__ __forceinline__ int32_t checked_length(const PagedAttnParams &p, int32_t b, bool report) {
   const int32_t n = p.paged.lengths[b], cap = p.paged.max_pages * p.paged.page_size;
@@ -581,7 +587,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     const StreamTask &task = tasks[unit & 1];
     const int32_t count_here = task.n, lo = task.lo, hi = task.hi, first_key = task.key0 + warp * 16;
     const int32_t rows_here = task.rows;
-    const bool whole = task.whole, prefix = task.prefix;
+    const bool whole = task.whole, prefix = task.prefix, few = rows_here <= 8;
     const int64_t slot0 = task.slot, head0 = task.head;
     const int32_t row0 = task.row0;
     uint32_t q[KS][4];
@@ -647,6 +653,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
       x0 = fmaxf(m0, fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2)));
       x1 = fmaxf(m1, fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2)));
+      if (few) x1 = x0;
       if (__any_sync(0xffffffffu, (x0 - m0) * c > kLazy || (x1 - m1) * c > kLazy)) {
         // (m = -inf: the factor is 0, as are l and O)
         const float a0 = x0 == -INFINITY ? 1.0f : ex2_approx((m0 - x0) * c);
@@ -665,15 +672,25 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       }
       // (m = -inf: every score so far is -inf and gives 0)
       const float n0 = m0 == -INFINITY ? 0.0f : kShift - m0 * c, n1 = m1 == -INFINITY ? 0.0f : kShift - m1 * c;
-      uint32_t a[4];
+      // A weight goes into the product in two f16 parts, hi + lo, so that its
+      // rounding (2^-11) does not add to the result's: in units of at most 8
+      // rows the lo parts take the fragments' idle rows 8 to 15, in larger ones
+      // a second product.  HBM bounds the kernel either way.
+      uint32_t a[4], a_lo[4];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const float p0 = ex2_approx(fmaf(s[x][0], c, n0)), p1 = ex2_approx(fmaf(s[x][1], c, n0));
-        const float p2 = ex2_approx(fmaf(s[x][2], c, n1)), p3 = ex2_approx(fmaf(s[x][3], c, n1));
         l0 += p0 + p1;
-        l1 += p2 + p3;
         a[2 * x] = to_h2(p0, p1);
-        a[2 * x + 1] = to_h2(p2, p3);
+        a_lo[2 * x] = rest_h2(p0, p1, a[2 * x]);
+        a[2 * x + 1] = a_lo[2 * x];
+        a_lo[2 * x + 1] = 0;
+        if (!few) {
+          const float p2 = ex2_approx(fmaf(s[x][2], c, n1)), p3 = ex2_approx(fmaf(s[x][3], c, n1));
+          l1 += p2 + p3;
+          a[2 * x + 1] = to_h2(p2, p3);
+          a_lo[2 * x + 1] = rest_h2(p2, p3, a[2 * x + 1]);
+        }
       }
 #pragma unroll
       for (int d = 0; d < NT; d += 2) {
@@ -681,6 +698,10 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         ldmatrix_x4_trans(vs + place(v_row, d + (mi >> 1)), b);
         mma_16816(o[d], a, b[0], b[1]);
         mma_16816(o[d + 1], a, b[2], b[3]);
+        if (!few) {
+          mma_16816(o[d], a_lo, b[0], b[1]);
+          mma_16816(o[d + 1], a_lo, b[2], b[3]);
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[st]);
@@ -707,6 +728,13 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       return m == -INFINITY ? 0.0f : ex2_approx((m - t) * c);
     };
     const float a0 = weight(m0, r0), a1 = weight(m1, r1);
+    if (few) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        o[i][0] += o[i][2];
+        o[i][1] += o[i][3];
+      }
+    }
     auto meet = [&](auto per_round) {
       constexpr int NI = decltype(per_round)::value, ROWS = 32 / NI, LD = NI * 8 + 4;  // n8 tiles a round; rows
       const int orow = (warp * 32 + lane) / (NI * 2), ocol = (lane % (NI * 2)) * 4;   // this thread's share of the sums
