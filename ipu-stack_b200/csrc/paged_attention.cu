@@ -102,17 +102,18 @@ struct PagedAttnParams {
   float *stream_o, *tile_o;
   float2 *stream_ml, *tile_ml;
   int32_t stream_rows, tile_slot_rows;  // rows of a slot
-  // Written by CTA 0 of either kernel for the join: key tiles before sequence
-  // b (stream) or row unit u (tile), then (tile) the whole line's, then the
-  // number of pieces; and row units before sequence b.
+  // Written by CTA 0 of either kernel for the join: the length per head of the
+  // own parts before row unit u, at max_units + 1 the line's, then the number of
+  // pieces; and the row units before sequence b.
   int64_t *stream_sums, *unit_sums;
-  int32_t *unit_base;
+  int32_t *stream_base, *unit_base;
   int32_t sms;                     // CTAs of each kernel
   int32_t stream, tile;            // which of the two run
   int32_t join_rows;               // rows of a block of the join: 8 or kJoinRows
   int32_t stream_prefix;  // the stream kernel takes the prefix too, for so many groups of 16 rows; or 0
-  int32_t tile_own;       // the tile kernel takes the own parts, in at most max_units row units
-  int32_t max_units;
+  int32_t tile_own;       // the tile kernel takes the own parts
+  uint64_t over_group;    // 2^36 / group, rounded up
+  int32_t max_units;      // of own parts, in the kernel that takes them, for sorted row offsets
   int32_t prefix_units;   // tile kernel: row units of the prefix
   int32_t tile_rows;      // tile kernel: batch rows per 128-row MMA tile, 128 / group
   uint32_t *err;
@@ -165,6 +166,38 @@ __device__ __forceinline__ int32_t checked_length(const PagedAttnParams &p, int3
   if (n > cap && report && n > p.prefix) record_device_error(p.err, ERR_KERNEL_PAGED_ATTENTION | ERR_SITE_LENGTH);
   return n < 0 ? 0 : min(n, max(cap, p.prefix));
 }
+
+// The call's first row of sequence b.
+__device__ __forceinline__ int32_t first_row(const PagedAttnParams &p, int32_t b) {
+  return p.paged.row_offsets ? max(0, min(p.paged.row_offsets[b], (int32_t)p.rows)) : b;
+}
+
+// x / group for 0 <= x < 2^31 and group <= 16: group * over_group exceeds 2^36 by
+// less than group, and x times that stays below 2^36.
+__device__ __forceinline__ int32_t over_group(const PagedAttnParams &p, int32_t x) {
+  return (int32_t)((uint64_t)(uint32_t)x * p.over_group >> 36);
+}
+
+// The call's rows of a sequence: [begin, end), the first at position pos0, and
+// its length.
+struct SequenceRows {
+  int32_t begin, end, length;
+  int64_t pos0;
+  __device__ __forceinline__ SequenceRows(const PagedAttnParams &p, int32_t b, bool report) {
+    begin = first_row(p, b);
+    end = first_row(p, b + 1);
+    length = checked_length(p, b, report);
+    pos0 = (int64_t)p.paged.lengths[b] - (end - begin);
+  }
+  // End of the keys that the rows up to row `last` of the sequence attend to.
+  __device__ __forceinline__ int32_t keys_to(int64_t last) const {
+    return (int32_t)max((int64_t)0, min((int64_t)length, pos0 + last + 1));
+  }
+};
+
+// Lines of units: sums over sequences carry the number of row units in front,
+// above 2^40, and the length in front of them per head.
+constexpr int64_t kLength = (1ll << 40) - 1;
 
 // A thread's contiguous share of [0, n) in a block of kThreads.
 template <int kThreads>
@@ -290,40 +323,88 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A worker's place on the line: unit (b, h), keys [lo, hi); b = -1: the prefix,
-// for rows [16 rows16, 16 rows16 + 16) of the call.
+// A worker's place on the line: unit (b, rows16, h): 16 rows of sequence b (of
+// the call for the prefix, b = -1), counted in query heads of key head h, from
+// row 16 rows16 on; keys [lo, hi).
 struct StreamWalk {
   LinePlace at;
-  int32_t b, h, rows16, lo, hi;
+  int32_t b, rows16, h, lo, hi;
+  int32_t unit, behind;     // own part: row units before this one; those of the sequence behind it
+  int32_t begin, rows;      // first batch row of the sequence; rows of the unit
+  int32_t pos0;             // own part: position of the sequence's first row
 
-  __device__ __forceinline__ static int32_t tiles(const PagedAttnParams &p, int32_t len) {
-    return len > p.prefix ? (len + kStreamKeys - 1) / kStreamKeys - p.prefix / kStreamKeys : 0;
+  __device__ __forceinline__ static int32_t units(const PagedAttnParams &p, const SequenceRows &r) {
+    return max(0, ((r.end - r.begin) * p.group + 15) / 16);
   }
-  __device__ __forceinline__ void enter(const PagedAttnParams &p, int32_t sequence) {
-    b = sequence;
-    if (b < 0) {
-      lo = 0;
-      hi = p.prefix;
-      at.n = (hi + kStreamKeys - 1) / kStreamKeys;
-    } else {
-      lo = p.prefix;
-      hi = checked_length(p, b, false);
-      at.n = tiles(p, hi);
-    }
+  // Key tiles of row unit `j`.
+  __device__ __forceinline__ static int32_t tiles(const PagedAttnParams &p, const SequenceRows &r, int32_t j) {
+    const int32_t to = r.keys_to(over_group(p, min((r.end - r.begin) * p.group, 16 * j + 16) - 1));
+    return to > p.prefix ? (to + kStreamKeys - 1) / kStreamKeys - p.prefix / kStreamKeys : 0;
+  }
+  // Row units and length of a sequence's own part (see kLength).
+  __device__ __forceinline__ static int64_t sequence(const PagedAttnParams &p, int32_t b, bool report) {
+    const SequenceRows r(p, b, report);
+    const int32_t n = units(p, r);
+    int64_t sum = (int64_t)n << 40;
+#pragma unroll 1
+    for (int32_t j = 0; j < n; ++j) sum += unit_cost(tiles(p, r, j));
+    return sum;
+  }
+  __device__ __forceinline__ void prefix(const PagedAttnParams &p, int32_t j) {
+    b = -1;
+    rows16 = j;
+    unit = -1;
+    begin = 0;
+    rows = min(16, (int32_t)p.rows * p.group - 16 * j);
+    pos0 = 0;
+    lo = 0;
+    hi = p.prefix;
+    at.n = (hi + kStreamKeys - 1) / kStreamKeys;
+  }
+  __device__ __forceinline__ void own(const PagedAttnParams &p, const SequenceRows &r, int32_t j) {
+    const int32_t all_rows = (r.end - r.begin) * p.group;
+    rows16 = j;
+    behind = units(p, r) - j - 1;
+    begin = r.begin;
+    rows = min(16, all_rows - 16 * j);
+    pos0 = (int32_t)max(r.pos0, (int64_t)INT32_MIN);
+    lo = p.prefix;
+    hi = r.keys_to(over_group(p, 16 * j + rows - 1));
+    at.n = tiles(p, r, j);
   }
   __device__ __noinline__ void next(const PagedAttnParams &p) {
     if (!at.pass()) return;
-    if (b < 0 && ++rows16 < p.stream_prefix) return;
-    rows16 = 0;
-    if (++h < p.heads) return;
-    h = 0;
-#pragma unroll 1
-    do {
-      if (b + 1 >= p.paged.sequences) {
-        at.left = 0;
+    if (b < 0) {  // units are in the order (head, rows)
+      if (rows16 + 1 < p.stream_prefix) {
+        prefix(p, rows16 + 1);
         return;
       }
-      enter(p, b + 1);
+      if (++h < p.heads) {
+        prefix(p, 0);
+        return;
+      }
+      behind = 0;
+    } else if (++h < p.heads) {
+      return;
+    }
+    h = 0;
+    do {  // the next row unit with keys
+      ++unit;
+      if (behind) {
+        own(p, SequenceRows(p, b, false), rows16 + 1);
+        continue;
+      }
+      int32_t n = 0;
+#pragma unroll 1
+      while (!n) {
+        if (++b >= p.paged.sequences) {
+          at.left = 0;
+          return;
+        }
+        const SequenceRows r(p, b, false);
+        n = units(p, r);
+        if (n) own(p, r, 0);
+      }
     } while (at.n == 0);
   }
 };
@@ -351,10 +432,11 @@ __device__ __forceinline__ int32_t stream_sms(const PagedAttnParams &p, int64_t 
 
 // One unit's share of a worker's piece, as the producer hands it to the others.
 struct StreamTask {
-  int64_t slot, head;        // of the partial result; (whole) output head of row 0
+  int64_t slot;              // of the partial result
   int32_t n, key0, lo, hi;   // key tiles from position key0 on, keys [lo, hi); n = 0: the piece is done
   int32_t rows, whole;       // rows of the unit; the result is final
-  int32_t prefix, row0;      // the prefix: first row (token, head of the group) of the unit
+  int32_t prefix, begin;     // the prefix, or a sequence whose rows start at batch row `begin`
+  int32_t row0, pos0, h;     // the unit's first row, in heads of the group from `begin` on; the position at `begin`
 };
 
 template <int DP>
@@ -369,7 +451,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   __shared__ uint64_t all_unit_full[kStreamWorkers][2], all_unit_empty[kStreamWorkers][2];  // queries and task
   __shared__ StreamTask all_tasks[kStreamWorkers][2];
   __shared__ int64_t scratch[kStreamThreads / 32];
-  __shared__ int32_t first_unit[kStreamWorkers][3];
+  __shared__ int32_t first_unit[kStreamWorkers][5];
   __shared__ float all_m[kStreamWorkers][4][16], all_l[kStreamWorkers][4][16];
   __shared__ int aborted;
   volatile int *abort_flag = &aborted;
@@ -401,65 +483,78 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  auto count = [&](int32_t b) { return unit_cost(StreamWalk::tiles(p, checked_length(p, b, blockIdx.x == 0))); };
   // Sums first, then this worker's piece [W c / C, W (c + 1) / C) of the line's W.
   int64_t before;
-  const int64_t total = block_sum<kStreamThreads>(p.paged.sequences, scratch, count, before);
+  const int64_t total = block_sum<kStreamThreads>(
+      p.paged.sequences, scratch, [&](int32_t b) { return StreamWalk::sequence(p, b, blockIdx.x == 0); }, before);
   const int64_t ahead = (int64_t)unit_cost((p.prefix + kStreamKeys - 1) / kStreamKeys) * p.stream_prefix * p.heads;
-  const int64_t line = ahead + total * p.heads;
-  const int64_t sms = p.stream_prefix ? p.sms : stream_sms(p, total);
+  const int64_t line = ahead + (total & kLength) * p.heads;
+  const int64_t sms = p.stream_prefix ? p.sms : stream_sms(p, total & kLength);
   const int64_t pieces = min(kStreamWorkers * sms, line);  // no piece is empty
   // Worker w of CTA c has piece w * sms + c: few pieces spread over many SMs.
   auto piece_of = [&](int w) { return w * sms + (int64_t)blockIdx.x; };
   auto start_of = [&](int w) { return line * piece_of(w) / pieces; };
   const bool idle = (int64_t)blockIdx.x >= min(sms, pieces);
-  if (blockIdx.x == 0) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    p.stream_sums[p.max_units + 1] = line;
+    p.stream_sums[p.max_units + 2] = pieces;
+  }
+  if (!idle || blockIdx.x == 0) {
+    const int64_t start0 = idle ? -1 : start_of(0), start1 = idle ? -1 : start_of(1);
+    static_assert(kStreamWorkers == 2, "two starts");
     const Share<kStreamThreads> mine(p.paged.sequences);
-    int64_t sum = before;
 #pragma unroll 1
     for (int32_t b = mine.lo; b < mine.hi; ++b) {
-      p.stream_sums[b] = sum;
-      sum += count(b);
-    }
-    if (threadIdx.x == 0) {
-      p.stream_sums[p.paged.sequences] = total;
-      p.stream_sums[p.paged.sequences + 1] = pieces;
-    }
-    if (idle) griddep_wait();  // (see the end)
-  }
-  if (idle) return;
-  const Share<kStreamThreads> mine(p.paged.sequences);
+      const SequenceRows r(p, b, false);
+      const int32_t n = StreamWalk::units(p, r), base = (int32_t)(before >> 40);
+      int64_t cost = before & kLength;
+      if (blockIdx.x == 0) p.stream_base[b] = base;
 #pragma unroll 1
-  for (int32_t b = mine.lo; b < mine.hi; ++b) {
-    const int32_t n = count(b);
+      for (int32_t j = 0; j < n; ++j) {
+        const int32_t here = unit_cost(StreamWalk::tiles(p, r, j));
 #pragma unroll 1
-    for (int w = 0; w < kStreamWorkers; ++w) {
-      const int64_t at = start_of(w) - ahead - before * p.heads;
-      if (at >= 0 && at < (int64_t)n * p.heads) {
-        first_unit[w][0] = b;
-        first_unit[w][1] = (int32_t)(at / n);
-        first_unit[w][2] = (int32_t)(at % n);
+        for (int w = 0; w < kStreamWorkers; ++w) {
+          const int64_t at = (w ? start1 : start0) - ahead - cost * p.heads;
+          if (at >= 0 && at < (int64_t)here * p.heads) {
+            first_unit[w][0] = b;
+            first_unit[w][1] = j;
+            first_unit[w][2] = (int32_t)(at / here);
+            first_unit[w][3] = (int32_t)(at % here);
+            first_unit[w][4] = base + j;
+          }
+        }
+        // (max_units holds for sorted row offsets)
+        if (blockIdx.x == 0 && base + j < p.max_units) {
+          p.stream_sums[base + j] = cost;
+          p.stream_sums[base + j + 1] = cost + here;
+        }
+        cost += here;
       }
+      before = ((before >> 40) + n) << 40 | cost;
     }
-    before += n;
+  }
+  if (idle) {
+    if (blockIdx.x == 0) griddep_wait();  // (see the end)
+    return;
   }
   __syncthreads();  // (the barriers' initialisation too)
   const int64_t cta = piece_of(worker), start = start_of(worker);
   if (cta >= pieces) return;  // (a second worker)
   StreamWalk w;
-  w.at.left = line * (cta + 1) / pieces - start;
   if (start < ahead) {
-    w.enter(p, -1);
+    w.prefix(p, 0);
     const int32_t unit = (int32_t)(start / unit_cost(w.at.n));
     w.h = unit / p.stream_prefix;
-    w.rows16 = unit % p.stream_prefix;
+    w.prefix(p, unit % p.stream_prefix);
     w.at.x = (int32_t)(start % unit_cost(w.at.n));
   } else {
-    w.rows16 = 0;
-    w.enter(p, first_unit[worker][0]);
-    w.h = first_unit[worker][1];
-    w.at.x = first_unit[worker][2];
+    w.b = first_unit[worker][0];
+    w.own(p, SequenceRows(p, w.b, false), first_unit[worker][1]);
+    w.h = first_unit[worker][2];
+    w.at.x = first_unit[worker][3];
+    w.unit = first_unit[worker][4];
   }
+  w.at.left = line * (cta + 1) / pieces - start;
 
   if (warp == 4) {
     // Producer: lane l issues boxes l, l + 32, ... of a tile: (K or V, half,
@@ -471,37 +566,37 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     int st = 0, filled = 0;
     uint32_t phase = 0;  // of the stage's barriers
     uint32_t unit = 0;
-    // Hands out the next task and its query rows: the group's heads, or (prefix)
-    // those of 16 rows of the call; zeros behind them and behind head_dim.
+    // Hands out the next task and its query rows; zeros behind them and behind head_dim.
     auto publish = [&](int32_t n) {
       const uint32_t buffer = unit & 1;
       if (!wait(&unit_empty[buffer], ((unit >> 1) & 1) ^ 1, abort_flag)) return false;
       ++unit;
-      const int32_t row0 = w.b < 0 ? w.rows16 * 16 : 0;
-      const int32_t rows = w.b < 0 ? min(16, (int32_t)p.rows * p.group - row0) : p.group;
       if (n) {
 #pragma unroll 1
         for (int x = lane; x < 16 * (DP / 8); x += 32) {
-          const int r = x / (DP / 8), col = x % (DP / 8) * 8, token = (row0 + r) / p.group;
-          const bool there = r < rows && col < p.head_dim;
-          const uint16_t *src = p.q + (w.b < 0 ? token : w.b) * p.q_stride +
-                                (w.h * p.group + row0 + r - token * p.group) * p.head_dim + col;
+          const int r = x / (DP / 8), col = x % (DP / 8) * 8, row = 16 * w.rows16 + r, token = over_group(p, row);
+          const bool there = r < w.rows && col < p.head_dim;
+          const uint16_t *src = p.q + (int64_t)(w.begin + token) * p.q_stride +
+                                (w.h * p.group + row - token * p.group) * p.head_dim + col;
           cp_async_16(smem_u32(queries) + buffer * kQueryBytes + (r * kQueryLd + col) * 2, there ? src : p.q, there ? 16 : 0);
         }
       }
       if (lane == 0) {
         StreamTask &task = tasks[buffer];
-        const int64_t at = w.b < 0 ? w.h * p.stream_prefix + w.rows16 : (int64_t)(w.b + p.stream_prefix) * p.heads + w.h;
+        const int64_t at = w.b < 0 ? w.h * p.stream_prefix + w.rows16 : (int64_t)(p.stream_prefix + w.unit) * p.heads + w.h;
         task.slot = (at + cta) * p.stream_rows;
-        task.head = (int64_t)w.b * p.q_heads + w.h * p.group;
         task.n = n;
         task.key0 = (w.lo / kStreamKeys + w.at.first()) * kStreamKeys;
         task.lo = w.lo;
         task.hi = w.hi;
-        task.rows = rows;
+        // (max_units holds for sorted row offsets; others write nothing past it)
+        task.rows = w.unit < p.max_units ? w.rows : 0;
         task.whole = p.prefix == 0 && n == w.at.n;
         task.prefix = w.b < 0;
-        task.row0 = row0;
+        task.row0 = 16 * w.rows16;
+        task.begin = w.begin;
+        task.pos0 = w.pos0;
+        task.h = w.h;
         mbar_arrive(&unit_full[buffer]);
       }
       cp_async_arrive(&unit_full[buffer]);
@@ -588,21 +683,27 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     const int32_t count_here = task.n, lo = task.lo, hi = task.hi, first_key = task.key0 + warp * 16;
     const int32_t rows_here = task.rows;
     const bool whole = task.whole, prefix = task.prefix, few = rows_here <= 8;
-    const int64_t slot0 = task.slot, head0 = task.head;
-    const int32_t row0 = task.row0;
+    const int64_t slot0 = task.slot;
+    const int32_t row0 = task.row0, begin = task.begin, pos0 = task.pos0, head = task.h * p.group;
     uint32_t q[KS][4];
 #pragma unroll
     for (int k = 0; k < KS; ++k) ldmatrix_x4(q_at + (unit & 1) * kQueryBytes + k * 32, q[k]);
     __syncwarp();
     if (lane == 0) mbar_arrive(&unit_empty[unit & 1]);
     if (count_here == 0) break;
-    // Keys a row attends to end at the unit's end, in the prefix perhaps before it.
-    int32_t end0 = hi, end1 = hi, end = hi;
-    if (prefix) {
-      if (r0 < rows_here) end0 = min(hi, max(0, p.paged.lengths[(row0 + r0) / p.group]));
-      if (r1 < rows_here) end1 = min(hi, max(0, p.paged.lengths[(row0 + r1) / p.group]));
-      end = __reduce_min_sync(0xffffffffu, min(end0, end1));
-    }
+    // Keys a row attends to end at its position, at the unit's end at the latest.
+    auto row_end = [&](int r) {
+      if (r >= rows_here) return hi;
+      const int32_t place = over_group(p, row0 + r);
+      int64_t position = (int64_t)pos0 + place;
+      if (prefix) {
+        PagedRow at;
+        position = paged_row(p.paged, place, at) ? at.position : -1;
+      }
+      return (int32_t)max((int64_t)0, min((int64_t)hi, position + 1));
+    };
+    const int32_t end0 = row_end(r0), end1 = row_end(r1);
+    const int32_t end = __reduce_min_sync(0xffffffffu, min(end0, end1));
     float o[NT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
@@ -774,7 +875,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
             uint2 h;
             h.x = to_h2(r.x * inv, r.y * inv);
             h.y = to_h2(r.z * inv, r.w * inv);
-            *reinterpret_cast<uint2 *>(p.out + (head0 + orow) * p.head_dim + col) = h;
+            const int32_t place = over_group(p, row0 + orow), in_group = row0 + orow - place * p.group;
+            *reinterpret_cast<uint2 *>(p.out + ((int64_t)(begin + place) * p.q_heads + head + in_group) * p.head_dim + col) = h;
           } else {
             *reinterpret_cast<float4 *>(p.stream_o + slot * p.head_dim + col) = r;
           }
@@ -816,10 +918,6 @@ constexpr int kTileRows = 128, kTileKeys = 128;
 constexpr int kTileBytes = 128 * 128 * 2, kTileHalf = kTileBytes / 2;
 constexpr int kTileThreads = 576, kTileSmem = 6 * kTileBytes + 1024;
 
-__device__ __forceinline__ int32_t first_row(const PagedAttnParams &p, int32_t b) {
-  return p.paged.row_offsets ? max(0, min(p.paged.row_offsets[b], (int32_t)p.rows)) : b;
-}
-
 // A CTA's place on the tile kernel's line: unit (row unit, head h); `seq` < 0:
 // the prefix, whose row units cover all rows.
 struct TileWalk {
@@ -829,23 +927,22 @@ struct TileWalk {
   int32_t rows, lo, hi;      // batch rows; keys [lo, hi)
   int64_t row0, pos0;        // first batch row and (own part) its position
 
-  // Key tiles of row unit j of a sequence with rows [begin, end), the first at position `pos`.
-  __device__ __forceinline__ static int32_t own_tiles(const PagedAttnParams &p, int32_t begin, int32_t end, int64_t pos,
-                                                      int32_t len, int32_t j) {
-    const int64_t to = min((int64_t)len, pos + min((int64_t)(end - begin), (int64_t)(j + 1) * 2 * p.tile_rows));
-    return to > p.prefix ? (int32_t)((to + kTileKeys - 1) / kTileKeys) - p.prefix / kTileKeys : 0;
+  // Key tiles of row unit j of a sequence.
+  __device__ __forceinline__ static int32_t tiles(const PagedAttnParams &p, const SequenceRows &r, int32_t j) {
+    const int32_t to = r.keys_to(min((int64_t)(r.end - r.begin), (int64_t)(j + 1) * 2 * p.tile_rows) - 1);
+    return to > p.prefix ? (to + kTileKeys - 1) / kTileKeys - p.prefix / kTileKeys : 0;
   }
   __device__ __noinline__ void own(const PagedAttnParams &p, int32_t b, int32_t row_unit) {
-    const int32_t begin = first_row(p, b), end = first_row(p, b + 1), per_unit = 2 * p.tile_rows;
+    const SequenceRows r(p, b, false);
+    const int32_t per_unit = 2 * p.tile_rows;
     seq = b;
     j = row_unit;
-    row0 = begin + (int64_t)j * per_unit;
-    rows = (int32_t)max((int64_t)0, min((int64_t)per_unit, end - row0));
-    pos0 = (int64_t)p.paged.lengths[b] - (end - begin) + (row0 - begin);
+    row0 = r.begin + (int64_t)j * per_unit;
+    rows = (int32_t)max((int64_t)0, min((int64_t)per_unit, r.end - row0));
+    pos0 = r.pos0 + (row0 - r.begin);
     lo = p.prefix;
-    const int32_t len = checked_length(p, b, false);
-    hi = (int32_t)max((int64_t)0, min((int64_t)len, pos0 + rows));
-    at.n = own_tiles(p, begin, end, pos0 - (row0 - begin), len, j);
+    hi = r.keys_to(row0 - r.begin + rows - 1);
+    at.n = tiles(p, r, j);
   }
   __device__ __forceinline__ void prefix(const PagedAttnParams &p, int32_t row_unit) {
     const int32_t per_unit = 2 * p.tile_rows;
@@ -858,9 +955,9 @@ struct TileWalk {
     hi = p.prefix;
     at.n = (hi + kTileKeys - 1) / kTileKeys;
   }
-  __device__ __forceinline__ static int32_t units(const PagedAttnParams &p, int32_t b) {
+  __device__ __forceinline__ static int32_t units(const PagedAttnParams &p, const SequenceRows &r) {
     const int32_t per_unit = 2 * p.tile_rows;
-    return max(0, (first_row(p, b + 1) - first_row(p, b) + per_unit - 1) / per_unit);
+    return max(0, (r.end - r.begin + per_unit - 1) / per_unit);
   }
   __device__ __forceinline__ int64_t slot_unit(const PagedAttnParams &p) const {
     return seq < 0 ? (int64_t)h * p.prefix_units + j : (int64_t)(p.prefix_units + unit) * p.heads + h;
@@ -891,7 +988,7 @@ struct TileWalk {
 #pragma unroll 1
     for (;; ++unit) {
 #pragma unroll 1
-      while (j >= units(p, seq)) {
+      while (j >= units(p, SequenceRows(p, seq, false))) {
         if (++seq >= p.paged.sequences) {
           at.left = 0;
           return;
@@ -1003,25 +1100,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   // This CTA's piece of the line's W, [W c / C, W (c + 1) / C).
   const int64_t cta = blockIdx.x;
   const int64_t ahead = (int64_t)p.prefix_units * p.heads * unit_cost((p.prefix + kTileKeys - 1) / kTileKeys);
-  // Row units (above 2^40) and the length of sequence b's own part per head, in one sum.
-  constexpr int64_t kLength = (1ll << 40) - 1;
-  auto count = [&](int32_t b) {
-    const int32_t begin = first_row(p, b), end = first_row(p, b + 1), u = TileWalk::units(p, b);
-    const int32_t len = checked_length(p, b, cta == 0);
-    const int64_t pos0 = (int64_t)p.paged.lengths[b] - (end - begin);
-    int64_t sum = (int64_t)u << 40;
-#pragma unroll 1
-    for (int32_t j = 0; j < u; ++j) sum += unit_cost(TileWalk::own_tiles(p, begin, end, pos0, len, j));
-    return sum;
-  };
   int64_t total = 0, before = 0;
   int32_t sms = p.sms;
   if (p.stream)
     sms -= stream_sms(p, block_sum<kTileThreads>(
-                             p.paged.sequences, scratch,
-                             [&](int32_t b) { return unit_cost(StreamWalk::tiles(p, checked_length(p, b, false))); },
-                             before));
-  if (p.tile_own) total = block_sum<kTileThreads>(p.paged.sequences, scratch, count, before);
+                             p.paged.sequences, scratch, [&](int32_t b) { return StreamWalk::sequence(p, b, false); },
+                             before) & kLength);
+  if (p.tile_own)
+    total = block_sum<kTileThreads>(
+        p.paged.sequences, scratch,
+        [&](int32_t b) {
+          const SequenceRows r(p, b, cta == 0);
+          const int32_t n = TileWalk::units(p, r);
+          int64_t sum = (int64_t)n << 40;
+#pragma unroll 1
+          for (int32_t j = 0; j < n; ++j) sum += unit_cost(TileWalk::tiles(p, r, j));
+          return sum;
+        },
+        before);
   const int64_t line = ahead + (total & kLength) * p.heads, ctas = min((int64_t)sms, line);
   const bool idle = cta >= ctas;  // no piece is empty
   const int64_t start = idle ? -1 : line * cta / ctas;
@@ -1030,14 +1126,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const Share<kTileThreads> mine(p.paged.sequences);
 #pragma unroll 1
     for (int32_t b = mine.lo; b < mine.hi; ++b) {
-      const int32_t begin = first_row(p, b), end = first_row(p, b + 1), u = TileWalk::units(p, b);
-      const int32_t base = (int32_t)(before >> 40), len = checked_length(p, b, false);
-      const int64_t pos0 = (int64_t)p.paged.lengths[b] - (end - begin);
+      const SequenceRows r(p, b, false);
+      const int32_t u = TileWalk::units(p, r), base = (int32_t)(before >> 40);
       int64_t cost = before & kLength;
       if (cta == 0) p.unit_base[b] = base;
 #pragma unroll 1
       for (int32_t j = 0; j < u; ++j) {
-        const int32_t n = unit_cost(TileWalk::own_tiles(p, begin, end, pos0, len, j));
+        const int32_t n = unit_cost(TileWalk::tiles(p, r, j));
         const int64_t at = start - ahead - cost * p.heads;
         if (at >= 0 && at < (int64_t)n * p.heads) {
           found[0] = b;
@@ -1590,20 +1685,22 @@ __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_cons
       r.count = 0;
       const int32_t tile_cost = unit_cost((p.prefix + kTileKeys - 1) / kTileKeys), per_unit = 2 * p.tile_rows;
       if (prefix && stream_cost) {
-        const int64_t line = ((int64_t)stream_cost * p.stream_prefix + p.stream_sums[p.paged.sequences]) * p.heads;
         const int32_t unit = kv * p.stream_prefix + (int32_t)index / 16;
-        r = pieces_of(line, p.stream_sums[p.paged.sequences + 1], (int64_t)unit * stream_cost, stream_cost, unit,
-                      (int32_t)index % 16);
+        r = pieces_of(p.stream_sums[p.max_units + 1], p.stream_sums[p.max_units + 2], (int64_t)unit * stream_cost, stream_cost,
+                      unit, (int32_t)index % 16);
       } else if (prefix && p.prefix_units) {
         const int32_t unit = kv * p.prefix_units + (int32_t)row / per_unit;
         r = pieces_of(p.unit_sums[p.max_units + 1], p.unit_sums[p.max_units + 2], (int64_t)unit * tile_cost, tile_cost, unit,
                       (int32_t)row % per_unit * p.group + in_group);
       } else if (!prefix && p.stream) {
-        const int64_t before = p.stream_sums[row], n = p.stream_sums[row + 1] - before;
-        const int64_t ahead = (int64_t)stream_cost * p.stream_prefix * p.heads;
-        const int64_t line = ahead + p.stream_sums[p.paged.sequences] * p.heads;
-        r = pieces_of(line, p.stream_sums[p.paged.sequences + 1], ahead + before * p.heads + kv * n, n,
-                      (int64_t)((int32_t)row + p.stream_prefix) * p.heads + kv, in_group);
+        const int32_t flat = ((int32_t)row - first_row(p, where.sequence)) * p.group + in_group;
+        const int32_t unit = p.stream_base[where.sequence] + flat / 16;
+        if (unit < p.max_units) {
+          const int64_t before = p.stream_sums[unit], n = p.stream_sums[unit + 1] - before;
+          r = pieces_of(p.stream_sums[p.max_units + 1], p.stream_sums[p.max_units + 2],
+                        ((int64_t)stream_cost * p.stream_prefix + before) * p.heads + kv * n, n,
+                        (int64_t)(p.stream_prefix + unit) * p.heads + kv, flat % 16);
+        }
       } else if (!prefix && p.tile_own) {
         const int32_t place = (int32_t)row - first_row(p, where.sequence);
         const int32_t unit = p.unit_base[where.sequence] + place / per_unit;
@@ -1692,12 +1789,12 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // How a call is cut up, from sizes the host knows, and its workspace.
 struct PagedPlan {
-  bool stream;                 // the stream kernel takes single rows
+  bool stream;                 // the stream kernel takes the own parts
   int32_t stream_prefix;       // and their prefix, for so many groups of 16 rows
   bool tile, tile_own;         // the tile kernel runs; takes the own parts
   int32_t sms, stream_rows, tile_rows, tile_slot_rows;
   int64_t prefix_units, max_units;
-  uint64_t stream_o, stream_ml, stream_sums, tile_o, tile_ml, unit_sums, unit_base, bytes;
+  uint64_t stream_o, stream_ml, stream_sums, stream_base, tile_o, tile_ml, unit_sums, unit_base, bytes;
 };
 
 PagedPlan paged_plan(int64_t rows, int64_t sequences, int64_t q_heads, int64_t heads, int64_t head_dim,
@@ -1705,18 +1802,23 @@ PagedPlan paged_plan(int64_t rows, int64_t sequences, int64_t q_heads, int64_t h
   PagedPlan plan = {};
   const int64_t group = q_heads / heads;
   plan.sms = sm_count();
-  plan.stream = !ragged && group <= 16;
+  // The stream kernel reads keys once per 16 rows (in query heads of a key
+  // head), the tile kernel once per 256 and pays for all of them. 32 sequences
+  // of 1 to 4 rows x 4 heads over 500 to 4000 keys take 67 us here and 84 us
+  // there, 16 sequences of 1 to 8 rows x 8 heads, two units each, 83 us both.
+  plan.stream = group <= 16 && (!ragged || rows * group <= 32 * sequences);
   plan.tile_own = !plan.stream;
   // The stream kernel takes the prefix too where its extra time, 0.6 us a key
-  // tile and SM, is below the tile kernel's start (23 rows of 16 heads behind
-  // 729 positions: XX against 27 us).
+  // tile and SM, is below the tile kernel's start: 23 rows of 16 heads behind
+  // 729 positions take 20 against 25 us, 4 rows of 32 heads on 8 behind 512 15
+  // against 22 us.
   const int64_t groups = ceil_div(rows * group, 16);
   if (plan.stream && prefix_rows > 0 && groups * heads * ceil_div(prefix_rows, kStreamKeys) * 0.6 < plan.sms * 8.0)
     plan.stream_prefix = (int32_t)groups;
   if (plan.stream && prefix_rows > 0 && groups == 1) plan.stream_prefix = 1;
   plan.tile_rows = (int32_t)(kTileRows / group);
   plan.tile_slot_rows = (int32_t)(2 * plan.tile_rows * group);
-  plan.stream_rows = (int32_t)(plan.stream_prefix ? 16 : group);
+  plan.stream_rows = (int32_t)(plan.stream_prefix || ragged ? 16 : group);
   const int64_t per_unit = 2 * plan.tile_rows;
   uint64_t at = 0;
   auto take = [&](uint64_t bytes) {
@@ -1725,11 +1827,13 @@ PagedPlan paged_plan(int64_t rows, int64_t sequences, int64_t q_heads, int64_t h
     return here;
   };
   if (plan.stream) {
+    plan.max_units = ragged ? rows * group / 16 + sequences : sequences;
     const int64_t slots =
-        ((sequences + plan.stream_prefix) * heads + kStreamWorkers * plan.sms) * plan.stream_rows;
+        ((plan.max_units + plan.stream_prefix) * heads + kStreamWorkers * plan.sms) * plan.stream_rows;
     plan.stream_o = take(slots * head_dim * 4);
     plan.stream_ml = take(slots * 8);
-    plan.stream_sums = take((sequences + 2) * 8);
+    plan.stream_sums = take((plan.max_units + 3) * 8);
+    plan.stream_base = take(sequences * 4);
   }
   if (prefix_rows > 0 && !plan.stream_prefix) plan.prefix_units = ceil_div(rows, per_unit);
   if (plan.tile_own) {
@@ -1738,7 +1842,7 @@ PagedPlan paged_plan(int64_t rows, int64_t sequences, int64_t q_heads, int64_t h
   }
   if (plan.prefix_units || plan.tile_own) {
     plan.tile = true;
-    const int64_t slots = ((plan.prefix_units + plan.max_units) * heads + plan.sms) * plan.tile_slot_rows;
+    const int64_t slots = ((plan.prefix_units + (plan.tile_own ? plan.max_units : 0)) * heads + plan.sms) * plan.tile_slot_rows;
     plan.tile_o = take(slots * head_dim * 4);
     plan.tile_ml = take(slots * 8);
     plan.unit_sums = take((plan.max_units + 3) * 8);
@@ -1834,6 +1938,7 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
   p.stream_o = reinterpret_cast<float *>(ws + plan.stream_o);
   p.stream_ml = reinterpret_cast<float2 *>(ws + plan.stream_ml);
   p.stream_sums = reinterpret_cast<int64_t *>(ws + plan.stream_sums);
+  p.stream_base = reinterpret_cast<int32_t *>(ws + plan.stream_base);
   p.stream_rows = plan.stream_rows;
   p.stream = plan.stream;
   p.sms = plan.sms;
@@ -1847,6 +1952,7 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
   p.tile_own = plan.tile_own;
   p.prefix_units = (int32_t)plan.prefix_units;
   p.max_units = (int32_t)plan.max_units;
+  p.over_group = ((1ull << 36) + (uint64_t)p.group - 1) / (uint64_t)p.group;
   p.tile_rows = plan.tile_rows;
   p.err = device_error_word();
   const int64_t tasks = p.rows * q_heads;

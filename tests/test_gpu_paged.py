@@ -325,6 +325,12 @@ RAGGED = [
     ([700], [129], 300, 128, 1, 1, 96, 0), ([64, 10, 90], [40, 10, 80], 50, 16, 1, 5, 128, 0),
     ([129, 1, 128], [129, 1, 128], 0, 16, 1, 24, 64, 0), ([40, 41], [1, 1], 16, 8, 1, 128, 128, 0),
     ([60, 41], [9, 30], 0, 1, 1, 4, 128, 0), ([200, 141], [70, 30], 100, 20, 1, 4, 72, 1), ([300, 290], [7, 9], 280, 2, 2, 2, 64, 0),
+    # few rows a sequence: units of 16 rows that begin and end inside a token's heads, sequences without rows
+    ([9], [2], 0, 16, 1, 16, 64, 0), ([70, 64, 65], [3, 1, 2], 0, 16, 2, 5, 128, 2), ([5, 2, 400], [5, 3, 9], 0, 16, 1, 4, 72, 0),
+    ([300, 0, 20, 310, 3], [4, 0, 0, 30, 3], 0, 64, 2, 3, 128, 1), ([900, 850], [1, 3], 0, 128, 1, 11, 96, 0),
+    ([130, 140, 128, 127], [2, 1, 3, 1], 128, 64, 2, 4, 128, 0), ([600] * 30, [4] * 30, 590, 16, 2, 4, 80, 3),
+    ([66, 90] * 5, [3, 2] * 5, 64, 32, 4, 8, 64, 0), ([1000, 20] * 20, [5, 2] * 20, 0, 16, 1, 6, 128, 4),
+    ([40] * 700, [1, 2, 0, 3, 1, 1, 2] * 100, 30, 8, 1, 2, 64, 5), ([7] * 400, [0] * 399 + [7], 0, 16, 1, 1, 64, 0),
 ]
 
 
