@@ -103,17 +103,16 @@ struct PagedAttnParams {
   float2 *stream_ml, *tile_ml;
   int32_t stream_rows, tile_slot_rows;  // rows of a slot
   // Written by CTA 0 of either kernel for the join: the length per head of the
-  // own parts before row unit u, at max_units + 1 the line's, then the number of
-  // pieces; and the row units before sequence b.
+  // own parts before row unit u, at (its) units + 1 the line's, then the number
+  // of pieces; and the row units before sequence b.
   int64_t *stream_sums, *unit_sums;
   int32_t *stream_base, *unit_base;
   int32_t sms;                     // CTAs of each kernel
-  int32_t stream, tile;            // which of the two run
+  int32_t stream, tile_own;        // which of the two take own parts (both: see few_rows)
   int32_t join_rows;               // rows of a block of the join: 8 or kJoinRows
   int32_t stream_prefix;  // the stream kernel takes the prefix too, for so many groups of 16 rows; or 0
-  int32_t tile_own;       // the tile kernel takes the own parts
   uint64_t over_group;    // 2^36 / group, rounded up
-  int32_t max_units;      // of own parts, in the kernel that takes them, for sorted row offsets
+  int32_t stream_units, tile_units;  // of own parts at most, for sorted row offsets
   int32_t prefix_units;   // tile kernel: row units of the prefix
   int32_t tile_rows;      // tile kernel: batch rows per 128-row MMA tile, 128 / group
   uint32_t *err;
@@ -195,6 +194,18 @@ struct SequenceRows {
   }
 };
 
+// Who takes a sequence's own part.  The stream kernel reads the keys once per 16
+// rows, counted in query heads of a key head, the tile kernel once per 256, and
+// pays for all of them.  Two units of 16 are where they meet: 32 sequences of 1
+// to 4 rows x 4 heads over 500 to 4000 keys take 72 us with the first and 84 us
+// with the second; 16 sequences of 1 to 8 rows x 8 heads 83 us with the second,
+// 90 us with those of 5 to 8 rows there and the others here, 116 us with the
+// first alone.
+constexpr int kFewRows = 32;
+__device__ __forceinline__ bool few_rows(const PagedAttnParams &p, const SequenceRows &r) {
+  return p.stream && (!p.tile_own || (int64_t)(r.end - r.begin) * p.group <= kFewRows);
+}
+
 // Lines of units: sums over sequences carry the number of row units in front,
 // above 2^40, and the length in front of them per head.
 constexpr int64_t kLength = (1ll << 40) - 1;
@@ -209,33 +220,6 @@ struct Share {
     hi = min(n, lo + size);
   }
 };
-
-// Sum of count(b) over [0, n) by the whole block; `before` becomes the sum in
-// front of this thread's share.
-template <int kThreads, typename Count>
-__device__ __forceinline__ int64_t block_sum(int32_t n, int64_t *scratch, Count count, int64_t &before) {
-  const Share<kThreads> share(n);
-  int64_t mine = 0;
-#pragma unroll 1
-  for (int32_t b = share.lo; b < share.hi; ++b) mine += count(b);
-  int64_t sum = mine;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll 1
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, sum, d);
-    if (lane >= d) sum += x;
-  }
-  if (lane == 31) scratch[warp] = sum;
-  __syncthreads();
-  int64_t total = 0;
-  before = sum - mine;
-#pragma unroll 1
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += scratch[w];
-    total += scratch[w];
-  }
-  return total;
-}
 
 // The page id of the chunk of keys at position `pos`, if the chunk has a key of
 // [lo, hi); checked_page makes a page coordinate of it, out of range (the TMA
@@ -334,21 +318,12 @@ struct StreamWalk {
   int32_t pos0;             // own part: position of the sequence's first row
 
   __device__ __forceinline__ static int32_t units(const PagedAttnParams &p, const SequenceRows &r) {
-    return max(0, ((r.end - r.begin) * p.group + 15) / 16);
+    return few_rows(p, r) ? max(0, ((r.end - r.begin) * p.group + 15) / 16) : 0;
   }
   // Key tiles of row unit `j`.
   __device__ __forceinline__ static int32_t tiles(const PagedAttnParams &p, const SequenceRows &r, int32_t j) {
     const int32_t to = r.keys_to(over_group(p, min((r.end - r.begin) * p.group, 16 * j + 16) - 1));
     return to > p.prefix ? (to + kStreamKeys - 1) / kStreamKeys - p.prefix / kStreamKeys : 0;
-  }
-  // Row units and length of a sequence's own part (see kLength).
-  __device__ __forceinline__ static int64_t sequence(const PagedAttnParams &p, int32_t b, bool report) {
-    const SequenceRows r(p, b, report);
-    const int32_t n = units(p, r);
-    int64_t sum = (int64_t)n << 40;
-#pragma unroll 1
-    for (int32_t j = 0; j < n; ++j) sum += unit_cost(tiles(p, r, j));
-    return sum;
   }
   __device__ __forceinline__ void prefix(const PagedAttnParams &p, int32_t j) {
     b = -1;
@@ -409,17 +384,105 @@ struct StreamWalk {
   }
 };
 
-// SMs that stream own parts while the others work on the prefix: so many that
-// both end together, by what was measured with both kernels running: a start of
-// 8 us and 0.6 us a key tile and SM (heads of 128) against 13 us and 2.15 us a
-// key tile (a row tile alone: 1.5).  More than kStreamSaturated saturate HBM.
+constexpr int kTileRows = 128, kTileKeys = 128;
+constexpr int kTileBytes = 128 * 128 * 2, kTileHalf = kTileBytes / 2;
+constexpr int kTileThreads = 576, kTileSmem = 6 * kTileBytes + 1024;
+
+// A CTA's place on the tile kernel's line: unit (row unit, head h); `seq` < 0:
+// the prefix, whose row units cover all rows.
+struct TileWalk {
+  LinePlace at;
+  int32_t seq, j, h;         // row unit j of its sequence (or of the prefix)
+  int32_t unit;              // own part: row units before it
+  int32_t rows, lo, hi;      // batch rows; keys [lo, hi)
+  int64_t row0, pos0;        // first batch row and (own part) its position
+
+  // Key tiles of row unit j of a sequence.
+  __device__ __forceinline__ static int32_t tiles(const PagedAttnParams &p, const SequenceRows &r, int32_t j) {
+    const int32_t to = r.keys_to(min((int64_t)(r.end - r.begin), (int64_t)(j + 1) * 2 * p.tile_rows) - 1);
+    return to > p.prefix ? (to + kTileKeys - 1) / kTileKeys - p.prefix / kTileKeys : 0;
+  }
+  __device__ __noinline__ void own(const PagedAttnParams &p, int32_t b, int32_t row_unit) {
+    const SequenceRows r(p, b, false);
+    const int32_t per_unit = 2 * p.tile_rows;
+    seq = b;
+    j = row_unit;
+    row0 = r.begin + (int64_t)j * per_unit;
+    rows = (int32_t)max((int64_t)0, min((int64_t)per_unit, r.end - row0));
+    pos0 = r.pos0 + (row0 - r.begin);
+    lo = p.prefix;
+    hi = r.keys_to(row0 - r.begin + rows - 1);
+    at.n = tiles(p, r, j);
+  }
+  __device__ __forceinline__ void prefix(const PagedAttnParams &p, int32_t row_unit) {
+    const int32_t per_unit = 2 * p.tile_rows;
+    seq = -1;
+    j = row_unit;
+    row0 = (int64_t)j * per_unit;
+    rows = (int32_t)min((int64_t)per_unit, p.rows - row0);
+    pos0 = 0;
+    lo = 0;
+    hi = p.prefix;
+    at.n = (hi + kTileKeys - 1) / kTileKeys;
+  }
+  __device__ __forceinline__ static int32_t units(const PagedAttnParams &p, const SequenceRows &r) {
+    const int32_t per_unit = 2 * p.tile_rows;
+    return few_rows(p, r) ? 0 : max(0, (r.end - r.begin + per_unit - 1) / per_unit);
+  }
+  __device__ __forceinline__ int64_t slot_unit(const PagedAttnParams &p) const {
+    return seq < 0 ? (int64_t)h * p.prefix_units + j : (int64_t)(p.prefix_units + unit) * p.heads + h;
+  }
+  __device__ __noinline__ void next(const PagedAttnParams &p) {
+    if (!at.pass()) return;
+    if (seq < 0) {  // units are in the order (head, row unit)
+      if (++j < p.prefix_units) {
+        prefix(p, j);
+        return;
+      }
+      if (++h < p.heads) {
+        prefix(p, 0);
+        return;
+      }
+      unit = -1;
+      j = 0;
+      h = 0;
+    } else if (++h < p.heads) {
+      return;
+    } else {
+      h = 0;
+      ++j;
+    }
+    // the next row unit with keys
+    ++unit;
+    if (seq < 0) seq = 0;
+#pragma unroll 1
+    for (;; ++unit) {
+#pragma unroll 1
+      while (j >= units(p, SequenceRows(p, seq, false))) {
+        if (++seq >= p.paged.sequences) {
+          at.left = 0;
+          return;
+        }
+        j = 0;
+      }
+      own(p, seq, j);
+      if (at.n > 0) return;
+      ++j;
+    }
+  }
+};
+
+// SMs that stream while the others work on row tiles, of two lines (key tiles):
+// so many that both end together, by what was measured with both kernels
+// running: a start of 8 us and 0.6 us a key tile and SM (heads of 128) against
+// 13 us and 2.15 us a key tile (a row tile alone: 1.5).  More than
+// kStreamSaturated saturate HBM.
 constexpr int kStreamSaturated = 112;
-__device__ __forceinline__ int32_t stream_sms(const PagedAttnParams &p, int64_t own_cost) {
-  if (own_cost == 0) return 0;
-  if (p.prefix_units == 0) return p.sms;
-  const float stream = (float)own_cost * p.heads * (0.25f + 0.35f / 128 * p.head_dim);
-  const float tile = (float)p.prefix_units * p.heads * unit_cost((p.prefix + 127) / 128) *
-                     (p.rows > p.tile_rows ? 2.15f : 1.5f);
+__device__ __forceinline__ int32_t stream_sms(const PagedAttnParams &p, int64_t stream_line, int64_t tile_line) {
+  if (stream_line == 0) return 0;
+  if (tile_line == 0) return p.sms;
+  const float stream = (float)stream_line * (0.25f + 0.35f / 128 * p.head_dim);
+  const float tile = (float)tile_line * (p.rows > p.tile_rows ? 2.15f : 1.5f);
   int32_t lo = 1, hi = min(kStreamSaturated, p.sms - 1);
 #pragma unroll 1
   while (lo < hi) {
@@ -429,6 +492,67 @@ __device__ __forceinline__ int32_t stream_sms(const PagedAttnParams &p, int64_t 
   }
   return lo;
 }
+
+// Row units and length of a sequence's own part (see kLength) in the kernel that takes it.
+template <typename Walk>
+__device__ __forceinline__ int64_t own_part(const PagedAttnParams &p, const SequenceRows &r) {
+  const int32_t n = Walk::units(p, r);
+  int64_t sum = (int64_t)n << 40;
+#pragma unroll 1
+  for (int32_t j = 0; j < n; ++j) sum += unit_cost(Walk::tiles(p, r, j));
+  return sum;
+}
+
+// Both kernels' lines, in key tiles: a CTA of either needs both to know how many
+// SMs each has.  Summed by the whole block.
+template <int kThreads>
+struct Lines {
+  int64_t stream_ahead, stream, tile_ahead, tile;  // the prefix's part, which is in front; the whole
+  int64_t stream_before, tile_before;              // sums of own_part() in front of this thread's share
+  int32_t sms_to_stream;
+  __device__ __forceinline__ Lines(const PagedAttnParams &p, int64_t (&scratch)[kThreads / 32][2], bool report) {
+    const Share<kThreads> share(p.paged.sequences);
+    int64_t mine[2] = {0, 0};
+#pragma unroll 1
+    for (int32_t b = share.lo; b < share.hi; ++b) {
+      const SequenceRows r(p, b, report);
+      if (few_rows(p, r)) mine[0] += own_part<StreamWalk>(p, r);
+      else mine[1] += own_part<TileWalk>(p, r);
+    }
+    int64_t sum[2] = {mine[0], mine[1]};
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll 1
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, sum[0], d), y = __shfl_up_sync(0xffffffffu, sum[1], d);
+      if (lane >= d) {
+        sum[0] += x;
+        sum[1] += y;
+      }
+    }
+    if (lane == 31) {
+      scratch[warp][0] = sum[0];
+      scratch[warp][1] = sum[1];
+    }
+    __syncthreads();
+    stream_before = sum[0] - mine[0];
+    tile_before = sum[1] - mine[1];
+    stream = tile = 0;
+#pragma unroll 1
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) {
+        stream_before += scratch[w][0];
+        tile_before += scratch[w][1];
+      }
+      stream += scratch[w][0];
+      tile += scratch[w][1];
+    }
+    stream_ahead = (int64_t)unit_cost((p.prefix + kStreamKeys - 1) / kStreamKeys) * p.stream_prefix * p.heads;
+    tile_ahead = (int64_t)unit_cost((p.prefix + kTileKeys - 1) / kTileKeys) * p.prefix_units * p.heads;
+    stream = stream_ahead + (stream & kLength) * p.heads;
+    tile = tile_ahead + (tile & kLength) * p.heads;
+    sms_to_stream = stream_sms(p, stream, tile);
+  }
+};
 
 // One unit's share of a worker's piece, as the producer hands it to the others.
 struct StreamTask {
@@ -450,7 +574,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   __shared__ uint64_t all_full[kStreamWorkers][kStreamStages], all_empty[kStreamWorkers][kStreamStages];
   __shared__ uint64_t all_unit_full[kStreamWorkers][2], all_unit_empty[kStreamWorkers][2];  // queries and task
   __shared__ StreamTask all_tasks[kStreamWorkers][2];
-  __shared__ int64_t scratch[kStreamThreads / 32];
+  __shared__ int64_t scratch[kStreamThreads / 32][2];
   __shared__ int32_t first_unit[kStreamWorkers][5];
   __shared__ float all_m[kStreamWorkers][4][16], all_l[kStreamWorkers][4][16];
   __shared__ int aborted;
@@ -483,21 +607,20 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
+  // (sums of unsorted row offsets may run over and find no first unit)
+  if (threadIdx.x >= 32 && threadIdx.x < 32 + kStreamWorkers * 5) (&first_unit[0][0])[threadIdx.x - 32] = 0;
   // Sums first, then this worker's piece [W c / C, W (c + 1) / C) of the line's W.
-  int64_t before;
-  const int64_t total = block_sum<kStreamThreads>(
-      p.paged.sequences, scratch, [&](int32_t b) { return StreamWalk::sequence(p, b, blockIdx.x == 0); }, before);
-  const int64_t ahead = (int64_t)unit_cost((p.prefix + kStreamKeys - 1) / kStreamKeys) * p.stream_prefix * p.heads;
-  const int64_t line = ahead + (total & kLength) * p.heads;
-  const int64_t sms = p.stream_prefix ? p.sms : stream_sms(p, total & kLength);
+  const Lines<kStreamThreads> lines(p, scratch, blockIdx.x == 0 && !p.tile_own);
+  const int64_t line = lines.stream, ahead = lines.stream_ahead, sms = lines.sms_to_stream;
+  int64_t before = lines.stream_before;
   const int64_t pieces = min(kStreamWorkers * sms, line);  // no piece is empty
   // Worker w of CTA c has piece w * sms + c: few pieces spread over many SMs.
   auto piece_of = [&](int w) { return w * sms + (int64_t)blockIdx.x; };
   auto start_of = [&](int w) { return line * piece_of(w) / pieces; };
   const bool idle = (int64_t)blockIdx.x >= min(sms, pieces);
   if (blockIdx.x == 0 && threadIdx.x == 0) {
-    p.stream_sums[p.max_units + 1] = line;
-    p.stream_sums[p.max_units + 2] = pieces;
+    p.stream_sums[p.stream_units + 1] = line;
+    p.stream_sums[p.stream_units + 2] = pieces;
   }
   if (!idle || blockIdx.x == 0) {
     const int64_t start0 = idle ? -1 : start_of(0), start1 = idle ? -1 : start_of(1);
@@ -523,8 +646,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
             first_unit[w][4] = base + j;
           }
         }
-        // (max_units holds for sorted row offsets)
-        if (blockIdx.x == 0 && base + j < p.max_units) {
+        // (stream_units holds for sorted row offsets; sums of others may even be negative)
+        if (blockIdx.x == 0 && (uint32_t)(base + j) < (uint32_t)p.stream_units) {
           p.stream_sums[base + j] = cost;
           p.stream_sums[base + j + 1] = cost + here;
         }
@@ -589,8 +712,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
         task.key0 = (w.lo / kStreamKeys + w.at.first()) * kStreamKeys;
         task.lo = w.lo;
         task.hi = w.hi;
-        // (max_units holds for sorted row offsets; others write nothing past it)
-        task.rows = w.unit < p.max_units ? w.rows : 0;
+        // (for unsorted row offsets nothing is written past the last unit)
+        task.rows = w.b < 0 || (uint32_t)w.unit < (uint32_t)p.stream_units ? w.rows : 0;
         task.whole = p.prefix == 0 && n == w.at.n;
         task.prefix = w.b < 0;
         task.row0 = 16 * w.rows16;
@@ -873,8 +996,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
           }
           if (whole) {
             uint2 h;
-            h.x = to_h2(r.x * inv, r.y * inv);
-            h.y = to_h2(r.z * inv, r.w * inv);
+            h.x = sum == 0.0f ? 0u : to_h2(r.x * inv, r.y * inv);  // (no keys: 0 * V, where V may be anything)
+            h.y = sum == 0.0f ? 0u : to_h2(r.z * inv, r.w * inv);
             const int32_t place = over_group(p, row0 + orow), in_group = row0 + orow - place * p.group;
             *reinterpret_cast<uint2 *>(p.out + ((int64_t)(begin + place) * p.q_heads + head + in_group) * p.head_dim + col) = h;
           } else {
@@ -914,94 +1037,6 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 // A unit whose rows fill one row tile only has it twice, for even and for odd
 // key tiles (`dual`), and joins both at its end: each row's two O lie in the same
 // TMEM lane.
-constexpr int kTileRows = 128, kTileKeys = 128;
-constexpr int kTileBytes = 128 * 128 * 2, kTileHalf = kTileBytes / 2;
-constexpr int kTileThreads = 576, kTileSmem = 6 * kTileBytes + 1024;
-
-// A CTA's place on the tile kernel's line: unit (row unit, head h); `seq` < 0:
-// the prefix, whose row units cover all rows.
-struct TileWalk {
-  LinePlace at;
-  int32_t seq, j, h;         // row unit j of its sequence (or of the prefix)
-  int32_t unit;              // own part: row units before it
-  int32_t rows, lo, hi;      // batch rows; keys [lo, hi)
-  int64_t row0, pos0;        // first batch row and (own part) its position
-
-  // Key tiles of row unit j of a sequence.
-  __device__ __forceinline__ static int32_t tiles(const PagedAttnParams &p, const SequenceRows &r, int32_t j) {
-    const int32_t to = r.keys_to(min((int64_t)(r.end - r.begin), (int64_t)(j + 1) * 2 * p.tile_rows) - 1);
-    return to > p.prefix ? (to + kTileKeys - 1) / kTileKeys - p.prefix / kTileKeys : 0;
-  }
-  __device__ __noinline__ void own(const PagedAttnParams &p, int32_t b, int32_t row_unit) {
-    const SequenceRows r(p, b, false);
-    const int32_t per_unit = 2 * p.tile_rows;
-    seq = b;
-    j = row_unit;
-    row0 = r.begin + (int64_t)j * per_unit;
-    rows = (int32_t)max((int64_t)0, min((int64_t)per_unit, r.end - row0));
-    pos0 = r.pos0 + (row0 - r.begin);
-    lo = p.prefix;
-    hi = r.keys_to(row0 - r.begin + rows - 1);
-    at.n = tiles(p, r, j);
-  }
-  __device__ __forceinline__ void prefix(const PagedAttnParams &p, int32_t row_unit) {
-    const int32_t per_unit = 2 * p.tile_rows;
-    seq = -1;
-    j = row_unit;
-    row0 = (int64_t)j * per_unit;
-    rows = (int32_t)min((int64_t)per_unit, p.rows - row0);
-    pos0 = 0;
-    lo = 0;
-    hi = p.prefix;
-    at.n = (hi + kTileKeys - 1) / kTileKeys;
-  }
-  __device__ __forceinline__ static int32_t units(const PagedAttnParams &p, const SequenceRows &r) {
-    const int32_t per_unit = 2 * p.tile_rows;
-    return max(0, (r.end - r.begin + per_unit - 1) / per_unit);
-  }
-  __device__ __forceinline__ int64_t slot_unit(const PagedAttnParams &p) const {
-    return seq < 0 ? (int64_t)h * p.prefix_units + j : (int64_t)(p.prefix_units + unit) * p.heads + h;
-  }
-  __device__ __noinline__ void next(const PagedAttnParams &p) {
-    if (!at.pass()) return;
-    if (seq < 0) {  // units are in the order (head, row unit)
-      if (++j < p.prefix_units) {
-        prefix(p, j);
-        return;
-      }
-      if (++h < p.heads) {
-        prefix(p, 0);
-        return;
-      }
-      unit = -1;
-      j = 0;
-      h = 0;
-    } else if (++h < p.heads) {
-      return;
-    } else {
-      h = 0;
-      ++j;
-    }
-    // the next row unit with keys
-    ++unit;
-    if (seq < 0) seq = 0;
-#pragma unroll 1
-    for (;; ++unit) {
-#pragma unroll 1
-      while (j >= units(p, SequenceRows(p, seq, false))) {
-        if (++seq >= p.paged.sequences) {
-          at.left = 0;
-          return;
-        }
-        j = 0;
-      }
-      own(p, seq, j);
-      if (at.n > 0) return;
-      ++j;
-    }
-  }
-};
-
 // One unit's share of a CTA's piece, as the load warp hands it to the others:
 // only that warp walks the line, which costs the softmax warps no registers.
 struct TileTask {
@@ -1067,7 +1102,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __shared__ uint32_t tmem_slot;
   __shared__ int aborted;
   __shared__ float x_max[2][2][kTileRows], x_sum[2][2][kTileRows];
-  __shared__ int64_t scratch[kTileThreads / 32];
+  __shared__ int64_t scratch[kTileThreads / 32][2];
   __shared__ int32_t found[5];
   __shared__ uint64_t task_full[2], task_empty[2];
   __shared__ TileTask tasks[2];
@@ -1097,28 +1132,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
+  if (threadIdx.x >= 32 && threadIdx.x < 37) found[threadIdx.x - 32] = 0;  // (as first_unit above)
   // This CTA's piece of the line's W, [W c / C, W (c + 1) / C).
   const int64_t cta = blockIdx.x;
-  const int64_t ahead = (int64_t)p.prefix_units * p.heads * unit_cost((p.prefix + kTileKeys - 1) / kTileKeys);
-  int64_t total = 0, before = 0;
-  int32_t sms = p.sms;
-  if (p.stream)
-    sms -= stream_sms(p, block_sum<kTileThreads>(
-                             p.paged.sequences, scratch, [&](int32_t b) { return StreamWalk::sequence(p, b, false); },
-                             before) & kLength);
-  if (p.tile_own)
-    total = block_sum<kTileThreads>(
-        p.paged.sequences, scratch,
-        [&](int32_t b) {
-          const SequenceRows r(p, b, cta == 0);
-          const int32_t n = TileWalk::units(p, r);
-          int64_t sum = (int64_t)n << 40;
-#pragma unroll 1
-          for (int32_t j = 0; j < n; ++j) sum += unit_cost(TileWalk::tiles(p, r, j));
-          return sum;
-        },
-        before);
-  const int64_t line = ahead + (total & kLength) * p.heads, ctas = min((int64_t)sms, line);
+  const Lines<kTileThreads> lines(p, scratch, cta == 0);
+  const int64_t line = lines.tile, ahead = lines.tile_ahead, ctas = min((int64_t)(p.sms - lines.sms_to_stream), line);
+  int64_t before = lines.tile_before;
   const bool idle = cta >= ctas;  // no piece is empty
   const int64_t start = idle ? -1 : line * cta / ctas;
   griddep_launch_dependents();
@@ -1141,7 +1160,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           found[3] = (int32_t)(at % n);
           found[4] = base + j;
         }
-        if (cta == 0 && base + j < p.max_units) {
+        if (cta == 0 && (uint32_t)(base + j) < (uint32_t)p.tile_units) {
           p.unit_sums[base + j] = cost;
           p.unit_sums[base + j + 1] = cost + n;
         }
@@ -1151,8 +1170,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
   }
   if (cta == 0 && threadIdx.x == 0) {
-    p.unit_sums[p.max_units + 1] = line;
-    p.unit_sums[p.max_units + 2] = ctas;
+    p.unit_sums[p.tile_units + 1] = line;
+    p.unit_sums[p.tile_units + 2] = ctas;
   }
   if (idle) return;
   __syncthreads();
@@ -1216,8 +1235,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       task.dual = walk.rows <= p.tile_rows;
       task.prefix = walk.seq < 0;
       task.direct = p.prefix == 0 && task.n == walk.at.n;
-      // (max_units holds for sorted row offsets; others write no partials past it)
-      task.store = walk.unit < p.max_units;
+      // (for unsorted row offsets nothing is written past the last unit)
+      task.store = walk.seq < 0 || (uint32_t)walk.unit < (uint32_t)p.tile_units;
       task.fix_first = task.first * kTileKeys < walk.lo && walk.lo % p.chunk != 0;
       task.fix_last = (task.first + task.n) * kTileKeys > walk.hi && walk.hi % p.chunk != 0;
       if (!publish(task, unit)) {
@@ -1641,16 +1660,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 // row by row (tile slots) or dim by dim (stream slots).  A row's partials are
 // the pieces of its prefix unit and those of its own unit, both runs of slots.
 struct Pieces {
-  int64_t slot;    // of the first
-  int32_t count, row;
+  const float2 *ml;  // of the first one's row; a piece is `rows` rows further
+  const float *o;    // its dim 0; four dims further on `dims`, a piece rows * head_dim
+  int32_t count, rows, dims;  // count < 0: padding
 };
 // Pieces of unit `unit`, at [first, first + cost) of a line of length `line`:
 // piece c of C is [line c / C, line (c + 1) / C), so place t is in c = ((t + 1) C
 // - 1) / line, and the unit's tiles are its places from kUnitCost on.
-__device__ __forceinline__ Pieces pieces_of(int64_t line, int64_t c, int64_t first, int64_t cost,
-                                            int64_t unit, int32_t row) {
-  Pieces r = {0, 0, row};
+__device__ __forceinline__ Pieces pieces_of(const PagedAttnParams &p, bool stream, int64_t first, int64_t cost, int64_t unit,
+                                            int32_t row) {
+  Pieces r = {p.stream ? p.stream_ml : p.tile_ml, p.stream ? p.stream_o : p.tile_o, 0, 0, 0};
   if (cost <= 0) return r;
+  const int64_t *sums = stream ? p.stream_sums + p.stream_units : p.unit_sums + p.tile_units, line = sums[1], c = sums[2];
   const int64_t last = first + cost;
   first += kUnitCost;
   int32_t c0, c1;
@@ -1664,8 +1685,19 @@ __device__ __forceinline__ Pieces pieces_of(int64_t line, int64_t c, int64_t fir
   // (in bounds whatever the sums of unsorted row offsets are)
   c0 = max(0, min(c0, (int32_t)c - 1));
   c1 = max(c0, min(c1, (int32_t)c - 1));
-  r.slot = unit + c0;
   r.count = c1 - c0 + 1;
+  const int64_t slot = unit + c0;
+  if (stream) {
+    r.rows = p.stream_rows;
+    r.dims = 4;
+    r.ml = p.stream_ml + slot * r.rows + row;
+    r.o = p.stream_o + (slot * r.rows + row) * p.head_dim;
+  } else {
+    r.rows = p.tile_slot_rows;
+    r.dims = r.rows * 4;
+    r.ml = p.tile_ml + slot * r.rows + row;
+    r.o = p.tile_o + (slot * (p.head_dim >> 2) * r.rows + row) * 4;
+  }
   return r;
 }
 
@@ -1679,36 +1711,34 @@ __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_cons
     const bool prefix = threadIdx.x >= kJoinRows;
     const uint32_t index = blockIdx.x * p.join_rows + threadIdx.x % kJoinRows, row = index / (uint32_t)p.group;
     const int32_t in_group = (int32_t)(index - row * (uint32_t)p.group);
-    Pieces r = {0, -1, 0};
+    Pieces r = {nullptr, nullptr, -1, 0, 0};
     PagedRow where;
     if (row < p.rows && paged_row(p.paged, row, where)) {
       r.count = 0;
       const int32_t tile_cost = unit_cost((p.prefix + kTileKeys - 1) / kTileKeys), per_unit = 2 * p.tile_rows;
       if (prefix && stream_cost) {
         const int32_t unit = kv * p.stream_prefix + (int32_t)index / 16;
-        r = pieces_of(p.stream_sums[p.max_units + 1], p.stream_sums[p.max_units + 2], (int64_t)unit * stream_cost, stream_cost,
-                      unit, (int32_t)index % 16);
+        r = pieces_of(p, true, (int64_t)unit * stream_cost, stream_cost, unit, (int32_t)index % 16);
       } else if (prefix && p.prefix_units) {
         const int32_t unit = kv * p.prefix_units + (int32_t)row / per_unit;
-        r = pieces_of(p.unit_sums[p.max_units + 1], p.unit_sums[p.max_units + 2], (int64_t)unit * tile_cost, tile_cost, unit,
-                      (int32_t)row % per_unit * p.group + in_group);
-      } else if (!prefix && p.stream) {
-        const int32_t flat = ((int32_t)row - first_row(p, where.sequence)) * p.group + in_group;
-        const int32_t unit = p.stream_base[where.sequence] + flat / 16;
-        if (unit < p.max_units) {
-          const int64_t before = p.stream_sums[unit], n = p.stream_sums[unit + 1] - before;
-          r = pieces_of(p.stream_sums[p.max_units + 1], p.stream_sums[p.max_units + 2],
-                        ((int64_t)stream_cost * p.stream_prefix + before) * p.heads + kv * n, n,
-                        (int64_t)(p.stream_prefix + unit) * p.heads + kv, flat % 16);
-        }
-      } else if (!prefix && p.tile_own) {
-        const int32_t place = (int32_t)row - first_row(p, where.sequence);
-        const int32_t unit = p.unit_base[where.sequence] + place / per_unit;
-        if (unit < p.max_units) {
-          const int64_t before = p.unit_sums[unit], n = p.unit_sums[unit + 1] - before;
-          r = pieces_of(p.unit_sums[p.max_units + 1], p.unit_sums[p.max_units + 2],
-                        ((int64_t)p.prefix_units * tile_cost + before) * p.heads + kv * n, n,
-                        (int64_t)(p.prefix_units + unit) * p.heads + kv, place % per_unit * p.group + in_group);
+        r = pieces_of(p, false, (int64_t)unit * tile_cost, tile_cost, unit, (int32_t)row % per_unit * p.group + in_group);
+      } else if (!prefix) {
+        const SequenceRows rows(p, where.sequence, false);
+        const int32_t place = (int32_t)row - rows.begin, flat = place * p.group + in_group;
+        if (few_rows(p, rows)) {
+          const int32_t unit = p.stream_base[where.sequence] + flat / 16;
+          if ((uint32_t)unit < (uint32_t)p.stream_units) {
+            const int64_t before = p.stream_sums[unit], n = p.stream_sums[unit + 1] - before;
+            r = pieces_of(p, true, ((int64_t)stream_cost * p.stream_prefix + before) * p.heads + kv * n, n,
+                          (int64_t)(p.stream_prefix + unit) * p.heads + kv, flat % 16);
+          }
+        } else {
+          const int32_t unit = p.unit_base[where.sequence] + place / per_unit;
+          if ((uint32_t)unit < (uint32_t)p.tile_units) {
+            const int64_t before = p.unit_sums[unit], n = p.unit_sums[unit + 1] - before;
+            r = pieces_of(p, false, ((int64_t)p.prefix_units * tile_cost + before) * p.heads + kv * n, n,
+                          (int64_t)(p.prefix_units + unit) * p.heads + kv, place % per_unit * p.group + in_group);
+          }
         }
       }
     }
@@ -1724,18 +1754,9 @@ __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_cons
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float l = 0.0f, top = -INFINITY;
     // Four partials' loads are issued before the first is used, with no branch between them.
-    const bool pre_stream = stream_cost != 0, own_stream = p.stream != 0;
-    const int32_t pre_rows = pre_stream ? p.stream_rows : p.tile_slot_rows, own_rows = own_stream ? p.stream_rows : p.tile_slot_rows;
-    auto ml_of = [&](const Pieces &r, bool stream, int32_t rows) {
-      return (stream ? p.stream_ml : p.tile_ml) + r.slot * rows + r.row;
-    };
-    auto part_of = [&](const Pieces &r, bool stream, int32_t rows) {
-      return stream ? p.stream_o + (r.slot * rows + r.row) * p.head_dim + dim
-                    : p.tile_o + ((r.slot * (p.head_dim >> 2) + (dim >> 2)) * rows + r.row) * 4;
-    };
-    const float2 *pre_ml = ml_of(pre, pre_stream, pre_rows), *own_ml = ml_of(own, own_stream, own_rows) - (int64_t)pre.count * own_rows;
-    const int64_t pre_step = (int64_t)pre_rows * p.head_dim, own_step = (int64_t)own_rows * p.head_dim;
-    const float *pre_part = part_of(pre, pre_stream, pre_rows), *own_part = part_of(own, own_stream, own_rows) - pre.count * own_step;
+    const int64_t pre_step = (int64_t)pre.rows * p.head_dim, own_step = (int64_t)own.rows * p.head_dim;
+    const float *pre_part = pre.o + (dim >> 2) * pre.dims, *own_part = own.o + (dim >> 2) * own.dims - pre.count * own_step;
+    const float2 *own_ml = own.ml - (int64_t)pre.count * own.rows;
     const int32_t count = pre.count + own.count;
 #pragma unroll 1
     for (int32_t i = 0; i < count; i += 4) {
@@ -1748,7 +1769,7 @@ __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_cons
         v[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (i + x < count) {
           const bool first = i + x < pre.count;
-          s[x] = first ? pre_ml[(int64_t)(i + x) * pre_rows] : own_ml[(int64_t)(i + x) * own_rows];
+          s[x] = first ? pre.ml[(int64_t)(i + x) * pre.rows] : own_ml[(int64_t)(i + x) * own.rows];
           v[x] = *reinterpret_cast<const float4 *>(first ? pre_part + (i + x) * pre_step : own_part + (i + x) * own_step);
         }
       }
@@ -1789,11 +1810,11 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // How a call is cut up, from sizes the host knows, and its workspace.
 struct PagedPlan {
-  bool stream;                 // the stream kernel takes the own parts
-  int32_t stream_prefix;       // and their prefix, for so many groups of 16 rows
-  bool tile, tile_own;         // the tile kernel runs; takes the own parts
+  bool stream, tile_own;       // which kernels take own parts
+  int32_t stream_prefix;       // the stream kernel takes the prefix, for so many groups of 16 rows
+  bool tile;                   // the tile kernel runs
   int32_t sms, stream_rows, tile_rows, tile_slot_rows;
-  int64_t prefix_units, max_units;
+  int64_t prefix_units, stream_units, tile_units;
   uint64_t stream_o, stream_ml, stream_sums, stream_base, tile_o, tile_ml, unit_sums, unit_base, bytes;
 };
 
@@ -1802,12 +1823,13 @@ PagedPlan paged_plan(int64_t rows, int64_t sequences, int64_t q_heads, int64_t h
   PagedPlan plan = {};
   const int64_t group = q_heads / heads;
   plan.sms = sm_count();
-  // The stream kernel reads keys once per 16 rows (in query heads of a key
-  // head), the tile kernel once per 256 and pays for all of them. 32 sequences
-  // of 1 to 4 rows x 4 heads over 500 to 4000 keys take 67 us here and 84 us
-  // there, 16 sequences of 1 to 8 rows x 8 heads, two units each, 83 us both.
-  plan.stream = group <= 16 && (!ragged || rows * group <= 32 * sequences);
-  plan.tile_own = !plan.stream;
+  // Sequences of few rows go to the stream kernel, the others to the tile kernel
+  // (few_rows): 63 single rows next to a prompt of 512 over 600 to 3000 keys take
+  // 108 us so and 188 us on the tile kernel alone.  No sequence can have many
+  // where the call has few; and where they fill a unit of the tile kernel on
+  // average, it takes all of them, which saves a launch.
+  plan.stream = group <= 16 && (!ragged || rows * group <= 2 * kTileRows * sequences);
+  plan.tile_own = !plan.stream || (ragged && rows * group > kFewRows);
   // The stream kernel takes the prefix too where its extra time, 0.6 us a key
   // tile and SM, is below the tile kernel's start: 23 rows of 16 heads behind
   // 729 positions take 20 against 25 us, 4 rows of 32 heads on 8 behind 512 15
@@ -1827,25 +1849,25 @@ PagedPlan paged_plan(int64_t rows, int64_t sequences, int64_t q_heads, int64_t h
     return here;
   };
   if (plan.stream) {
-    plan.max_units = ragged ? rows * group / 16 + sequences : sequences;
+    plan.stream_units = ragged ? rows * group / 16 + sequences : sequences;
     const int64_t slots =
-        ((plan.max_units + plan.stream_prefix) * heads + kStreamWorkers * plan.sms) * plan.stream_rows;
+        ((plan.stream_units + plan.stream_prefix) * heads + kStreamWorkers * plan.sms) * plan.stream_rows;
     plan.stream_o = take(slots * head_dim * 4);
     plan.stream_ml = take(slots * 8);
-    plan.stream_sums = take((plan.max_units + 3) * 8);
+    plan.stream_sums = take((plan.stream_units + 3) * 8);
     plan.stream_base = take(sequences * 4);
   }
   if (prefix_rows > 0 && !plan.stream_prefix) plan.prefix_units = ceil_div(rows, per_unit);
   if (plan.tile_own) {
-    plan.max_units = rows / per_unit + sequences;
-    if (plan.max_units > rows) plan.max_units = rows;
+    const int64_t several = plan.stream ? rows * group / (kFewRows + 1) : rows;  // sequences with that many rows
+    plan.tile_units = rows / per_unit + (sequences < several ? sequences : several);
   }
   if (plan.prefix_units || plan.tile_own) {
     plan.tile = true;
-    const int64_t slots = ((plan.prefix_units + (plan.tile_own ? plan.max_units : 0)) * heads + plan.sms) * plan.tile_slot_rows;
+    const int64_t slots = ((plan.prefix_units + plan.tile_units) * heads + plan.sms) * plan.tile_slot_rows;
     plan.tile_o = take(slots * head_dim * 4);
     plan.tile_ml = take(slots * 8);
-    plan.unit_sums = take((plan.max_units + 3) * 8);
+    plan.unit_sums = take((plan.tile_units + 3) * 8);
     plan.unit_base = take(sequences * 4);
   }
   plan.bytes = at > 256 ? at : 256;
@@ -1948,15 +1970,20 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
   p.unit_sums = reinterpret_cast<int64_t *>(ws + plan.unit_sums);
   p.unit_base = reinterpret_cast<int32_t *>(ws + plan.unit_base);
   p.tile_slot_rows = plan.tile_slot_rows;
-  p.tile = plan.tile;
   p.tile_own = plan.tile_own;
   p.prefix_units = (int32_t)plan.prefix_units;
-  p.max_units = (int32_t)plan.max_units;
+  p.stream_units = (int32_t)plan.stream_units;
+  p.tile_units = (int32_t)plan.tile_units;
   p.over_group = ((1ull << 36) + (uint64_t)p.group - 1) / (uint64_t)p.group;
   p.tile_rows = plan.tile_rows;
   p.err = device_error_word();
   const int64_t tasks = p.rows * q_heads;
-  IPUC_CHECK_ARG(tasks < (1ll << 31) && plan.max_units < (1ll << 23), "paged_attention: extent too large");
+  // (sums over units are held in 23 bits, their key tiles in 40)
+  const int64_t units = plan.prefix_units + plan.tile_units + plan.stream_prefix + plan.stream_units;
+  const int64_t keys = (int64_t)batch->max_pages * cache->page_size;
+  IPUC_CHECK_ARG(tasks < (1ll << 31) - 256 && units < (1ll << 23) &&
+                     units * p.heads < (1ll << 40) / ((keys > prefix_rows ? keys : prefix_rows) / kStreamKeys + 4),
+                 "paged_attention: extent too large");
   CUtensorMap tm_q, tm_k, tm_v;
   auto cache_map = [&](CUtensorMap *map, const void *base, int32_t box) {
     return make_map_paged(map, base, d, cache->page_size, cache->heads, cache->pages, cache->row_stride,

@@ -330,6 +330,10 @@ RAGGED = [
     ([300, 0, 20, 310, 3], [4, 0, 0, 30, 3], 0, 64, 2, 3, 128, 1), ([900, 850], [1, 3], 0, 128, 1, 11, 96, 0),
     ([130, 140, 128, 127], [2, 1, 3, 1], 128, 64, 2, 4, 128, 0), ([600] * 30, [4] * 30, 590, 16, 2, 4, 80, 3),
     ([66, 90] * 5, [3, 2] * 5, 64, 32, 4, 8, 64, 0), ([1000, 20] * 20, [5, 2] * 20, 0, 16, 1, 6, 128, 4),
+    # sequences of few rows next to sequences of many
+    ([500, 90, 30, 333, 0, 40], [100, 1, 9, 2, 0, 8], 0, 16, 2, 4, 128, 2), ([64, 1, 70], [64, 1, 33], 0, 64, 1, 1, 64, 0),
+    ([300] * 20 + [410], [1] * 20 + [120], 200, 32, 2, 4, 128, 0), ([150] * 9, [3, 40, 1] * 3, 0, 12, 1, 5, 80, 1),
+    ([700, 30] * 4, [2, 30] * 4, 26, 16, 1, 16, 72, 0), ([5, 60], [7, 80], 0, 16, 2, 2, 96, 3),
     ([40] * 700, [1, 2, 0, 3, 1, 1, 2] * 100, 30, 8, 1, 2, 64, 5), ([7] * 400, [0] * 399 + [7], 0, 16, 1, 1, 64, 0),
 ]
 
