@@ -509,7 +509,8 @@ ipuc_status ipuc_rotary_f16(void *out, int64_t out_stride, const void *in, int64
 
 /* Norm of queries and keys over each head, y = x / sqrt(mean(x^2) + eps) *
  * weight (f16 [head_dim], NULL for ones), and their rotation (NULL: none) in
- * one pass.  Rows, precisions, positions and in-place use as ipuc_rotary_f16;
+ * one pass.  Rows, precisions, positions (without a rotation only their sign
+ * counts) and in-place use as ipuc_rotary_f16;
  * q_heads or k_heads may be 0 (that tensor's pointers are then not read). */
 ipuc_status ipuc_qk_norm_rotary_f16(void *q_out, int64_t q_out_stride, void *k_out, int64_t k_out_stride,
                                     const void *q, int64_t q_stride, const void *k, int64_t k_stride,
@@ -556,7 +557,8 @@ ipuc_status ipuc_paged_append_f16(const ipuc_paged_cache *cache, const ipuc_page
  * position p attends to positions 0..p of its sequence, softmax(q k^T * scale)
  * v per head; query head h reads key head h / (q_heads / heads).  q [rows]
  * [q_heads][head_dim] f16 at stride q_stride, out [rows][q_heads][head_dim]
- * f16, dense.  scale <= 0 selects 1/sqrt(head_dim).  A row that attends to
+ * f16, dense, apart from q (refused where the two overlap).  scale <= 0 selects
+ * 1/sqrt(head_dim).  A row that attends to
  * nothing gives 0.
  * prefix_rows: positions below it are the same for all sequences and are read
  * through prefix_pages (device int32, ceil(prefix_rows / page_size) entries)

@@ -45,6 +45,7 @@ enum : uint32_t {
   ERR_SITE_POSITION = 16,
   ERR_SITE_LENGTH = 17,
   ERR_SITE_PAGE = 18,
+  ERR_SITE_OFFSET = 19,
   ERR_KERNEL_GEMM_F16 = 1u << 16,
   ERR_KERNEL_GEMM_F32 = 2u << 16,
   ERR_KERNEL_ATTENTION = 3u << 16,

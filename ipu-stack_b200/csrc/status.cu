@@ -86,9 +86,9 @@ extern "C" ipuc_status ipuc_device_status(ipuc_stream stream) {
     char buf[128];
     const uint32_t site = value & 0xffffu;
     if (site >= ERR_SITE_INDEX) {
-      static const char *const what[] = {"position", "length", "page id"};
+      static const char *const what[] = {"position", "length", "page id", "row offset"};
       snprintf(buf, sizeof(buf), "index in device memory out of range: kernel %u, %s", value >> 16,
-               site - ERR_SITE_INDEX < 3 ? what[site - ERR_SITE_INDEX] : "index");
+               site - ERR_SITE_INDEX < 4 ? what[site - ERR_SITE_INDEX] : "index");
       return fail(IPUC_ERR_DEVICE_INDEX, buf);
     }
     snprintf(buf, sizeof(buf), "device wait timed out: kernel %u site %u", value >> 16, value & 0xffffu);

@@ -524,6 +524,13 @@ def _want(fn, name, t, device, dtype, ndim):
     return t.shape, stride
 
 
+def _on(fn, device, *specs):
+    """Refuses a table, cache or batch that was made for another device than the call's."""
+    for s in specs:
+        if s is not None and s._on != device:
+            _refuse(fn, f"{type(s).__name__} is not on the current device")
+
+
 def _vector(fn, name, t, device, dtype, size):
     """Address of a dense vector."""
     shape, stride = _want(fn, name, t, device, dtype, 1)
@@ -570,13 +577,14 @@ class Rotary:
         (positions, columns), stride = _want(fn, "table", table, device, torch.float32, 2)
         if stride[1] != 1 or (positions > 1 and stride[0] != columns):
             _refuse(fn, "table must be dense")
-        self.table = table
+        self.table, self._on = table, device
         self._spec = _pack_rotary(table.data_ptr(), positions, columns, layout)
 
 
 def rotary_f16(out, x, rotary, positions=None, stream=None):
     """out = x with the heads rotated: x [tokens, heads, head_dim] f16 or f32, out f16 of that shape."""
     fn, (torch, device) = "ipuc_rotary_f16", _device()
+    _on(fn, device, rotary)
     dtype, precision = _precision(fn, "x", x)
     shape, xs = _token_rows(fn, "x", x, device, dtype)
     _, os_ = _token_rows(fn, "out", out, device, torch.float16, shape)
@@ -590,6 +598,7 @@ def qk_norm_rotary_f16(q_out, k_out, q, k, q_weight=None, k_weight=None, eps=1e-
     """Per-head norm of q and k, then their rotation: q [tokens, q_heads, head_dim], k [tokens, k_heads, head_dim]
     of one type, weights f16 [head_dim] (None: ones)."""
     fn, (torch, device) = "ipuc_qk_norm_rotary_f16", _device()
+    _on(fn, device, rotary)
     dtype, precision = _precision(fn, "q", q)
     q_shape, qs = _token_rows(fn, "q", q, device, dtype)
     tokens, q_heads, d = q_shape
@@ -625,6 +634,7 @@ class PagedCache:
         if page_size == 1:
             row_stride = max(row_stride, d)
         self.keys, self.values, self.heads, self.page_size, self.head_dim = keys, values, heads, page_size, d
+        self._on = device
         self._spec = _pack_cache(keys.data_ptr(), values.data_ptr(), pages, page_size, heads, d, page_stride,
                                  head_stride, row_stride)
 
@@ -641,7 +651,7 @@ class PagedBatch:
             _refuse(fn, "page_table must be dense in its last dimension")
         at = _vector(fn, "lengths", lengths, device, torch.int32, n)
         offsets = None if row_offsets is None else _vector(fn, "row_offsets", row_offsets, device, torch.int32, n + 1)
-        self._keep = (page_table, lengths, row_offsets)
+        self._keep, self._on = (page_table, lengths, row_offsets), device
         self._spec = (page_table.data_ptr(), at, offsets, stride[0] if n > 1 else width, n, width)
 
     def _with_rows(self, rows):
@@ -652,6 +662,7 @@ class PagedBatch:
 def paged_append_f16(cache, batch, k, v, rotary=None, stream=None):
     """Writes the new rows k, v [rows, heads, head_dim] (f16 or f32) into the cache, keys rotated by their positions."""
     fn, (_, device) = "ipuc_paged_append_f16", _device()
+    _on(fn, device, cache, batch, rotary)
     dtype, precision = _precision(fn, "k", k)
     rows = k.shape[0] if k.dim() else 0
     shape = (rows, cache.heads, cache.head_dim)
@@ -671,6 +682,7 @@ def paged_attention_f16(out, q, cache, batch, workspace, prefix_rows=0, prefix_p
     """Attention of q [rows, q_heads, head_dim] over the cache into out (dense); positions below prefix_rows are read
     once for all rows through prefix_pages."""
     fn, (torch, device) = "ipuc_paged_attention_f16", _device()
+    _on(fn, device, cache, batch)
     shape, qs = _token_rows(fn, "q", q, device, torch.float16)
     rows, heads, d = shape
     _, os_ = _token_rows(fn, "out", out, device, torch.float16, shape)

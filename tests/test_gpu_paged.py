@@ -168,6 +168,19 @@ def test_qk_norm_without_weights_in_place_and_one_side():
     within(fused, want, ref.rounded(want, want.abs(), 64 / 2 + 8))
 
 
+def test_qk_norm_without_rotation_leaves_padding():
+    """Without a rotation a negative position still marks padding; others may lie behind any table."""
+    g = gen(6)
+    x = randn(g, (5, 2, 64))
+    out = torch.full_like(x, 7.0)
+    positions = torch.tensor([0, -1, 2 ** 31 - 1, -2 ** 31, 3], dtype=torch.int32, device="cuda")
+    ipuc.qk_norm_rotary_f16(out[:, :1], out[:, 1:], x[:, :1], x[:, 1:], eps=1e-6, positions=positions)
+    want = ref.norm(f64(x), None, 1e-6)
+    keep = torch.tensor([0, 2, 4])
+    within(out[keep.cuda()], want[keep], ref.rounded(want, want.abs(), 64 / 2 + 8)[keep])
+    assert (out[[1, 3]] == 7).all()
+
+
 def test_qk_norm_extremes():
     x = torch.zeros((3, 1, 128), dtype=F16, device="cuda")
     x[1] = 65504.0
@@ -405,6 +418,17 @@ def test_attention_reports_bad_pages_and_lengths():
                 assert (f64(out)[1] - want).abs().max() <= 4 * ref.F16_HALF_STEP * v.abs().max()
 
 
+@pytest.mark.parametrize("rows,offsets", [(8, [0, 5, 3, 8]), (8, [-1, 2, 4, 8]), (8, [0, 2, 4, 9]), (200, [0, 200, 0, 200]),
+                                          (200, [0, 190, 3, 200])])
+def test_attention_reports_row_offsets_out_of_order_and_range(rows, offsets):
+    c = Case(25, [60, 40, 50], heads=2, dim=64, page=16).device()
+    c.rows, c.offsets = rows, offsets
+    c.device()
+    run_attention(c, 4)
+    with pytest.raises(ipuc.IpucError, match="row offset"):
+        ipuc.device_status()
+
+
 # ---- together ---------------------------------------------------------------------
 
 def serve_step(c, fused, wq, wk, rotary, positions, heads, kv, ws, bufs):
@@ -488,6 +512,31 @@ def test_graph_follows_lengths_and_tables_in_device_memory():
         want, bound, _ = ref.attention(f64(q), f64(c.keys).nan_to_num(), f64(c.values).nan_to_num(), c.table, now, None, 0, [],
                                        0.125)
         within(out, want, bound)
+
+
+def test_attention_rows_without_keys_next_to_values_that_are_not_finite():
+    """More rows than positions: the first attend to nothing and give 0, whatever the values of the others' keys are."""
+    for new in ([6], [80]):
+        c = Case(23, [3], new, heads=1, dim=64, page=16).device()
+        c.values[c.table[0][0], :, :3] = math.inf
+        _, out, _ = run_attention(c, 4)
+        ipuc.device_status()
+        assert (out[:-3] == 0).all() and (out[-1] != 0).all()
+
+
+def test_attention_strides_and_a_wide_table():
+    """q a slice of a fused projection, table rows longer than max_pages, lengths and offsets inside larger tensors."""
+    c = Case(24, [70, 5, 33], [2, 5, 20], heads=2, dim=128, page=16).device()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    wide = i32([r + [-1] * 3 for r in c.table])
+    lengths, offsets = i32([9, 70, 5, 33, 9])[1:4], i32([-1] + c.offsets + [99])[1:-1]
+    c.batch = ipuc.PagedBatch(wide[:, :len(c.table[0])], lengths, offsets)
+    fused = randn(c.g, (c.rows, 12, 128))
+    q, out, _ = run_attention(c, 4, q=fused[:, 2:10])
+    ipuc.device_status()
+    want, bound, _ = ref.attention(f64(q), f64(c.keys).nan_to_num(), f64(c.values).nan_to_num(), c.table, c.lengths, c.offsets,
+                                   0, [], 1.0 / math.sqrt(128))
+    within(out, want, bound)
 
 
 def test_results_do_not_change_from_run_to_run():

@@ -106,12 +106,21 @@ def test_paged_refusals(c, b, status, text):
     (dict(prefix=-1), INV, "prefix_rows"), (dict(prefix=16), INV, "prefix_pages"), (dict(stride=255), INV, "stride"),
     (dict(stride=260), ALI, "multiples of 8"), (dict(c=cache(row_stride=68)), ALI, "multiples of 8"), (dict(q=FAKE + 2), ALI, "16-byte"),
     (dict(out=None), INV, "null"), (dict(ws=None), INV, "workspace"), (dict(size=0), INV, "workspace smaller"),
-    (dict(ws=FAKE + 16), ALI, "256-byte"), (dict(prefix=16, pages=FAKE + 1), ALI, "4-byte")])
+    (dict(ws=FAKE + 16), ALI, "256-byte"), (dict(prefix=16, pages=FAKE + 1), ALI, "4-byte"),
+    (dict(scale=math.inf), INV, "scale"), (dict(scale=math.nan), INV, "scale"),
+    # q's rows end 66,048 bytes behind q (2 strides and a row), out's 1536 behind out
+    (dict(q=5 * FAKE), INV, "overlaps"), (dict(q=5 * FAKE - 66032), INV, "overlaps"), (dict(q=5 * FAKE + 1520), INV, "overlaps"),
+    (dict(b=batch(sequences=2 ** 30, rows=2 ** 30)), INV, "extent too large"),
+    (dict(b=batch(sequences=1, rows=2 ** 29, row_offsets=FAKE), stride=256), INV, "extent too large"),
+    # 2^20 sequences of 2^30 positions: 2^44 key tiles a head
+    (dict(b=batch(sequences=1 << 20, rows=1 << 20, max_pages=1 << 26, table_stride=1 << 26), stride=256, q=1 << 40), INV,
+     "extent too large")])
 def test_attention_refusals(change, status, text):
-    a = dict(out=5 * FAKE, q=6 * FAKE, stride=256 * 64, heads=4, c=cache(), prefix=0, pages=None, ws=FAKE, size=1 << 40)
+    a = dict(out=5 * FAKE, q=6 * FAKE, stride=256 * 64, heads=4, c=cache(), prefix=0, pages=None, ws=FAKE, size=1 << 40,
+             scale=0.0, b=batch())
     a.update(change)
-    refused("ipuc_paged_attention_f16", (a["out"], a["q"], a["stride"], a["heads"], a["c"], batch(), a["prefix"], a["pages"], 0.0,
-                                         a["ws"], a["size"], None), status, text)
+    refused("ipuc_paged_attention_f16", (a["out"], a["q"], a["stride"], a["heads"], a["c"], a["b"], a["prefix"], a["pages"],
+                                         a["scale"], a["ws"], a["size"], None), status, text)
 
 
 def test_empty_calls_launch_nothing():
@@ -131,6 +140,18 @@ def test_wrappers_refuse_host_tensors_and_wrong_shapes():
     if torch.cuda.is_available():
         with pytest.raises(ipuc.IpucError, match="current device"):
             ipuc.rotary_f16(x, x, None)
+
+
+def test_wrappers_refuse_tables_caches_and_batches_of_another_device(monkeypatch):
+    """Made for device 1, called with device 0 current: the kernels could not address them."""
+    class Made:
+        _on, _spec, heads, head_dim = 1, None, 2, 64
+    x = torch.zeros((4, 2, 64), dtype=torch.float16)
+    monkeypatch.setattr(ipuc, "_device", lambda: (torch, 0))
+    for fn, args in ((ipuc.rotary_f16, (x, x, Made())), (ipuc.qk_norm_rotary_f16, (x, x, x, x, None, None, 1e-6, Made())),
+                     (ipuc.paged_append_f16, (Made(), Made(), x, x)), (ipuc.paged_attention_f16, (x, x, Made(), Made(), None))):
+        with pytest.raises(ipuc.IpucError, match="Made is not on the current device"):
+            fn(*args)
 
 
 def test_status_of_a_bad_index():
