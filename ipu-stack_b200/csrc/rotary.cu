@@ -149,17 +149,21 @@ __device__ __forceinline__ void store(uint16_t *p, const Vec<uint16_t, V> &v) {
 // sum is a shuffle tree.
 //
 // HBM-bound: x is read and written once, and the rows' loads are issued before
-// the chain position -> table row, which they do not depend on.  One head per
-// group: two or four heads that share the lookups and the table row measured
-// the same on 8192 x 32 x 128 (27.8 us, torch's copy of the same bytes 22.4) and
-// slower on 32 tokens (2.6 and 3.4 against 2.2 us), and so did resident blocks
-// that loop with the next group's loads in flight (35.8 us).
+// the chain position -> table row, which they do not depend on.  8192 x 32 x 128
+// takes 24.9 us (5.6 TB/s; torch's copy of the same bytes 22.4), the norm of
+// 8191 x 40 x 128 in f32 with the rotation 42.5 (6.0 TB/s).  One head per group:
+// two or four heads that share the lookups and the table row measured the same
+// and slower on 32 tokens (2.6 and 3.4 against 2.2 us); resident blocks that
+// loop with the next group's loads in flight 35.8 us; fewer registers for more
+// resident warps (42 of 47) 31 us; 8-byte loads 30.8 us.  Small blocks, which
+// end and begin one by one: 25.6 and 45.9 us with 256 threads, 43.2 with 64.
+constexpr int kHeadsThreads = 128;
 template <int V, typename TIN, bool kNorm, bool kPaged>
-__global__ void __launch_bounds__(256) heads_kernel(const __grid_constant__ HeadsParams p) {
+__global__ void __launch_bounds__(kHeadsThreads) heads_kernel(const __grid_constant__ HeadsParams p) {
   constexpr int IPL = V >= 4 ? 1 : V == 2 ? 2 : 4;  // head_dim <= 256
   const uint32_t lanes = 1u << p.lane_shift;
   const uint32_t lane = threadIdx.x & (lanes - 1);
-  const uint32_t group = blockIdx.x * (256u >> p.lane_shift) + (threadIdx.x >> p.lane_shift);
+  const uint32_t group = blockIdx.x * ((uint32_t)kHeadsThreads >> p.lane_shift) + (threadIdx.x >> p.lane_shift);
   const uint32_t token = group / (uint32_t)p.heads, head = group - token * (uint32_t)p.heads;
   const bool inside = token < p.tokens;
   const int items = p.head_dim / (2 * V), turned = p.rotary_dim / (2 * V);
@@ -315,14 +319,14 @@ ipuc_status launch_heads(HeadsParams &p, cudaStream_t stream) {
   while ((1 << p.lane_shift) < items && p.lane_shift < 5) ++p.lane_shift;
   p.heads = p.seg[0].heads + p.seg[1].heads;
   p.inv_dim = 1.0f / (float)p.head_dim;
-  const int64_t groups = p.tokens * p.heads, per_block = 256 >> p.lane_shift;
+  const int64_t groups = p.tokens * p.heads, per_block = kHeadsThreads >> p.lane_shift;
   IPUC_CHECK_ARG(groups < (1ll << 31), "heads: extent too large");
   const unsigned grid = (unsigned)((groups + per_block - 1) / per_block);
   switch (v) {
-    case 8: heads_kernel<8, TIN, kNorm, kPaged><<<grid, 256, 0, stream>>>(p); break;
-    case 4: heads_kernel<4, TIN, kNorm, kPaged><<<grid, 256, 0, stream>>>(p); break;
-    case 2: heads_kernel<2, TIN, kNorm, kPaged><<<grid, 256, 0, stream>>>(p); break;
-    default: heads_kernel<1, TIN, kNorm, kPaged><<<grid, 256, 0, stream>>>(p); break;
+    case 8: heads_kernel<8, TIN, kNorm, kPaged><<<grid, kHeadsThreads, 0, stream>>>(p); break;
+    case 4: heads_kernel<4, TIN, kNorm, kPaged><<<grid, kHeadsThreads, 0, stream>>>(p); break;
+    case 2: heads_kernel<2, TIN, kNorm, kPaged><<<grid, kHeadsThreads, 0, stream>>>(p); break;
+    default: heads_kernel<1, TIN, kNorm, kPaged><<<grid, kHeadsThreads, 0, stream>>>(p); break;
   }
   return check_launch("heads_kernel");
 }
