@@ -59,11 +59,12 @@ using namespace sm100;
 // Both factors cancel in O / l as long as every partial result has them.
 constexpr float kLazy = 8.0f, kShift = 4.0f;
 
-// What loading a unit's queries and storing its result costs, in key tiles:
-// measured 5-6 us against 2.5 for a tile of the tile kernel, 2 us against 1.2
-// of the stream kernel.  With 0, pieces of many short units ended last (long
-// batch: mean 141 us, last 180).
-constexpr int kUnitCost = 2;
+// What loading a unit's queries and storing its result costs, in key tiles: it
+// takes 5 to 6 us of a CTA of the tile kernel against 2.15 for a key tile, and
+// 2 to 3 us of a worker of the stream kernel against 1.2.  With 0, 1, 2, 3 and 4:
+// a batch of 128 behind 32768 shared positions 189, 172, 159, 152 and 153 us,
+// pieces of 8 prompts behind 4096 181, 146, 134, 122 and 122 us.
+constexpr int kUnitCost = 3;
 __device__ __forceinline__ int32_t unit_cost(int32_t tiles) { return tiles > 0 ? tiles + kUnitCost : 0; }
 
 // A place on a line: offset `x` in a unit of `n` key tiles, `left` to the
