@@ -97,9 +97,10 @@ struct PagedAttnParams {
   float scale_log2;       // softmax scale * log2(e)
   // Each kernel lays its units (rows that read the same keys of one head) on a
   // line, a unit's length being its key tiles and kUnitCost more for its start
-  // and end, and cuts the line into equal pieces, one per CTA or worker.  A
-  // unit that a piece ends in has several partial results: unnormalised O (f32, head_dim wide) and (running
-  // maximum in log2 units, sum of weights) per row, in slot (unit + CTA).
+  // and end, and cuts the line into equal pieces, one per CTA or worker.  A unit
+  // that a piece ends in has several partial results: unnormalised O (f32,
+  // head_dim wide) and (running maximum in log2 units, sum of weights) per row,
+  // in slot (unit + piece).
   float *stream_o, *tile_o;
   float2 *stream_ml, *tile_ml;
   int32_t stream_rows, tile_slot_rows;  // rows of a slot
@@ -240,20 +241,26 @@ __device__ __forceinline__ int32_t checked_page(const PagedAttnParams &p, int32_
   return p.paged.pages;
 }
 
-// ---- single rows: the sequences' own parts ------------------------------------
-
-// One row per sequence and at most 16 query heads per key head: the group is
-// one m16n8k16 tile, so a key costs 16 x 128 multiply-adds whatever the group,
-// and K and V are streamed once: HBM-bound.  The key tiles (64 keys, at
-// absolute multiples of 64) of all (sequence, head) units form one line that
-// is cut into equal pieces, one per CTA, so ragged lengths leave no CTA idle.
-// When the call has so few rows that the tile kernel's start would cost more,
-// the shared prefix is on the line too, in front, as a unit per head and group
-// of 16 rows (the later groups' reads of it come from L2).
+// ---- few rows: the sequences' own parts ----------------------------------------
+//
+// O = sum_j 2^(s_j - m) v_j / sum_j 2^(s_j - m) with s = q k scale log2(e), in one
+// pass with a running maximum m: when m grows, O and the sum so far are scaled.
+//
+// At most 16 query heads per key head: the group of a row (or rows) is one
+// m16n8k16 tile, so a key costs 16 x 128 multiply-adds whatever the group, and K
+// and V are streamed once: HBM-bound.  64 rows over 2000 to 4000 keys of 8 heads
+// of 128 (790 MB) take 145 us, 5.5 TB/s.  (tcgen05's tile has 128 rows, an eighth
+// of it filled: see few_rows for the two side by side.)  The key tiles
+// (64 keys, at absolute multiples of 64) of all units (16 rows of a sequence,
+// head) form one line that is cut into equal pieces, one per worker, so ragged
+// lengths leave no CTA idle.  When the call has so few rows that the tile
+// kernel's start would cost more, the shared prefix is on the line too, in front,
+// as a unit per head and group of 16 rows (the later groups' reads of it come
+// from L2).
 // A CTA is two workers with a piece each: a producer warp fills a ring of
-// tiles by TMA, box by box of gcd(page_size, 64) keys; four warps take 16 keys
-// of every tile each, with a running maximum, sum and O of their own, and meet
-// once per unit.
+// tiles by TMA, box by box of gcd(page_size, 64) keys, and hands out units with
+// their queries; four warps take 16 keys of every tile each, with a running
+// maximum, sum and O of their own, and meet once per unit.
 // Two layouts of K and V in shared memory.  Heads of 64 and 128 lie in halves
 // of 64 elements with the 128-byte swizzle.  Others would waste up to half of
 // that (72 elements: 9 KB of keys in 16, 0.52 of HBM): their rows are single
@@ -1025,6 +1032,11 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 
 // ---- many rows: tiles of 128 on the tensor cores --------------------------------
 
+// The same sums as above, bound by the softmax and the tensor core together: a
+// key tile takes 2.15 us of an SM, 4 x 256 x 128 x 128 operations, which is 1.15
+// PFLOP/s on all SMs; 128 rows of 32 heads behind 32768 shared positions take 84
+// us, 820 TFLOP/s with start and end (K and V, read once by each row unit, come
+// to 3.2 TB/s).
 // Rows that read the same keys (all rows of the call for the shared prefix;
 // one sequence's rows for its own part) are packed group by group into
 // 128-row MMA tiles, tile_rows = 128 / group batch rows to a tile, two tiles
@@ -1663,6 +1675,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 // group), a thread four dims of one of them: so 16-byte reads are neighbours
 // row by row (tile slots) or dim by dim (stream slots).  A row's partials are
 // the pieces of its prefix unit and those of its own unit, both runs of slots.
+// Bound by latency, two lookups and two rounds of loads: 64 rows of 32 heads take
+// 7 us.  Weights are 2^(m_i - m), sums and O stay in f32 up to the one rounding.
 struct Pieces {
   const float2 *ml;  // of the first one's row; a piece is `rows` rows further
   const float *o;    // its dim 0; four dims further on `dims`, a piece rows * head_dim
