@@ -157,6 +157,9 @@ __device__ __forceinline__ void store(uint16_t *p, const Vec<uint16_t, V> &v) {
 // loop with the next group's loads in flight 35.8 us; fewer registers for more
 // resident warps (42 of 47) 31 us; 8-byte loads 30.8 us.  Small blocks, which
 // end and begin one by one: 25.6 and 45.9 us with 256 threads, 43.2 with 64.
+// In a cache a group takes a key head and its value head: the chain there is
+// longer (row -> sequence -> length -> page), and 8000 x 8 x 128 of each, 16
+// sequences, take 14.8 us (4.7 TB/s) for 18.1 with a group for each.
 constexpr int kHeadsThreads = 128;
 template <int V, typename TIN, bool kNorm, bool kPaged>
 __global__ void __launch_bounds__(kHeadsThreads) heads_kernel(const __grid_constant__ HeadsParams p) {
@@ -167,8 +170,10 @@ __global__ void __launch_bounds__(kHeadsThreads) heads_kernel(const __grid_const
   const uint32_t token = group / (uint32_t)p.heads, head = group - token * (uint32_t)p.heads;
   const bool inside = token < p.tokens;
   const int items = p.head_dim / (2 * V), turned = p.rotary_dim / (2 * V);
-  const bool second = head >= (uint32_t)p.seg[0].heads;
-  const Segment &g = p.seg[second ? 1 : 0];
+  // Dense: heads of the first tensor, then of the second.  Cache: a key head and
+  // its value head, which share the lookups.
+  constexpr int S = kPaged ? 2 : 1;
+  const bool second = !kPaged && head >= (uint32_t)p.seg[0].heads;
   const int at = second ? (int)head - p.seg[0].heads : (int)head;
   int e0[IPL], e1[IPL];
 #pragma unroll
@@ -178,16 +183,20 @@ __global__ void __launch_bounds__(kHeadsThreads) heads_kernel(const __grid_const
     e0[k] = split ? item * V : 2 * V * item;
     e1[k] = split ? p.rotary_dim / 2 + item * V : e0[k] + V;
   }
-  Vec<TIN, V> x[IPL][2];
-  const TIN *in = static_cast<const TIN *>(g.in) + token * g.in_stride + at * p.head_dim;
+  Vec<TIN, V> x[S][IPL][2];
 #pragma unroll
-  for (int k = 0; k < IPL; ++k) {
-    if (inside && (int)(lane + k * lanes) < items) {
-      x[k][0] = load<TIN, V>(in + e0[k]);
-      x[k][1] = load<TIN, V>(in + e1[k]);
-    } else {
+  for (int t = 0; t < S; ++t) {
+    const Segment &g = p.seg[kPaged ? t : second ? 1 : 0];
+    const TIN *in = static_cast<const TIN *>(g.in) + token * g.in_stride + at * p.head_dim;
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[k][0].v[j] = x[k][1].v[j] = TIN(0);
+    for (int k = 0; k < IPL; ++k) {
+      if (inside && (int)(lane + k * lanes) < items) {
+        x[t][k][0] = load<TIN, V>(in + e0[k]);
+        x[t][k][1] = load<TIN, V>(in + e1[k]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[t][k][0].v[j] = x[t][k][1].v[j] = TIN(0);
+      }
     }
   }
   // The token's position (-1: nothing is written) and, in a cache, its slot.
@@ -236,58 +245,62 @@ __global__ void __launch_bounds__(kHeadsThreads) heads_kernel(const __grid_const
     for (int k = 0; k < IPL; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float a = to_f32(x[k][0].v[j]), b = to_f32(x[k][1].v[j]);
+        const float a = to_f32(x[0][k][0].v[j]), b = to_f32(x[0][k][1].v[j]);
         sum = fmaf(a, a, fmaf(b, b, sum));
       }
     for (uint32_t m = lanes >> 1; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
     rstd = rsqrtf(sum * p.inv_dim + p.eps);
   }
   if (position < 0) return;
-  uint16_t *out = g.out + (kPaged ? page_at + at * p.paged.head_stride : token * g.out_stride + at * p.head_dim);
 #pragma unroll
-  for (int k = 0; k < IPL; ++k) {
-    const int item = (int)(lane + k * lanes);
-    if (item >= items) continue;
-    float y[2 * V];
+  for (int t = 0; t < S; ++t) {
+    const Segment &g = p.seg[kPaged ? t : second ? 1 : 0];
+    uint16_t *out = g.out + (kPaged ? page_at + at * p.paged.head_stride : token * g.out_stride + at * p.head_dim);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      y[j] = to_f32(x[k][0].v[j]);
-      y[V + j] = to_f32(x[k][1].v[j]);
-    }
-    if constexpr (kNorm) {
-      if (g.weight) {
-        const Vec<uint16_t, V> w0 = *reinterpret_cast<const Vec<uint16_t, V> *>(g.weight + e0[k]);
-        const Vec<uint16_t, V> w1 = *reinterpret_cast<const Vec<uint16_t, V> *>(g.weight + e1[k]);
+    for (int k = 0; k < IPL; ++k) {
+      const int item = (int)(lane + k * lanes);
+      if (item >= items) continue;
+      float y[2 * V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          y[j] *= rstd * h2f(w0.v[j]);
-          y[V + j] *= rstd * h2f(w1.v[j]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 2 * V; ++j) y[j] *= rstd;
+      for (int j = 0; j < V; ++j) {
+        y[j] = to_f32(x[t][k][0].v[j]);
+        y[V + j] = to_f32(x[t][k][1].v[j]);
       }
-    }
-    if (p.table && g.rotate && item < turned) {
-      // (two loops: indices known at compile time keep y in registers)
-      if (p.interleaved) {
+      if constexpr (kNorm) {
+        if (g.weight) {
+          const Vec<uint16_t, V> w0 = *reinterpret_cast<const Vec<uint16_t, V> *>(g.weight + e0[k]);
+          const Vec<uint16_t, V> w1 = *reinterpret_cast<const Vec<uint16_t, V> *>(g.weight + e1[k]);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float a = y[2 * j], b = y[2 * j + 1];
-          y[2 * j] = a * cs[k].v[j] - b * sn[k].v[j];
-          y[2 * j + 1] = b * cs[k].v[j] + a * sn[k].v[j];
-        }
-      } else {
+          for (int j = 0; j < V; ++j) {
+            y[j] *= rstd * h2f(w0.v[j]);
+            y[V + j] *= rstd * h2f(w1.v[j]);
+          }
+        } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float a = y[j], b = y[V + j];
-          y[j] = a * cs[k].v[j] - b * sn[k].v[j];
-          y[V + j] = b * cs[k].v[j] + a * sn[k].v[j];
+          for (int j = 0; j < 2 * V; ++j) y[j] *= rstd;
         }
       }
+      if (p.table && g.rotate && item < turned) {
+        // (two loops: indices known at compile time keep y in registers)
+        if (p.interleaved) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float a = y[2 * j], b = y[2 * j + 1];
+            y[2 * j] = a * cs[k].v[j] - b * sn[k].v[j];
+            y[2 * j + 1] = b * cs[k].v[j] + a * sn[k].v[j];
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float a = y[j], b = y[V + j];
+            y[j] = a * cs[k].v[j] - b * sn[k].v[j];
+            y[V + j] = b * cs[k].v[j] + a * sn[k].v[j];
+          }
+        }
+      }
+      store(out + e0[k], to_f16<V>(y));
+      store(out + e1[k], to_f16<V>(y + V));
     }
-    store(out + e0[k], to_f16<V>(y));
-    store(out + e1[k], to_f16<V>(y + V));
   }
 }
 
@@ -317,7 +330,7 @@ ipuc_status launch_heads(HeadsParams &p, cudaStream_t stream) {
   const int items = p.head_dim / (2 * v);
   p.lane_shift = 0;
   while ((1 << p.lane_shift) < items && p.lane_shift < 5) ++p.lane_shift;
-  p.heads = p.seg[0].heads + p.seg[1].heads;
+  p.heads = p.seg[0].heads + (kPaged ? 0 : p.seg[1].heads);
   p.inv_dim = 1.0f / (float)p.head_dim;
   const int64_t groups = p.tokens * p.heads, per_block = kHeadsThreads >> p.lane_shift;
   IPUC_CHECK_ARG(groups < (1ll << 31), "heads: extent too large");
