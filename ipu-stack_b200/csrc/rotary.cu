@@ -24,41 +24,58 @@ struct TableParams {
   float *table;
   int64_t positions;
   int32_t pairs;
-  float magnitude;
-  double quarter_turns[kMaxPairs];  // f_i * 2 / pi: quarter turns per position
+  float magnitude, magnitude_rest;  // in two parts: 1.1 alone is off by 2^-25 of it in f32
+  uint64_t turns[kMaxPairs];  // f_i / 2pi, turns per position, in units of 2^-64
 };
 
 // Angles of far positions need more than 32 bits (131072 * f leaves 7 bits of
-// a fraction in f32), so position times frequency is formed in f64 in units of
-// a quarter turn; what is left after the nearest whole quarter is at most half
-// a quarter, which f32 holds to 2^-26 of a turn, and the whole quarters swap
-// and negate the f32 sine and cosine.  The whole quarters come from adding
-// 1.5 * 2^52, whose sum has them in its low bits (positions are below 2^31 and
-// frequencies below 1, so they fit); conversions between f64 and integers run
-// at a quarter of the adds' rate.  A thread writes V neighbouring pairs.
-// Bound by the stores: 131072 x 128 takes 17.7 us (3.8 TB/s), torch's fill of it
-// 17.9, a bare loop of 16-byte stores 12.6.
+// a fraction in f32).  An angle is a fraction of a turn in 64-bit fixed point, so
+// position times frequency drops the whole turns by itself; the nearest whole
+// quarter is its rounded top two bits, and what is left, t in [-1/2, 1/2) of a
+// quarter, goes to f32 with 2^-32 of a quarter kept.  Sine and cosine of pi/2 t
+// are their Taylor polynomials to t^9 and t^10 (the next terms are below 2e-9);
+// pi/2 in two parts keeps the sine to half a step and the rounding of t.  The
+// whole quarters swap and negate the two.  A thread writes V neighbouring pairs.
+// Bound by the stores: 131072 x 128 takes 13.4 us (5.0 TB/s), torch's fill of it
+// 17.9, a bare loop of 16-byte stores 12.6.  Products and the remainder in f64
+// with CUDA's sincospif took 17.7: bound by the instructions.
+__device__ __forceinline__ void sincos_quarter(float t, float &s, float &c) {
+  constexpr double h = 1.57079632679489661923;  // pi / 2
+  constexpr float h0 = (float)h, h1 = (float)(h - (double)h0);
+  constexpr float s3 = (float)(-h * h * h / 6), s5 = (float)(h * h * h * h * h / 120);
+  constexpr float s7 = (float)(-h * h * h * h * h * h * h / 5040);
+  constexpr float s9 = (float)(h * h * h * h * h * h * h * h * h / 362880);
+  constexpr float c2 = (float)(-h * h / 2), c4 = (float)(h * h * h * h / 24);
+  constexpr float c6 = (float)(-h * h * h * h * h * h / 720), c8 = (float)(h * h * h * h * h * h * h * h / 40320);
+  constexpr float c10 = (float)(-h * h * h * h * h * h * h * h * h * h / 3628800);
+  const float t2 = t * t;
+  const float p = fmaf(t2, fmaf(t2, fmaf(t2, fmaf(t2, s9, s7), s5), s3), h1);
+  s = fmaf(t, h0, t * p);
+  c = fmaf(t2, fmaf(t2, fmaf(t2, fmaf(t2, fmaf(t2, c10, c8), c6), c4), c2), 1.0f);
+}
+
 template <int V>
 __global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant__ TableParams p) {
   const int groups = p.pairs / V, rows = 256 / groups;  // positions per block and step
   const int i = (threadIdx.x % groups) * V;
   if ((int)threadIdx.x >= rows * groups) return;
-  double f[V];
+  uint64_t f[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) f[j] = p.quarter_turns[i + j];
-  constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52
+  for (int j = 0; j < V; ++j) f[j] = p.turns[i + j];
   for (int64_t pos = (int64_t)blockIdx.x * rows + threadIdx.x / groups; pos < p.positions;
        pos += (int64_t)gridDim.x * rows) {
     float cs[V], sn[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const double t = (double)pos * f[j], shifted = t + kRound;
+      const uint64_t angle = (uint64_t)pos * f[j];
       float s, c;
-      sincospif(0.5f * (float)(t - (shifted - kRound)), &s, &c);
-      const int q = __double2loint(shifted) & 3;
-      const float a = q & 1 ? s : c, b = q & 1 ? c : s;
-      cs[j] = (q == 1 || q == 2 ? -a : a) * p.magnitude;
-      sn[j] = (q >= 2 ? -b : b) * p.magnitude;
+      sincos_quarter((float)(int32_t)(uint32_t)(angle >> 30) * 0x1p-32f, s, c);
+      const uint32_t q = ((uint32_t)(angle >> 61) + 1) >> 1;  // (the carry out of two bits is a whole turn)
+      // cosine, sine of the quarters: (c, s), (-s, c), (-c, -s), (s, -c)
+      const float a = __uint_as_float(__float_as_uint(q & 1 ? s : c) ^ ((q + 1) & 2) << 30);
+      const float b = __uint_as_float(__float_as_uint(q & 1 ? c : s) ^ (q & 2) << 30);
+      cs[j] = fmaf(a, p.magnitude, a * p.magnitude_rest);
+      sn[j] = fmaf(b, p.magnitude, b * p.magnitude_rest);
     }
     float *row = p.table + pos * 2 * p.pairs + i;
     if constexpr (V == 4) {
@@ -425,6 +442,7 @@ extern "C" ipuc_status ipuc_rotary_table(float *table, int64_t positions, int64_
   p.positions = positions;
   p.pairs = (int32_t)(rotary_dim / 2);
   p.magnitude = (float)c.magnitude;
+  p.magnitude_rest = (float)(c.magnitude - (double)p.magnitude);
   const double pi = 3.14159265358979323846, r = (double)rotary_dim;
   const double base = c.kind == IPUC_ROTARY_SCALE_BASE ? c.base * pow(c.factor, r / (r - 2.0)) : c.base;
   for (int i = 0; i < p.pairs; ++i) {
@@ -435,7 +453,7 @@ extern "C" ipuc_status ipuc_rotary_table(float *table, int64_t positions, int64_
       const double keep = fmin(1.0, fmax(0.0, (turns - c.low) / (c.high - c.low)));
       f *= keep + (1.0 - keep) / c.factor;
     }
-    p.quarter_turns[i] = f * (2.0 / pi);
+    p.turns[i] = (uint64_t)(f / (2.0 * pi) * 0x1p64);  // (f is at most 1)
   }
   const bool wide = p.pairs % 4 == 0 && aligned(table, 16);
   const int64_t rows = 256 / (wide ? p.pairs / 4 : p.pairs), want = (positions + rows - 1) / rows, cap = (int64_t)sm_count() * 8;
