@@ -568,8 +568,9 @@ ipuc_status ipuc_paged_append_f16(const ipuc_paged_cache *cache, const ipuc_page
  * turn the call's earlier rows of that sequence NaN too (0 * inf).
  * head_dim a multiple of 8, at most 128; q_heads / heads at most 128; 16-byte
  * aligned pointers, strides multiples of 8 elements.
- * workspace: ipuc_paged_attention_workspace_bytes() bytes, 256-byte aligned,
- * contents need no clearing; two calls that may overlap need one each. */
+ * workspace: ipuc_paged_attention_workspace_bytes() bytes (ragged: whether the
+ * batch has row_offsets), 256-byte aligned, contents need no clearing; two
+ * calls that may overlap need one each. */
 uint64_t ipuc_paged_attention_workspace_bytes(int64_t rows, int64_t sequences, int64_t q_heads, int64_t heads,
                                               int64_t head_dim, int64_t prefix_rows, int32_t ragged);
 ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_t q_stride, int64_t q_heads,

@@ -563,6 +563,90 @@ def test_two_calls_at_once_with_a_workspace_each():
             assert torch.equal(o, a)
 
 
+@pytest.mark.parametrize("lengths,new,prefix", [([700] * 40, None, 640), ([500] * 20 + [900], [1] * 20 + [200], 0),
+                                                ([600] * 20 + [900], [2] * 20 + [200], 512)])
+def test_graphs_at_once_with_both_kernels_each(lengths, new, prefix):
+    """Each call has a tile kernel and a stream kernel beside it; two captured calls are replayed on two streams."""
+    cases = [Case(40 + i, [n + 13 * i for n in lengths], new, heads=2, dim=128, page=16, prefix=prefix).device() for i in range(2)]
+    made = [run_attention(c, 4) for c in cases]
+    alone = [out.clone() for _, out, _ in made]
+    graphs, streams = [], [torch.cuda.Stream() for _ in cases]
+    for c, (q, out, ws) in zip(cases, made):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            ipuc.paged_attention_f16(out, q, c.cache, c.batch, ws, c.prefix, c.pages)
+    for _ in range(20):
+        for _, out, ws in made:
+            out.fill_(7.0)
+            ws.fill_(255)
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+                g.replay()
+        torch.cuda.synchronize()
+        for (_, out, _), a in zip(made, alone):
+            assert torch.equal(out, a)
+    ipuc.device_status()
+
+
+def test_offsets_beyond_32_bits():
+    """Pages and rows that lie more than 2^31 elements behind their base; the rest of the memory is as it was allocated."""
+    pages, page, dim = 300000, 64, 128     # 2.46e9 elements
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    keys, values = (torch.empty((pages, 1, page, dim), dtype=F16, device="cuda") for _ in range(2))
+    g = gen(50)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    far = [pages - 1, pages - 7, 3, pages // 2 + 20000]
+    cache, lengths, new = ipuc.PagedCache(keys, values), [100, 120], [100, 120]
+    batch = ipuc.PagedBatch(i32([far[:2], far[2:]]), i32(lengths), i32([0, 100, 220]))
+    table = make_table(128, dim)
+    # rows 2^24 elements apart: the last one 3.7e9 behind the first
+    rows = torch.empty((220, 1 << 24), dtype=F16, device="cuda")
+    k, v = rows[:, :dim].unflatten(1, (1, dim)), rows[:, dim:2 * dim].unflatten(1, (1, dim))
+    k.copy_(randn(g, k.shape))
+    v.copy_(randn(g, v.shape))
+    ipuc.paged_append_f16(cache, batch, k, v, ipuc.Rotary(table))
+    q = rows[:, 2 * dim:6 * dim].unflatten(1, (4, dim))
+    q.copy_(randn(g, q.shape))
+    positions = i32(list(range(100)) + list(range(120)))
+    ipuc.rotary_f16(q, q, ipuc.Rotary(table), positions)
+    used = torch.tensor(far)
+    small_k, small_v = f64(keys[used.cuda()]), f64(values[used.cuda()])
+    assert torch.equal(small_v[0, 0, :page], f64(v)[:page, 0]) and torch.equal(small_v[3, 0, :56], f64(v)[164:, 0])
+    for prefix, prefix_pages in ((0, []), (64, [far[2]])):     # (any page may be shared: the first 64 keys are then others)
+        out = torch.empty((220, 4, dim), dtype=F16, device="cuda")
+        ws = torch.empty(ipuc.paged_attention_workspace_bytes(220, 2, 4, 1, dim, prefix, True), dtype=torch.uint8, device="cuda")
+        ipuc.paged_attention_f16(out, q, cache, batch, ws, prefix, i32(prefix_pages) if prefix else None)
+        torch.cuda.synchronize()
+        ipuc.device_status()
+        want, bound, _ = ref.attention(f64(q), small_k.nan_to_num(), small_v.nan_to_num(), [[0, 1], [2, 3]], lengths, [0, 100, 220],
+                                       prefix, [2] if prefix else [], 1.0 / math.sqrt(dim))
+        within(out, want, bound)
+
+
+def test_a_long_sequence():
+    """One row over 200000 positions, all SMs on it, and 70 rows over the same as a shared prefix."""
+    g = gen(51)
+    pages = 200000 // 64 + 1
+    keys, values = randn(g, (pages, 1, 64, 64)), randn(g, (pages, 1, 64, 64))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    order = list(range(pages))
+    random.Random(51).shuffle(order)
+    cache = ipuc.PagedCache(keys, values)
+    for rows, prefix in ((1, 0), (70, 199999)):
+        q = randn(g, (rows, 4, 64))
+        batch = ipuc.PagedBatch(i32([order] * rows), i32([200000] * rows))
+        out = torch.empty_like(q)
+        ws = torch.empty(ipuc.paged_attention_workspace_bytes(rows, rows, 4, 1, 64, prefix), dtype=torch.uint8, device="cuda")
+        ipuc.paged_attention_f16(out, q, cache, batch, ws, prefix, i32(order) if prefix else None)
+        torch.cuda.synchronize()
+        ipuc.device_status()
+        want, bound, _ = ref.attention(f64(q[:2]), f64(keys), f64(values), [order] * 2, [200000] * min(rows, 2), None, 0, [], 0.125)
+        within(out[:2], want, bound)
+
+
 def test_against_flash_attention():
     """A cache that holds one sequence's keys in order, all rows at its last position: ipuc_flash_attention_f16's result."""
     heads, n, d = 2, 384, 128
