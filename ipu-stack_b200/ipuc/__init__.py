@@ -486,17 +486,17 @@ def _refuse(fn, text):
     raise IpucError(fn, ERR_INVALID_ARGUMENT, f"{fn[5:]}: {text}")
 
 
-_torch = _get_device = _raw_stream = None
+_torch = _Tensor = _get_device = _raw_stream = None
 
 
 def _load_torch():
     """torch and its two per-call queries, looked up once: a decode step makes these calls for every layer, and
     torch.cuda.current_stream() alone costs as much host time as a launch."""
-    global _torch, _get_device, _raw_stream
+    global _torch, _Tensor, _get_device, _raw_stream
     import torch
     _get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
     _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    _torch = torch
+    _torch, _Tensor = torch, torch.Tensor
     return torch
 
 
@@ -514,7 +514,7 @@ def _stream_on(device, stream):
 
 def _want(fn, name, t, device, dtype, ndim):
     """Shape and strides of `t`, a CUDA tensor of the current device with this type and rank."""
-    if not isinstance(t, _torch.Tensor) or t.dtype is not dtype:
+    if not isinstance(t, _Tensor) or t.dtype is not dtype:
         _refuse(fn, f"{name} has the wrong type")
     stride = t.stride()
     if len(stride) != ndim:
@@ -533,21 +533,25 @@ def _on(fn, device, *specs):
 
 def _vector(fn, name, t, device, dtype, size):
     """Address of a dense vector."""
-    shape, stride = _want(fn, name, t, device, dtype, 1)
-    if shape[0] != size or (size > 1 and stride[0] != 1):
+    if not (isinstance(t, _Tensor) and t.dtype is dtype and t.get_device() == device and t.shape == (size,)
+            and t.is_contiguous()):
+        _want(fn, name, t, device, dtype, 1)
         _refuse(fn, f"{name} must be a dense vector of {size} entries")
     return t.data_ptr()
 
 
 def _token_rows(fn, name, t, device, dtype, shape=None):
     """[tokens, heads, head_dim] with dense heads: (shape, token stride)."""
-    size, stride = _want(fn, name, t, device, dtype, 3)
-    tokens, heads, d = size
-    if shape is not None and (tokens, heads, d) != tuple(shape):
+    if not isinstance(t, _Tensor) or t.dtype is not dtype or t.get_device() != device or t.dim() != 3:
+        _want(fn, name, t, device, dtype, 3)
+    size = t.shape
+    if shape is not None and size != shape:
         _refuse(fn, f"{name} has the wrong shape")
-    if (d > 1 and stride[2] != 1) or (heads > 1 and stride[1] != d):
+    tokens, heads, d = size
+    s0, s1, s2 = t.stride()
+    if (s2 != 1 and d > 1) or (s1 != d and heads > 1):
         _refuse(fn, f"{name} must be dense in its last 2 dimensions")
-    return size, stride[0] if tokens > 1 else heads * d
+    return size, s0 if tokens > 1 else heads * d
 
 
 def _precision(fn, name, t):
@@ -574,8 +578,8 @@ class Rotary:
 
     def __init__(self, table, layout=ROTARY_HALF):
         fn, (torch, device) = "ipuc_rotary_table", _device()
-        (positions, columns), stride = _want(fn, "table", table, device, torch.float32, 2)
-        if stride[1] != 1 or (positions > 1 and stride[0] != columns):
+        (positions, columns), _ = _want(fn, "table", table, device, torch.float32, 2)
+        if not table.is_contiguous():
             _refuse(fn, "table must be dense")
         self.table, self._on = table, device
         self._spec = _pack_rotary(table.data_ptr(), positions, columns, layout)
