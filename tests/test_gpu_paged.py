@@ -590,6 +590,50 @@ def test_graphs_at_once_with_both_kernels_each(lengths, new, prefix):
     ipuc.device_status()
 
 
+@pytest.mark.parametrize("new", [None, [3, 40]])
+def test_a_page_at_several_places(new):
+    """One page in two places of a table, in two sequences and in the prefix."""
+    g = gen(52)
+    keys, values = randn(g, (4, 2, 16, 64)), randn(g, (4, 2, 16, 64))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    table, lengths = [[2, 1, 2, 3], [2, 2, 1, 0]], [60, 50]
+    offsets = None if new is None else [0, new[0], sum(new)]
+    rows = 2 if new is None else sum(new)
+    q = randn(g, (rows, 6, 64))
+    for prefix, prefix_pages in ((0, []), (20, [1, 2])):
+        out = torch.empty_like(q)
+        ws = torch.empty(ipuc.paged_attention_workspace_bytes(rows, 2, 6, 2, 64, prefix, new is not None), dtype=torch.uint8,
+                         device="cuda")
+        batch = ipuc.PagedBatch(i32(table), i32(lengths), None if new is None else i32(offsets))
+        ipuc.paged_attention_f16(out, q, ipuc.PagedCache(keys, values), batch, ws, prefix, i32(prefix_pages) if prefix else None)
+        want, bound, _ = ref.attention(f64(q), f64(keys), f64(values), table, lengths, offsets, prefix, prefix_pages, 0.125)
+        within(out, want, bound)
+        ipuc.device_status()
+
+
+def test_a_stream_that_is_given():
+    """stream= as a torch stream and as a handle, with the current stream busy elsewhere."""
+    c = Case(53, [300, 20, 90], heads=2, dim=64, page=16).device()
+    x = randn(c.g, (3, 8, 64))
+    table = make_table(512, 64)
+    positions = torch.tensor([299, 19, 89], dtype=torch.int32, device="cuda")
+    turned, out = torch.empty_like(x), torch.empty_like(x)
+    ws = torch.empty(ipuc.paged_attention_workspace_bytes(3, 3, 8, 2, 64), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    results = []
+    for stream in (None, torch.cuda.Stream(), torch.cuda.Stream().cuda_stream):
+        turned.zero_()
+        out.zero_()
+        torch.cuda.synchronize()
+        ipuc.rotary_f16(turned, x, ipuc.Rotary(table), positions, stream=stream)
+        ipuc.paged_append_f16(c.cache, c.batch, turned[:, :2], x[:, :2], stream=stream)
+        ipuc.paged_attention_f16(out, turned, c.cache, c.batch, ws, stream=stream)
+        torch.cuda.synchronize()
+        results.append(out.clone())
+    ipuc.device_status()
+    assert torch.equal(results[0], results[1]) and torch.equal(results[0], results[2]) and (results[0] != 0).any()
+
+
 def test_offsets_beyond_32_bits():
     """Pages and rows that lie more than 2^31 elements behind their base; the rest of the memory is as it was allocated."""
     pages, page, dim = 300000, 64, 128     # 2.46e9 elements
