@@ -356,6 +356,18 @@ def test_attention_ragged_rows(lengths, new, prefix, page, heads, group, dim, pa
     check_attention(Case(8, lengths, new, heads=heads, dim=dim, page=page, prefix=prefix, pad=pad).device(), group)
 
 
+@pytest.mark.parametrize("new,prefix", [(None, 0), ([2, 70, 1], 0), ([2, 70, 1], 40)])
+@pytest.mark.parametrize("dim", range(8, 129, 8))
+def test_attention_every_head_dim(dim, new, prefix):
+    check_attention(Case(13, [90, 130, 41], new, heads=2, dim=dim, page=16, prefix=prefix).device(), 3)
+
+
+@pytest.mark.parametrize("new", [None, [1, 6, 2, 40]])
+@pytest.mark.parametrize("group", [1, 2, 7, 8, 9, 12, 15, 16, 17, 33, 64, 100, 128])
+def test_attention_groups(group, new):
+    check_attention(Case(14, [100, 70, 2, 129], new, heads=2, dim=64, page=32, prefix=20).device(), group)
+
+
 @pytest.mark.parametrize("layout", ["hnd", "nhd"])
 @pytest.mark.parametrize("new", [None, [3, 1, 90]])
 def test_attention_layouts_scale_and_sharp_scores(layout, new):
