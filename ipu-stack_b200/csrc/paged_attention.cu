@@ -111,7 +111,7 @@ struct PagedAttnParams {
   int32_t *stream_base, *unit_base;
   int32_t sms;                     // CTAs of each kernel
   int32_t stream, tile_own;        // which of the two take own parts (both: see few_rows)
-  int32_t join_rows;               // rows of a block of the join: 8 or kJoinRows
+  int32_t join_rows;               // rows of a block of the join: 1, 8 or kJoinRows
   int32_t stream_prefix;  // the stream kernel takes the prefix too, for so many groups of 16 rows; or 0
   uint64_t over_group;    // 2^36 / group, rounded up
   int32_t stream_units, tile_units;  // of own parts at most, for sorted row offsets
@@ -624,7 +624,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   const Lines<kStreamThreads> lines(p, scratch, blockIdx.x == 0 && !p.tile_own);
   const int64_t line = lines.stream, ahead = lines.stream_ahead, sms = lines.sms_to_stream;
   int64_t before = lines.stream_before;
-  const int64_t pieces = min(kStreamWorkers * sms, line);  // no piece is empty
+  // (no piece is empty; shorter ones than two key tiles cost more in the join: 16.0
+  // against 15.5 us for 4 rows of 32 heads behind 512)
+  const int64_t pieces = min(kStreamWorkers * sms, (line + 1) / 2);
   // Worker w of CTA c has piece w * sms + c: few pieces spread over many SMs.
   auto piece_of = [&](int w) { return w * sms + (int64_t)blockIdx.x; };
   auto start_of = [&](int w) { return line * piece_of(w) / pieces; };
@@ -1719,8 +1721,16 @@ __device__ __forceinline__ Pieces pieces_of(const PagedAttnParams &p, bool strea
   return r;
 }
 
+// kSplit: a block joins one row, eight neighbouring threads sharing its partials:
+// for calls whose rows would leave most of the GPU idle and have many.  A call in
+// all, without and with it: a row of 32 heads over 8000 keys (37 partials) 25.1
+// and 20.3 us, 4 rows of 32 heads behind 512 15.5 and 14.3, 11 rows in 4
+// sequences over 500 to 4000 29.3 and 27.1, but 16 rows over 100 to 900 (3
+// partials) 21.5 and 21.9.
 constexpr int kJoinRows = 32;
+template <bool kSplit>
 __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_constant__ PagedAttnParams p) {
+  constexpr int32_t step = kSplit ? 8 : 1;
   const int32_t dim = (threadIdx.x >> 3) * 4, kv = blockIdx.y;
   const int32_t stream_cost = p.stream_prefix ? unit_cost((p.prefix + kStreamKeys - 1) / kStreamKeys) : 0;
   __shared__ Pieces shared_pieces[2][kJoinRows];  // own, prefix
@@ -1763,9 +1773,9 @@ __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_cons
     shared_pieces[prefix][threadIdx.x % kJoinRows] = r;
   }
   __syncthreads();
-  if (dim >= p.head_dim) return;
+  if (!kSplit && dim >= p.head_dim) return;
 #pragma unroll 1
-  for (int32_t sub = threadIdx.x & 7; sub < p.join_rows; sub += 8) {
+  for (int32_t sub = kSplit ? 0 : threadIdx.x & 7; sub < p.join_rows; sub += 8) {
     const Pieces own = shared_pieces[0][sub], pre = shared_pieces[1][sub];
     if (own.count < 0) continue;  // padding
     if (p.prefix == 0 && own.count == 1) continue;  // the whole unit was one CTA's, which wrote the result
@@ -1775,9 +1785,9 @@ __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_cons
     const int64_t pre_step = (int64_t)pre.rows * p.head_dim, own_step = (int64_t)own.rows * p.head_dim;
     const float *pre_part = pre.o + (dim >> 2) * pre.dims, *own_part = own.o + (dim >> 2) * own.dims - pre.count * own_step;
     const float2 *own_ml = own.ml - (int64_t)pre.count * own.rows;
-    const int32_t count = pre.count + own.count;
+    const int32_t count = dim < p.head_dim ? pre.count + own.count : 0;
 #pragma unroll 1
-    for (int32_t i = 0; i < count; i += 4) {
+    for (int32_t first = kSplit ? threadIdx.x & 7 : 0; first < count; first += 4 * step) {
       float2 s[4];
       float4 v[4];
       float t = top;
@@ -1785,10 +1795,11 @@ __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_cons
       for (int32_t x = 0; x < 4; ++x) {
         s[x] = make_float2(-INFINITY, 0.0f);
         v[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (i + x < count) {
-          const bool first = i + x < pre.count;
-          s[x] = first ? pre.ml[(int64_t)(i + x) * pre.rows] : own_ml[(int64_t)(i + x) * own.rows];
-          v[x] = *reinterpret_cast<const float4 *>(first ? pre_part + (i + x) * pre_step : own_part + (i + x) * own_step);
+        const int32_t i = first + x * step;
+        if (i < count) {
+          const bool shared = i < pre.count;
+          s[x] = shared ? pre.ml[(int64_t)i * pre.rows] : own_ml[(int64_t)i * own.rows];
+          v[x] = *reinterpret_cast<const float4 *>(shared ? pre_part + i * pre_step : own_part + i * own_step);
         }
       }
 #pragma unroll
@@ -1811,6 +1822,18 @@ __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_cons
         o.z = fmaf(v[x].z, w, o.z);
         o.w = fmaf(v[x].w, w, o.w);
       }
+    }
+    if (kSplit) {
+#pragma unroll
+      for (int m = 1; m < 8; m <<= 1) {
+        const float other = __shfl_xor_sync(0xffffffffu, top, m), t = fmaxf(top, other);
+        const float a = top == -INFINITY ? 0.0f : ex2_approx(top - t), b = other == -INFINITY ? 0.0f : ex2_approx(other - t);
+        auto join = [&](float x) { return fmaf(x, a, __shfl_xor_sync(0xffffffffu, x, m) * b); };
+        top = t;
+        l = join(l);
+        o = make_float4(join(o.x), join(o.y), join(o.z), join(o.w));
+      }
+      if ((threadIdx.x & 7) || dim >= p.head_dim) continue;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     uint2 v;
@@ -2015,7 +2038,8 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
   };
   // The stream kernel runs beside the tile kernel, whose start takes longer, on
   // the SMs that leaves it (programmatic dependent launch).  The join is an
-  // ordinary launch: an early one measured 3.5 us slower for few rows.
+  // ordinary launch: an early one gained nothing (15.9 against 16.0 us for few
+  // rows, 31 against 29 for few rows of ragged batches).
   auto launch = [&](auto kernel, dim3 grid, int threads, int bytes, bool beside, auto... args) -> ipuc_status {
     if (bytes) IPUC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
     cudaLaunchConfig_t cfg = {};
@@ -2059,7 +2083,10 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
     if (st != IPUC_OK) return st;
   }
   // Few rows: many small blocks; more than fill the GPU: fewer, which find their pieces at once.
-  p.join_rows = p.rows * q_heads >= 8 * 4 * (int64_t)p.sms ? kJoinRows : 8;
-  return launch(paged_combine_kernel, dim3((unsigned)ceil_div(p.rows * p.group, p.join_rows), (unsigned)p.heads), 256, 0,
-                false, p);
+  const int64_t heads_rows = p.rows * q_heads, resident = 4 * (int64_t)p.sms;
+  const bool split = heads_rows <= 3 * p.sms;
+  p.join_rows = split ? 1 : heads_rows >= 8 * resident ? kJoinRows : 8;
+  const dim3 grid((unsigned)ceil_div(p.rows * p.group, p.join_rows), (unsigned)p.heads);
+  return split ? launch(paged_combine_kernel<true>, grid, 256, 0, false, p)
+               : launch(paged_combine_kernel<false>, grid, 256, 0, false, p);
 }
