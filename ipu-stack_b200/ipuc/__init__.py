@@ -144,8 +144,9 @@ def _check(fn: str, status: int):
 
 def call(name: str, *args):
     """Call an entry point by name with raw arguments; raises IpucError on failure."""
-    st = getattr(lib(), name)(*args)
-    _check(name, st)
+    st = getattr(_lib or lib(), name)(*args)
+    if st != OK:
+        _check(name, st)
     return st
 
 
@@ -575,6 +576,7 @@ def rotary_table(out, base=10000.0, scaling=ROTARY_SCALE_NONE, factor=1.0, low=1
 
 class Rotary:
     """A rotary table (rotary_table's output) with the layout of the pairs; keeps the table alive."""
+    __slots__ = ("table", "_on", "_spec")
 
     def __init__(self, table, layout=ROTARY_HALF):
         fn, (torch, device) = "ipuc_rotary_table", _device()
@@ -588,7 +590,8 @@ class Rotary:
 def rotary_f16(out, x, rotary, positions=None, stream=None):
     """out = x with the heads rotated: x [tokens, heads, head_dim] f16 or f32, out f16 of that shape."""
     fn, (torch, device) = "ipuc_rotary_f16", _device()
-    _on(fn, device, rotary)
+    if rotary is not None and rotary._on != device:
+        _on(fn, device, rotary)
     dtype, precision = _precision(fn, "x", x)
     shape, xs = _token_rows(fn, "x", x, device, dtype)
     _, os_ = _token_rows(fn, "out", out, device, torch.float16, shape)
@@ -602,7 +605,8 @@ def qk_norm_rotary_f16(q_out, k_out, q, k, q_weight=None, k_weight=None, eps=1e-
     """Per-head norm of q and k, then their rotation: q [tokens, q_heads, head_dim], k [tokens, k_heads, head_dim]
     of one type, weights f16 [head_dim] (None: ones)."""
     fn, (torch, device) = "ipuc_qk_norm_rotary_f16", _device()
-    _on(fn, device, rotary)
+    if rotary is not None and rotary._on != device:
+        _on(fn, device, rotary)
     dtype, precision = _precision(fn, "q", q)
     q_shape, qs = _token_rows(fn, "q", q, device, dtype)
     tokens, q_heads, d = q_shape
@@ -620,11 +624,14 @@ def qk_norm_rotary_f16(q_out, k_out, q, k, q_weight=None, k_weight=None, eps=1e-
 class PagedCache:
     """Keys and values [pages, heads, page_size, head_dim] f16 of equal strides (any order of the first three
     dimensions in memory: pass a transposed view of [pages, page_size, heads, head_dim]); keeps them alive."""
+    __slots__ = ("keys", "values", "heads", "page_size", "head_dim", "_on", "_spec")
 
     def __init__(self, keys, values):
         fn, (torch, device) = "ipuc_paged_cache", _device()
         shape, stride = _want(fn, "keys", keys, device, torch.float16, 4)
-        if _want(fn, "values", values, device, torch.float16, 4) != (shape, stride):
+        if not (isinstance(values, _Tensor) and values.dtype is keys.dtype and values.get_device() == device
+                and values.stride() == stride and values.shape == shape):
+            _want(fn, "values", values, device, torch.float16, 4)
             _refuse(fn, "keys and values must have the same shape and strides")
         pages, heads, page_size, d = shape
         if d > 1 and stride[3] != 1:
@@ -647,6 +654,7 @@ class PagedBatch:
     """The sequences of a call: page_table [sequences, max_pages], lengths [sequences] and, unless every sequence
     has one row, row_offsets [sequences + 1], int32.  The number of rows is that of the tensors of each call (with
     row_offsets: its last entry, or more; the rest is padding)."""
+    __slots__ = ("_keep", "_on", "_spec")
 
     def __init__(self, page_table, lengths, row_offsets=None):
         fn, (torch, device) = "ipuc_paged_batch", _device()
@@ -666,7 +674,8 @@ class PagedBatch:
 def paged_append_f16(cache, batch, k, v, rotary=None, stream=None):
     """Writes the new rows k, v [rows, heads, head_dim] (f16 or f32) into the cache, keys rotated by their positions."""
     fn, (_, device) = "ipuc_paged_append_f16", _device()
-    _on(fn, device, cache, batch, rotary)
+    if cache._on != device or batch._on != device or (rotary is not None and rotary._on != device):
+        _on(fn, device, cache, batch, rotary)
     dtype, precision = _precision(fn, "k", k)
     rows = k.shape[0] if k.dim() else 0
     shape = (rows, cache.heads, cache.head_dim)
@@ -686,7 +695,8 @@ def paged_attention_f16(out, q, cache, batch, workspace, prefix_rows=0, prefix_p
     """Attention of q [rows, q_heads, head_dim] over the cache into out (dense); positions below prefix_rows are read
     once for all rows through prefix_pages."""
     fn, (torch, device) = "ipuc_paged_attention_f16", _device()
-    _on(fn, device, cache, batch)
+    if cache._on != device or batch._on != device:
+        _on(fn, device, cache, batch)
     shape, qs = _token_rows(fn, "q", q, device, torch.float16)
     rows, heads, d = shape
     _, os_ = _token_rows(fn, "out", out, device, torch.float16, shape)
