@@ -62,9 +62,21 @@ def test_table(kind, code, scaling, positions, rotary, magnitude):
     got = make_table(positions, rotary, scaling=code, magnitude=magnitude, **scaling)
     want = ref.table(positions, rotary, magnitude, kind=kind, **scaling)
     torch.cuda.synchronize()
-    # sincospif within 2 steps, its argument, the magnitude and the product rounded once each: 6 half
-    # steps of 1; the angle itself is f64 (131072 rad: 2^-52 of that, 3e-11).
+    # The remainder of the angle rounded once (at most pi/4 of a half step), the polynomial's last product and
+    # sum, the products with the magnitude's two parts: 6 half steps of 1 hold them and the terms left out
+    # (2e-9); the angle itself is as exact as an f64 frequency (131072 rad: 2^-52 of that, 3e-11).
     assert (f64(got) - want).abs().max() <= 6 * ref.F32_HALF_STEP * magnitude + 1e-10
+
+
+def test_table_far_positions():
+    """Positions around 2^24 and behind, where f32 holds no fraction of the angle."""
+    positions = (1 << 24) + 5000
+    got = f64(make_table(positions, 4, base=100.0)[-10000:])
+    # frequencies 1 and 1/10, the second off by 2^-54 of a turn a position at most
+    at = torch.arange(positions - 10000, positions, dtype=torch.float64)
+    angle = torch.stack((at, at / 10.0), 1)
+    # as above, and the f64 angles here and in the table: 2 x 2^-53 of 1.7e7 rad
+    assert (got - torch.cat((angle.cos(), angle.sin()), 1)).abs().max() <= 6 * ref.F32_HALF_STEP + 4e-9
 
 
 # ---- rotary --------------------------------------------------------------------
