@@ -547,8 +547,9 @@ typedef struct {
 
 /* Writes the new rows' keys (rotated by their positions unless rotary is
  * NULL) and values into the cache: k, v [rows][heads][head_dim] at strides
- * k_stride, v_stride, f16 or f32, apart from the cache.  A slot that two rows of the call share
- * (one page in two places of the table) holds either's elements. */
+ * k_stride, v_stride, f16 or f32, apart from the cache.  A slot that two rows
+ * of the call share (one page in two places of the table) holds either's
+ * elements. */
 ipuc_status ipuc_paged_append_f16(const ipuc_paged_cache *cache, const ipuc_paged_batch *batch, const void *k,
                                   int64_t k_stride, const void *v, int64_t v_stride, ipuc_precision in_precision,
                                   const ipuc_rotary *rotary, ipuc_stream stream);
