@@ -161,6 +161,12 @@ __device__ __forceinline__ uint32_t rest_h2(float lo, float hi, uint32_t h) {
   return to_h2(lo - f.x, hi - f.y);
 }
 
+// (Maximum in log2 units, sum) of a partial result.  A maximum drops NaN scores,
+// the sum keeps them: with scores of NaN alone the maximum is that of no keys.
+__device__ __forceinline__ float2 partial_ml(float m, float l, float c) {
+  return make_float2(l != l ? l : m == -INFINITY ? m : m * c, l);
+}
+
 // Length of sequence b as far as its table row can hold it.
 __device__ __forceinline__ int32_t checked_length(const PagedAttnParams &p, int32_t b, bool report) {
   const int32_t n = p.paged.lengths[b], cap = p.paged.max_pages * p.paged.page_size;
@@ -980,10 +986,10 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       for (int x = 0; x < 4; ++x) top = fmaxf(top, warp_m[x][orow & 15]);
 #pragma unroll
       for (int x = 0; x < 4; ++x)
-        if (warp_m[x][orow & 15] != -INFINITY) sum += warp_l[x][orow & 15] * ex2_approx((warp_m[x][orow & 15] - top) * c);
+        if (warp_l[x][orow & 15] != 0.0f) sum += warp_l[x][orow & 15] * ex2_approx((warp_m[x][orow & 15] - top) * c);
       const int64_t slot = slot0 + orow;
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      if (!whole && orow < rows_here && ocol == 0) p.stream_ml[slot] = make_float2(top == -INFINITY ? top : top * c, sum);
+      if (!whole && orow < rows_here && ocol == 0) p.stream_ml[slot] = partial_ml(top, sum, c);
 #pragma unroll
       for (int round = 0; round < (NT + NI - 1) / NI; ++round) {
         if (round) named_barrier_sync(1 + worker, 128);
@@ -1600,7 +1606,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         named_barrier_sync(9 + quarter, 128);  // read before the next unit's maxima are written
       }
       if (row_ok && !direct && half == 0 && (!dual || t == 0))
-        p.tile_ml[slot * p.tile_slot_rows + slot_row] = make_float2(m == -INFINITY ? m : m * c, l);
+        p.tile_ml[slot * p.tile_slot_rows + slot_row] = partial_ml(m, l, c);
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
       for (int ch = 0; ch < 2; ++ch) {
@@ -1803,7 +1809,7 @@ __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_cons
         }
       }
 #pragma unroll
-      for (int32_t x = 0; x < 4; ++x) t = fmaxf(t, s[x].x);
+      for (int32_t x = 0; x < 4; ++x) t = max_nan(t, s[x].x);
       if (t == -INFINITY) continue;  // no keys
       const float a = ex2_approx(top - t);
       top = t;
@@ -1826,7 +1832,7 @@ __global__ void __launch_bounds__(256, 4) paged_combine_kernel(const __grid_cons
     if (kSplit) {
 #pragma unroll
       for (int m = 1; m < 8; m <<= 1) {
-        const float other = __shfl_xor_sync(0xffffffffu, top, m), t = fmaxf(top, other);
+        const float other = __shfl_xor_sync(0xffffffffu, top, m), t = max_nan(top, other);
         const float a = top == -INFINITY ? 0.0f : ex2_approx(top - t), b = other == -INFINITY ? 0.0f : ex2_approx(other - t);
         auto join = [&](float x) { return fmaf(x, a, __shfl_xor_sync(0xffffffffu, x, m) * b); };
         top = t;

@@ -399,6 +399,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// The larger one, NaN where either is (fmaxf drops NaN).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 // 2^t for a pair, on the FMA pipe instead of the MUFU unit.  t = n + f with
 // n = round(t) (the 1.5*2^23 shifter) and f in [-0.5, 0.5]; 2^f is a degree-3

@@ -1,0 +1,97 @@
+"""Paged attention with NaN and infinities in queries, in keys that are attended
+to and in values: what softmax makes of them, on every path of the call.
+
+A row whose scores hold NaN or +inf is NaN in every element; a key of score -inf
+has weight 0; every other row is what it is without them."""
+import math
+
+import pytest
+import torch
+
+import ipuc
+import paged_ref as ref
+from test_gpu_paged import NAN, Case, f64, randn, run_attention
+
+pytestmark = pytest.mark.gpu
+
+# name: lengths, new, prefix, page, heads, group, dim
+REGIMES = {
+    "single rows, short": ([100, 64, 1, 37], None, 0, 16, 2, 4, 64),
+    "single rows of 16 heads": ([100, 130], None, 0, 16, 1, 16, 128),
+    "one row over many pieces": ([3000], None, 0, 64, 2, 4, 128),
+    "few rows behind a prefix": ([300, 290, 280], None, 256, 16, 2, 4, 72),
+    "many rows behind a prefix": ([2100 + i for i in range(64)], None, 2048, 64, 2, 8, 64),
+    "few rows a sequence": ([90, 200, 70], [3, 2, 4], 0, 16, 2, 4, 128),
+    "a prompt of two row tiles": ([100], [60], 0, 16, 1, 4, 64),
+    "a prompt of one row tile": ([200], [30], 0, 16, 1, 4, 128),
+    "prompts over several key tiles": ([700, 600], [100, 300], 0, 64, 1, 4, 128),
+    "prompts behind a prefix": ([600, 560], [70, 40], 500, 64, 2, 4, 128),
+    "prompts in whole units": ([390] * 24, [100] * 24, 0, 64, 8, 4, 64),
+    "a group of 24": ([150, 140], None, 0, 16, 1, 24, 64),
+}
+
+
+def make(seed, regime):
+    lengths, new, prefix, page, heads, group, dim = REGIMES[regime]
+    c = Case(seed, lengths, new, heads=heads, dim=dim, page=page, prefix=prefix).device()
+    q = randn(c.g, (c.rows, heads * group, dim))
+    return c, group, q
+
+
+def put(c, b, position, value, at=slice(None)):
+    """Writes `value` into the keys at a position of sequence b (of all where the prefix has it)."""
+    ids = c.prefix_pages if position < c.prefix else c.table[b]
+    c.keys[ids[position // c.page], :, position % c.page, at] = value
+
+
+def expected(c, q, scale):
+    """(out, bound) in f64, as paged_ref.attention's, for scores of any kind; rows of `want` are NaN as a whole or finite."""
+    q, keys, values = f64(q), f64(c.keys), f64(c.values)
+    group = q.shape[1] // keys.shape[1]
+    want, bound = torch.zeros_like(q), torch.full_like(q, ref.F16_TINY)
+    made = {}
+    for r, b, position in ref.rows_of(c.lengths, c.offsets, c.rows):
+        if position < 0:
+            continue
+        if b not in made:
+            at = torch.arange(c.lengths[b])
+            ids = torch.tensor([(c.prefix_pages if i < c.prefix else c.table[b])[i // c.page] for i in range(c.lengths[b])])
+            made = {b: (keys[ids, :, at % c.page], values[ids, :, at % c.page])}
+        k, v = (x[:position + 1].repeat_interleave(group, 1) for x in made[b])
+        s = torch.einsum("hd,nhd->hn", q[r], k) * scale
+        dead = torch.isnan(s).any(-1) | (s == math.inf).any(-1)
+        kept = torch.isfinite(s) & ~dead[:, None]
+        top = s.masked_fill(~kept, -math.inf).amax(-1, keepdim=True)
+        w = torch.where(kept, (s - torch.where(torch.isfinite(top), top, 0.0)).exp(), 0.0)
+        w = w / w.sum(-1, keepdim=True).clamp(min=1e-300)
+        want[r] = torch.einsum("hn,nhd->hd", w, v)
+        mass = torch.einsum("hn,nhd->hd", w, v.abs())
+        # (the bound's terms are paged_ref.attention's)
+        size = torch.einsum("hd,nhd->hn", q[r].nan_to_num(0, 0, 0).abs(), k.nan_to_num(0, 0, 0).abs()) * scale
+        delta = 2 * q.shape[2] * ref.F32_HALF_STEP * size.amax(-1)
+        bound[r] = ref.rounded(want[r], torch.zeros(()), 0) + (ref.F16_HALF_STEP + 1e-4 + 2 * delta)[:, None] * mass \
+            + (position + 1) * 2.0 ** -31 * v.abs().amax(0)
+        want[r][dead] = NAN
+    return want, bound
+
+
+def check(c, group, q):
+    _, out, _ = run_attention(c, group, q=q)
+    torch.cuda.synchronize()
+    ipuc.device_status()
+    want, bound = expected(c, q, 1.0 / math.sqrt(c.dim))
+    got, dead = f64(out), torch.isnan(want)
+    assert torch.equal(torch.isnan(got), dead), \
+        f"{int((torch.isnan(got) != dead).any(-1).sum())} rows differ in what is NaN, {int(dead.any(-1).sum())} should be"
+    off = (got - want).abs()[~dead]
+    assert (off <= bound[~dead]).all(), f"worst {(off / bound[~dead]).max():.3f} of the bound"
+    return dead
+
+
+@pytest.mark.parametrize("regime", REGIMES)
+def test_a_query_that_holds_nan(regime):
+    c, group, q = make(60, regime)
+    for i, r in enumerate(range(0, c.rows, 3)):
+        q[r, (5 * i) % q.shape[1], (7 * i) % c.dim] = NAN
+    dead = check(c, group, q)
+    assert dead.any() and not dead.all()
