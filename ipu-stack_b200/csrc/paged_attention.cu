@@ -1515,20 +1515,23 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         float mx = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
-          mx = max3(mx, __uint_as_float(a[i]), __uint_as_float(a[i + 1]));
-          mx1 = max3(mx1, __uint_as_float(a[i + 2]), __uint_as_float(a[i + 3]));
-          mx = max3(mx, __uint_as_float(b[i]), __uint_as_float(b[i + 1]));
-          mx1 = max3(mx1, __uint_as_float(b[i + 2]), __uint_as_float(b[i + 3]));
+          mx = max3_nan(mx, __uint_as_float(a[i]), __uint_as_float(a[i + 1]));
+          mx1 = max3_nan(mx1, __uint_as_float(a[i + 2]), __uint_as_float(a[i + 3]));
+          mx = max3_nan(mx, __uint_as_float(b[i]), __uint_as_float(b[i + 1]));
+          mx1 = max3_nan(mx1, __uint_as_float(b[i + 2]), __uint_as_float(b[i + 3]));
         }
-        mx = fmaxf(mx, mx1);
+        mx = max_nan(mx, mx1);
         x_max[t][half][row] = mx;
         named_barrier_sync(bar_id, 64);
-        const float m_new = fmaxf(m, fmaxf(mx, x_max[t][half ^ 1][row]));
+        // A score of NaN or +inf makes the row NaN.  The maximum carries that: the
+        // polynomial below, which takes one pair in three, does not.
+        float m_new = max_nan(m, max_nan(mx, x_max[t][half ^ 1][row]));
+        if (m_new == INFINITY) m_new = NAN;
         bool rescale = false;
         float alpha = 1.0f;
         if (j == 0) {
           m = m_new;
-        } else if ((m_new - m) * c > kLazy) {
+        } else if ((m_new - m) * c > kLazy || isnan(m_new)) {
           alpha = ex2_approx((m - m_new) * c);  // 0 where m = -inf: so are O and l
           rescale = true;
           m = m_new;
@@ -1598,7 +1601,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           x_max[t][1][row] = l;
         }
         named_barrier_sync(9 + quarter, 128);
-        const float m2 = x_max[t ^ 1][0][row], l2 = x_max[t ^ 1][1][row], top = fmaxf(m, m2);
+        const float m2 = x_max[t ^ 1][0][row], l2 = x_max[t ^ 1][1][row], top = max_nan(m, m2);
         own = m == -INFINITY ? 0.0f : ex2_approx((m - top) * c);
         other = m2 == -INFINITY ? 0.0f : ex2_approx((m2 - top) * c);
         l = l * own + l2 * other;

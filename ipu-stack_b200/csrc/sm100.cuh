@@ -399,7 +399,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// The larger one, NaN where either is (fmaxf drops NaN).
+// The largest, NaN where any is (fmaxf and max3 drop NaN).
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -413,7 +418,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // an f16 ulp), and 2^n is added to the exponent field.
 // Inputs are clamped at -125: with 2^f in [0.70, 1.42] the exponent field
 // then stays in [1, 254], so adding n to it can neither wrap nor underflow
-// (2^-125 rounds to 0 in the f16 P anyway).
+// (2^-125 rounds to 0 in the f16 P anyway).  NaN gives 2^-125 too: callers
+// carry it in the maximum that t is taken relative to.
 __device__ __forceinline__ uint64_t exp2_poly2(uint64_t t) {
   float t0, t1;
   f2_unpack(t, t0, t1);

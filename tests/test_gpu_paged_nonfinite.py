@@ -26,7 +26,7 @@ REGIMES = {
     "a prompt of one row tile": ([200], [30], 0, 16, 1, 4, 128),
     "prompts over several key tiles": ([700, 600], [100, 300], 0, 64, 1, 4, 128),
     "prompts behind a prefix": ([600, 560], [70, 40], 500, 64, 2, 4, 128),
-    "prompts in whole units": ([390] * 24, [100] * 24, 0, 64, 8, 4, 64),
+    "prompts in whole units": ([390] * 24, [70] * 24, 0, 64, 8, 4, 64),
     "a group of 24": ([150, 140], None, 0, 16, 1, 24, 64),
 }
 
@@ -44,34 +44,50 @@ def put(c, b, position, value, at=slice(None)):
     c.keys[ids[position // c.page], :, position % c.page, at] = value
 
 
+def with_keys(c, value, at):
+    """The case with `value` in one key of each sequence's own part, at six neighbouring positions in turn or in
+    different sequences (kernels take pairs of scores in threes), then in the shared part (a position of a third pair)."""
+    keys = c.keys.clone()
+    several = len(c.lengths) >= 6
+    for shift in range(1 if several else 6):
+        for b, n in enumerate(c.lengths):
+            put(c, b, max(0, n - 40 + (b + shift if several else shift) % 6), value, at)
+        yield c
+        c.keys.copy_(keys)
+    if c.prefix:
+        put(c, 0, 196, value, at)
+        yield c
+
+
 def expected(c, q, scale):
     """(out, bound) in f64, as paged_ref.attention's, for scores of any kind; rows of `want` are NaN as a whole or finite."""
     q, keys, values = f64(q), f64(c.keys), f64(c.values)
     group = q.shape[1] // keys.shape[1]
     want, bound = torch.zeros_like(q), torch.full_like(q, ref.F16_TINY)
-    made = {}
-    for r, b, position in ref.rows_of(c.lengths, c.offsets, c.rows):
-        if position < 0:
+    rows = ref.rows_of(c.lengths, c.offsets, c.rows)
+    for b, n in enumerate(c.lengths):
+        mine = [(r, position) for r, x, position in rows if x == b and position >= 0]
+        if not mine:
             continue
-        if b not in made:
-            at = torch.arange(c.lengths[b])
-            ids = torch.tensor([(c.prefix_pages if i < c.prefix else c.table[b])[i // c.page] for i in range(c.lengths[b])])
-            made = {b: (keys[ids, :, at % c.page], values[ids, :, at % c.page])}
-        k, v = (x[:position + 1].repeat_interleave(group, 1) for x in made[b])
-        s = torch.einsum("hd,nhd->hn", q[r], k) * scale
-        dead = torch.isnan(s).any(-1) | (s == math.inf).any(-1)
-        kept = torch.isfinite(s) & ~dead[:, None]
-        top = s.masked_fill(~kept, -math.inf).amax(-1, keepdim=True)
-        w = torch.where(kept, (s - torch.where(torch.isfinite(top), top, 0.0)).exp(), 0.0)
+        r, position = (torch.tensor(x) for x in zip(*mine))
+        at = torch.arange(n)
+        ids = torch.tensor([(c.prefix_pages if i < c.prefix else c.table[b])[i // c.page] for i in range(n)])
+        k, v = (x[ids, :, at % c.page].repeat_interleave(group, 1) for x in (keys, values))
+        there = at <= position[:, None, None]                                    # [rows, 1, keys]
+        s = torch.einsum("rhd,nhd->rhn", q[r], k) * scale
+        dead = ((torch.isnan(s) | (s == math.inf)) & there).any(-1)
+        s = s.masked_fill(~there | ~torch.isfinite(s), -math.inf)
+        top = s.amax(-1, keepdim=True)
+        w = (s - top.masked_fill(top == -math.inf, 0.0)).exp()
         w = w / w.sum(-1, keepdim=True).clamp(min=1e-300)
-        want[r] = torch.einsum("hn,nhd->hd", w, v)
-        mass = torch.einsum("hn,nhd->hd", w, v.abs())
+        out, mass = torch.einsum("rhn,nhd->rhd", w, v), torch.einsum("rhn,nhd->rhd", w, v.abs())
         # (the bound's terms are paged_ref.attention's)
-        size = torch.einsum("hd,nhd->hn", q[r].nan_to_num(0, 0, 0).abs(), k.nan_to_num(0, 0, 0).abs()) * scale
-        delta = 2 * q.shape[2] * ref.F32_HALF_STEP * size.amax(-1)
-        bound[r] = ref.rounded(want[r], torch.zeros(()), 0) + (ref.F16_HALF_STEP + 1e-4 + 2 * delta)[:, None] * mass \
-            + (position + 1) * 2.0 ** -31 * v.abs().amax(0)
-        want[r][dead] = NAN
+        size = torch.einsum("rhd,nhd->rhn", q[r].nan_to_num(0, 0, 0).abs(), k.nan_to_num(0, 0, 0).abs()) * scale
+        delta = 2 * q.shape[2] * ref.F32_HALF_STEP * size.masked_fill(~there, 0.0).amax(-1)
+        bound[r] = ref.rounded(out, torch.zeros(()), 0) + (ref.F16_HALF_STEP + 1e-4 + 2 * delta)[..., None] * mass \
+            + (position[:, None, None] + 1) * 2.0 ** -31 * v.abs().amax(0)
+        out[dead] = NAN
+        want[r] = out
     return want, bound
 
 
@@ -95,3 +111,33 @@ def test_a_query_that_holds_nan(regime):
         q[r, (5 * i) % q.shape[1], (7 * i) % c.dim] = NAN
     dead = check(c, group, q)
     assert dead.any() and not dead.all()
+
+
+@pytest.mark.parametrize("regime", REGIMES)
+def test_a_key_of_nan(regime):
+    c, group, q = make(61, regime)
+    for c in with_keys(c, NAN, 3):
+        assert check(c, group, q).any()
+
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf])
+@pytest.mark.parametrize("regime", REGIMES)
+def test_a_key_of_infinity(regime, value):
+    """Scores of +inf (the row is NaN) and of -inf (the key has no weight), by the sign of the query's element."""
+    c, group, q = make(62, regime)
+    q[..., 5] = torch.where(q[..., 5] == 0, torch.ones_like(q[..., 5]), q[..., 5])
+    for c in with_keys(c, value, 5):
+        dead = check(c, group, q)
+        assert dead.any() and not dead.all()
+
+
+def test_keys_of_minus_infinity_alone():
+    """No key has any weight: 0, as for a row without keys."""
+    for new in (None, [40]):
+        c = Case(63, [40], new, heads=1, dim=64, page=16).device()
+        c.keys[..., 0] = -math.inf
+        q = randn(c.g, (c.rows, 4, 64))
+        q[..., 0] = 1.0
+        _, out, _ = run_attention(c, 4, q=q)
+        ipuc.device_status()
+        assert (out == 0).all()
