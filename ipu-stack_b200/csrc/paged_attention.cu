@@ -1610,7 +1610,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       if (row_ok && !direct && half == 0 && (!dual || t == 0))
         p.tile_ml[slot * p.tile_slot_rows + slot_row] = partial_ml(m, l, c);
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const float inv = 1.0f / l;
 #pragma unroll
       for (int ch = 0; ch < 2; ++ch) {
         const int32_t at = dual ? t * 32 : ch * 32;  // column in this thread's half
@@ -1641,7 +1641,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const int col0 = half * 64 + at;
         if (!row_ok || (dual && ch == 1)) continue;
         if (direct) {
-          // (a row without keys: O is 0 * V, which a non-finite V of another row's keys makes NaN)
+          // (a row without keys: O is 0 * V, which a non-finite V of another row's keys makes NaN.
+          // Its sum is not 0: the polynomial makes 2^-125 of a masked score.)
           uint16_t *o = p.out + head * p.head_dim + col0;
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
@@ -1651,7 +1652,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             v.y = to_h2(__uint_as_float(r[i + 2]) * inv, __uint_as_float(r[i + 3]) * inv);
             v.z = to_h2(__uint_as_float(r[i + 4]) * inv, __uint_as_float(r[i + 5]) * inv);
             v.w = to_h2(__uint_as_float(r[i + 6]) * inv, __uint_as_float(r[i + 7]) * inv);
-            *reinterpret_cast<uint4 *>(o + i) = l == 0.0f ? make_uint4(0u, 0u, 0u, 0u) : v;
+            *reinterpret_cast<uint4 *>(o + i) = m == -INFINITY ? make_uint4(0u, 0u, 0u, 0u) : v;
           }
         } else {
           // [slot][dim / 4][row][4]: a lane holds a row, so a warp's 16-byte stores are

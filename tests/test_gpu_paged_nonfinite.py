@@ -141,3 +141,15 @@ def test_keys_of_minus_infinity_alone():
         _, out, _ = run_attention(c, 4, q=q)
         ipuc.device_status()
         assert (out == 0).all()
+
+
+@pytest.mark.parametrize("length,new,prefix,group", [
+    (3, 6, 0, 4), (3, 20, 0, 4), (3, 60, 0, 4), (3, 110, 0, 4), (3, 250, 0, 1), (3, 60, 0, 24), (130, 200, 0, 4), (60, 100, 40, 4)])
+def test_rows_without_keys_next_to_infinite_values(length, new, prefix, group):
+    """More rows than positions: the first attend to nothing and give 0 whatever the values of the others' keys are."""
+    c = Case(64, [length], [new], heads=1, dim=64, page=16, prefix=prefix).device()
+    for i in range(3):
+        c.values[(c.prefix_pages if prefix else c.table[0])[0], :, i] = math.inf
+    _, out, _ = run_attention(c, group)
+    ipuc.device_status()
+    assert (out[:-length] == 0).all() and (out[-1] != 0).all()
