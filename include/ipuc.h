@@ -565,9 +565,10 @@ ipuc_status ipuc_paged_append_f16(const ipuc_paged_cache *cache, const ipuc_page
  * prefix_rows: positions below it are the same for all sequences and are read
  * through prefix_pages (device int32, ceil(prefix_rows / page_size) entries)
  * once for all rows, not through the table, whose entries for them are not
- * read.  Slots behind a sequence's length may hold anything, NaN included.
- * A non-finite value at a position that a sequence's later rows attend to may
- * turn the call's earlier rows of that sequence NaN too (0 * inf).
+ * read.  Slots behind a sequence's length (of the prefix: behind the longest
+ * sequence's) may hold anything, NaN included.  A non-finite value at a position
+ * that some row attends to may turn rows that end in front of it NaN too
+ * (0 * inf): rows of the same sequence, for a position of the prefix any row.
  * head_dim a multiple of 8, at most 128; q_heads / heads at most 128; 16-byte
  * aligned pointers, strides multiples of 8 elements.
  * workspace: ipuc_paged_attention_workspace_bytes() bytes (ragged: whether the

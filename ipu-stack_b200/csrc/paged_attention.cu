@@ -333,6 +333,7 @@ struct StreamWalk {
   int32_t unit, behind;     // own part: row units before this one; those of the sequence behind it
   int32_t begin, rows;      // first batch row of the sequence; rows of the unit
   int32_t pos0;             // own part: position of the sequence's first row
+  int32_t prefix_end;       // of the prefix's keys that any sequence reaches
 
   __device__ __forceinline__ static int32_t units(const PagedAttnParams &p, const SequenceRows &r) {
     return few_rows(p, r) ? max(0, ((r.end - r.begin) * p.group + 15) / 16) : 0;
@@ -350,8 +351,8 @@ struct StreamWalk {
     rows = min(16, (int32_t)p.rows * p.group - 16 * j);
     pos0 = 0;
     lo = 0;
-    hi = p.prefix;
-    at.n = (hi + kStreamKeys - 1) / kStreamKeys;
+    hi = prefix_end;
+    at.n = (p.prefix + kStreamKeys - 1) / kStreamKeys;
   }
   __device__ __forceinline__ void own(const PagedAttnParams &p, const SequenceRows &r, int32_t j) {
     const int32_t all_rows = (r.end - r.begin) * p.group;
@@ -413,6 +414,7 @@ struct TileWalk {
   int32_t unit;              // own part: row units before it
   int32_t rows, lo, hi;      // batch rows; keys [lo, hi)
   int64_t row0, pos0;        // first batch row and (own part) its position
+  int32_t prefix_end;        // as in StreamWalk
 
   // Key tiles of row unit j of a sequence.
   __device__ __forceinline__ static int32_t tiles(const PagedAttnParams &p, const SequenceRows &r, int32_t j) {
@@ -439,8 +441,8 @@ struct TileWalk {
     rows = (int32_t)min((int64_t)per_unit, p.rows - row0);
     pos0 = 0;
     lo = 0;
-    hi = p.prefix;
-    at.n = (hi + kTileKeys - 1) / kTileKeys;
+    hi = prefix_end;
+    at.n = (p.prefix + kTileKeys - 1) / kTileKeys;
   }
   __device__ __forceinline__ static int32_t units(const PagedAttnParams &p, const SequenceRows &r) {
     const int32_t per_unit = 2 * p.tile_rows;
@@ -527,12 +529,18 @@ struct Lines {
   int64_t stream_ahead, stream, tile_ahead, tile;  // the prefix's part, which is in front; the whole
   int64_t stream_before, tile_before;              // sums of own_part() in front of this thread's share
   int32_t sms_to_stream;
-  __device__ __forceinline__ Lines(const PagedAttnParams &p, int64_t (&scratch)[kThreads / 32][2], bool report) {
+  // End of the prefix's keys: the longest sequence's length, where all are shorter
+  // than the prefix.  Slots behind it may hold anything.
+  int32_t prefix_end;
+  __device__ __forceinline__ Lines(const PagedAttnParams &p, int64_t (&scratch)[kThreads / 32][2],
+                                   int32_t (&longest)[kThreads / 32], bool report) {
     const Share<kThreads> share(p.paged.sequences);
     int64_t mine[2] = {0, 0};
+    int32_t length = 0;
 #pragma unroll 1
     for (int32_t b = share.lo; b < share.hi; ++b) {
       const SequenceRows r(p, b, report);
+      length = max(length, r.length);
       if (few_rows(p, r)) mine[0] += own_part<StreamWalk>(p, r);
       else mine[1] += own_part<TileWalk>(p, r);
     }
@@ -546,16 +554,20 @@ struct Lines {
         sum[1] += y;
       }
     }
+    length = __reduce_max_sync(0xffffffffu, length);
     if (lane == 31) {
       scratch[warp][0] = sum[0];
       scratch[warp][1] = sum[1];
+      longest[warp] = length;
     }
     __syncthreads();
     stream_before = sum[0] - mine[0];
     tile_before = sum[1] - mine[1];
     stream = tile = 0;
+    length = 0;
 #pragma unroll 1
     for (int w = 0; w < kThreads / 32; ++w) {
+      length = max(length, longest[w]);
       if (w < warp) {
         stream_before += scratch[w][0];
         tile_before += scratch[w][1];
@@ -568,6 +580,7 @@ struct Lines {
     stream = stream_ahead + (stream & kLength) * p.heads;
     tile = tile_ahead + (tile & kLength) * p.heads;
     sms_to_stream = stream_sms(p, stream, tile);
+    prefix_end = min(p.prefix, length);
   }
 };
 
@@ -592,6 +605,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   __shared__ uint64_t all_unit_full[kStreamWorkers][2], all_unit_empty[kStreamWorkers][2];  // queries and task
   __shared__ StreamTask all_tasks[kStreamWorkers][2];
   __shared__ int64_t scratch[kStreamThreads / 32][2];
+  __shared__ int32_t longest[kStreamThreads / 32];
   __shared__ int32_t first_unit[kStreamWorkers][5];
   __shared__ float all_m[kStreamWorkers][4][16], all_l[kStreamWorkers][4][16];
   __shared__ int aborted;
@@ -627,7 +641,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   // (sums of unsorted row offsets may run over and find no first unit)
   if (threadIdx.x >= 32 && threadIdx.x < 32 + kStreamWorkers * 5) (&first_unit[0][0])[threadIdx.x - 32] = 0;
   // Sums first, then this worker's piece [W c / C, W (c + 1) / C) of the line's W.
-  const Lines<kStreamThreads> lines(p, scratch, blockIdx.x == 0 && !p.tile_own);
+  const Lines<kStreamThreads> lines(p, scratch, longest, blockIdx.x == 0 && !p.tile_own);
   const int64_t line = lines.stream, ahead = lines.stream_ahead, sms = lines.sms_to_stream;
   int64_t before = lines.stream_before;
   // (no piece is empty; shorter ones than two key tiles cost more in the join: 16.0
@@ -683,6 +697,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
   const int64_t cta = piece_of(worker), start = start_of(worker);
   if (cta >= pieces) return;  // (a second worker)
   StreamWalk w;
+  w.prefix_end = lines.prefix_end;
   if (start < ahead) {
     w.prefix(p, 0);
     const int32_t unit = (int32_t)(start / unit_cost(w.at.n));
@@ -1070,8 +1085,10 @@ struct TileTask {
   int32_t prefix, direct, store;
   // V rows outside [lo, hi) of a chunk that has both kinds may hold anything
   // and are zeroed in shared memory (0 * NaN is NaN); whole chunks outside are
-  // zero-filled by the TMA.
-  int32_t fix_first, fix_last;
+  // zero-filled by the TMA.  Chunks with lo and hi inside: in the first key tile,
+  // and in the one with this index in the task (-1: none; the unit's last, or an
+  // earlier one of the prefix where no sequence reaches its end).
+  int32_t fix_first, fix_at;
 };
 
 // The MMA warp runs as a whole and one elected lane issues: in code that only
@@ -1127,6 +1144,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __shared__ int aborted;
   __shared__ float x_max[2][2][kTileRows], x_sum[2][2][kTileRows];
   __shared__ int64_t scratch[kTileThreads / 32][2];
+  __shared__ int32_t longest[kTileThreads / 32];
   __shared__ int32_t found[5];
   __shared__ uint64_t task_full[2], task_empty[2];
   __shared__ TileTask tasks[2];
@@ -1159,7 +1177,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   if (threadIdx.x >= 32 && threadIdx.x < 37) found[threadIdx.x - 32] = 0;  // (as first_unit above)
   // This CTA's piece of the line's W, [W c / C, W (c + 1) / C).
   const int64_t cta = blockIdx.x;
-  const Lines<kTileThreads> lines(p, scratch, cta == 0);
+  const Lines<kTileThreads> lines(p, scratch, longest, cta == 0);
   const int64_t line = lines.tile, ahead = lines.tile_ahead, ctas = min((int64_t)(p.sms - lines.sms_to_stream), line);
   int64_t before = lines.tile_before;
   const bool idle = cta >= ctas;  // no piece is empty
@@ -1201,6 +1219,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   __syncthreads();
   TileWalk walk;
   walk.unit = -1;
+  walk.prefix_end = lines.prefix_end;
   if (start < ahead) {
     walk.prefix(p, 0);
     const int64_t u = start / unit_cost(walk.at.n);
@@ -1262,7 +1281,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       // (for unsorted row offsets nothing is written past the last unit)
       task.store = walk.seq < 0 || (uint32_t)walk.unit < (uint32_t)p.tile_units;
       task.fix_first = task.first * kTileKeys < walk.lo && walk.lo % p.chunk != 0;
-      task.fix_last = (task.first + task.n) * kTileKeys > walk.hi && walk.hi % p.chunk != 0;
+      task.fix_at = walk.hi % p.chunk != 0 ? walk.hi / kTileKeys - task.first : -1;
       if (!publish(task, unit)) {
         ok = false;
         break;
@@ -1323,7 +1342,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           if (!ok) break;
           load(s_v + st * kTileBytes, &tm_v, &v_full[st], key0, v_slot, v_page);
           ++v_issued;
-          if ((task.fix_first && j == 1) || (task.fix_last && j == task.n)) {
+          if ((task.fix_first && j == 1) || j - 1 == task.fix_at) {
             ok = wait(&v_full[st], ((v_issued - 1) >> 1) & 1, abort_flag);
             if (!ok) break;
 #pragma unroll 1
@@ -1387,8 +1406,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       ok = there(&task_full[unit & 1], unit >> 1);
       if (!ok) break;
       const TileTask &task = tasks[unit & 1];
-      const int32_t n = uniform(task.n), flags = uniform(task.fix_first | task.fix_last << 1 | task.dual << 2);
-      const bool fix_first = flags & 1, fix_last = flags & 2, dual = flags & 4;
+      const int32_t n = uniform(task.n), flags = uniform(task.fix_first | task.dual << 1), fix_at = uniform(task.fix_at);
+      const bool fix_first = flags & 1, dual = flags & 2;
       if (lane == 0) mbar_arrive(&task_empty[unit & 1]);
       __syncwarp();
       if (n == 0) break;
@@ -1414,7 +1433,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const int st = i & 1;
         const bool more = j + step < n;
         const uint64_t vd = v_desc + (uint64_t)(st * (kTileBytes >> 4));
-        if ((fix_first && j == 0) || (fix_last && j == n - 1)) ok = there(&v_fixed[st], fixes[st]++);
+        if ((fix_first && j == 0) || j == fix_at) ok = there(&v_fixed[st], fixes[st]++);
         else ok = there(&v_full[st], i >> 1);
 #pragma unroll 1
         for (int x = dual ? 1 : 0; x < 2 && ok; ++x) {

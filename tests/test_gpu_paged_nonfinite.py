@@ -153,3 +153,19 @@ def test_rows_without_keys_next_to_infinite_values(length, new, prefix, group):
     _, out, _ = run_attention(c, group)
     ipuc.device_status()
     assert (out[:-length] == 0).all() and (out[-1] != 0).all()
+
+
+@pytest.mark.parametrize("lengths,new,prefix,page,heads,group,dim", [
+    ([20, 30], None, 100, 16, 2, 4, 64), ([20, 30], [5, 9], 100, 64, 1, 2, 72), ([1], None, 700, 256, 2, 16, 128), ([0, 0], None, 50, 16, 1, 4, 64),
+    ([20, 0, 30], None, 100, 16, 1, 24, 64), ([0, 0], None, 300, 16, 1, 24, 64), ([129, 5], [40, 1], 300, 64, 1, 33, 128),
+    ([257, 200], None, 400, 12, 2, 24, 80), ([900 - i for i in range(64)], None, 2048, 64, 2, 8, 64),
+    ([128 + i for i in range(40)], [3, 30] * 20, 2000, 128, 2, 8, 128), ([5] * 64, None, 2048, 64, 2, 8, 96)])
+def test_slots_of_the_prefix_behind_every_length(lengths, new, prefix, page, heads, group, dim):
+    """No sequence reaches the prefix's end; its slots behind the longest one hold NaN and infinities."""
+    c = Case(65, lengths, new, heads=heads, dim=dim, page=page, prefix=prefix).device()
+    for i in range(max(lengths), prefix):
+        at = (c.prefix_pages[i // page], slice(None), i % page)
+        c.keys[at] = NAN if i % 2 else math.inf
+        c.values[at] = NAN if i % 3 else -math.inf
+    q = randn(c.g, (c.rows, heads * group, dim))
+    assert not check(c, group, q).any()
