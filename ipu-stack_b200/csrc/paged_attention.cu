@@ -1960,12 +1960,11 @@ ipuc_status make_map_paged(CUtensorMap *map, const void *base, int64_t head_dim,
   if (!fn) return fail(IPUC_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
   const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)d1, (cuuint64_t)d2, (cuuint64_t)d3};
   const cuuint64_t strides[3] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2, (cuuint64_t)s3 * 2};
-  const cuuint32_t box[4] = {(cuuint32_t)b0, (cuuint32_t)b1, 1, (cuuint32_t)b3}, ones[4] = {1, 1, 1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(base), dims, strides, box, ones,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, b0 == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(IPUC_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled failed");
+  const cuuint32_t box[4] = {(cuuint32_t)b0, (cuuint32_t)b1, 1, (cuuint32_t)b3};
+  const CUresult r = encode_tiled(fn, map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims, strides, box,
+                                  b0 == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(IPUC_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
   return IPUC_OK;
 }
 
