@@ -287,14 +287,22 @@ struct StreamShape {
   int32_t pitch, stages, bytes;  // bytes: dynamic shared memory
 };
 constexpr bool stream_swizzled(int padded_dim) { return padded_dim % 64 == 0; }
-StreamShape stream_shape(int32_t padded_dim, int32_t chunk) {
-  StreamShape r;
+constexpr StreamShape stream_shape(int32_t padded_dim, int32_t chunk) {
+  StreamShape r = {};
   const int32_t align = 128 / (chunk < 8 ? chunk : 8);
   r.pitch = stream_swizzled(padded_dim) ? padded_dim * 2 : (padded_dim * 2 + 16 + align - 1) / align * align;
   const int32_t stage = 2 * kStreamKeys * r.pitch;
   r.stages = kStreamRingBytes / stage < kStreamStages ? kStreamRingBytes / stage : kStreamStages;
   r.bytes = kStreamWorkers * (r.stages * stage + kMergeBytes + 2 * kQueryBytes) + 1024;
   return r;
+}
+// The most that a kernel takes with any page size: its limit, which all host threads
+// share, is the same in every call.
+constexpr int32_t stream_bytes(int32_t padded_dim) {
+  int32_t most = 0;
+  for (int32_t chunk = 1; chunk <= kStreamKeys; chunk *= 2)
+    if (stream_shape(padded_dim, chunk).bytes > most) most = stream_shape(padded_dim, chunk).bytes;
+  return most;
 }
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
@@ -2068,8 +2076,8 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
   // the SMs that leaves it (programmatic dependent launch).  The join is an
   // ordinary launch: an early one gained nothing (15.9 against 16.0 us for few
   // rows, 31 against 29 for few rows of ragged batches).
-  auto launch = [&](auto kernel, dim3 grid, int threads, int bytes, bool beside, auto... args) -> ipuc_status {
-    if (bytes) IPUC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  auto launch = [&](auto kernel, dim3 grid, int threads, int bytes, int most, bool beside, auto... args) -> ipuc_status {
+    if (most) IPUC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
@@ -2087,7 +2095,7 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
     st = make_map_paged(&tm_q, q, d, p.group, cache->heads, p.rows, d, p.group * d, q_stride, 64, p.group, p.tile_rows);
     if (st == IPUC_OK) st = cache_map(&tm_k, cache->keys, 64);
     if (st == IPUC_OK) st = cache_map(&tm_v, cache->values, 64);
-    if (st == IPUC_OK) st = launch(paged_tile_kernel, p.sms, kTileThreads, kTileSmem, false, tm_q, tm_k, tm_v, p);
+    if (st == IPUC_OK) st = launch(paged_tile_kernel, p.sms, kTileThreads, kTileSmem, kTileSmem, false, tm_q, tm_k, tm_v, p);
     if (st != IPUC_OK) return st;
   }
   if (plan.stream) {
@@ -2101,13 +2109,13 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
       if (st == IPUC_OK) st = cache_map(&tm_v, cache->values, box);
       if (st != IPUC_OK) return st;
     }
-    auto stream_kernel = [&](auto kernel) {
-      return launch(kernel, p.sms, kStreamThreads, shape.bytes, plan.tile, tm_k, tm_v, p);
+    auto stream_kernel = [&](auto kernel, int most) {
+      return launch(kernel, p.sms, kStreamThreads, shape.bytes, most, plan.tile, tm_k, tm_v, p);
     };
-    st = padded == 64   ? stream_kernel(paged_stream_kernel<64>)
-         : padded == 80 ? stream_kernel(paged_stream_kernel<80>)
-         : padded == 96 ? stream_kernel(paged_stream_kernel<96>)
-                        : stream_kernel(paged_stream_kernel<128>);
+    st = padded == 64   ? stream_kernel(paged_stream_kernel<64>, stream_bytes(64))
+         : padded == 80 ? stream_kernel(paged_stream_kernel<80>, stream_bytes(80))
+         : padded == 96 ? stream_kernel(paged_stream_kernel<96>, stream_bytes(96))
+                        : stream_kernel(paged_stream_kernel<128>, stream_bytes(128));
     if (st != IPUC_OK) return st;
   }
   // Few rows: many small blocks; more than fill the GPU: fewer, which find their pieces at once.
@@ -2115,6 +2123,6 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
   const bool split = heads_rows <= 3 * p.sms;
   p.join_rows = split ? 1 : heads_rows >= 8 * resident ? kJoinRows : 8;
   const dim3 grid((unsigned)ceil_div(p.rows * p.group, p.join_rows), (unsigned)p.heads);
-  return split ? launch(paged_combine_kernel<true>, grid, 256, 0, false, p)
-               : launch(paged_combine_kernel<false>, grid, 256, 0, false, p);
+  return split ? launch(paged_combine_kernel<true>, grid, 256, 0, 0, false, p)
+               : launch(paged_combine_kernel<false>, grid, 256, 0, 0, false, p);
 }

@@ -56,3 +56,43 @@ def test_the_first_product_of_a_host_thread():
     # f32 sums of 256 products (256 half steps of the magnitudes) and the store
     want, size = f64(a) @ f64(b), f64(a).abs() @ f64(b).abs()
     within(c, want, ref.rounded(want, size, 256))
+
+
+@pytest.mark.parametrize("dim", [72, 96, 128])
+def test_host_threads_with_caches_of_other_page_sizes(dim):
+    """Threads with a cache, a stream and a workspace each.  The page size decides how much shared memory a call takes,
+    the limit of it belongs to the kernel: no thread's calls may lower it for the others'."""
+    cases = [Case(70 + i, [9, 4, 13], heads=1, dim=dim, page=page).device() for i, page in enumerate((2, 16, 2, 16))]
+    failed, outs, made = [], [], []
+    for c in cases:
+        q = randn(c.g, (3, 4, dim))
+        ws = torch.empty(ipuc.paged_attention_workspace_bytes(3, 3, 4, 1, dim), dtype=torch.uint8, device="cuda")
+        made.append((q, ws, torch.cuda.Stream()))
+        outs.append(torch.empty_like(q))
+    torch.cuda.synchronize()
+    start = threading.Barrier(len(cases))
+
+    def work(i):
+        (q, ws, stream), out, c = made[i], outs[i], cases[i]
+        # (the wrapper's arguments, packed once: as many calls at once as possible)
+        args = (out.data_ptr(), q.data_ptr(), 4 * dim, 4, c.cache._spec, c.batch._with_rows(3), 0, None, 0.0, ws.data_ptr(),
+                ws.numel(), stream.cuda_stream)
+        start.wait()
+        try:
+            for _ in range(5000):
+                ipuc.call("ipuc_paged_attention_f16", *args)
+        except Exception as e:  # noqa: BLE001  (a thread's failure is the test's)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    ipuc.device_status()
+    for c, (q, _, _), out in zip(cases, made, outs):
+        want, bound, _ = ref.attention(f64(q), f64(c.keys).nan_to_num(), f64(c.values).nan_to_num(), c.table, c.lengths, None, 0,
+                                       [], 1.0 / math.sqrt(dim))
+        within(out, want, bound)
