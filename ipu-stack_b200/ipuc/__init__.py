@@ -712,10 +712,14 @@ def paged_attention_f16(out, q, cache, batch, workspace, prefix_rows=0, prefix_p
         if n * cache.page_size < prefix_rows or (n > 1 and stride[0] != 1):
             _refuse(fn, "prefix_pages must be dense and hold prefix_rows")
         at = prefix_pages.data_ptr()
-    if workspace is not None and workspace.get_device() != device:
-        _refuse(fn, "workspace is not on the current device")
-    call(fn, out.data_ptr(), q.data_ptr(), qs, heads, cache._spec, batch._with_rows(rows), prefix_rows, at, scale,
-         _ptr(workspace), workspace.numel() * workspace.element_size() if workspace is not None else 0,
+    ws, size = None, 0
+    if workspace is not None:
+        if not isinstance(workspace, _Tensor) or workspace.get_device() != device:
+            _refuse(fn, "workspace is not a tensor on the current device")
+        if not workspace.is_contiguous():
+            _refuse(fn, "workspace must be dense")
+        ws, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    call(fn, out.data_ptr(), q.data_ptr(), qs, heads, cache._spec, batch._with_rows(rows), prefix_rows, at, scale, ws, size,
          _stream_on(device, stream))
 
 
