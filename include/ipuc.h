@@ -569,6 +569,9 @@ ipuc_status ipuc_paged_append_f16(const ipuc_paged_cache *cache, const ipuc_page
  * sequence's) may hold anything, NaN included.  A non-finite value at a position
  * that some row attends to may turn rows that end in front of it NaN too
  * (0 * inf): rows of the same sequence, for a position of the prefix any row.
+ * Rows that give it weight are not finite in that element: NaN in most calls,
+ * also where the value is an infinity (weights enter the product in two parts,
+ * of which one may be 0 or negative).
  * head_dim a multiple of 8, at most 128; q_heads / heads at most 128; 16-byte
  * aligned pointers, strides multiples of 8 elements.
  * workspace: ipuc_paged_attention_workspace_bytes() bytes (ragged: whether the

@@ -941,7 +941,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
       // A weight goes into the product in two f16 parts, hi + lo, so that its
       // rounding (2^-11) does not add to the result's: in units of at most 8
       // rows the lo parts take the fragments' idle rows 8 to 15, in larger ones
-      // a second product.  HBM bounds the kernel either way.
+      // a second product.  HBM bounds the kernel either way.  An infinite value
+      // meets a part that is 0 or negative and gives NaN.
       uint32_t a[4], a_lo[4];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {

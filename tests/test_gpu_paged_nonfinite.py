@@ -169,3 +169,24 @@ def test_slots_of_the_prefix_behind_every_length(lengths, new, prefix, page, hea
         c.values[at] = NAN if i % 3 else -math.inf
     q = randn(c.g, (c.rows, heads * group, dim))
     assert not check(c, group, q).any()
+
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf, NAN])
+@pytest.mark.parametrize("regime", REGIMES)
+def test_a_value_that_is_not_finite(regime, value):
+    """It shows in its element of every row that gives it weight, and in no other element."""
+    c, group, q = make(66, regime)
+    values = c.values.clone()
+    at = [max(0, n - 40 + b % 6) for b, n in enumerate(c.lengths)]
+    for b, n in enumerate(c.lengths):
+        ids = c.prefix_pages if at[b] < c.prefix else c.table[b]
+        c.values[ids[at[b] // c.page], :, at[b] % c.page, 7] = value
+    _, out, _ = run_attention(c, group, q=q)
+    torch.cuda.synchronize()
+    ipuc.device_status()
+    c.values.copy_(values)
+    want, bound = expected(c, q, 1.0 / math.sqrt(c.dim))
+    got, others = f64(out), torch.arange(c.dim) != 7
+    assert ((got - want).abs() <= bound)[..., others].all()
+    for r, b, position in ref.rows_of(c.lengths, c.offsets, c.rows):
+        assert position < at[b] or not torch.isfinite(got[r, :, 7]).any()
