@@ -217,7 +217,8 @@ ipuc_status ipuc_cast(void *out, ipuc_precision to, const void *in, ipuc_precisi
  * scale <= 0 selects 1/sqrt(head_dim) (AttentionScale::InverseSqrtQueryWidth).
  * fp32 running max/denominator.  head_dim % 8 == 0 and head_dim <= 128
  * (smaller head dims are zero-padded to 128 inside the kernel); larger head
- * dims return IPUC_ERR_UNSUPPORTED.  Any query/key row counts >= 1. */
+ * dims return IPUC_ERR_UNSUPPORTED.  Any query/key row counts >= 1.  A score of
+ * NaN or +inf makes its row NaN. */
 ipuc_status ipuc_flash_attention_f16(void *out, ipuc_precision out_precision, const void *q,
                                      const void *k, const void *v, int64_t matrices,
                                      int64_t query_rows, int64_t key_rows, int64_t head_dim,

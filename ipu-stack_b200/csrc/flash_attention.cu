@@ -378,29 +378,31 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           float mx1 = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            mx = max3(mx, __uint_as_float(a[i]), __uint_as_float(a[i + 1]));
-            mx1 = max3(mx1, __uint_as_float(a[i + 2]), __uint_as_float(a[i + 3]));
-            mx = max3(mx, __uint_as_float(b[i]), __uint_as_float(b[i + 1]));
-            mx1 = max3(mx1, __uint_as_float(b[i + 2]), __uint_as_float(b[i + 3]));
+            mx = max3_nan(mx, __uint_as_float(a[i]), __uint_as_float(a[i + 1]));
+            mx1 = max3_nan(mx1, __uint_as_float(a[i + 2]), __uint_as_float(a[i + 3]));
+            mx = max3_nan(mx, __uint_as_float(b[i]), __uint_as_float(b[i + 1]));
+            mx1 = max3_nan(mx1, __uint_as_float(b[i + 2]), __uint_as_float(b[i + 3]));
           }
-          mx = fmaxf(mx, mx1);
+          mx = max_nan(mx, mx1);
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             if (i >= valid) a[i] = __float_as_uint(-INFINITY);
             if (i + 32 >= valid) b[i] = __float_as_uint(-INFINITY);
-            mx = fmaxf(mx, fmaxf(__uint_as_float(a[i]), __uint_as_float(b[i])));
+            mx = max3_nan(mx, __uint_as_float(a[i]), __uint_as_float(b[i]));
           }
         }
         xmax[t][h][row] = mx;
         named_barrier_sync(bar_id, 64);
-        mx = fmaxf(mx, xmax[t][h ^ 1][row]);
-        const float m_new = fmaxf(m, mx);
+        // A score of NaN or +inf makes the row NaN: the maximum carries it, which the
+        // polynomial below does not.
+        float m_new = max3_nan(m, mx, xmax[t][h ^ 1][row]);
+        if (m_new == INFINITY) m_new = NAN;
         bool rescale = false;
         float alpha = 1.0f;
         if (j == 0) {
           m = m_new;
-        } else if ((m_new - m) * c > RESCALE_THRESHOLD) {
+        } else if ((m_new - m) * c > RESCALE_THRESHOLD || isnan(m_new)) {
           alpha = ex2_approx((m - m_new) * c);
           rescale = true;
           m = m_new;
@@ -515,7 +517,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           store = false;
         } else {
           const float m_peer = recv_m[r2], l_peer = recv_l[r2];
-          const float mf = fmaxf(m, m_peer);
+          const float mf = max_nan(m, m_peer);
           a_own = ex2_approx((m - mf) * c);
           a_peer = ex2_approx((m_peer - mf) * c);
           l = l * a_own + l_peer * a_peer;
