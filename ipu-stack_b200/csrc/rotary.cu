@@ -32,7 +32,8 @@ struct TableParams {
 // a fraction in f32).  An angle is a fraction of a turn in 64-bit fixed point, so
 // position times frequency drops the whole turns by itself; the nearest whole
 // quarter is its rounded top two bits, and what is left, t in [-1/2, 1/2) of a
-// quarter, goes to f32 with 2^-32 of a quarter kept.  Sine and cosine of pi/2 t
+// quarter, comes in steps of 2^-32 and goes to f32, which rounds it by 2^-26 at
+// most.  Sine and cosine of pi/2 t
 // are their Taylor polynomials to t^9 and t^10 (the next terms are below 2e-9);
 // pi/2 in two parts keeps the sine to half a step and the rounding of t.  The
 // whole quarters swap and negate the two.  A thread writes V neighbouring pairs.
