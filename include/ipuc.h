@@ -560,9 +560,9 @@ ipuc_status ipuc_paged_append_f16(const ipuc_paged_cache *cache, const ipuc_page
  * v per head; query head h reads key head h / (q_heads / heads).  q [rows]
  * [q_heads][head_dim] f16 at stride q_stride, out [rows][q_heads][head_dim]
  * f16, dense, apart from q (refused where the two overlap).  scale <= 0 selects
- * 1/sqrt(head_dim).  A row that attends to
- * nothing gives 0.  A score of NaN or +inf makes its row NaN; a key of score
- * -inf has weight 0, and a row of such keys alone gives 0.
+ * 1/sqrt(head_dim); scale * log2(e) must be finite in f32.  A row that attends to
+ * nothing gives 0.  A score of NaN or +inf makes its row NaN; a key of score -inf
+ * has weight 0, and a row of such keys alone gives 0.
  * prefix_rows: positions below it are the same for all sequences and are read
  * through prefix_pages (device int32, ceil(prefix_rows / page_size) entries)
  * once for all rows, not through the table, whose entries for them are not

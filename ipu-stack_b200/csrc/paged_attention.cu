@@ -58,6 +58,7 @@ using namespace sm100;
 // within f16 (at most 2^12) and those down to 2^-18 of the largest normal.
 // Both factors cancel in O / l as long as every partial result has them.
 constexpr float kLazy = 8.0f, kShift = 4.0f;
+constexpr float kLog2e = 1.4426950408889634f;
 
 // What loading a unit's queries and storing its result costs, in key tiles: it
 // takes 5 to 6 us of a CTA of the tile kernel against 2.15 for a key tile, and
@@ -2017,7 +2018,7 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
     return fail(IPUC_ERR_UNSUPPORTED, "paged_attention: more than 128 query heads per key head are not supported");
   IPUC_CHECK_ARG(prefix_rows >= 0 && prefix_rows < (1ll << 31) - 256, "paged_attention: prefix_rows out of range");
   IPUC_CHECK_ARG(prefix_rows == 0 || prefix_pages, "paged_attention: null prefix_pages");
-  IPUC_CHECK_ARG(isfinite(scale), "paged_attention: scale must be finite");
+  IPUC_CHECK_ARG(isfinite(scale) && (scale <= 0.0f || isfinite(scale * kLog2e)), "paged_attention: scale must be finite");
   IPUC_CHECK_ARG(q_stride >= q_heads * d, "paged_attention: token stride shorter than q_heads * head_dim");
   IPUC_CHECK_ALIGN(q_stride % 8 == 0 && cache->page_stride % 8 == 0 && cache->head_stride % 8 == 0 &&
                        cache->row_stride % 8 == 0,
@@ -2051,7 +2052,7 @@ extern "C" ipuc_status ipuc_paged_attention_f16(void *out, const void *q, int64_
   p.head_dim = (int32_t)d;
   p.prefix = (int32_t)prefix_rows;
   p.chunk = gcd(cache->page_size, kStreamKeys);
-  p.scale_log2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float)d)) * 1.4426950408889634f;
+  p.scale_log2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float)d)) * kLog2e;
   p.stream_o = reinterpret_cast<float *>(ws + plan.stream_o);
   p.stream_ml = reinterpret_cast<float2 *>(ws + plan.stream_ml);
   p.stream_sums = reinterpret_cast<int64_t *>(ws + plan.stream_sums);

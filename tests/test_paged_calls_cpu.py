@@ -1,4 +1,6 @@
 """Refusals of the paged attention wrapper that need no GPU."""
+import ctypes
+
 import pytest
 import torch
 
@@ -41,3 +43,15 @@ def test_a_dense_workspace_is_passed_on_with_its_size(made, workspace, size):
     args, calls = made
     ipuc.paged_attention_f16(*args, workspace)
     assert calls[0][-2] == size and calls[0][-3] == (None if workspace is None else workspace.data_ptr())
+
+
+@pytest.mark.parametrize("scale,refused", [(3e38, True), (2.5e38, True), (2.3e38, False), (1e-45, False), (-3e38, False)])
+def test_a_scale_that_leaves_f32_in_the_exponent_is_refused(scale, refused):
+    """The kernels work in powers of two: scale * log2(e) has to be finite (a scale that is not positive selects the default)."""
+    fake = 1 << 20   # (a workspace of 0 bytes ends the calls whose scale is fine, before anything is launched)
+    cache = ipuc._PagedCache(fake, 2 * fake, 8, 16, 2, 64, 2048, 1024, 64)
+    batch = ipuc._PagedBatch(fake, fake, None, 4, 3, 3, 4)
+    status = ipuc.lib().ipuc_paged_attention_f16(5 * fake, 6 * fake, 256, 4, ctypes.byref(cache), ctypes.byref(batch), 0, None,
+                                                 scale, fake, 0, None)
+    assert status == ipuc.ERR_INVALID_ARGUMENT
+    assert (b"scale" if refused else b"workspace") in ipuc.lib().ipuc_last_error_string()
