@@ -394,10 +394,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         }
         xmax[t][h][row] = mx;
         named_barrier_sync(bar_id, 64);
-        // A score of NaN or +inf makes the row NaN: the maximum carries it, which the
-        // polynomial below does not.
-        float m_new = max3_nan(m, mx, xmax[t][h ^ 1][row]);
-        if (m_new == INFINITY) m_new = NAN;
+        // A score of NaN or +inf makes the row NaN: the maximum carries it (+inf up to
+        // the epilogue), which the polynomial below does not.
+        const float m_new = max3_nan(m, mx, xmax[t][h ^ 1][row]);
         bool rescale = false;
         float alpha = 1.0f;
         if (j == 0) {
@@ -464,6 +463,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       if (!ok) break;
       // Epilogue: combine the two partial row sums, then O_t / l -> out for this
       // warp's 64 columns.
+      if (m == INFINITY) l = NAN;
       xsum[t][h][row] = l;
       named_barrier_sync(bar_id, 64);
       l += xsum[t][h ^ 1][row];

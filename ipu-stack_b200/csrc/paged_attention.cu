@@ -1555,10 +1555,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         mx = max_nan(mx, mx1);
         x_max[t][half][row] = mx;
         named_barrier_sync(bar_id, 64);
-        // A score of NaN or +inf makes the row NaN.  The maximum carries that: the
-        // polynomial below, which takes one pair in three, does not.
-        float m_new = max_nan(m, max_nan(mx, x_max[t][half ^ 1][row]));
-        if (m_new == INFINITY) m_new = NAN;
+        // A score of NaN or +inf makes the row NaN.  The maximum carries that (+inf up
+        // to the unit's end): the polynomial below, which takes one pair in three, does not.
+        const float m_new = max3_nan(m, mx, x_max[t][half ^ 1][row]);
         bool rescale = false;
         float alpha = 1.0f;
         if (j == 0) {
@@ -1622,6 +1621,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_ready[t]);
       }
+      if (m == INFINITY) l = NAN;
       x_sum[t][half][row] = l;
       named_barrier_sync(bar_id, 64);
       l += x_sum[t][half ^ 1][row];
